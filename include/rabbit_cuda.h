@@ -459,6 +459,155 @@ int rabbit_cuda_refv2_position(const rabbit_cuda_refv2 *c);
  * the copies of its outputs to the host are outside it. */
 int rabbit_cuda_refv2_device_ms(const rabbit_cuda_refv2 *c, float *ms);
 
+/* ------------------------------------------------- rotary positions -- */
+
+/* Element types of the activations the entry points below take. */
+#define RABBIT_CUDA_F32 0
+#define RABBIT_CUDA_F16 1
+#define RABBIT_CUDA_BF16 2
+
+/* Which channels of a head rotate together: (2 i, 2 i + 1), the reference's
+ * (src/forward_v2.c:92-104), or (i, i + rot_dim / 2). */
+#define RABBIT_CUDA_ROPE_INTERLEAVED 0
+#define RABBIT_CUDA_ROPE_HALF 1
+
+/* How the pair frequencies f_i = base^(-2 i / rot_dim) are scaled for contexts
+ * longer than the model's first one. */
+#define RABBIT_CUDA_ROPE_SCALE_NONE 0
+#define RABBIT_CUDA_ROPE_SCALE_LINEAR 1 /* f_i / factor */
+#define RABBIT_CUDA_ROPE_SCALE_NTK 2    /* base * factor^(rot_dim / (rot_dim - 2)) */
+#define RABBIT_CUDA_ROPE_SCALE_BANDS 3  /* by turns over the first context, n_i = original_ctx
+                                           f_i / 2 pi: n_i <= low: f_i / factor; n_i >= high:
+                                           f_i; linear in n_i between */
+#define RABBIT_CUDA_ROPE_SCALE_YARN 4   /* YaRN: by pair index, from f_i at the pair that turns
+                                           `high` times over original_ctx (rounded down) to
+                                           f_i / factor at the one that turns `low` times
+                                           (rounded up), linear in i between */
+
+typedef struct {
+    int head_dim;       /* 2..1024 */
+    int rot_dim;        /* channels that rotate, the first of each head: even, 2..512 and at
+                           most head_dim; 0 means head_dim */
+    int layout;         /* RABBIT_CUDA_ROPE_INTERLEAVED / _HALF */
+    int scaling;        /* RABBIT_CUDA_ROPE_SCALE_* */
+    double base;        /* 0 means 10000 (forward_v2.c:96) */
+    double factor;      /* > 0; 0 means 1; not read without scaling */
+    double low, high;   /* BANDS / YARN; 0 means 1 and 4 (BANDS), 1 and 32 (YARN) */
+    int original_ctx;   /* BANDS / YARN: the first context's length, > 0 */
+    double magnitude;   /* multiplies the rotated channels; 0 means 1, with YARN
+                           1 + 0.1 ln(factor) (factor above 1) */
+} rabbit_cuda_rope_desc;
+
+typedef struct rabbit_cuda_rope rabbit_cuda_rope;
+
+/* The frequencies of `desc` in 64 bits (host only: touches no GPU). One object
+ * serves every device, stream and thread. */
+int rabbit_cuda_rope_create(const rabbit_cuda_rope_desc *desc, rabbit_cuda_rope **out);
+int rabbit_cuda_rope_free(rabbit_cuda_rope *r);
+/* The angle per position of each pair, freq[rot_dim / 2], and the magnitude.
+ * Any pointer may be NULL. */
+int rabbit_cuda_rope_freqs(const rabbit_cuda_rope *r, double *freq, double *magnitude);
+/* Rotate n_tokens rows of n_heads heads: row t at x + t * x_stride elements
+ * (0: n_heads * head_dim), its heads head_dim apart; d_positions [n_tokens].
+ * With the pair's angle a = position * f_i taken in 64 bits,
+ *   y_1 = m (x_1 cos a - x_2 sin a),  y_2 = m (x_2 cos a + x_1 sin a)
+ * in 32 bits, rounded to `dtype` once; channels from rot_dim on are copied.
+ * y may be x (with the same stride); otherwise they must not overlap. DEVICE
+ * buffers aligned to their element, asynchronous on `stream`, on the calling
+ * thread's device (rabbit_cuda_set_device); may be captured into a graph.
+ * n_tokens 0 does nothing. */
+int rabbit_cuda_rope_dev(const rabbit_cuda_rope *r, int dtype, const void *d_x, int64_t x_stride,
+                         void *d_y, int64_t y_stride, const int *d_positions, int n_tokens,
+                         int n_heads, void *stream);
+
+/* ------------------------------------------- paged key / value cache, 4 bit -- */
+
+/* Keys and values of many sequences in pages of page_size tokens, in 4 bits
+ * (no counterpart in the reference, whose KV cache is fp32 and holds one
+ * sequence of at most 256 tokens, src/forward_v2.c:16-26). For each token, KV
+ * head and 32 consecutive channels x (the last group of a head may be
+ * shorter): scale s = bf16(max|x| / 7) (the fp32 product with 1/7, rounded),
+ * codes rint(x / s), a channel read back as code * s; s = 0: all zero. Each group has its own codes, so a token
+ * can be written without touching its neighbours: 18 bytes per 32 channels. A
+ * group that holds an infinity or a NaN reads back as NaN. Slot = page *
+ * page_size + place in the page; every layer has the same pages. */
+typedef struct {
+    int n_layers;    /* >= 1 */
+    int n_kv_heads;  /* 1..1024 */
+    int head_dim;    /* a multiple of 8, 8..256 */
+    int page_size;   /* tokens, a multiple of 16, 16..1024 */
+    int n_pages;     /* >= 1 */
+} rabbit_cuda_kv4_desc;
+
+typedef struct rabbit_cuda_kv4 rabbit_cuda_kv4;
+
+/* Allocates the pages on `device` and zeroes them. */
+int rabbit_cuda_kv4_create(const rabbit_cuda_kv4_desc *desc, int device, rabbit_cuda_kv4 **out);
+int rabbit_cuda_kv4_free(rabbit_cuda_kv4 *kv);
+/* Bytes in HBM of every layer's pages. */
+uint64_t rabbit_cuda_kv4_bytes(const rabbit_cuda_kv4 *kv);
+/* Write n_tokens rows of n_kv_heads heads of keys and values (row t at
+ * t * stride elements, 0: n_kv_heads * head_dim) into slots d_slots[t] of
+ * `layer`. A negative slot is skipped (padding). With `rope` (of the same
+ * head_dim; may be NULL) the keys are first rotated by d_positions[t], in 64
+ * bits, so the codes are those of the exactly rotated key. Slots of one call
+ * should differ: of two rows written to one slot the slot holds a mix. A slot
+ * past the cache is skipped and reported by rabbit_cuda_kv4_check. DEVICE
+ * buffers aligned to their element, asynchronous on `stream`; may be captured
+ * into a graph. n_tokens 0 does nothing. */
+int rabbit_cuda_kv4_append_dev(rabbit_cuda_kv4 *kv, int layer, int dtype, const void *d_k,
+                               int64_t k_stride, const void *d_v, int64_t v_stride,
+                               const int64_t *d_slots, int n_tokens, const rabbit_cuda_rope *rope,
+                               const int *d_positions, void *stream);
+/* The rows of slots d_slots[t] as the cache holds them (code * s, rounded to
+ * `dtype`): [n_tokens][n_kv_heads][head_dim], d_k or d_v may be NULL. Rows of
+ * negative slots, and of slots past the cache (reported by
+ * rabbit_cuda_kv4_check), are left as they were. */
+int rabbit_cuda_kv4_read_dev(rabbit_cuda_kv4 *kv, int layer, int dtype, const int64_t *d_slots,
+                             int n_tokens, void *d_k, void *d_v, void *stream);
+
+/* The sequences of an attention call, in DEVICE arrays that are read when the
+ * call runs (so a captured graph sees their values at replay). */
+typedef struct {
+    int n_seqs;              /* 0..65535 */
+    int max_pages;           /* entries of a page_table row */
+    int max_q_len;           /* at least the longest sequence's query rows; 0 means 1 */
+    const int *d_q_start;    /* [n_seqs + 1] ascending: query rows of sequence i are
+                                [q_start[i], q_start[i + 1]); NULL: row i is sequence i's only one */
+    const int *d_kv_len;     /* [n_seqs] cached positions, the query rows' own included */
+    const int *d_page_table; /* [n_seqs][max_pages] page of positions j * page_size .. */
+} rabbit_cuda_kv4_batch;
+
+/* What an attention call needs while it runs (partial sums of sequences split
+ * over the SMs), allocated once; it serves any layer, batch and head count of
+ * `kv`. Calls, and graphs that hold them, that may run at the same time need
+ * one each. */
+typedef struct rabbit_cuda_kv4_scratch rabbit_cuda_kv4_scratch;
+int rabbit_cuda_kv4_scratch_create(const rabbit_cuda_kv4 *kv, rabbit_cuda_kv4_scratch **out);
+int rabbit_cuda_kv4_scratch_free(rabbit_cuda_kv4_scratch *ws);
+
+/* Attention of n_tokens query rows (n_heads heads, a multiple of n_kv_heads;
+ * query head h reads KV head h / (n_heads / n_kv_heads)) over `layer`'s cache.
+ * The last query row of a sequence is its last cached position, the row before
+ * it one earlier, and so on; a row at position p sees positions 0..p, with
+ * window > 0 only the last `window` of them. out = sum_j softmax_j(scale q.k_j)
+ * v_j; scale 0 means 1 / sqrt(head_dim); a row that sees nothing gives 0. Rows
+ * behind the last sequence are left as they were; a row past n_tokens is not
+ * written. Strides in elements between rows (0: n_heads * head_dim); out may be
+ * q with the same stride. Positions past max_pages pages, pages past the cache
+ * and q_start not ascending read as nothing there and are reported by
+ * rabbit_cuda_kv4_check. DEVICE buffers aligned to their element, asynchronous on
+ * `stream`; may be captured into a graph. */
+int rabbit_cuda_kv4_attention_dev(rabbit_cuda_kv4 *kv, int layer, rabbit_cuda_kv4_scratch *ws,
+                                  int dtype, const void *d_q, int64_t q_stride, void *d_out,
+                                  int64_t out_stride, int n_tokens, int n_heads,
+                                  const rabbit_cuda_kv4_batch *batch, float scale, int window,
+                                  void *stream);
+/* Synchronises `stream` and reports, once, what calls on this cache found out
+ * of range since the last check (RABBIT_CUDA_ERR_ARGS) or a bounded wait that
+ * gave up (RABBIT_CUDA_ERR_TIMEOUT). */
+int rabbit_cuda_kv4_check(rabbit_cuda_kv4 *kv, void *stream);
+
 #if defined(__GNUC__)
 #pragma GCC visibility pop
 #endif

@@ -44,8 +44,29 @@ class DenseDesc(C.Structure):
                 ("w_v", C.POINTER(C.c_void_p)), ("w_o", C.POINTER(C.c_void_p))]
 
 
+class RopeDesc(C.Structure):
+    """rabbit_cuda_rope_desc"""
+    _fields_ = [("head_dim", C.c_int), ("rot_dim", C.c_int), ("layout", C.c_int),
+                ("scaling", C.c_int), ("base", C.c_double), ("factor", C.c_double),
+                ("low", C.c_double), ("high", C.c_double), ("original_ctx", C.c_int),
+                ("magnitude", C.c_double)]
+
+
+class Kv4Desc(C.Structure):
+    """rabbit_cuda_kv4_desc"""
+    _fields_ = [("n_layers", C.c_int), ("n_kv_heads", C.c_int), ("head_dim", C.c_int),
+                ("page_size", C.c_int), ("n_pages", C.c_int)]
+
+
+class Kv4Batch(C.Structure):
+    """rabbit_cuda_kv4_batch: device arrays as ints (kept alive by the caller)."""
+    _fields_ = [("n_seqs", C.c_int), ("max_pages", C.c_int), ("max_q_len", C.c_int),
+                ("d_q_start", C.c_void_p), ("d_kv_len", C.c_void_p), ("d_page_table", C.c_void_p)]
+
+
 _P = C.c_void_p
 _I = C.c_int
+_L = C.c_int64
 # name -> (restype, argtypes)
 SIGNATURES = {
     "rabbit_cuda_version": (C.c_char_p, []),
@@ -117,6 +138,20 @@ SIGNATURES = {
     "rabbit_cuda_refv2_generate": (_I, [_P, _I, _P]),
     "rabbit_cuda_refv2_position": (_I, [_P]),
     "rabbit_cuda_refv2_device_ms": (_I, [_P, C.POINTER(C.c_float)]),
+    "rabbit_cuda_rope_create": (_I, [C.POINTER(RopeDesc), C.POINTER(_P)]),
+    "rabbit_cuda_rope_free": (_I, [_P]),
+    "rabbit_cuda_rope_freqs": (_I, [_P, _P, C.POINTER(C.c_double)]),
+    "rabbit_cuda_rope_dev": (_I, [_P, _I, _P, _L, _P, _L, _P, _I, _I, _P]),
+    "rabbit_cuda_kv4_create": (_I, [C.POINTER(Kv4Desc), _I, C.POINTER(_P)]),
+    "rabbit_cuda_kv4_free": (_I, [_P]),
+    "rabbit_cuda_kv4_bytes": (C.c_uint64, [_P]),
+    "rabbit_cuda_kv4_append_dev": (_I, [_P, _I, _I, _P, _L, _P, _L, _P, _I, _P, _P, _P]),
+    "rabbit_cuda_kv4_read_dev": (_I, [_P, _I, _I, _P, _I, _P, _P, _P]),
+    "rabbit_cuda_kv4_scratch_create": (_I, [_P, C.POINTER(_P)]),
+    "rabbit_cuda_kv4_scratch_free": (_I, [_P]),
+    "rabbit_cuda_kv4_attention_dev": (_I, [_P, _I, _P, _I, _P, _L, _P, _L, _I, _I,
+                                           C.POINTER(Kv4Batch), C.c_float, _I, _P]),
+    "rabbit_cuda_kv4_check": (_I, [_P, _P]),
 }
 
 _LIB: C.CDLL | None = None
@@ -545,3 +580,126 @@ class Cache:
         if self.handle:
             lib().rabbit_cuda_cache_free(self.handle)
             self.handle = None
+
+
+F32, F16, BF16 = range(3)  # RABBIT_CUDA_F32 ...
+ROPE_INTERLEAVED, ROPE_HALF = range(2)
+(ROPE_SCALE_NONE, ROPE_SCALE_LINEAR, ROPE_SCALE_NTK, ROPE_SCALE_BANDS,
+ ROPE_SCALE_YARN) = range(5)
+
+
+class Rope:
+    """Rotary positions (rabbit_cuda_rope): the frequencies, in 64 bits on the
+    host; 0 for an argument means its default."""
+
+    def __init__(self, head_dim: int, *, rot_dim: int = 0, layout: int = ROPE_INTERLEAVED,
+                 scaling: int = ROPE_SCALE_NONE, base: float = 0.0, factor: float = 0.0,
+                 low: float = 0.0, high: float = 0.0, original_ctx: int = 0,
+                 magnitude: float = 0.0):
+        d = RopeDesc(head_dim, rot_dim, layout, scaling, base, factor, low, high, original_ctx,
+                     magnitude)
+        h = C.c_void_p()
+        check(lib().rabbit_cuda_rope_create(C.byref(d), C.byref(h)))
+        self.handle = h
+        self.head_dim, self.rot_dim = head_dim, rot_dim or head_dim
+
+    def freqs(self):
+        """(angle per position of each pair [rot_dim / 2], magnitude)"""
+        f = np.zeros(self.rot_dim // 2, np.float64)
+        m = C.c_double()
+        check(lib().rabbit_cuda_rope_freqs(self.handle, _ptr(f), C.byref(m)))
+        return f, m.value
+
+    def apply_dev(self, dtype: int, d_x: int, d_y: int, d_positions: int, n_tokens: int,
+                  n_heads: int, *, x_stride: int = 0, y_stride: int = 0, stream: int = 0) -> None:
+        """y = x rotated (rabbit_cuda_rope_dev); strides in elements between rows."""
+        check(lib().rabbit_cuda_rope_dev(self.handle, dtype, d_x, x_stride, d_y, y_stride,
+                                         d_positions, n_tokens, n_heads, stream or None))
+
+    def free(self) -> None:
+        if self.handle:
+            check(lib().rabbit_cuda_rope_free(self.handle))
+            self.handle = C.c_void_p()
+
+    def __del__(self):
+        try:
+            self.free()
+        except Exception:
+            pass
+
+
+class Kv4:
+    """A paged key / value cache in 4 bits (rabbit_cuda_kv4); slot =
+    page * page_size + place in the page. Device pointers as ints."""
+
+    def __init__(self, *, n_layers: int, n_kv_heads: int, head_dim: int, page_size: int,
+                 n_pages: int, device: int = 0):
+        d = Kv4Desc(n_layers, n_kv_heads, head_dim, page_size, n_pages)
+        h = C.c_void_p()
+        check(lib().rabbit_cuda_kv4_create(C.byref(d), device, C.byref(h)))
+        self.handle = h
+        self.n_layers, self.n_kv_heads, self.head_dim = n_layers, n_kv_heads, head_dim
+        self.page_size, self.n_pages = page_size, n_pages
+
+    @property
+    def nbytes(self) -> int:
+        return int(lib().rabbit_cuda_kv4_bytes(self.handle))
+
+    def append_dev(self, layer: int, dtype: int, d_k: int, d_v: int, d_slots: int, n_tokens: int, *,
+                   rope: Rope | None = None, d_positions: int = 0, k_stride: int = 0,
+                   v_stride: int = 0, stream: int = 0) -> None:
+        """Rows of keys (rotated by `rope`) and values into int64 slots
+        (rabbit_cuda_kv4_append_dev); negative slots are skipped."""
+        check(lib().rabbit_cuda_kv4_append_dev(
+            self.handle, layer, dtype, d_k, k_stride, d_v, v_stride, d_slots, n_tokens,
+            rope.handle if rope else None, d_positions or None, stream or None))
+
+    def read_dev(self, layer: int, dtype: int, d_slots: int, n_tokens: int, d_k: int, d_v: int,
+                 stream: int = 0) -> None:
+        """The rows of int64 slots as the cache holds them (rabbit_cuda_kv4_read_dev)."""
+        check(lib().rabbit_cuda_kv4_read_dev(self.handle, layer, dtype, d_slots, n_tokens,
+                                             d_k or None, d_v or None, stream or None))
+
+    def attention_dev(self, layer: int, scratch: "Kv4Scratch", dtype: int, d_q: int, d_out: int,
+                      n_tokens: int, n_heads: int, batch: Kv4Batch, *, scale: float = 0.0,
+                      window: int = 0, q_stride: int = 0, out_stride: int = 0,
+                      stream: int = 0) -> None:
+        """Attention of n_tokens query rows over the cache (rabbit_cuda_kv4_attention_dev)."""
+        check(lib().rabbit_cuda_kv4_attention_dev(
+            self.handle, layer, scratch.handle, dtype, d_q, q_stride, d_out, out_stride, n_tokens,
+            n_heads, C.byref(batch), scale, window, stream or None))
+
+    def check(self, stream: int = 0) -> None:
+        check(lib().rabbit_cuda_kv4_check(self.handle, stream or None))
+
+    def free(self) -> None:
+        if self.handle:
+            check(lib().rabbit_cuda_kv4_free(self.handle))
+            self.handle = C.c_void_p()
+
+    def __del__(self):
+        try:
+            self.free()
+        except Exception:
+            pass
+
+
+class Kv4Scratch:
+    """Workspace of attention calls on a Kv4 (rabbit_cuda_kv4_scratch): one for
+    each chain of calls that may run at the same time as another."""
+
+    def __init__(self, kv: Kv4):
+        h = C.c_void_p()
+        check(lib().rabbit_cuda_kv4_scratch_create(kv.handle, C.byref(h)))
+        self.handle = h
+
+    def free(self) -> None:
+        if self.handle:
+            check(lib().rabbit_cuda_kv4_scratch_free(self.handle))
+            self.handle = C.c_void_p()
+
+    def __del__(self):
+        try:
+            self.free()
+        except Exception:
+            pass
