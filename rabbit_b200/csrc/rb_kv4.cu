@@ -113,10 +113,12 @@ __global__ void __launch_bounds__(kAppendThreads) k_kv4_append(const __grid_cons
         top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
         if (!write) continue;
-        const __nv_bfloat16 sb = __float2bfloat16_rn(__fmul_rn(__uint_as_float(top), 1.0f / 7.0f));
+        // a group with an infinity or a NaN has a NaN for its scale
+        const float top7 = __fmul_rn(__uint_as_float(top), 1.0f / 7.0f);
+        const __nv_bfloat16 sb = __float2bfloat16_rn(top7 < INFINITY ? top7 : __uint_as_float(0x7fc00000u));
         const float s = __bfloat162float(sb), inv = 1.0f / s;
         uint32_t word = 0x88888888u;
-        if (s > 0.f && s < INFINITY) {
+        if (s > 0.f) {
             word = 0;
 #pragma unroll
             for (int n = 0; n < 8; ++n) word |= (uint32_t)(kv4_code(x[n], s, inv) + 8) << (4 * n);
