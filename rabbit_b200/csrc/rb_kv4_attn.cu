@@ -15,8 +15,6 @@ struct rabbit_cuda_kv4_scratch {
 
 namespace rb {
 
-constexpr int kDecodeGrid = 2;  // CTAs per SM at most
-
 template <int NG, int RB, bool SPLIT>
 static cudaError_t launch_decode(const Kv4AttnArgs &a, const rabbit_cuda_kv4 *kv, cudaStream_t s) {
     using C = DecodeCfg<NG, RB, SPLIT>;
@@ -28,7 +26,8 @@ static cudaError_t launch_decode(const Kv4AttnArgs &a, const rabbit_cuda_kv4 *kv
         if (e != cudaSuccess) return e;
         ready.fetch_or(1u << kv->device);
     }
-    return launch_pdl(kern, dim3(C::kCtas * kv->ctx->sm_count), dim3(C::kThreads), C::kSmem, s, a);
+    const int grid = C::kCtas * kv->ctx->sm_count;
+    return launch_pdl(kern, dim3(grid < kDecodeMaxGrid ? grid : kDecodeMaxGrid), dim3(C::kThreads), C::kSmem, s, a);
 }
 
 // Rows of a tile: 16 where a KV head has more than 8 query rows and the output
@@ -69,7 +68,7 @@ int rabbit_cuda_kv4_scratch_create(const rabbit_cuda_kv4 *kv, rabbit_cuda_kv4_sc
     ws->ng = kv->view.ng;
     // two partial results a CTA (the item its run continues, the one it leaves
     // unfinished) of the largest tile: outputs, then (reference, sum) pairs
-    const size_t ctas = (size_t)kDecodeGrid * kv->ctx->sm_count;
+    const size_t ctas = kDecodeMaxGrid;
     const size_t rows = ws->ng <= 4 ? 16 : 8;
     const size_t bytes = sizeof(float) * 2 * ctas * rows * (32 * ws->ng + 2);
     DeviceScope scope(kv->device);

@@ -55,21 +55,58 @@ __host__ __device__ inline int kv4_seq(int s0, int s1, int len, int T, int max_q
     return bad;
 }
 
-// Work is counted in units: a granule of one item (sequence, row tile, KV head);
-// an item that sees no granule has one unit, for the zeros it writes. The units
-// of all items in order are cut into `parts` runs of equal length, run b of
-// [u(b), u(b + 1)), u(b) = floor(b total / parts); with parts <= total none is
-// empty.
-__host__ __device__ inline int64_t kv4_items(const Kv4Seq &s, int group, int rows, int nkv) {
-    return s.nq ? (int64_t)nkv * (((int64_t)s.nq * group + rows - 1) / rows) : 0;
+// Work is counted in units: an item (sequence, row tile, KV head) has kKv4Fixed
+// units for what it costs whatever its length (its query operands, its merge)
+// and one for each granule it sees, at least one (for the zeros of an item
+// that sees none). The units of all items in order are cut into `parts` runs
+// of equal length, run b of [u(b), u(b + 1)), u(b) = floor(b total / parts). A run
+// works on the granules whose units are in it; one that ends within an item's
+// fixed units leaves the whole item to the next. Runs are at least kKv4MinRun
+// long, more than an item's fixed units, so each has some granule's unit.
+constexpr int kKv4Fixed = 8, kKv4MinRun = 14;
+__host__ __device__ inline int kv4_items(const Kv4Seq &s, int group, int rows, int nkv) {
+    return s.nq ? nkv * ((s.nq * group + rows - 1) / rows) : 0;
 }
-__host__ __device__ inline int kv4_units(const Kv4Seq &s) { return s.n > 0 ? s.n : 1; }
+__host__ __device__ inline int kv4_granules(const Kv4Seq &s) { return s.n > 0 ? s.n : 1; }
+__host__ __device__ inline int64_t kv4_cost(const Kv4Seq &s, int group, int rows, int nkv) {
+    return (int64_t)kv4_items(s, group, rows, nkv) * (kv4_granules(s) + kKv4Fixed);
+}
+__host__ __device__ inline int64_t kv4_parts(int64_t total, int grid) {
+    const int64_t most = total / kKv4MinRun;
+    return most < 1 ? 1 : most < grid ? most : grid;
+}
 __host__ __device__ inline int64_t kv4_cut(int64_t b, int64_t total, int64_t parts) {
     return b * total / parts;
 }
 // The run that unit x falls into.
 __host__ __device__ inline int kv4_run_of(int64_t x, int64_t total, int64_t parts) {
     return (int)(((x + 1) * parts - 1) / total);
+}
+
+// A run's share of one item.
+struct Kv4Share {
+    int from, take;   // granules [from, from + take) of the item's
+    bool begins, ends;
+    int first, last;  // the runs that have a share of the item
+};
+// A walk over a run's items: `off` units of item `sub` of sequence `s` lie before
+// unit `u`. The share of the item in [u, u1), or take 0 where it has none.
+__host__ __device__ inline Kv4Share kv4_share(const Kv4Seq &s, int off, int64_t u, int64_t u1,
+                                              int64_t total, int64_t parts) {
+    Kv4Share r;
+    const int n = kv4_granules(s);
+    const int64_t start = u - off + kKv4Fixed;  // the first granule's unit
+    const int64_t to = u1 < start + n ? u1 : start + n;
+    r.from = off > kKv4Fixed ? off - kKv4Fixed : 0;
+    r.take = to > start + r.from ? (int)(to - start) - r.from : 0;
+    r.begins = r.from == 0;
+    r.ends = r.from + r.take == n;
+    r.first = r.last = 0;
+    if (!(r.begins && r.ends)) {
+        r.first = kv4_run_of(start, total, parts);
+        r.last = kv4_run_of(start + n - 1, total, parts);
+    }
+    return r;
 }
 
 #ifdef __CUDACC__
@@ -142,32 +179,61 @@ __device__ __forceinline__ float piece_bf16(const uint32_t (&w)[NW], int i) {
     return __uint_as_float(i & 1 ? w[i >> 1] & 0xffff0000u : w[i >> 1] << 16);
 }
 
-// Token of a granule's first half that column j of a score tile stands for;
-// the same in the second half, 8 later. The order keeps the lanes' loads of K
-// (columns 2 i and 2 i + 1) and of V (columns 2 t, then 2 t + 1, of the four t)
-// in different banks.
+// Token of a granule's first half that row j of a score tile stands for; the
+// same in the second half, 8 later. The order keeps the lanes' loads of K (rows
+// 2 i and 2 i + 1) and of V (rows 2 t, then 2 t + 1, of the four t) in different
+// banks.
 __device__ __forceinline__ int kv4_token(int j) { return j & 1 ? 4 + ((j >> 1) ^ 1) : j >> 1; }
 
-// The value pieces of two tokens (a: even column, b: odd) as fp16 pairs of
-// signed codes, channel 4 g + i of group `grp` in e[i]: a nibble under the
-// exponent of 1024 is 1024 + u, of 16 u in the next nibble 1024 + 16 u; one
-// addition or multiply-add, exact, leaves u - 8. Signed here, where the K side
-// takes its bias off by the accumulator's start: sums of values over a long
-// context cancel, and with the bias in them would keep 2^-24 of 8 sum w
-// instead of 2^-24 of themselves.
-template <int NW>
-__device__ __forceinline__ void value_codes(uint32_t (&e)[4], const uint32_t (&a)[NW],
-                                            const uint32_t (&b)[NW], int grp) {
-    const uint32_t x = __byte_perm(a[grp >> 1], b[grp >> 1], grp & 1 ? 0x7632 : 0x5410), y = x >> 8;
+// Signed codes of the lowest nibble of each half word, and of the next one, as
+// fp16 pairs: a nibble under the exponent of 1024 is 1024 + u, of the next
+// nibble 1024 + 16 u; one addition or multiply-add, exact, leaves u - 8.
+__device__ __forceinline__ void signed_codes(uint32_t &e0, uint32_t &e1, uint32_t x) {
     const __half2 bias = __half2half2(__ushort_as_half(0xE408)),   // -1032
         sixteenth = __half2half2(__ushort_as_half(0x2C00)),        // 1 / 16
         bias16 = __half2half2(__ushort_as_half(0xD480));           // -72
     auto half2_of = [](uint32_t v) { return *reinterpret_cast<__half2 *>(&v); };
     auto bits = [](__half2 v) { return *reinterpret_cast<uint32_t *>(&v); };
-    e[0] = bits(__hadd2(half2_of(and_or<0x000f000fu, 0x64006400u>(x)), bias));
-    e[1] = bits(__hfma2(half2_of(and_or<0x00f000f0u, 0x64006400u>(x)), sixteenth, bias16));
-    e[2] = bits(__hadd2(half2_of(and_or<0x000f000fu, 0x64006400u>(y)), bias));
-    e[3] = bits(__hfma2(half2_of(and_or<0x00f000f0u, 0x64006400u>(y)), sixteenth, bias16));
+    e0 = bits(__hadd2(half2_of(and_or<0x000f000fu, 0x64006400u>(x)), bias));
+    e1 = bits(__hfma2(half2_of(and_or<0x00f000f0u, 0x64006400u>(x)), sixteenth, bias16));
+}
+
+// The value pieces of two tokens (a: even column, b: odd) as fp16 pairs of
+// signed codes, channel 4 g + i of group `grp` in e[i]. Signed, where the K side
+// may take its bias off by the accumulator's start: sums of values over a long
+// context cancel, and with the bias in them would keep 2^-24 of 8 sum w
+// instead of 2^-24 of themselves.
+template <int NW>
+__device__ __forceinline__ void value_codes(uint32_t (&e)[4], const uint32_t (&a)[NW],
+                                            const uint32_t (&b)[NW], int grp) {
+    const uint32_t x = __byte_perm(a[grp >> 1], b[grp >> 1], grp & 1 ? 0x7632 : 0x5410);
+    signed_codes(e[0], e[1], x);
+    signed_codes(e[2], e[3], x >> 8);
+}
+
+// The transpose of an 8 x 8 matrix of fp16 whose row g, columns 2 t and 2 t + 1
+// are lane (g, t)'s pair.
+__device__ __forceinline__ uint32_t transpose8(uint32_t a) {
+    uint32_t d;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+    return d;
+}
+
+// A key word as fp16 pairs, nibbles (0, 4), (2, 6), (1, 5), (3, 7) of it.
+// SIGNED: the codes; else u 2^-24 for the first two and 16 u 2^-24 for the
+// others, as they lie.
+template <bool SIGNED>
+__device__ __forceinline__ void key_codes(uint32_t (&e)[4], uint32_t x) {
+    const uint32_t y = x >> 8;
+    if constexpr (SIGNED) {
+        signed_codes(e[0], e[2], x);
+        signed_codes(e[1], e[3], y);
+    } else {
+        e[0] = x & 0x000f000fu;
+        e[1] = y & 0x000f000fu;
+        e[2] = x & 0x00f000f0u;
+        e[3] = y & 0x00f000f0u;
+    }
 }
 #endif
 
