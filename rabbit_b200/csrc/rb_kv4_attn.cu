@@ -18,7 +18,7 @@ namespace rb {
 template <int NG, int RB, bool SPLIT>
 static cudaError_t launch_decode(const Kv4AttnArgs &a, const rabbit_cuda_kv4 *kv, cudaStream_t s) {
     using C = DecodeCfg<NG, RB, SPLIT>;
-    static_assert(C::kSmem <= kMaxDynSmem, "shared memory of a CTA");
+    static_assert(C::kSmem + 5120 <= kMaxDynSmem, "shared memory of a CTA, the static part with it");
     auto kern = k_kv4_decode<NG, RB, SPLIT>;
     static std::atomic<uint32_t> ready{0};  // devices whose limit is raised
     if (!(ready.load() >> kv->device & 1u)) {
@@ -26,7 +26,7 @@ static cudaError_t launch_decode(const Kv4AttnArgs &a, const rabbit_cuda_kv4 *kv
         if (e != cudaSuccess) return e;
         ready.fetch_or(1u << kv->device);
     }
-    const int grid = C::kCtas * kv->ctx->sm_count;
+    const int grid = kv->ctx->sm_count;
     return launch_pdl(kern, dim3(grid < kDecodeMaxGrid ? grid : kDecodeMaxGrid), dim3(C::kThreads), C::kSmem, s, a);
 }
 

@@ -55,21 +55,20 @@ __host__ __device__ inline int kv4_seq(int s0, int s1, int len, int T, int max_q
     return bad;
 }
 
-// Work is counted in units: an item (sequence, row tile, KV head) has kKv4Fixed
-// units for what it costs whatever its length (its query operands, its merge)
-// and one for each granule it sees, at least one (for the zeros of an item
-// that sees none). The units of all items in order are cut into `parts` runs
-// of equal length, run b of [u(b), u(b + 1)), u(b) = floor(b total / parts). A run
-// works on the granules whose units are in it; one that ends within an item's
-// fixed units leaves the whole item to the next. Runs are at least kKv4MinRun
-// long, more than an item's fixed units, so each has some granule's unit.
-constexpr int kKv4Fixed = 8, kKv4MinRun = 14;
+// Work is counted in units: an item (sequence, row tile, KV head) that sees some
+// granule has kKv4Fixed units for what it costs whatever its length (its query
+// operands, its merge) and one for each granule. The units of all items in
+// order are cut into `parts` runs of equal length, run b of [u(b), u(b + 1)), u(b)
+// = floor(b total / parts). A run works on the granules whose units are in it; one
+// that ends within an item's fixed units leaves the whole item to the next. Runs
+// are at least kKv4MinRun long, more than an item's fixed units, so each has some
+// granule's unit.
+constexpr int kKv4Fixed = 12, kKv4MinRun = 16;
 __host__ __device__ inline int kv4_items(const Kv4Seq &s, int group, int rows, int nkv) {
-    return s.nq ? nkv * ((s.nq * group + rows - 1) / rows) : 0;
+    return s.nq && s.n > 0 ? nkv * ((s.nq * group + rows - 1) / rows) : 0;
 }
-__host__ __device__ inline int kv4_granules(const Kv4Seq &s) { return s.n > 0 ? s.n : 1; }
 __host__ __device__ inline int64_t kv4_cost(const Kv4Seq &s, int group, int rows, int nkv) {
-    return (int64_t)kv4_items(s, group, rows, nkv) * (kv4_granules(s) + kKv4Fixed);
+    return (int64_t)kv4_items(s, group, rows, nkv) * (s.n + kKv4Fixed);
 }
 __host__ __device__ inline int64_t kv4_parts(int64_t total, int grid) {
     const int64_t most = total / kKv4MinRun;
@@ -94,7 +93,7 @@ struct Kv4Share {
 __host__ __device__ inline Kv4Share kv4_share(const Kv4Seq &s, int off, int64_t u, int64_t u1,
                                               int64_t total, int64_t parts) {
     Kv4Share r;
-    const int n = kv4_granules(s);
+    const int n = s.n;
     const int64_t start = u - off + kKv4Fixed;  // the first granule's unit
     const int64_t to = u1 < start + n ? u1 : start + n;
     r.from = off > kKv4Fixed ? off - kKv4Fixed : 0;
