@@ -63,7 +63,7 @@ __host__ __device__ inline int kv4_seq(int s0, int s1, int len, int T, int max_q
 // that ends within an item's fixed units leaves the whole item to the next. Runs
 // are at least kKv4MinRun long, more than an item's fixed units, so each has some
 // granule's unit.
-constexpr int kKv4Fixed = 12, kKv4MinRun = 16;
+constexpr int kKv4Fixed = 24, kKv4MinRun = 28;
 __host__ __device__ inline int kv4_items(const Kv4Seq &s, int group, int rows, int nkv) {
     return s.nq && s.n > 0 ? nkv * ((s.nq * group + rows - 1) / rows) : 0;
 }
@@ -86,25 +86,18 @@ __host__ __device__ inline int kv4_run_of(int64_t x, int64_t total, int64_t part
 struct Kv4Share {
     int from, take;   // granules [from, from + take) of the item's
     bool begins, ends;
-    int first, last;  // the runs that have a share of the item
+    int64_t start;    // the unit of the item's first granule
 };
-// A walk over a run's items: `off` units of item `sub` of sequence `s` lie before
+// A walk over a run's items: `off` units of an item of sequence `s` lie before
 // unit `u`. The share of the item in [u, u1), or take 0 where it has none.
-__host__ __device__ inline Kv4Share kv4_share(const Kv4Seq &s, int off, int64_t u, int64_t u1,
-                                              int64_t total, int64_t parts) {
+__host__ __device__ inline Kv4Share kv4_share(const Kv4Seq &s, int off, int64_t u, int64_t u1) {
     Kv4Share r;
-    const int n = s.n;
-    const int64_t start = u - off + kKv4Fixed;  // the first granule's unit
-    const int64_t to = u1 < start + n ? u1 : start + n;
+    r.start = u - off + kKv4Fixed;
+    const int64_t to = u1 < r.start + s.n ? u1 : r.start + s.n;
     r.from = off > kKv4Fixed ? off - kKv4Fixed : 0;
-    r.take = to > start + r.from ? (int)(to - start) - r.from : 0;
+    r.take = to > r.start + r.from ? (int)(to - r.start) - r.from : 0;
     r.begins = r.from == 0;
-    r.ends = r.from + r.take == n;
-    r.first = r.last = 0;
-    if (!(r.begins && r.ends)) {
-        r.first = kv4_run_of(start, total, parts);
-        r.last = kv4_run_of(start + n - 1, total, parts);
-    }
+    r.ends = r.from + r.take == s.n;
     return r;
 }
 

@@ -57,11 +57,11 @@ struct DecodeCfg {
     static constexpr int kStride = kCh + 4;          // merge rows: spreads a quarter warp over the banks
     static constexpr int NT = SPLIT ? 2 : 1;         // terms of a query
     static constexpr size_t kRing = (size_t)S * kv4_bytes(NG);
-    // a step's outputs, a row each of every warp; at the run's end also (factor,
-    // sum) pairs of an item's pieces, one a run
+    // a step's outputs, a row each of every warp; at the run's end also what the
+    // threads make of an item's pieces, 6 values each
     static constexpr size_t kOut = sizeof(float) * (size_t)W * kRows * kStride;
-    static constexpr size_t kPairs = sizeof(float2) * (size_t)kRows * kDecodeMaxGrid;
-    static constexpr size_t kMerge = kOut > kPairs ? kOut : kPairs;
+    static constexpr size_t kPieces = sizeof(float) * 6 * kThreads;
+    static constexpr size_t kMerge = kOut > kPieces ? kOut : kPieces;
     static constexpr size_t kQuery = 16 * (size_t)RB * NG * (32 * NT + 4);  // operands, bias
     static constexpr size_t kSmem = kRing + kMerge + K * kQuery;
 };
@@ -72,7 +72,8 @@ struct DecodeStep {
     int p0;                    // position of the first
     int rho0, rows, kvh;       // row tile, KV head
     int row0, at0;             // sequence's first query row, and its position
-    int whole, slot, first, last;  // merge of its output
+    int whole, slot, n;        // of its output: the item's granules,
+    int64_t start;             // and the unit of the first
     int owner;                 // the warp that takes all of a short whole item; -1: in turn
     int more;
 };
@@ -81,7 +82,7 @@ constexpr int kShort = 4;  // granules of a short item
 // The walk over a run's steps, the same in every warp that makes it.
 struct DecodeWalk {
     Kv4Seq s;
-    int64_t u, u1, total, parts;
+    int64_t u, u1;
     int seq, sub, off, item, base, shorts;
     bool more;
 };
@@ -123,7 +124,7 @@ __device__ __forceinline__ Kv4Seq load_seq(const Kv4AttnArgs &a, int i, int *bad
 __device__ __forceinline__ bool next_step(const Kv4AttnArgs &a, int G, int rows, int warps, DecodeWalk &w, DecodeStep &d,
                                           Kv4Seq &now, int &seq) {
     while (w.more) {
-        const Kv4Share sh = kv4_share(w.s, w.off, w.u, w.u1, w.total, w.parts);
+        const Kv4Share sh = kv4_share(w.s, w.off, w.u, w.u1);
         now = w.s;
         seq = w.seq;
         const int sub = w.sub;
@@ -148,8 +149,8 @@ __device__ __forceinline__ bool next_step(const Kv4AttnArgs &a, int G, int rows,
         d.at0 = now.len - now.nq;
         d.whole = sh.begins && sh.ends;
         d.slot = 2 * blockIdx.x + (sh.begins ? 1 : 0);
-        d.first = sh.first;
-        d.last = sh.last;
+        d.n = now.n;
+        d.start = sh.start;
         d.owner = d.whole && sh.take <= kShort ? w.shorts++ % warps : -1;
         d.more = w.more;
         w.base += d.granules;
@@ -182,20 +183,40 @@ __device__ __forceinline__ void store4(const Kv4AttnArgs &a, int64_t at, const f
     }
 }
 
-// 8 channels of a query row as fp32.
-__device__ __forceinline__ void load_q8(const Kv4AttnArgs &a, int64_t at, float (&v)[8]) {
-    if (a.dtype == RABBIT_CUDA_F32) {
-        const float *p = static_cast<const float *>(a.q) + at;
-        if (a.vec) load8<true>(v, p);
-        else load8<false>(v, p);
-    } else if (a.dtype == RABBIT_CUDA_F16) {
-        const __half *p = static_cast<const __half *>(a.q) + at;
-        if (a.vec) load8<true>(v, p);
-        else load8<false>(v, p);
+// 8 channels of a query row as they lie (NV vectors of 16 bytes), and as fp32:
+// apart, so that the loads of several pieces are under way at once.
+template <int NV>
+__device__ __forceinline__ void load_q8(const Kv4AttnArgs &a, int64_t at, uint4 (&w)[NV]) {
+    if (a.vec) {
+        const uint4 *p = reinterpret_cast<const uint4 *>(static_cast<const char *>(a.q) + at * (2 * NV));
+#pragma unroll
+        for (int i = 0; i < NV; ++i) w[i] = p[i];
+    } else if constexpr (NV == 2) {
+        const uint32_t *p = static_cast<const uint32_t *>(a.q) + at;
+        w[0] = make_uint4(p[0], p[1], p[2], p[3]);
+        w[1] = make_uint4(p[4], p[5], p[6], p[7]);
     } else {
-        const __nv_bfloat16 *p = static_cast<const __nv_bfloat16 *>(a.q) + at;
-        if (a.vec) load8<true>(v, p);
-        else load8<false>(v, p);
+        const uint16_t *p = static_cast<const uint16_t *>(a.q) + at;
+        w[0] = make_uint4(p[0] | (uint32_t)p[1] << 16, p[2] | (uint32_t)p[3] << 16,
+                          p[4] | (uint32_t)p[5] << 16, p[6] | (uint32_t)p[7] << 16);
+    }
+}
+template <int NV>
+__device__ __forceinline__ void q8_f32(const uint4 (&w)[NV], bool bf16, float (&v)[8]) {
+    const uint32_t *x = &w[0].x;
+    if constexpr (NV == 2) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            v[i] = __uint_as_float((&w[0].x)[i]);
+            v[4 + i] = __uint_as_float((&w[1].x)[i]);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float2 h = __half22float2(*reinterpret_cast<const __half2 *>(x + i));
+            v[2 * i] = bf16 ? __uint_as_float(x[i] << 16) : h.x;
+            v[2 * i + 1] = bf16 ? __uint_as_float(x[i] & 0xffff0000u) : h.y;
+        }
     }
 }
 
@@ -215,23 +236,26 @@ __global__ void __launch_bounds__(DecodeCfg<NG, RB, SPLIT>::kThreads, 1)
     __shared__ int64_t warp_sums[C::kThreads / 32];
     __shared__ int64_t found_before;
     __shared__ int found_seq;
+    __shared__ Kv4Seq found;
     __shared__ float wm[W][C::kRows], wl[W][C::kRows];
     __shared__ float suml[C::kRows];
     launch_dependents();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    if (tid == 0) {
-        for (int i = 0; i < S; ++i) {
-            tag[i] = -2;  // no round
-            mbar_init(&full[i], 1);
-            mbar_init(&empty[i], 1);
+    if (tid < S) {
+        tag[tid] = -2;  // no round
+        mbar_init(&full[tid], 1);
+        mbar_init(&empty[tid], 1);
+        if (tid < K) {
+            mbar_init(&asked[tid], 1);
+            mbar_init(&done[tid], W);
         }
-        for (int i = 0; i < K; ++i) {
-            mbar_init(&asked[i], 1);
-            mbar_init(&done[i], W);
+        if (tid == 0) {
+            mbar_init(&left, W);
+            mbar_init(&merged, 1);
         }
-        mbar_init(&left, W);
-        mbar_init(&merged, 1);
         mbar_init_fence();
+    }
+    if (tid == 0) {
         pending = 0;
     }
     wait_prerequisite();
@@ -240,9 +264,10 @@ __global__ void __launch_bounds__(DecodeCfg<NG, RB, SPLIT>::kThreads, 1)
 
     // ---- this CTA's run of units
     int64_t mine = 0, total;
+    Kv4Seq s = {};
     for (int i = tid; i < a.n_seqs; i += C::kThreads) {
         int bad;
-        const Kv4Seq s = load_seq(a, i, &bad);
+        s = load_seq(a, i, &bad);
         if (bad && blockIdx.x == 0) atomicOr(c.err, bad);
         mine += kv4_cost(s, G, C::kRows, c.nkv);
     }
@@ -263,6 +288,7 @@ __global__ void __launch_bounds__(DecodeCfg<NG, RB, SPLIT>::kThreads, 1)
     const int64_t u0 = kv4_cut(blockIdx.x, total, parts);
     if (a.n_seqs <= C::kThreads) {
         if (mine > 0 && excl <= u0 && u0 < excl + mine) {
+            found = s;
             found_seq = tid;
             found_before = excl;
         }
@@ -270,10 +296,14 @@ __global__ void __launch_bounds__(DecodeCfg<NG, RB, SPLIT>::kThreads, 1)
         int64_t base = 0;
         for (int i0 = 0; i0 < a.n_seqs && base <= u0; i0 += C::kThreads) {
             const int i = i0 + tid;
-            const int64_t cost = i < a.n_seqs ? kv4_cost(load_seq(a, i), G, C::kRows, c.nkv) : 0;
-            int64_t all;
+            int64_t all, cost = 0;
+            if (i < a.n_seqs) {
+                s = load_seq(a, i);
+                cost = kv4_cost(s, G, C::kRows, c.nkv);
+            }
             const int64_t before = base + block_scan<C::kThreads>(cost, warp_sums, all);
             if (cost > 0 && before <= u0 && u0 < before + cost) {
+                found = s;
                 found_seq = i;
                 found_before = before;
             }
@@ -283,15 +313,13 @@ __global__ void __launch_bounds__(DecodeCfg<NG, RB, SPLIT>::kThreads, 1)
     __syncthreads();
     auto start_walk = [&](DecodeWalk &w) {
         w.seq = found_seq;
-        w.s = load_seq(a, w.seq);
+        w.s = found;
         w.u = u0;
         w.u1 = kv4_cut(blockIdx.x + 1, total, parts);
-        w.total = total;
-        w.parts = parts;
         w.item = w.s.n + kKv4Fixed;
         const int64_t r = u0 - found_before;
-        w.sub = (int)(r / w.item);
-        w.off = (int)(r % w.item);
+        w.sub = r >> 31 ? (int)(r / w.item) : (int)r / w.item;
+        w.off = (int)(r - (int64_t)w.sub * w.item);
         w.base = 0;
         w.shorts = 0;
         w.more = true;
@@ -369,7 +397,8 @@ __global__ void __launch_bounds__(DecodeCfg<NG, RB, SPLIT>::kThreads, 1)
         DecodeStep d;
         Kv4Seq now;
         int seq;
-        float x8[RB][NG][8];  // the next step's query rows, loaded ahead
+        uint4 x8[RB][NG][NT];  // the next step's query rows, loaded ahead
+        const bool bf16 = a.dtype == RABBIT_CUDA_BF16;
         auto load_rows = [&]() {
 #pragma unroll
             for (int rb = 0; rb < RB; ++rb) {
@@ -379,7 +408,7 @@ __global__ void __launch_bounds__(DecodeCfg<NG, RB, SPLIT>::kThreads, 1)
 #pragma unroll
                 for (int grp = 0; grp < NG; ++grp) {
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) x8[rb][grp][i] = 0.f;
+                    for (int i = 0; i < NT; ++i) x8[rb][grp][i] = make_uint4(0, 0, 0, 0);
                     if (in && 32 * grp + 8 * t < c.hd) load_q8(a, base + 32 * grp + 8 * t, x8[rb][grp]);
                 }
             }
@@ -403,9 +432,12 @@ __global__ void __launch_bounds__(DecodeCfg<NG, RB, SPLIT>::kThreads, 1)
                 for (int rb = 0; rb < RB; ++rb) {
                     float top = 0.f;
 #pragma unroll
-                    for (int grp = 0; grp < NG; ++grp)
+                    for (int grp = 0; grp < NG; ++grp) {
+                        float v[8];
+                        q8_f32(x8[rb][grp], bf16, v);
 #pragma unroll
-                        for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(x8[rb][grp][i]));
+                        for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(v[i]));
+                    }
                     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
                     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
                     // 2^(14 - e), 2^e <= top: the largest goes to [2^14, 2^15)
@@ -416,12 +448,13 @@ __global__ void __launch_bounds__(DecodeCfg<NG, RB, SPLIT>::kThreads, 1)
                     if (t == 0) unit[buf][8 * rb + g] = fabsf(a.scale) * down * (SPLIT ? 1.0f : 16777216.0f);
 #pragma unroll
                     for (int grp = 0; grp < NG; ++grp) {
-                        float sum = 0.f;
+                        float sum = 0.f, y[8];
+                        q8_f32(x8[rb][grp], bf16, y);
                         uint32_t f[NT][4];
 #pragma unroll
                         for (int i = 0; i < 2; ++i) {  // the instruction's two steps
                             const float by = !SPLIT && i ? 0.0625f : 1.0f, back = !SPLIT && i ? 16.f : 1.0f;
-                            float v[4] = {x8[rb][grp][i], x8[rb][grp][i + 4], x8[rb][grp][i + 2], x8[rb][grp][i + 6]};
+                            float v[4] = {y[i], y[i + 4], y[i + 2], y[i + 6]};
 #pragma unroll
                             for (int x = 0; x < 4; ++x) v[x] *= sup * by;
 #pragma unroll
@@ -518,12 +551,15 @@ __global__ void __launch_bounds__(DecodeCfg<NG, RB, SPLIT>::kThreads, 1)
                         __threadfence();
                         __syncwarp();
                         if (lane == 0) {
-                            const unsigned before = atomicAdd(a.count + m.first, 1u);
-                            if (before == (unsigned)(m.last - m.first)) {
-                                a.count[m.first] = 0u;  // ready for the next call
+                            // the runs that have a share of the item
+                            const int first = kv4_run_of(m.start, total, parts);
+                            const int last = kv4_run_of(m.start + m.n - 1, total, parts);
+                            const unsigned before = atomicAdd(a.count + first, 1u);
+                            if (before == (unsigned)(last - first)) {
+                                a.count[first] = 0u;  // ready for the next call
                                 int *p = pend[pending++];
-                                p[0] = m.first;
-                                p[1] = m.last;
+                                p[0] = first;
+                                p[1] = last;
                                 p[2] = m.rows;
                                 p[3] = m.row0;
                                 p[4] = m.kvh;
@@ -871,62 +907,66 @@ __global__ void __launch_bounds__(DecodeCfg<NG, RB, SPLIT>::kThreads, 1)
         }
     }
 
-    // ---- items whose last piece came from this run: merged by the whole CTA. The
-    // pieces' factors into shared memory (all else in it is done with), then
-    // their outputs, eight loads in flight a thread.
+    // ---- items whose last piece came from this run: merged by the whole CTA, in
+    // the pieces' order. A thread takes 4 channels of a row and every `ways`-th
+    // run of pieces, then the ways are merged (in shared memory: all else in it
+    // is done with).
     __syncthreads();
     for (int x = 0; x < pending; ++x) {
         __threadfence();
-        const int first = pend[x][0], np = pend[x][1] - first + 1, R = pend[x][2];
-        auto piece = [&](int b, int r) { return (size_t)(2 * (first + b) + (b == 0)) * C::kRows + r; };
-        float2 *pf = reinterpret_cast<float2 *>(mo);  // [rows][np]
-        for (int i = tid; i < R * np; i += C::kThreads) {
-            const int r = i / np;
-            pf[i] = __ldcg(reinterpret_cast<const float2 *>(stats) + piece(i - r * np, r));
-        }
-        __syncthreads();
-        for (int r = warp; r < R; r += C::kThreads / 32) {
-            float mx = kNoRef, L = 0.f;
-            for (int b = lane; b < np; b += 32) mx = fmaxf(mx, pf[r * np + b].x);
-#pragma unroll
-            for (int s = 16; s; s >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, s));
-            for (int b = lane; b < np; b += 32) {
-                const float f = exp2_fast(pf[r * np + b].x - mx);
-                L = fmaf(pf[r * np + b].y, f, L);
-                pf[r * np + b].x = f;
-            }
-#pragma unroll
-            for (int s = 16; s; s >>= 1) L += __shfl_xor_sync(0xffffffffu, L, s);
-            if (lane == 0) suml[r] = L;
-        }
-        __syncthreads();
-        for (int i = tid; i < R * (C::kCh / 4); i += C::kThreads) {
+        const int first = pend[x][0], np = pend[x][1] - first + 1, R = pend[x][2], n4 = R * (C::kCh / 4);
+        const int ways = max(1, min(8, C::kThreads / n4)), each = (np + ways - 1) / ways;
+        float *part = mo;  // [ways][6][n4]
+        auto fold = [](float &mx, float &L, float (&v)[4], float m, float l, const float4 &y) {
+            const float up = fmaxf(mx, m), f = exp2_fast(mx - up), h = exp2_fast(m - up);
+            mx = up;
+            L = fmaf(L, f, l * h);
+            v[0] = fmaf(v[0], f, y.x * h);
+            v[1] = fmaf(v[1], f, y.y * h);
+            v[2] = fmaf(v[2], f, y.z * h);
+            v[3] = fmaf(v[3], f, y.w * h);
+        };
+        for (int i0 = 0; i0 < n4; i0 += C::kThreads) {
+            const int way = ways > 1 ? tid / n4 : 0, i = ways > 1 ? tid - way * n4 : i0 + tid;
             const int r = i / (C::kCh / 4), ch = 4 * (i % (C::kCh / 4));
-            float v[4] = {0.f, 0.f, 0.f, 0.f};
-            for (int b0 = 0; b0 < np; b0 += 8) {
-                float4 p[8];
+            float mx = kNoRef, L = 0.f, v[4] = {0.f, 0.f, 0.f, 0.f};
+            if (way < ways && i < n4) {
+                const int end = min(np, (way + 1) * each);
+                for (int b0 = way * each; b0 < end; b0 += 8) {
+                    float4 y[8];
+                    float2 ml[8];
 #pragma unroll
-                for (int b = 0; b < 8; ++b)
-                    if (b0 + b < np)
-                        p[b] = __ldcg(reinterpret_cast<const float4 *>(a.part + piece(b0 + b, r) * C::kCh + ch));
+                    for (int b = 0; b < 8; ++b)
+                        if (b0 + b < end) {
+                            const size_t s = (size_t)(2 * (first + b0 + b) + (b0 + b == 0)) * C::kRows + r;
+                            ml[b] = __ldcg(reinterpret_cast<const float2 *>(stats) + s);
+                            y[b] = __ldcg(reinterpret_cast<const float4 *>(a.part + s * C::kCh + ch));
+                        }
 #pragma unroll
-                for (int b = 0; b < 8; ++b)
-                    if (b0 + b < np) {
-                        const float f = pf[r * np + b0 + b].x;
-                        v[0] = fmaf(p[b].x, f, v[0]);
-                        v[1] = fmaf(p[b].y, f, v[1]);
-                        v[2] = fmaf(p[b].z, f, v[2]);
-                        v[3] = fmaf(p[b].w, f, v[3]);
-                    }
+                    for (int b = 0; b < 8; ++b)
+                        if (b0 + b < end) fold(mx, L, v, ml[b].x, ml[b].y, y[b]);
+                }
+                if (way > 0) {
+                    float *p = part + (size_t)way * 6 * n4 + i;
+                    p[0] = mx;
+                    p[n4] = L;
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) p[(2 + k) * n4] = v[k];
+                }
             }
-            if (ch < c.hd) {
-                const float inv = suml[r] != 0.f ? 1.0f / suml[r] : 0.f;
+            __syncthreads();
+            if (way == 0 && i < n4 && ch < c.hd) {
+                for (int k = 1; k < ways; ++k) {
+                    const float *p = part + (size_t)k * 6 * n4 + i;
+                    fold(mx, L, v, p[0], p[n4], make_float4(p[2 * n4], p[3 * n4], p[4 * n4], p[5 * n4]));
+                }
+                const float inv = L != 0.f ? 1.0f / L : 0.f;
 #pragma unroll
                 for (int k = 0; k < 4; ++k) v[k] *= inv;
                 store4(a, row_at(pend[x][3], pend[x][4], pend[x][5] + r) + ch, v, min(4, c.hd - ch));
             }
+            __syncthreads();
         }
-        __syncthreads();
     }
 }
 
