@@ -51,7 +51,7 @@ struct DecodeCfg {
     // ring slots, SL for each lane of the fetching warp: a warp holds two while it
     // works, the others are on their way
     static constexpr int SL = W == 14 ? 2 : 1, S = 32 * SL;
-    static constexpr int K = NG <= 4 ? 4 : 2;        // steps whose operands are held
+    static constexpr int K = NG > 4 ? 2 : RB == 1 && !SPLIT ? 6 : 4;  // steps whose operands are held
     static constexpr int kRows = 8 * RB;
     static constexpr int kCh = 32 * NG;
     static constexpr int kStride = kCh + 4;          // merge rows: spreads a quarter warp over the banks
@@ -77,7 +77,7 @@ struct DecodeStep {
     int owner;                 // the warp that takes all of a short whole item; -1: in turn
     int more;
 };
-constexpr int kShort = 4;  // granules of a short item
+constexpr int kShort = 6;  // granules of a short item
 
 // The walk over a run's steps, the same in every warp that makes it.
 struct DecodeWalk {
@@ -216,6 +216,95 @@ __device__ __forceinline__ void q8_f32(const uint4 (&w)[NV], bool bf16, float (&
             const float2 h = __half22float2(*reinterpret_cast<const __half2 *>(x + i));
             v[2 * i] = bf16 ? __uint_as_float(x[i] << 16) : h.x;
             v[2 * i + 1] = bf16 ? __uint_as_float(x[i] & 0xffff0000u) : h.y;
+        }
+    }
+}
+
+// A warp loads a step's query rows: lane (g, t) the channels of words t of row g.
+template <int NG, int RB, bool SPLIT>
+__device__ __forceinline__ void load_rows(const Kv4AttnArgs &a, const DecodeStep &d, int G,
+                                          uint4 (&x8)[RB][NG][SPLIT ? 2 : 1]) {
+    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+#pragma unroll
+    for (int rb = 0; rb < RB; ++rb) {
+        const int rho = d.rho0 + 8 * rb + g, qi = rho / G;
+        const bool in = 8 * rb + g < d.rows;
+        const int64_t base = (int64_t)(d.row0 + qi) * a.qs + (int64_t)(d.kvh * G + rho - qi * G) * a.c.hd;
+#pragma unroll
+        for (int grp = 0; grp < NG; ++grp) {
+#pragma unroll
+            for (int i = 0; i < (SPLIT ? 2 : 1); ++i) x8[rb][grp][i] = make_uint4(0, 0, 0, 0);
+            if (in && 32 * grp + 8 * t < a.c.hd) load_q8(a, base + 32 * grp + 8 * t, x8[rb][grp]);
+        }
+    }
+}
+
+// and makes them the step's operands, for lane (g, t): row g's channels (nibbles
+// 0, 4 | 2, 6 | 1, 5 | 3, 7 of word t of a group); for rows 2 t, 2 t + 1 the bias
+// their columns start from; a row's unit: one of its scores as a power of two.
+template <int NG, int RB, bool SPLIT>
+__device__ __forceinline__ void make_operands(const Kv4AttnArgs &a, uint8_t *query, float *unit,
+                                              const uint4 (&x8)[RB][NG][SPLIT ? 2 : 1]) {
+    constexpr int NT = SPLIT ? 2 : 1;
+    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const bool bf16 = a.dtype == RABBIT_CUDA_BF16;
+    uint4 *q = reinterpret_cast<uint4 *>(query);
+    float4 *c0 = reinterpret_cast<float4 *>(q + RB * NT * NG * 32);
+#pragma unroll
+    for (int rb = 0; rb < RB; ++rb) {
+        float top = 0.f;
+#pragma unroll
+        for (int grp = 0; grp < NG; ++grp) {
+            float v[8];
+            q8_f32(x8[rb][grp], bf16, v);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(v[i]));
+        }
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        // 2^(14 - e), 2^e <= top: the largest goes to [2^14, 2^15)
+        const int e = max((int)(__float_as_uint(top) >> 23) - 127, -100);
+        const float up = __uint_as_float((uint32_t)(127 + 14 - e) << 23);
+        const float down = __uint_as_float((uint32_t)(127 - 14 + e) << 23);
+        const float sup = a.scale < 0.f ? -up : up;
+        if (t == 0) unit[8 * rb + g] = fabsf(a.scale) * down * (SPLIT ? 1.0f : 16777216.0f);
+#pragma unroll
+        for (int grp = 0; grp < NG; ++grp) {
+            float sum = 0.f, y[8];
+            q8_f32(x8[rb][grp], bf16, y);
+            uint32_t f[NT][4];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {  // the instruction's two steps
+                const float by = !SPLIT && i ? 0.0625f : 1.0f, back = !SPLIT && i ? 16.f : 1.0f;
+                float v[4] = {y[i], y[i + 4], y[i + 2], y[i + 6]};
+#pragma unroll
+                for (int x = 0; x < 4; ++x) v[x] *= sup * by;
+#pragma unroll
+                for (int term = 0; term < NT; ++term) {
+                    const uint32_t x0 = pack_f16(v[0], v[1]), x1 = pack_f16(v[2], v[3]);
+                    f[term][2 * i] = x0;
+                    f[term][2 * i + 1] = x1;
+                    const float2 r0 = __half22float2(*reinterpret_cast<const __half2 *>(&x0));
+                    const float2 r1 = __half22float2(*reinterpret_cast<const __half2 *>(&x1));
+                    sum += ((r0.x + r0.y) + (r1.x + r1.y)) * back;
+                    v[0] -= r0.x;  // what this term leaves to the next
+                    v[1] -= r0.y;
+                    v[2] -= r1.x;
+                    v[3] -= r1.y;
+                }
+            }
+#pragma unroll
+            for (int term = 0; term < NT; ++term)
+                q[((rb * NT + term) * NG + grp) * 32 + lane] =
+                    make_uint4(f[term][0], f[term][1], f[term][2], f[term][3]);
+            if constexpr (!SPLIT) {
+                sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+                sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+                sum *= -8.0f / 16777216.0f;
+                const float s0 = __shfl_sync(0xffffffffu, sum, 8 * t);
+                const float s1 = __shfl_sync(0xffffffffu, sum, 8 * t + 4);
+                if (g == 0) c0[(rb * NG + grp) * 4 + t] = make_float4(s0, s1, s0, s1);
+            }
         }
     }
 }
@@ -392,30 +481,14 @@ __global__ void __launch_bounds__(DecodeCfg<NG, RB, SPLIT>::kThreads, 1)
             mbar_wait(&full[lane + 32 * (i % C::SL)], (i / C::SL) & 1, a.wait_ns, nullptr, 0);
     } else if (warp == W + 1) {
         // ---- operands of the coming steps, as far ahead as there is room, and merges
-        const int g = lane >> 2, t = lane & 3;
         DecodeWalk w;
         DecodeStep d;
         Kv4Seq now;
         int seq;
         uint4 x8[RB][NG][NT];  // the next step's query rows, loaded ahead
-        const bool bf16 = a.dtype == RABBIT_CUDA_BF16;
-        auto load_rows = [&]() {
-#pragma unroll
-            for (int rb = 0; rb < RB; ++rb) {
-                const int rho = d.rho0 + 8 * rb + g, qi = rho / G;
-                const bool in = 8 * rb + g < d.rows;
-                const int64_t base = (int64_t)(d.row0 + qi) * a.qs + (int64_t)(d.kvh * G + rho - qi * G) * c.hd;
-#pragma unroll
-                for (int grp = 0; grp < NG; ++grp) {
-#pragma unroll
-                    for (int i = 0; i < NT; ++i) x8[rb][grp][i] = make_uint4(0, 0, 0, 0);
-                    if (in && 32 * grp + 8 * t < c.hd) load_q8(a, base + 32 * grp + 8 * t, x8[rb][grp]);
-                }
-            }
-        };
         start_walk(w);
         bool has = next_step(a, G, C::kRows, W, w, d, now, seq);
-        if (has) load_rows();
+        if (has && d.owner < 0) load_rows<NG, RB, SPLIT>(a, d, G, x8);
         int asked_n = 0, seen_n = 0, merged_n = 0;  // steps made; steps looked at for a merge; merges
         for (uint64_t t0 = 0; has || seen_n < asked_n;) {
             bool did = false;
@@ -424,73 +497,14 @@ __global__ void __launch_bounds__(DecodeCfg<NG, RB, SPLIT>::kThreads, 1)
             if (has && asked_n - seen_n < K &&
                 (asked_n < K || mbar_test(&done[buf], (asked_n / K - 1) & 1))) {
                 did = true;
-                // For lane (g, t): row g's channels (nibbles 0, 4 | 2, 6 | 1, 5 | 3, 7 of word t
-                // of the group); for rows 2 t, 2 t + 1 the bias their columns start from.
-                uint4 *q = reinterpret_cast<uint4 *>(queries + buf * C::kQuery);
-                float4 *c0 = reinterpret_cast<float4 *>(q + RB * NT * NG * 32);
-#pragma unroll
-                for (int rb = 0; rb < RB; ++rb) {
-                    float top = 0.f;
-#pragma unroll
-                    for (int grp = 0; grp < NG; ++grp) {
-                        float v[8];
-                        q8_f32(x8[rb][grp], bf16, v);
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(v[i]));
-                    }
-                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-                    // 2^(14 - e), 2^e <= top: the largest goes to [2^14, 2^15)
-                    const int e = max((int)(__float_as_uint(top) >> 23) - 127, -100);
-                    const float up = __uint_as_float((uint32_t)(127 + 14 - e) << 23);
-                    const float down = __uint_as_float((uint32_t)(127 - 14 + e) << 23);
-                    const float sup = a.scale < 0.f ? -up : up;
-                    if (t == 0) unit[buf][8 * rb + g] = fabsf(a.scale) * down * (SPLIT ? 1.0f : 16777216.0f);
-#pragma unroll
-                    for (int grp = 0; grp < NG; ++grp) {
-                        float sum = 0.f, y[8];
-                        q8_f32(x8[rb][grp], bf16, y);
-                        uint32_t f[NT][4];
-#pragma unroll
-                        for (int i = 0; i < 2; ++i) {  // the instruction's two steps
-                            const float by = !SPLIT && i ? 0.0625f : 1.0f, back = !SPLIT && i ? 16.f : 1.0f;
-                            float v[4] = {y[i], y[i + 4], y[i + 2], y[i + 6]};
-#pragma unroll
-                            for (int x = 0; x < 4; ++x) v[x] *= sup * by;
-#pragma unroll
-                            for (int term = 0; term < NT; ++term) {
-                                const uint32_t x0 = pack_f16(v[0], v[1]), x1 = pack_f16(v[2], v[3]);
-                                f[term][2 * i] = x0;
-                                f[term][2 * i + 1] = x1;
-                                const float2 r0 = __half22float2(*reinterpret_cast<const __half2 *>(&x0));
-                                const float2 r1 = __half22float2(*reinterpret_cast<const __half2 *>(&x1));
-                                sum += ((r0.x + r0.y) + (r1.x + r1.y)) * back;
-                                v[0] -= r0.x;  // what this term leaves to the next
-                                v[1] -= r0.y;
-                                v[2] -= r1.x;
-                                v[3] -= r1.y;
-                            }
-                        }
-#pragma unroll
-                        for (int term = 0; term < NT; ++term)
-                            q[((rb * NT + term) * NG + grp) * 32 + lane] =
-                                make_uint4(f[term][0], f[term][1], f[term][2], f[term][3]);
-                        if constexpr (!SPLIT) {
-                            sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-                            sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-                            sum *= -8.0f / 16777216.0f;
-                            const float s0 = __shfl_sync(0xffffffffu, sum, 8 * t);
-                            const float s1 = __shfl_sync(0xffffffffu, sum, 8 * t + 4);
-                            if (g == 0) c0[(rb * NG + grp) * 4 + t] = make_float4(s0, s1, s0, s1);
-                        }
-                    }
-                }
+                if (d.owner < 0)
+                    make_operands<NG, RB, SPLIT>(a, queries + buf * C::kQuery, unit[buf], x8);
                 if (lane == 0) steps[buf] = d;
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&asked[buf]);
                 ++asked_n;
                 has = next_step(a, G, C::kRows, W, w, d, now, seq);
-                if (has) load_rows();
+                if (has && d.owner < 0) load_rows<NG, RB, SPLIT>(a, d, G, x8);
             }
             if (seen_n < asked_n) {
                 const DecodeStep &st = steps[seen_n % K];
@@ -608,6 +622,12 @@ __global__ void __launch_bounds__(DecodeCfg<NG, RB, SPLIT>::kThreads, 1)
                 continue;
             }
             const int R = st.rows, rho0 = st.rho0, kvh = st.kvh, p00 = st.p0 - kKv4Granule * st.base;
+            if (owner >= 0) {  // a short item's warp makes its operands itself
+                uint4 x8[RB][NG][NT];
+                load_rows<NG, RB, SPLIT>(a, st, G, x8);
+                make_operands<NG, RB, SPLIT>(a, queries + buf * C::kQuery, unit[buf], x8);
+                __syncwarp();
+            }
             const int at_lo = st.at0 + rho0 / G, at_hi = st.at0 + (rho0 + R - 1) / G;
             const uint4 *q = reinterpret_cast<const uint4 *>(queries + buf * C::kQuery);
             const float4 *c0 = reinterpret_cast<const float4 *>(q + RB * NT * NG * 32);
