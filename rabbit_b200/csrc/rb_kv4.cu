@@ -26,22 +26,48 @@ struct Kv4AppendRopeArgs {
     RopeTab tab;
 };
 
-// rint(x / s) of the real quotient, halves to even. The fp32 product with the
-// reciprocal is within 2^-20 of the quotient (|x / s| < 8), so only a quotient
-// within 2^-12 of a half needs the division in 64 bits. Scales near the
-// smallest fp32 have no finite reciprocal and always take it.
-__device__ __forceinline__ int kv4_code(double x, float s, float inv) {
-    const float t = (float)x * inv;
-    float q = rintf(t);
-    if (fabsf(fabsf(t - q) - 0.5f) < 2.44140625e-4f || s < 1e-30f) q = (float)rint(x / (double)s);
-    return (int)q;
+// Channel `ch` of a head's row in 64 bits; its first `rot` channels rotated by
+// the token's table.
+template <typename T>
+__device__ __forceinline__ double exact_channel(const T *row, int ch, const double2 *table, int rot, bool halves) {
+    if (ch >= rot) return to_f32(row[ch]);
+    const int np = rot / 2;
+    const bool first = halves ? ch < np : !(ch & 1);
+    const int other = halves ? (first ? ch + np : ch - np) : ch ^ 1;
+    const double2 k = table[halves ? (first ? ch : other) : ch >> 1];
+    return (double)to_f32(row[ch]) * k.x + (double)to_f32(row[other]) * (first ? -k.y : k.y);
+}
+// Channels ch .. ch + 7 again where 32 bits leave a rounding open: the bits of the
+// largest magnitude in fp32, and the codes (4 bits each).
+template <typename T>
+__device__ __noinline__ uint32_t exact_top(const T *row, int ch, const double2 *table, int rot, bool halves) {
+    uint32_t top = 0;
+#pragma unroll 1
+    for (int n = 0; n < 8; ++n)
+        top = max(top, __float_as_uint(fabsf((float)exact_channel(row, ch + n, table, rot, halves))));
+    return top;
+}
+template <typename T>
+__device__ __noinline__ uint32_t exact_codes(const T *row, int ch, const double2 *table, int rot, bool halves, float s) {
+    uint32_t word = 0;
+#pragma unroll 1
+    for (int n = 0; n < 8; ++n)
+        word |= ((uint32_t)(int)rint(exact_channel(row, ch + n, table, rot, halves) / (double)s) & 15u) << (4 * n);
+    return word;
 }
 
-// A thread: 8 consecutive channels of one (token, head) of the keys
-// (blockIdx.z = 0) or the values; 4 threads a group.
+// One CTA: tpc tokens, a thread 8 consecutive channels of one (token, head) of
+// the keys (blockIdx.z = 0) or the values, 4 threads a group.
+//
+// The codes are those of the exact value, at the cost of 32-bit arithmetic: the
+// rotation, the scale and the quotients are made in fp32 with a bound on their
+// error, and only where the bound leaves the rounding open (the scale's to bf16, a
+// quotient's to a whole number: about one value in 10^4) once more in 64 bits, from
+// the 64-bit cosine and sine that the token's table holds too. All in 64 bits the
+// conversions alone took 40 us for 8191 x 8 x 80 fp16 with a rotation; so 18 us.
 template <typename T, bool VEC, bool ROPE>
-__global__ void __launch_bounds__(kAppendThreads) k_kv4_append(const __grid_constant__ Kv4AppendRopeArgs aa) {
-    extern __shared__ __align__(16) double2 cs[];  // [tpc][rot / 2], keys only
+__global__ void __launch_bounds__(kAppendThreads, 4) k_kv4_append(const __grid_constant__ Kv4AppendRopeArgs aa) {
+    extern __shared__ __align__(16) double2 cs[];  // [tpc][rot / 2], keys only; then the same in fp32
     const Kv4AppendArgs &a = aa.a;
     const RopeTab &tab = aa.tab;
     const Kv4View &c = a.c;
@@ -50,81 +76,139 @@ __global__ void __launch_bounds__(kAppendThreads) k_kv4_append(const __grid_cons
     const int kv = blockIdx.z, t0 = blockIdx.x * a.tpc, nt = min(a.tpc, a.T - t0);
     const bool rot = ROPE && kv == 0;
     const int np = ROPE ? tab.rot / 2 : 0;
+    float2 *cs32 = reinterpret_cast<float2 *>(cs + a.tpc * np);
+    float mag = 0.f;
     if constexpr (ROPE) {
+        mag = fabsf((float)tab.mag);
         if (rot) {
             for (int i = threadIdx.x; i < nt * np; i += kAppendThreads) {
                 double2 v = rope_cs(a.pos[t0 + i / np], tab.turns[i % np]);
                 v.x *= tab.mag;
                 v.y *= tab.mag;
                 cs[i] = v;
+                cs32[i] = make_float2((float)v.x, (float)v.y);
             }
             __syncthreads();
         }
     }
-    const int per = c.nkv * c.ng * 4, total = nt * per;
     const bool halves = ROPE && tab.layout == RABBIT_CUDA_ROPE_HALF;
-    for (int i0 = blockIdx.y * kAppendThreads; i0 < total; i0 += gridDim.y * kAppendThreads) {
-        const int i = i0 + threadIdx.x;
-        const bool in = i < total;
-        const int tl = in ? i / per : 0, u = in ? i - tl * per : 0;
-        const int head = u / (c.ng * 4), w = u - head * c.ng * 4, grp = w >> 2, t = w & 3;
-        const int c0 = 8 * w;  // first channel
+    // a thread keeps its item of the row and goes through the tokens; short rows:
+    // several tokens side by side
+    const int per = c.nkv * c.ng * 4;
+    const int side = per <= kAppendThreads / 2 ? kAppendThreads / per : 1;
+    const int first = side > 1 ? threadIdx.x / per : 0;
+    for (int u0 = side > 1 ? 0 : blockIdx.y * kAppendThreads; u0 < per; u0 += gridDim.y * kAppendThreads) {
+    const int u = u0 + threadIdx.x - first * per;
+    const bool mine = u < per && first < side;
+    const int head = u / (c.ng * 4), w = u - head * c.ng * 4, grp = w >> 2, t = w & 3;
+    const int c0 = 8 * w;  // first channel
+    for (int ta = 0; ta < nt; ta += side) {
+        const int tl = ta + first;
+        const bool in = mine && tl < nt;
         const int64_t slot = in ? a.slots[t0 + tl] : -1;
         const bool write = slot >= 0 && slot < c.slots();
-        if (in && slot >= c.slots() && c.err) atomicOr(c.err, RB_KV4_ERR_SLOT);
-        double x[8];
-        uint32_t top = 0;  // bits of max |x|: an integer maximum keeps a NaN
+        if (in && slot >= c.slots()) atomicOr(c.err, RB_KV4_ERR_SLOT);
+        const bool turn = ROPE && rot && c0 < tab.rot;
+        // v, p: each channel and the other of its pair before the rotation; x: after it
+        float x[8], v[8], p[8], big = 0.f;  // big: the largest |v| + |p|
 #pragma unroll
-        for (int n = 0; n < 8; ++n) x[n] = 0.0;
+        for (int n = 0; n < 8; ++n) x[n] = v[n] = p[n] = 0.f;
+        const T *row = static_cast<const T *>(a.x[kv]) + (t0 + tl) * a.xs[kv] + (int64_t)head * c.hd;
         if (write && c0 < c.hd) {
-            const T *row = static_cast<const T *>(a.x[kv]) + (t0 + tl) * a.xs[kv] + (int64_t)head * c.hd;
-            float v[8];
             load8<VEC>(v, row + c0);
 #pragma unroll
             for (int n = 0; n < 8; ++n) x[n] = v[n];
-            if (rot && c0 < tab.rot) {
-                // partners: the other channel of each pair
-                float p[8];
-                if (!halves) {
+            if constexpr (ROPE) {
+                if (turn) {
+                    float2 k[8];  // x = v k.x + p k.y
+                    const float2 *ct = cs32 + tl * np;
+                    if (!halves) {
 #pragma unroll
-                    for (int n = 0; n < 8; ++n) p[n] = v[n ^ 1];
-                } else if (np % 8 == 0) {
-                    load8<VEC>(p, row + (c0 < np ? c0 + np : c0 - np));
-                } else {
+                        for (int n = 0; n < 8; ++n) {
+                            p[n] = v[n ^ 1];
+                            if (!(n & 1)) k[n] = k[n + 1] = c0 + n < tab.rot ? ct[(c0 + n) / 2] : make_float2(1.f, 0.f);
+                            if (!(n & 1)) k[n].y = -k[n].y;
+                        }
+                    } else if (np % 8 == 0) {  // all 8 are first or second
+                        const bool first = c0 < np;
+                        load8<VEC>(p, row + (first ? c0 + np : c0 - np));
+                        const float4 *c4 = reinterpret_cast<const float4 *>(ct + (first ? c0 : c0 - np));
+#pragma unroll
+                        for (int n = 0; n < 8; n += 2) {
+                            const float4 y = c4[n / 2];
+                            k[n] = make_float2(y.x, first ? -y.y : y.y);
+                            k[n + 1] = make_float2(y.z, first ? -y.w : y.w);
+                        }
+                    } else {
+#pragma unroll
+                        for (int n = 0; n < 8; ++n) {
+                            const int ch = c0 + n;
+                            k[n] = make_float2(1.f, 0.f);
+                            if (ch < tab.rot) {
+                                p[n] = to_f32(row[ch < np ? ch + np : ch - np]);
+                                k[n] = ct[ch < np ? ch : ch - np];
+                                if (ch < np) k[n].y = -k[n].y;
+                            }
+                        }
+                    }
 #pragma unroll
                     for (int n = 0; n < 8; ++n) {
-                        const int ch = c0 + n;
-                        p[n] = ch < tab.rot ? to_f32(row[ch < np ? ch + np : ch - np]) : 0.f;
-                    }
-                }
-#pragma unroll
-                for (int n = 0; n < 8; ++n) {
-                    const int ch = c0 + n;
-                    if (ch < tab.rot) {
-                        const bool first = halves ? ch < np : !(ch & 1);
-                        const double2 k = cs[tl * np + (halves ? (first ? ch : ch - np) : ch >> 1)];
-                        x[n] = (double)v[n] * k.x + (double)p[n] * (first ? -k.y : k.y);
+                        x[n] = fmaf(v[n], k[n].x, p[n] * k[n].y);
+                        big = fmaxf(big, fabsf(v[n]) + fabsf(p[n]));
                     }
                 }
             }
-#pragma unroll
-            for (int n = 0; n < 8; ++n) top = max(top, __float_as_uint(fabsf((float)x[n])));
         }
+        auto scale_of = [](float top) {
+            const float top7 = __fmul_rn(top, 1.0f / 7.0f);
+            // a group with an infinity or a NaN has a NaN for its scale
+            return __float2bfloat16_rn(top7 < INFINITY ? top7 : __uint_as_float(0x7fc00000u));
+        };
+        // the group's largest: an integer maximum of the bits keeps a NaN
+        uint32_t top = 0;
+#pragma unroll
+        for (int n = 0; n < 8; ++n) top = max(top, __float_as_uint(fabsf(x[n])));
         top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        __nv_bfloat16 sb = scale_of(__uint_as_float(top));
+        float off = 0.f;  // how far the rotated values may be off
+        if constexpr (ROPE) {
+            big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
+            big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
+            // cosine and sine half a step off, a product and a sum rounded: at most
+            // 4 2^-24 (|v| + |p|) of the magnitude
+            off = big * mag * 2.4e-7f;
+            const float a0 = __uint_as_float(top) - off, a1 = __uint_as_float(top) + off;
+            const bool open = off > 0.f && !(__bfloat162float(scale_of(fmaxf(a0, 0.f))) == __bfloat162float(scale_of(a1)));
+            if (__any_sync(0xffffffffu, open)) {
+                uint32_t e = 0;
+                if (write && c0 < c.hd) e = exact_top(row, c0, cs + tl * np, turn ? tab.rot : 0, halves);
+                e = max(e, __shfl_xor_sync(0xffffffffu, e, 1));
+                e = max(e, __shfl_xor_sync(0xffffffffu, e, 2));
+                if (open) sb = scale_of(__uint_as_float(e));
+            }
+        }
         if (!write) continue;
-        // a group with an infinity or a NaN has a NaN for its scale
-        const float top7 = __fmul_rn(__uint_as_float(top), 1.0f / 7.0f);
-        const __nv_bfloat16 sb = __float2bfloat16_rn(top7 < INFINITY ? top7 : __uint_as_float(0x7fc00000u));
         const float s = __bfloat162float(sb), inv = 1.0f / s;
         uint32_t word = 0x88888888u;
         if (s > 0.f) {
+            // quotients off by off / s and 2^-22 |q|, |q| < 8; a scale near the smallest
+            // fp32 has no finite reciprocal
+            const float room = fmaf(off, inv, 4e-6f);
+            float least = s < 1e-30f ? -1.f : 1.f;  // the least distance from a half
             word = 0;
 #pragma unroll
-            for (int n = 0; n < 8; ++n) word |= (uint32_t)(kv4_code(x[n], s, inv) + 8) << (4 * n);
+            for (int n = 0; n < 8; ++n) {
+                // the whole number lies in the low bits of a sum with 3 2^22
+                const float q = x[n] * inv, m = q + 12582912.0f;
+                word |= (__float_as_uint(m) & 15u) << (4 * n);
+                least = fminf(least, fabsf(fabsf(q - (m - 12582912.0f)) - 0.5f));
+            }
+            if (!(least > room))
+                word = c0 < c.hd ? exact_codes(row, c0, ROPE ? cs + tl * np : nullptr, turn ? tab.rot : 0, halves, s) : 0u;
+            word ^= 0x88888888u;  // plus 8
         }
-        const int64_t pg = slot / c.page;
-        const int j = (int)(slot - pg * c.page) & (kKv4Granule - 1);
+        const int j = (int)slot & (kKv4Granule - 1);  // pages are whole granules
         uint8_t *g = c.granule(slot, head) + (kv ? kv4_v(c.ng) : 0);
         uint8_t *codes = g + j * kv4_row(c.ng);
         if (kv == 0) {
@@ -137,34 +221,38 @@ __global__ void __launch_bounds__(kAppendThreads) k_kv4_append(const __grid_cons
         if (t == 0)
             reinterpret_cast<__nv_bfloat16 *>(g + kv4_ks(c.ng))[j * c.ng + grp] = sb;
     }
+    }
 }
 
 struct Kv4ReadArgs {
     Kv4View c;
     void *y[2];
     const int64_t *slots;
-    int T;
+    int T, tpc;
 };
 
 // A thread: 8 channels of one (token, head); keys in y[0], values in y[1].
 template <typename T, bool VEC>
-__global__ void __launch_bounds__(256) k_kv4_read(const __grid_constant__ Kv4ReadArgs a) {
+__global__ void __launch_bounds__(kAppendThreads) k_kv4_read(const __grid_constant__ Kv4ReadArgs a) {
     launch_dependents();
     wait_prerequisite();
     const Kv4View &c = a.c;
-    const int kv = blockIdx.z, per = c.nkv * c.ng * 4;
+    const int kv = blockIdx.z, per = c.nkv * c.ng * 4, t0 = blockIdx.x * a.tpc, nt = min(a.tpc, a.T - t0);
     if (!a.y[kv]) return;
-    const int64_t total = (int64_t)a.T * per;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
-        const int tl = (int)(i / per), u = (int)(i - (int64_t)tl * per);
-        const int head = u / (c.ng * 4), w = u - head * c.ng * 4, grp = w >> 2, t = w & 3;
-        const int64_t slot = a.slots[tl];
+    const int side = per <= kAppendThreads / 2 ? kAppendThreads / per : 1;
+    const int first = side > 1 ? threadIdx.x / per : 0;
+    if (first >= side) return;
+    for (int u = side > 1 ? threadIdx.x - first * per : blockIdx.y * kAppendThreads + threadIdx.x; u < per;
+         u += gridDim.y * kAppendThreads) {
+    const int head = u / (c.ng * 4), w = u - head * c.ng * 4, grp = w >> 2, t = w & 3;
+    for (int tl = first; tl < nt; tl += side) {
+        const int64_t slot = a.slots[t0 + tl];
         if (slot < 0 || 8 * w >= c.hd) continue;
         if (slot >= c.slots()) {
             atomicOr(c.err, RB_KV4_ERR_SLOT);
             continue;
         }
-        const int j = (int)(slot % c.page) & (kKv4Granule - 1);
+        const int j = (int)slot & (kKv4Granule - 1);  // pages are whole granules
         const uint8_t *g = c.granule(slot, head) + (kv ? kv4_v(c.ng) : 0);
         const uint8_t *codes = g + j * kv4_row(c.ng);
         uint32_t word;
@@ -180,8 +268,16 @@ __global__ void __launch_bounds__(256) k_kv4_read(const __grid_constant__ Kv4Rea
         float v[8];
 #pragma unroll
         for (int n = 0; n < 8; ++n) v[n] = (float)((int)(word >> (4 * n) & 15u) - 8) * s;
-        store8<VEC>(static_cast<T *>(a.y[kv]) + (int64_t)tl * c.nkv * c.hd + head * c.hd + 8 * w, v);
+        store8<VEC>(static_cast<T *>(a.y[kv]) + (int64_t)(t0 + tl) * c.nkv * c.hd + head * c.hd + 8 * w, v);
     }
+    }
+}
+
+// Tokens per CTA of the append and the read: one wave of four CTAs an SM for each
+// of keys and values, up to 8; a token's items in one CTA each 256 (blockIdx.y).
+static int tokens_per_cta(int n_tokens) {
+    const int n = (n_tokens + 591) / 592;
+    return n > 8 ? 8 : n;
 }
 
 static bool aligned(const void *p, uintptr_t n) {
@@ -225,6 +321,9 @@ int rabbit_cuda_kv4_create(const rabbit_cuda_kv4_desc *d, int device, rabbit_cud
     c->view.ng = (d->head_dim + kKv4Group - 1) / kKv4Group;
     c->view.page = d->page_size;
     c->view.n_pages = d->n_pages;
+    c->view.shift = -1;
+    for (int i = 4; i <= 10; ++i)
+        if (d->page_size == 1 << i) c->view.shift = i;
     c->layer_bytes = (size_t)d->n_pages * c->view.page_bytes();
     const size_t bytes = (size_t)d->n_layers * c->layer_bytes;
     void *base = nullptr;
@@ -300,14 +399,14 @@ int rabbit_cuda_kv4_append_dev(rabbit_cuda_kv4 *kv, int layer, int dtype, const 
     a.slots = d_slots;
     a.pos = rope ? d_positions : nullptr;
     a.T = n_tokens;
-    a.tpc = 1;
+    a.tpc = tokens_per_cta(n_tokens);
     const bool vec = aligned(d_k, 16) && aligned(d_v, 16) && a.xs[0] * size % 16 == 0 &&
                      a.xs[1] * size % 16 == 0 && (int64_t)a.c.hd * size % 16 == 0;
     DeviceScope scope(kv->device);
     if (scope.status != RABBIT_CUDA_OK) return scope.status;
-    const int items = a.tpc * a.c.nkv * a.c.ng * 4;
+    const int items = a.c.nkv * a.c.ng * 4;
     const dim3 grid((n_tokens + a.tpc - 1) / a.tpc, (items + kAppendThreads - 1) / kAppendThreads, 2);
-    const size_t smem = sizeof(double2) * (size_t)a.tpc * np;
+    const size_t smem = (sizeof(double2) + sizeof(float2)) * (size_t)a.tpc * np;
     with_dtype(dtype, [&](auto t) {
         using T = decltype(t);
         auto k = rope ? (vec ? k_kv4_append<T, true, true> : k_kv4_append<T, false, true>)
@@ -336,14 +435,15 @@ int rabbit_cuda_kv4_read_dev(rabbit_cuda_kv4 *kv, int layer, int dtype, const in
     a.slots = d_slots;
     a.T = n_tokens;
     const bool vec = aligned(d_k, 16) && aligned(d_v, 16) && (int64_t)a.c.hd * size % 16 == 0;
-    const int64_t items = (int64_t)n_tokens * a.c.nkv * a.c.ng * 4;
-    const int64_t blocks = (items + 255) / 256, most = 16ll * kv->ctx->sm_count;
+    a.tpc = tokens_per_cta(n_tokens);
+    const int items = a.c.nkv * a.c.ng * 4;
+    const dim3 grid((n_tokens + a.tpc - 1) / a.tpc, (items + kAppendThreads - 1) / kAppendThreads, 2);
     DeviceScope scope(kv->device);
     if (scope.status != RABBIT_CUDA_OK) return scope.status;
     with_dtype(dtype, [&](auto t) {
         using T = decltype(t);
         scope.launch(launch_pdl(vec ? k_kv4_read<T, true> : k_kv4_read<T, false>,
-                                dim3((unsigned)(blocks < most ? blocks : most), 1, 2), dim3(256), 0,
+                                grid, dim3(kAppendThreads), 0,
                                 static_cast<cudaStream_t>(stream), a),
                      "kv4_read");
         return 0;

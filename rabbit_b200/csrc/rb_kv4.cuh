@@ -55,6 +55,7 @@ __host__ __device__ constexpr int kv4_vplace(int j, int g) { return g ^ ((j & 2)
 struct Kv4View {
     uint8_t *base;
     int nkv, hd, ng, page, n_pages;
+    int shift;  // page = 2^shift, or -1
     int *err;
     __host__ __device__ size_t head_bytes() const {
         return (size_t)(page / kKv4Granule) * kv4_bytes(ng);
@@ -62,10 +63,14 @@ struct Kv4View {
     __host__ __device__ size_t page_bytes() const { return nkv * head_bytes(); }
     __host__ __device__ int64_t slots() const { return (int64_t)n_pages * page; }
     __device__ __forceinline__ uint8_t *granule(int64_t slot, int head) const {
-        const int64_t p = slot / page;
+        return row(slot) + (size_t)head * head_bytes();
+    }
+    // The slot's granule of KV head 0.
+    __device__ __forceinline__ uint8_t *row(int64_t slot) const {
+        // (a division in 64 bits takes five times the instructions of one in 32)
+        const int64_t p = shift >= 0 ? slot >> shift : slot >> 31 ? slot / page : (int)slot / page;
         const int r = (int)(slot - p * page);
-        return base + (size_t)p * page_bytes() + (size_t)head * head_bytes() +
-               (size_t)(r / kKv4Granule) * kv4_bytes(ng);
+        return base + (size_t)p * page_bytes() + (size_t)(r / kKv4Granule) * kv4_bytes(ng);
     }
 };
 

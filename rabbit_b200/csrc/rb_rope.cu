@@ -31,40 +31,91 @@ struct RopeArgs {
     const int *pos;
     int64_t xs, ys;  // elements between rows
     int T, heads, hd;
-    int tpc;       // tokens per CTA
-    bool copy;     // y is not x: the channels that do not rotate are copied
+    int tpc;         // tokens per CTA
+    int nrot, per;   // items of a head that rotate, and all of them
 };
 
 constexpr int kRopeThreads = 256;
 
-// One CTA: tpc tokens. Their angles once into shared memory, then a thread per
-// pair of a (token, head).
-template <typename T>
-__global__ void __launch_bounds__(kRopeThreads) k_rope(const __grid_constant__ RopeArgs a) {
+// Bound by memory: each element is read and written once. One CTA takes tpc
+// tokens (and a part of a token's items, blockIdx.y): their angles are made in 64
+// bits and shared by the heads; then a thread keeps its item of the row and goes
+// through the tokens, BATCH of them in flight. An item is V channels (16 bytes;
+// scalar form: one) that rotate with V others (HALF), or 16 bytes of whole pairs
+// (INTERLEAVED; scalar form: one pair), or 16 bytes of the rest to copy.
+template <typename T, int V, bool HALF>
+__global__ void __launch_bounds__(kRopeThreads, 4) k_rope(const __grid_constant__ RopeArgs a) {
     extern __shared__ __align__(16) float2 cs[];  // [tpc][rot / 2]
+    // a vector holds one side of V pairs (HALF), or both sides of V / 2 (the scalar
+    // form has two elements of one pair)
+    constexpr int NV = HALF || V == 1 ? 2 : 1;    // vectors of an item
+    constexpr int NP = NV == 2 ? V : V / 2;       // pairs of an item
+    constexpr int BATCH = 4 / NV;
+    struct alignas(V * sizeof(T)) Vec {
+        T e[V];
+    };
     launch_dependents();
     wait_prerequisite();
     const int np = a.tab.rot / 2, t0 = blockIdx.x * a.tpc, nt = min(a.tpc, a.T - t0);
     for (int i = threadIdx.x; i < nt * np; i += kRopeThreads) {
-        const double2 v = rope_cs(a.pos[t0 + i / np], a.tab.turns[i % np]);
-        cs[i] = make_float2((float)(v.x * a.tab.mag), (float)(v.y * a.tab.mag));
+        const int t = i / np;
+        const double2 k = rope_cs(a.pos[t0 + t], a.tab.turns[i - t * np]);
+        cs[i] = make_float2((float)(k.x * a.tab.mag), (float)(k.y * a.tab.mag));
     }
     __syncthreads();
-    const int rest = a.copy ? a.hd - a.tab.rot : 0, per = np + rest;
-    const bool half = a.tab.layout == RABBIT_CUDA_ROPE_HALF;
-    for (int64_t i = threadIdx.x; i < (int64_t)nt * a.heads * per; i += kRopeThreads) {
-        const int u = (int)(i % per), h = (int)(i / per % a.heads), t = (int)(i / per / a.heads);
-        const T *x = static_cast<const T *>(a.x) + (t0 + t) * a.xs + (int64_t)h * a.hd;
-        T *y = static_cast<T *>(a.y) + (t0 + t) * a.ys + (int64_t)h * a.hd;
-        if (u >= np) {
-            y[a.tab.rot + u - np] = x[a.tab.rot + u - np];
-            continue;
+    const int row = a.heads * a.per, second = HALF ? np : V;
+    // short rows: several tokens side by side
+    const int side = row <= kRopeThreads / 2 ? kRopeThreads / row : 1;
+    const int first = side > 1 ? threadIdx.x / row : 0;
+    if (first >= side) return;
+    for (int r = side > 1 ? threadIdx.x - first * row : blockIdx.y * kRopeThreads + threadIdx.x; r < row;
+         r += gridDim.y * kRopeThreads) {
+        const int h = r / a.per, u = r - h * a.per;
+        const bool turn = u < a.nrot;
+        const int c = h * a.hd + (turn ? (HALF ? u * V : u * V * NV) : a.tab.rot + (u - a.nrot) * V);
+        const float2 *k0 = cs + (turn ? u * NP : 0);
+        const T *x = static_cast<const T *>(a.x) + (int64_t)(t0 + first) * a.xs + c;
+        T *y = static_cast<T *>(a.y) + (int64_t)(t0 + first) * a.ys + c;
+        for (int t = first; t < nt; t += BATCH * side) {
+            Vec v[BATCH][NV];
+#pragma unroll
+            for (int b = 0; b < BATCH; ++b)
+                if (t + b * side < nt) {
+                    const T *at = x + b * side * a.xs;
+                    v[b][0] = *reinterpret_cast<const Vec *>(at);
+                    if (NV == 2 && turn) v[b][NV - 1] = *reinterpret_cast<const Vec *>(at + second);
+                }
+#pragma unroll
+            for (int b = 0; b < BATCH; ++b) {
+                if (t + b * side >= nt) continue;
+                T *to = y + b * side * a.ys;
+                if (turn) {
+                    const float2 *kt = k0 + (t + b * side) * np;
+                    float2 ks[NP];
+                    if constexpr (NP % 2 == 0) {  // an even pair of the table
+#pragma unroll
+                        for (int e = 0; e < NP; e += 2) {
+                            const float4 k = *reinterpret_cast<const float4 *>(kt + e);
+                            ks[e] = make_float2(k.x, k.y);
+                            ks[e + 1] = make_float2(k.z, k.w);
+                        }
+                    } else {
+                        ks[0] = kt[0];
+                    }
+#pragma unroll
+                    for (int e = 0; e < NP; ++e) {
+                        T &e1 = v[b][0].e[NV == 2 ? e : 2 * e], &e2 = NV == 2 ? v[b][NV - 1].e[e] : v[b][0].e[(2 * e + 1) % V];
+                        const float x1 = to_f32(e1), x2 = to_f32(e2);
+                        e1 = from_f32<T>(x1 * ks[e].x - x2 * ks[e].y);
+                        e2 = from_f32<T>(x2 * ks[e].x + x1 * ks[e].y);
+                    }
+                    if (NV == 2) *reinterpret_cast<Vec *>(to + second) = v[b][NV - 1];
+                }
+                *reinterpret_cast<Vec *>(to) = v[b][0];
+            }
+            x += BATCH * side * a.xs;
+            y += BATCH * side * a.ys;
         }
-        const int c1 = half ? u : 2 * u, c2 = half ? u + np : 2 * u + 1;
-        const float x1 = to_f32(x[c1]), x2 = to_f32(x[c2]);
-        const float2 v = cs[t * np + u];
-        y[c1] = from_f32<T>(x1 * v.x - x2 * v.y);
-        y[c2] = from_f32<T>(x2 * v.x + x1 * v.y);
     }
 }
 
@@ -164,8 +215,9 @@ int rabbit_cuda_rope_dev(const rabbit_cuda_rope *r, int dtype, const void *d_x, 
     const int64_t row = (int64_t)n_heads * a.hd;
     a.xs = x_stride ? x_stride : row;
     a.ys = y_stride ? y_stride : row;
+    const int size = dtype_size(dtype);
     const uintptr_t off = reinterpret_cast<uintptr_t>(d_x) | reinterpret_cast<uintptr_t>(d_y);
-    if (a.xs < row || a.ys < row || (off & (dtype_size(dtype) - 1)) || (d_x == d_y && a.xs != a.ys))
+    if (a.xs < row || a.ys < row || (off & (size - 1)) || (d_x == d_y && a.xs != a.ys))
         return fail(RABBIT_CUDA_ERR_ARGS,
                     "rope_dev: strides below n_heads * head_dim (or different in place), or a "
                     "pointer not aligned to its element");
@@ -174,14 +226,36 @@ int rabbit_cuda_rope_dev(const rabbit_cuda_rope *r, int dtype, const void *d_x, 
     a.pos = d_positions;
     a.T = n_tokens;
     a.heads = n_heads;
-    a.copy = d_x != d_y;
-    a.tpc = 1;
+    const bool half = a.tab.layout == RABBIT_CUDA_ROPE_HALF;
+    // 16-byte vectors where rows, heads and both sides of the pairs allow them
+    const int side = half ? a.tab.rot / 2 : a.tab.rot;
+    const bool vec = (off & 15) == 0 && a.xs * size % 16 == 0 && a.ys * size % 16 == 0 &&
+                     a.hd * size % 16 == 0 && side * size % 16 == 0 && a.tab.rot * size % 16 == 0;
+    const int V = vec ? 16 / size : 1;
+    a.nrot = half || !vec ? a.tab.rot / 2 / V : a.tab.rot / V;
+    a.per = a.nrot + (d_x != d_y ? (a.hd - a.tab.rot) / V : 0);
+    // Tokens per CTA: all tokens in one wave of four CTAs an SM (a CTA makes its
+    // tokens' angles before it can rotate, so few and long ones), up to 32; where
+    // there are fewer tokens than SMs, a token's items are spread over blockIdx.y,
+    // up to a CTA an SM in all. 16384 x 32 x 128 bf16: 28 tokens a CTA 50 us, 2 tokens
+    // 74 us.
+    const int64_t items = (int64_t)n_heads * a.per;
+    const int sms = 148;
+    const int64_t wave = ((int64_t)n_tokens + 4 * sms - 1) / (4 * sms);
+    a.tpc = wave > 32 ? 32 : (int)wave;
+    const int groups = (n_tokens + a.tpc - 1) / a.tpc;
+    int64_t split = (items + kRopeThreads - 1) / kRopeThreads;
+    if (split > sms / groups) split = sms / groups;
+    const dim3 grid(groups, split < 1 ? 1 : (unsigned)split);
+    const size_t smem = sizeof(float2) * (size_t)a.tpc * (a.tab.rot / 2);
     DeviceScope scope(current_device());
     if (scope.status != RABBIT_CUDA_OK) return scope.status;
-    const size_t smem = sizeof(float2) * (size_t)a.tpc * (a.tab.rot / 2);
     with_dtype(dtype, [&](auto t) {
-        scope.launch(launch_pdl(k_rope<decltype(t)>, dim3((n_tokens + a.tpc - 1) / a.tpc),
-                                dim3(kRopeThreads), smem, static_cast<cudaStream_t>(stream), a),
+        using T = decltype(t);
+        constexpr int VT = 16 / sizeof(T);
+        auto k = half ? (vec ? k_rope<T, VT, true> : k_rope<T, 1, true>)
+                      : (vec ? k_rope<T, VT, false> : k_rope<T, 1, false>);
+        scope.launch(launch_pdl(k, grid, dim3(kRopeThreads), smem, static_cast<cudaStream_t>(stream), a),
                      "rope_dev");
         return 0;
     });
