@@ -102,8 +102,12 @@ __global__ void __launch_bounds__(kAppendThreads, 4) k_kv4_append(const __grid_c
     const bool mine = u < per && first < side;
     const int head = u / (c.ng * 4), w = u - head * c.ng * 4, grp = w >> 2, t = w & 3;
     const int c0 = 8 * w;  // first channel
+    const T *row = static_cast<const T *>(a.x[kv]) + (t0 + first - side) * a.xs[kv] + (int64_t)head * c.hd;
+    const int64_t step = side * a.xs[kv];
+    const size_t part = (size_t)head * c.head_bytes() + (kv ? kv4_v(c.ng) : 0);
     for (int ta = 0; ta < nt; ta += side) {
         const int tl = ta + first;
+        row += step;
         const bool in = mine && tl < nt;
         const int64_t slot = in ? a.slots[t0 + tl] : -1;
         const bool write = slot >= 0 && slot < c.slots();
@@ -113,7 +117,6 @@ __global__ void __launch_bounds__(kAppendThreads, 4) k_kv4_append(const __grid_c
         float x[8], v[8], p[8], big = 0.f;  // big: the largest |v| + |p|
 #pragma unroll
         for (int n = 0; n < 8; ++n) x[n] = v[n] = p[n] = 0.f;
-        const T *row = static_cast<const T *>(a.x[kv]) + (t0 + tl) * a.xs[kv] + (int64_t)head * c.hd;
         if (write && c0 < c.hd) {
             load8<VEC>(v, row + c0);
 #pragma unroll
@@ -189,10 +192,10 @@ __global__ void __launch_bounds__(kAppendThreads, 4) k_kv4_append(const __grid_c
             }
         }
         if (!write) continue;
-        const float s = __bfloat162float(sb), inv = 1.0f / s;
+        const float s = __bfloat162float(sb), inv = __fdividef(1.0f, s);
         uint32_t word = 0x88888888u;
         if (s > 0.f) {
-            // quotients off by off / s and 2^-22 |q|, |q| < 8; a scale near the smallest
+            // quotients off by off / s and 2^-21 |q|, |q| < 8; a scale near the smallest
             // fp32 has no finite reciprocal
             const float room = fmaf(off, inv, 4e-6f);
             float least = s < 1e-30f ? -1.f : 1.f;  // the least distance from a half
@@ -204,12 +207,22 @@ __global__ void __launch_bounds__(kAppendThreads, 4) k_kv4_append(const __grid_c
                 word |= (__float_as_uint(m) & 15u) << (4 * n);
                 least = fminf(least, fabsf(fabsf(q - (m - 12582912.0f)) - 0.5f));
             }
-            if (!(least > room))
+            if (!(least > room) && off == 0.f && s >= 1e-30f) {
+                // Values as they came (of few bits, often halves exactly): (k + 1/2) s has 12
+                // bits, so the sign of x - (k + 1/2) s in fp32 is exact.
+                word = 0;
+#pragma unroll
+                for (int n = 0; n < 8; ++n) {
+                    const float k = floorf(x[n] * inv), r = fmaf(-(k + 0.5f), s, x[n]);
+                    const int code = (int)k;
+                    word |= (uint32_t)((r > 0.f || (r == 0.f && (code & 1)) ? code + 1 : code) & 15) << (4 * n);
+                }
+            } else if (!(least > room))
                 word = c0 < c.hd ? exact_codes(row, c0, ROPE ? cs + tl * np : nullptr, turn ? tab.rot : 0, halves, s) : 0u;
             word ^= 0x88888888u;  // plus 8
         }
         const int j = (int)slot & (kKv4Granule - 1);  // pages are whole granules
-        uint8_t *g = c.granule(slot, head) + (kv ? kv4_v(c.ng) : 0);
+        uint8_t *g = c.row(slot) + part;
         uint8_t *codes = g + j * kv4_row(c.ng);
         if (kv == 0) {
             reinterpret_cast<uint32_t *>(codes)[t * c.ng + grp] = word;
@@ -321,6 +334,9 @@ int rabbit_cuda_kv4_create(const rabbit_cuda_kv4_desc *d, int device, rabbit_cud
     c->view.ng = (d->head_dim + kKv4Group - 1) / kKv4Group;
     c->view.page = d->page_size;
     c->view.n_pages = d->n_pages;
+    c->view.head = (size_t)(d->page_size / kKv4Granule) * kv4_bytes(c->view.ng);
+    c->view.page_size = d->n_kv_heads * c->view.head;
+    c->view.n_slots = (int64_t)d->n_pages * d->page_size;
     c->view.shift = -1;
     for (int i = 4; i <= 10; ++i)
         if (d->page_size == 1 << i) c->view.shift = i;
