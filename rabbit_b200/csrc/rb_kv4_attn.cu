@@ -4,6 +4,7 @@
 #include <atomic>
 #include <new>
 
+#include "rb_kv4_chunk.cuh"
 #include "rb_kv4_decode.cuh"
 #include "rb_launch.h"
 
@@ -30,12 +31,39 @@ static cudaError_t launch_decode(const Kv4AttnArgs &a, const rabbit_cuda_kv4 *kv
     return launch_pdl(kern, dim3(grid < kDecodeMaxGrid ? grid : kDecodeMaxGrid), dim3(C::kThreads), C::kSmem, s, a);
 }
 
-// Rows of a tile: 16 where a KV head has more than 8 query rows and the output
-// of 16 fits the registers, else 8.
+// CTAs of the chunk kernel from which it is taken: it does the work of 64 query
+// rows in the time the other takes for some 17, but only that spreads a KV head's
+// positions over the SMs (measured at 256 rows x 4 heads over 4352 positions:
+// 148 us there, 49 us here with 128 CTAs; 75 us against 84 us with 32).
+constexpr int kChunkMinCtas = 40;
+
+template <int NG>
+static cudaError_t launch_chunk(const Kv4AttnArgs &a, int tiles, const rabbit_cuda_kv4 *kv, cudaStream_t s) {
+    using C = ChunkCfg<NG>;
+    static_assert(C::kSmem + 2048 <= kMaxDynSmem, "shared memory of a CTA, the static part with it");
+    auto kern = k_kv4_chunk<NG>;
+    static std::atomic<uint32_t> ready{0};  // devices whose limit is raised
+    if (!(ready.load() >> kv->device & 1u)) {
+        const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
+        if (e != cudaSuccess) return e;
+        ready.fetch_or(1u << kv->device);
+    }
+    return launch_pdl(kern, dim3(tiles, a.c.nkv, a.n_seqs), dim3(C::kThreads), C::kSmem, s, a);
+}
+
+// Rows of a tile: as many as a KV head has query rows of a sequence, up to what
+// the output leaves of the registers; a granule's codes are made once for all.
 template <int NG, bool SPLIT>
 static cudaError_t launch_rows(const Kv4AttnArgs &a, const rabbit_cuda_kv4 *kv, cudaStream_t s) {
-    if constexpr (NG <= 4)
-        if ((int64_t)a.max_q * (a.nh / a.c.nkv) > 8) return launch_decode<NG, 2, SPLIT>(a, kv, s);
+    if constexpr (NG <= 4) {
+        const int64_t rows = (int64_t)a.max_q * (a.nh / a.c.nkv);
+        if constexpr (!SPLIT) {
+            const int64_t tiles = (rows + ChunkCfg<NG>::kRows - 1) / ChunkCfg<NG>::kRows;
+            if (rows > 16 && tiles * a.c.nkv * a.n_seqs >= kChunkMinCtas && tiles < (1 << 30))
+                return launch_chunk<NG>(a, (int)tiles, kv, s);
+        }
+        if (rows > 8) return launch_decode<NG, 2, SPLIT>(a, kv, s);
+    }
     return launch_decode<NG, 1, SPLIT>(a, kv, s);
 }
 

@@ -419,6 +419,14 @@ ATTN = [
     dict(dtype="bf16", nh=16, nkv=2, hd=64, page=64, lens=[257, 65], qs=[65, 65], window=64),
     dict(dtype="f32", nh=16, nkv=1, hd=32, page=16, lens=[70], qs=[70]),
     dict(dtype="f16", nh=32, nkv=8, hd=128, page=64, lens=[600], qs=[256]),
+    # chunks on many SMs: 64 query rows a CTA, tiles of 64 positions
+    dict(dtype="bf16", nh=16, nkv=8, hd=64, page=16, lens=[300, 90, 70], qs=[90, 90, 70], pad=2),
+    dict(dtype="f16", nh=8, nkv=8, hd=80, page=32, lens=[257, 200, 64, 65], qs=[129, 1, 64, 100]),
+    dict(dtype="bf16", nh=10, nkv=10, hd=96, page=48, lens=[511, 130], qs=[130, 130], window=100),
+    dict(dtype="f16", nh=40, nkv=20, hd=32, page=16, lens=[100, 0, 20], qs=[64, 3, 33], window=1, gap=3, off=1),
+    dict(dtype="bf16", nh=48, nkv=8, hd=128, page=64, lens=[333, 77], qs=[77, 77], gap=8, scale=0.2),
+    dict(dtype="f16", nh=8, nkv=8, hd=40, page=16, lens=[700], qs=[320], q_gain=30.0),
+    dict(dtype="bf16", nh=16, nkv=16, hd=8, page=16, lens=[150], qs=[150], q_gain=1e-3),
     # a long sequence beside short ones: split over many SMs
     dict(dtype="bf16", nh=8, nkv=2, hd=128, page=64, lens=[9000, 1, 0, 200], poison=False),
     dict(dtype="f32", nh=4, nkv=1, hd=64, page=16, lens=[6000], poison=False),
@@ -467,6 +475,27 @@ def test_attention_of_values_that_are_not_finite(torch, rc):
     assert nan[1].all()
 
 
+@pytest.mark.parametrize("dtype,nq", [("bf16", 20), ("f16", 200), ("f32", 200)])
+def test_values_that_are_not_finite_in_a_chunk(torch, rc, dtype, nq):
+    """Within a chunk only the rows behind a position see it: a NaN key there
+    makes them NaN, a NaN value their channels of its group, and the rows
+    before it stay as they are."""
+    c = Case(torch, rc, dtype=dtype, nh=16, nkv=8, hd=64, page=16, lens=[nq + 50], qs=[nq], seed=6)
+    bad_k, bad_v = nq + 50 - 7, nq + 50 - 12  # positions near the chunk's end
+    x = torch.randn(2, 8, 64, device="cuda")
+    k, v = x.clone(), x.clone()
+    k[0, 3, 5] = float("nan")
+    v[1, 2, 40] = float("-inf")
+    s = torch.from_numpy(c.slots[0][[bad_k, bad_v]]).cuda()
+    c.kv.append_dev(0, rc.F32, k.data_ptr(), v.data_ptr(), s.data_ptr(), 2, stream=stream(torch))
+    c.call()
+    nan = np.isnan(c.rows_of(c.out).reshape(nq, 16, 64))
+    want = np.zeros_like(nan)
+    want[nq - 7:, 6:8] = True
+    want[nq - 12:, 4:6, 32:] = True
+    np.testing.assert_array_equal(nan, want)
+
+
 def test_attention_reports_what_is_out_of_range(torch, rc):
     """Lengths past the table, pages past the cache, q_start out of order:
     reported once each, nothing read there, the other sequences unharmed."""
@@ -495,6 +524,17 @@ def test_attention_reports_what_is_out_of_range(torch, rc):
             good(c, [0, 2])
         c.kv.check(stream(torch))
         assert np.isfinite(c.rows_of(c.out)).all()
+    # the same in a chunk: a page of the second sequence
+    c = Case(torch, rc, dtype="bf16", nh=16, nkv=8, hd=64, page=16, lens=[200, 150, 90],
+             qs=[100, 100, 90], seed=10)
+    c.table[1, 2] = 12345
+    c.call()
+    with pytest.raises(rc.RabbitCudaError, match="page"):
+        c.kv.check(stream(torch))
+    want, bar = c.oracle(c.rows_of(c.qbuf).reshape(c.rows, c.nh, c.hd))
+    got = c.rows_of(c.out).reshape(want.shape)
+    assert (np.abs(got - want) <= bar)[:100].all() and (np.abs(got - want) <= bar)[200:].all()
+    assert np.isfinite(got).all()
 
 
 def test_attention_in_a_graph_and_on_two_streams(torch, rc):
