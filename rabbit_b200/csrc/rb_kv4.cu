@@ -64,7 +64,7 @@ __device__ __noinline__ uint32_t exact_codes(const T *row, int ch, const double2
 // error, and only where the bound leaves the rounding open (the scale's to bf16, a
 // quotient's to a whole number: about one value in 10^4) once more in 64 bits, from
 // the 64-bit cosine and sine that the token's table holds too. All in 64 bits the
-// conversions alone took 40 us for 8191 x 8 x 80 fp16 with a rotation; so 18 us.
+// conversions alone took 40 us for 8191 x 8 x 80 fp16 with a rotation; so 27 us.
 template <typename T, bool VEC, bool ROPE>
 __global__ void __launch_bounds__(kAppendThreads, 4) k_kv4_append(const __grid_constant__ Kv4AppendRopeArgs aa) {
     extern __shared__ __align__(16) double2 cs[];  // [tpc][rot / 2], keys only; then the same in fp32
@@ -98,142 +98,142 @@ __global__ void __launch_bounds__(kAppendThreads, 4) k_kv4_append(const __grid_c
     const int side = per <= kAppendThreads / 2 ? kAppendThreads / per : 1;
     const int first = side > 1 ? threadIdx.x / per : 0;
     for (int u0 = side > 1 ? 0 : blockIdx.y * kAppendThreads; u0 < per; u0 += gridDim.y * kAppendThreads) {
-    const int u = u0 + threadIdx.x - first * per;
-    const bool mine = u < per && first < side;
-    const int head = u / (c.ng * 4), w = u - head * c.ng * 4, grp = w >> 2, t = w & 3;
-    const int c0 = 8 * w;  // first channel
-    const T *row = static_cast<const T *>(a.x[kv]) + (t0 + first - side) * a.xs[kv] + (int64_t)head * c.hd;
-    const int64_t step = side * a.xs[kv];
-    const size_t part = (size_t)head * c.head_bytes() + (kv ? kv4_v(c.ng) : 0);
-    for (int ta = 0; ta < nt; ta += side) {
-        const int tl = ta + first;
-        row += step;
-        const bool in = mine && tl < nt;
-        const int64_t slot = in ? a.slots[t0 + tl] : -1;
-        const bool write = slot >= 0 && slot < c.slots();
-        if (in && slot >= c.slots()) atomicOr(c.err, RB_KV4_ERR_SLOT);
-        const bool turn = ROPE && rot && c0 < tab.rot;
-        // v, p: each channel and the other of its pair before the rotation; x: after it
-        float x[8], v[8], p[8], big = 0.f;  // big: the largest |v| + |p|
+        const int u = u0 + threadIdx.x - first * per;
+        const bool mine = u < per && first < side;
+        const int head = u / (c.ng * 4), w = u - head * c.ng * 4, grp = w >> 2, t = w & 3;
+        const int c0 = 8 * w;  // first channel
+        const T *row = static_cast<const T *>(a.x[kv]) + (t0 + first - side) * a.xs[kv] + (int64_t)head * c.hd;
+        const int64_t step = side * a.xs[kv];
+        const size_t part = (size_t)head * c.head_bytes() + (kv ? kv4_v(c.ng) : 0);
+        for (int ta = 0; ta < nt; ta += side) {
+            const int tl = ta + first;
+            row += step;
+            const bool in = mine && tl < nt;
+            const int64_t slot = in ? a.slots[t0 + tl] : -1;
+            const bool write = slot >= 0 && slot < c.slots();
+            if (in && slot >= c.slots()) atomicOr(c.err, RB_KV4_ERR_SLOT);
+            const bool turn = ROPE && rot && c0 < tab.rot;
+            // v, p: each channel and the other of its pair before the rotation; x: after it
+            float x[8], v[8], p[8], big = 0.f;  // big: the largest |v| + |p|
 #pragma unroll
-        for (int n = 0; n < 8; ++n) x[n] = v[n] = p[n] = 0.f;
-        if (write && c0 < c.hd) {
-            load8<VEC>(v, row + c0);
+            for (int n = 0; n < 8; ++n) x[n] = v[n] = p[n] = 0.f;
+            if (write && c0 < c.hd) {
+                load8<VEC>(v, row + c0);
 #pragma unroll
-            for (int n = 0; n < 8; ++n) x[n] = v[n];
-            if constexpr (ROPE) {
-                if (turn) {
-                    float2 k[8];  // x = v k.x + p k.y
-                    const float2 *ct = cs32 + tl * np;
-                    if (!halves) {
+                for (int n = 0; n < 8; ++n) x[n] = v[n];
+                if constexpr (ROPE) {
+                    if (turn) {
+                        float2 k[8];  // x = v k.x + p k.y
+                        const float2 *ct = cs32 + tl * np;
+                        if (!halves) {
 #pragma unroll
-                        for (int n = 0; n < 8; ++n) {
-                            p[n] = v[n ^ 1];
-                            if (!(n & 1)) k[n] = k[n + 1] = c0 + n < tab.rot ? ct[(c0 + n) / 2] : make_float2(1.f, 0.f);
-                            if (!(n & 1)) k[n].y = -k[n].y;
-                        }
-                    } else if (np % 8 == 0) {  // all 8 are first or second
-                        const bool first = c0 < np;
-                        load8<VEC>(p, row + (first ? c0 + np : c0 - np));
-                        const float4 *c4 = reinterpret_cast<const float4 *>(ct + (first ? c0 : c0 - np));
+                            for (int n = 0; n < 8; ++n) {
+                                p[n] = v[n ^ 1];
+                                if (!(n & 1)) k[n] = k[n + 1] = c0 + n < tab.rot ? ct[(c0 + n) / 2] : make_float2(1.f, 0.f);
+                                if (!(n & 1)) k[n].y = -k[n].y;
+                            }
+                        } else if (np % 8 == 0) {  // all 8 are first or second
+                            const bool first = c0 < np;
+                            load8<VEC>(p, row + (first ? c0 + np : c0 - np));
+                            const float4 *c4 = reinterpret_cast<const float4 *>(ct + (first ? c0 : c0 - np));
 #pragma unroll
-                        for (int n = 0; n < 8; n += 2) {
-                            const float4 y = c4[n / 2];
-                            k[n] = make_float2(y.x, first ? -y.y : y.y);
-                            k[n + 1] = make_float2(y.z, first ? -y.w : y.w);
-                        }
-                    } else {
+                            for (int n = 0; n < 8; n += 2) {
+                                const float4 y = c4[n / 2];
+                                k[n] = make_float2(y.x, first ? -y.y : y.y);
+                                k[n + 1] = make_float2(y.z, first ? -y.w : y.w);
+                            }
+                        } else {
 #pragma unroll
-                        for (int n = 0; n < 8; ++n) {
-                            const int ch = c0 + n;
-                            k[n] = make_float2(1.f, 0.f);
-                            if (ch < tab.rot) {
-                                p[n] = to_f32(row[ch < np ? ch + np : ch - np]);
-                                k[n] = ct[ch < np ? ch : ch - np];
-                                if (ch < np) k[n].y = -k[n].y;
+                            for (int n = 0; n < 8; ++n) {
+                                const int ch = c0 + n;
+                                k[n] = make_float2(1.f, 0.f);
+                                if (ch < tab.rot) {
+                                    p[n] = to_f32(row[ch < np ? ch + np : ch - np]);
+                                    k[n] = ct[ch < np ? ch : ch - np];
+                                    if (ch < np) k[n].y = -k[n].y;
+                                }
                             }
                         }
-                    }
 #pragma unroll
-                    for (int n = 0; n < 8; ++n) {
-                        x[n] = fmaf(v[n], k[n].x, p[n] * k[n].y);
-                        big = fmaxf(big, fabsf(v[n]) + fabsf(p[n]));
+                        for (int n = 0; n < 8; ++n) {
+                            x[n] = fmaf(v[n], k[n].x, p[n] * k[n].y);
+                            big = fmaxf(big, fabsf(v[n]) + fabsf(p[n]));
+                        }
                     }
                 }
             }
-        }
-        auto scale_of = [](float top) {
-            const float top7 = __fmul_rn(top, 1.0f / 7.0f);
-            // a group with an infinity or a NaN has a NaN for its scale
-            return __float2bfloat16_rn(top7 < INFINITY ? top7 : __uint_as_float(0x7fc00000u));
-        };
-        // the group's largest: an integer maximum of the bits keeps a NaN
-        uint32_t top = 0;
+            auto scale_of = [](float top) {
+                const float top7 = __fmul_rn(top, 1.0f / 7.0f);
+                // a group with an infinity or a NaN has a NaN for its scale
+                return __float2bfloat16_rn(top7 < INFINITY ? top7 : __uint_as_float(0x7fc00000u));
+            };
+            // the group's largest: an integer maximum of the bits keeps a NaN
+            uint32_t top = 0;
 #pragma unroll
-        for (int n = 0; n < 8; ++n) top = max(top, __float_as_uint(fabsf(x[n])));
-        top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-        top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        __nv_bfloat16 sb = scale_of(__uint_as_float(top));
-        float off = 0.f;  // how far the rotated values may be off
-        if constexpr (ROPE) {
-            big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
-            big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
-            // cosine and sine half a step off, a product and a sum rounded: at most
-            // 4 2^-24 (|v| + |p|) of the magnitude
-            off = big * mag * 2.4e-7f;
-            const float a0 = __uint_as_float(top) - off, a1 = __uint_as_float(top) + off;
-            const bool open = off > 0.f && !(__bfloat162float(scale_of(fmaxf(a0, 0.f))) == __bfloat162float(scale_of(a1)));
-            if (__any_sync(0xffffffffu, open)) {
-                uint32_t e = 0;
-                if (write && c0 < c.hd) e = exact_top(row, c0, cs + tl * np, turn ? tab.rot : 0, halves);
-                e = max(e, __shfl_xor_sync(0xffffffffu, e, 1));
-                e = max(e, __shfl_xor_sync(0xffffffffu, e, 2));
-                if (open) sb = scale_of(__uint_as_float(e));
+            for (int n = 0; n < 8; ++n) top = max(top, __float_as_uint(fabsf(x[n])));
+            top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+            __nv_bfloat16 sb = scale_of(__uint_as_float(top));
+            float off = 0.f;  // how far the rotated values may be off
+            if constexpr (ROPE) {
+                big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
+                big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
+                // cosine and sine half a step off, a product and a sum rounded: at most
+                // 4 2^-24 (|v| + |p|) of the magnitude
+                off = big * mag * 2.4e-7f;
+                const float a0 = __uint_as_float(top) - off, a1 = __uint_as_float(top) + off;
+                const bool open = off > 0.f && !(__bfloat162float(scale_of(fmaxf(a0, 0.f))) == __bfloat162float(scale_of(a1)));
+                if (__any_sync(0xffffffffu, open)) {
+                    uint32_t e = 0;
+                    if (write && c0 < c.hd) e = exact_top(row, c0, cs + tl * np, turn ? tab.rot : 0, halves);
+                    e = max(e, __shfl_xor_sync(0xffffffffu, e, 1));
+                    e = max(e, __shfl_xor_sync(0xffffffffu, e, 2));
+                    if (open) sb = scale_of(__uint_as_float(e));
+                }
             }
-        }
-        if (!write) continue;
-        const float s = __bfloat162float(sb), inv = __fdividef(1.0f, s);
-        uint32_t word = 0x88888888u;
-        if (s > 0.f) {
-            // quotients off by off / s and 2^-21 |q|, |q| < 8; a scale near the smallest
-            // fp32 has no finite reciprocal
-            const float room = fmaf(off, inv, 4e-6f);
-            float least = s < 1e-30f ? -1.f : 1.f;  // the least distance from a half
-            word = 0;
-#pragma unroll
-            for (int n = 0; n < 8; ++n) {
-                // the whole number lies in the low bits of a sum with 3 2^22
-                const float q = x[n] * inv, m = q + 12582912.0f;
-                word |= (__float_as_uint(m) & 15u) << (4 * n);
-                least = fminf(least, fabsf(fabsf(q - (m - 12582912.0f)) - 0.5f));
-            }
-            if (!(least > room) && off == 0.f && s >= 1e-30f) {
-                // Values as they came (of few bits, often halves exactly): (k + 1/2) s has 12
-                // bits, so the sign of x - (k + 1/2) s in fp32 is exact.
+            if (!write) continue;
+            const float s = __bfloat162float(sb), inv = __fdividef(1.0f, s);
+            uint32_t word = 0x88888888u;
+            if (s > 0.f) {
+                // quotients off by off / s and 2^-21 |q|, |q| < 8; a scale near the smallest
+                // fp32 has no finite reciprocal
+                const float room = fmaf(off, inv, 4e-6f);
+                float least = s < 1e-30f ? -1.f : 1.f;  // the least distance from a half
                 word = 0;
 #pragma unroll
                 for (int n = 0; n < 8; ++n) {
-                    const float k = floorf(x[n] * inv), r = fmaf(-(k + 0.5f), s, x[n]);
-                    const int code = (int)k;
-                    word |= (uint32_t)((r > 0.f || (r == 0.f && (code & 1)) ? code + 1 : code) & 15) << (4 * n);
+                    // the whole number lies in the low bits of a sum with 3 2^22
+                    const float q = x[n] * inv, m = q + 12582912.0f;
+                    word |= (__float_as_uint(m) & 15u) << (4 * n);
+                    least = fminf(least, fabsf(fabsf(q - (m - 12582912.0f)) - 0.5f));
                 }
-            } else if (!(least > room))
-                word = c0 < c.hd ? exact_codes(row, c0, ROPE ? cs + tl * np : nullptr, turn ? tab.rot : 0, halves, s) : 0u;
-            word ^= 0x88888888u;  // plus 8
+                if (!(least > room) && off == 0.f && s >= 1e-30f) {
+                    // Values as they came (of few bits, often halves exactly): (k + 1/2) s has 12
+                    // bits, so the sign of x - (k + 1/2) s in fp32 is exact.
+                    word = 0;
+#pragma unroll
+                    for (int n = 0; n < 8; ++n) {
+                        const float k = floorf(x[n] * inv), r = fmaf(-(k + 0.5f), s, x[n]);
+                        const int code = (int)k;
+                        word |= (uint32_t)((r > 0.f || (r == 0.f && (code & 1)) ? code + 1 : code) & 15) << (4 * n);
+                    }
+                } else if (!(least > room))
+                    word = c0 < c.hd ? exact_codes(row, c0, ROPE ? cs + tl * np : nullptr, turn ? tab.rot : 0, halves, s) : 0u;
+                word ^= 0x88888888u;  // plus 8
+            }
+            const int j = (int)slot & (kKv4Granule - 1);  // pages are whole granules
+            uint8_t *g = c.row(slot) + part;
+            uint8_t *codes = g + j * kv4_row(c.ng);
+            if (kv == 0) {
+                reinterpret_cast<uint32_t *>(codes)[t * c.ng + grp] = word;
+            } else {
+                uint16_t *h = reinterpret_cast<uint16_t *>(codes);
+                h[kv4_vplace(j, 2 * t) * c.ng + grp] = (uint16_t)word;
+                h[kv4_vplace(j, 2 * t + 1) * c.ng + grp] = (uint16_t)(word >> 16);
+            }
+            if (t == 0)
+                reinterpret_cast<__nv_bfloat16 *>(g + kv4_ks(c.ng))[j * c.ng + grp] = sb;
         }
-        const int j = (int)slot & (kKv4Granule - 1);  // pages are whole granules
-        uint8_t *g = c.row(slot) + part;
-        uint8_t *codes = g + j * kv4_row(c.ng);
-        if (kv == 0) {
-            reinterpret_cast<uint32_t *>(codes)[t * c.ng + grp] = word;
-        } else {
-            uint16_t *h = reinterpret_cast<uint16_t *>(codes);
-            h[kv4_vplace(j, 2 * t) * c.ng + grp] = (uint16_t)word;
-            h[kv4_vplace(j, 2 * t + 1) * c.ng + grp] = (uint16_t)(word >> 16);
-        }
-        if (t == 0)
-            reinterpret_cast<__nv_bfloat16 *>(g + kv4_ks(c.ng))[j * c.ng + grp] = sb;
-    }
     }
 }
 
@@ -257,40 +257,40 @@ __global__ void __launch_bounds__(kAppendThreads) k_kv4_read(const __grid_consta
     if (first >= side) return;
     for (int u = side > 1 ? threadIdx.x - first * per : blockIdx.y * kAppendThreads + threadIdx.x; u < per;
          u += gridDim.y * kAppendThreads) {
-    const int head = u / (c.ng * 4), w = u - head * c.ng * 4, grp = w >> 2, t = w & 3;
-    for (int tl = first; tl < nt; tl += side) {
-        const int64_t slot = a.slots[t0 + tl];
-        if (slot < 0 || 8 * w >= c.hd) continue;
-        if (slot >= c.slots()) {
-            atomicOr(c.err, RB_KV4_ERR_SLOT);
-            continue;
-        }
-        const int j = (int)slot & (kKv4Granule - 1);  // pages are whole granules
-        const uint8_t *g = c.granule(slot, head) + (kv ? kv4_v(c.ng) : 0);
-        const uint8_t *codes = g + j * kv4_row(c.ng);
-        uint32_t word;
-        if (kv == 0) {
-            word = reinterpret_cast<const uint32_t *>(codes)[t * c.ng + grp];
-        } else {
-            const uint16_t *h = reinterpret_cast<const uint16_t *>(codes);
-            word = h[kv4_vplace(j, 2 * t) * c.ng + grp] |
-                   (uint32_t)h[kv4_vplace(j, 2 * t + 1) * c.ng + grp] << 16;
-        }
-        const float s = __bfloat162float(
-            reinterpret_cast<const __nv_bfloat16 *>(g + kv4_ks(c.ng))[j * c.ng + grp]);
-        float v[8];
+        const int head = u / (c.ng * 4), w = u - head * c.ng * 4, grp = w >> 2, t = w & 3;
+        for (int tl = first; tl < nt; tl += side) {
+            const int64_t slot = a.slots[t0 + tl];
+            if (slot < 0 || 8 * w >= c.hd) continue;
+            if (slot >= c.slots()) {
+                atomicOr(c.err, RB_KV4_ERR_SLOT);
+                continue;
+            }
+            const int j = (int)slot & (kKv4Granule - 1);  // pages are whole granules
+            const uint8_t *g = c.granule(slot, head) + (kv ? kv4_v(c.ng) : 0);
+            const uint8_t *codes = g + j * kv4_row(c.ng);
+            uint32_t word;
+            if (kv == 0) {
+                word = reinterpret_cast<const uint32_t *>(codes)[t * c.ng + grp];
+            } else {
+                const uint16_t *h = reinterpret_cast<const uint16_t *>(codes);
+                word = h[kv4_vplace(j, 2 * t) * c.ng + grp] |
+                       (uint32_t)h[kv4_vplace(j, 2 * t + 1) * c.ng + grp] << 16;
+            }
+            const float s = __bfloat162float(
+                reinterpret_cast<const __nv_bfloat16 *>(g + kv4_ks(c.ng))[j * c.ng + grp]);
+            float v[8];
 #pragma unroll
-        for (int n = 0; n < 8; ++n) v[n] = (float)((int)(word >> (4 * n) & 15u) - 8) * s;
-        store8<VEC>(static_cast<T *>(a.y[kv]) + (int64_t)(t0 + tl) * c.nkv * c.hd + head * c.hd + 8 * w, v);
-    }
+            for (int n = 0; n < 8; ++n) v[n] = (float)((int)(word >> (4 * n) & 15u) - 8) * s;
+            store8<VEC>(static_cast<T *>(a.y[kv]) + (int64_t)(t0 + tl) * c.nkv * c.hd + head * c.hd + 8 * w, v);
+        }
     }
 }
 
 // Tokens per CTA of the append and the read: one wave of four CTAs an SM for each
 // of keys and values, up to 8; a token's items in one CTA each 256 (blockIdx.y).
 static int tokens_per_cta(int n_tokens) {
-    const int n = (n_tokens + 591) / 592;
-    return n > 8 ? 8 : n;
+    const int64_t n = ((int64_t)n_tokens + 591) / 592;
+    return n > 8 ? 8 : (int)n;
 }
 
 static bool aligned(const void *p, uintptr_t n) {
@@ -340,10 +340,11 @@ int rabbit_cuda_kv4_create(const rabbit_cuda_kv4_desc *d, int device, rabbit_cud
     c->view.shift = -1;
     for (int i = 4; i <= 10; ++i)
         if (d->page_size == 1 << i) c->view.shift = i;
-    c->layer_bytes = (size_t)d->n_pages * c->view.page_bytes();
-    const size_t bytes = (size_t)d->n_layers * c->layer_bytes;
+    c->layer_bytes = (size_t)d->n_pages * c->view.page_bytes();  // below 2^60
+    size_t bytes = 0;
     void *base = nullptr;
-    cudaError_t e = cudaMalloc(&base, bytes);
+    cudaError_t e = __builtin_mul_overflow((size_t)d->n_layers, c->layer_bytes, &bytes) ? cudaErrorMemoryAllocation
+                                                                                      : cudaMalloc(&base, bytes);
     if (e == cudaSuccess) {
         c->view.base = static_cast<uint8_t *>(base);
         if ((e = cudaMalloc(&c->d_err, sizeof(int))) == cudaSuccess &&
@@ -421,7 +422,7 @@ int rabbit_cuda_kv4_append_dev(rabbit_cuda_kv4 *kv, int layer, int dtype, const 
     DeviceScope scope(kv->device);
     if (scope.status != RABBIT_CUDA_OK) return scope.status;
     const int items = a.c.nkv * a.c.ng * 4;
-    const dim3 grid((n_tokens + a.tpc - 1) / a.tpc, (items + kAppendThreads - 1) / kAppendThreads, 2);
+    const dim3 grid((unsigned)(((int64_t)n_tokens + a.tpc - 1) / a.tpc), (items + kAppendThreads - 1) / kAppendThreads, 2);
     const size_t smem = (sizeof(double2) + sizeof(float2)) * (size_t)a.tpc * np;
     with_dtype(dtype, [&](auto t) {
         using T = decltype(t);
@@ -453,7 +454,7 @@ int rabbit_cuda_kv4_read_dev(rabbit_cuda_kv4 *kv, int layer, int dtype, const in
     const bool vec = aligned(d_k, 16) && aligned(d_v, 16) && (int64_t)a.c.hd * size % 16 == 0;
     a.tpc = tokens_per_cta(n_tokens);
     const int items = a.c.nkv * a.c.ng * 4;
-    const dim3 grid((n_tokens + a.tpc - 1) / a.tpc, (items + kAppendThreads - 1) / kAppendThreads, 2);
+    const dim3 grid((unsigned)(((int64_t)n_tokens + a.tpc - 1) / a.tpc), (items + kAppendThreads - 1) / kAppendThreads, 2);
     DeviceScope scope(kv->device);
     if (scope.status != RABBIT_CUDA_OK) return scope.status;
     with_dtype(dtype, [&](auto t) {

@@ -217,7 +217,8 @@ int rabbit_cuda_rope_dev(const rabbit_cuda_rope *r, int dtype, const void *d_x, 
     a.ys = y_stride ? y_stride : row;
     const int size = dtype_size(dtype);
     const uintptr_t off = reinterpret_cast<uintptr_t>(d_x) | reinterpret_cast<uintptr_t>(d_y);
-    if (a.xs < row || a.ys < row || (off & (size - 1)) || (d_x == d_y && a.xs != a.ys))
+    if (a.xs < row || a.ys < row || (off & (size - 1)) ||
+        (reinterpret_cast<uintptr_t>(d_positions) & 3) || (d_x == d_y && a.xs != a.ys))
         return fail(RABBIT_CUDA_ERR_ARGS,
                     "rope_dev: strides below n_heads * head_dim (or different in place), or a "
                     "pointer not aligned to its element");
@@ -237,13 +238,15 @@ int rabbit_cuda_rope_dev(const rabbit_cuda_rope *r, int dtype, const void *d_x, 
     // Tokens per CTA: all tokens in one wave of four CTAs an SM (a CTA makes its
     // tokens' angles before it can rotate, so few and long ones), up to 32; where
     // there are fewer tokens than SMs, a token's items are spread over blockIdx.y,
-    // up to a CTA an SM in all. 16384 x 32 x 128 bf16: 28 tokens a CTA 50 us, 2 tokens
-    // 74 us.
+    // up to a CTA an SM in all. 16384 x 32 x 128 bf16: 28 tokens a CTA 55 us (4.9
+    // TB/s), 2 tokens 74 us.
     const int64_t items = (int64_t)n_heads * a.per;
     const int sms = 148;
     const int64_t wave = ((int64_t)n_tokens + 4 * sms - 1) / (4 * sms);
+    const int most = 48 * 1024 / (int)(sizeof(float2) * (a.tab.rot / 2));  // their angles' shared memory
     a.tpc = wave > 32 ? 32 : (int)wave;
-    const int groups = (n_tokens + a.tpc - 1) / a.tpc;
+    if (a.tpc > most) a.tpc = most;
+    const int groups = (int)(((int64_t)n_tokens + a.tpc - 1) / a.tpc);
     int64_t split = (items + kRopeThreads - 1) / kRopeThreads;
     if (split > sms / groups) split = sms / groups;
     const dim3 grid(groups, split < 1 ? 1 : (unsigned)split);

@@ -88,7 +88,7 @@ def test_null_arguments_are_refused(rc):
 @pytest.mark.parametrize("kw", [
     dict(n_layers=0), dict(n_kv_heads=0), dict(n_kv_heads=1025), dict(head_dim=0), dict(head_dim=12),
     dict(head_dim=264), dict(page_size=8), dict(page_size=24), dict(page_size=2048),
-    dict(n_pages=0), dict(n_pages=-1), dict(device=-1), dict(device=99),
+    dict(n_pages=0), dict(n_pages=-1), dict(device=-1), dict(device=99), dict(n_layers=1 << 20),
 ])
 def test_cache_refuses(rc, kw):
     base = dict(n_layers=1, n_kv_heads=1, head_dim=64, page_size=16, n_pages=1)
