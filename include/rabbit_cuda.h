@@ -527,10 +527,11 @@ int rabbit_cuda_rope_dev(const rabbit_cuda_rope *r, int dtype, const void *d_x, 
  * sequence of at most 256 tokens, src/forward_v2.c:16-26). For each token, KV
  * head and 32 consecutive channels x (the last group of a head may be
  * shorter): scale s = bf16(max|x| / 7) (the fp32 product with 1/7, rounded),
- * codes rint(x / s), a channel read back as code * s; s = 0: all zero. Each group has its own codes, so a token
- * can be written without touching its neighbours: 18 bytes per 32 channels. A
- * group that holds an infinity or a NaN reads back as NaN. Slot = page *
- * page_size + place in the page; every layer has the same pages. */
+ * codes rint(x / s), a channel read back as code * s; s = 0: all zero. Each
+ * group has its own codes, so a token can be written without touching its
+ * neighbours: 18 bytes per 32 channels. A group that holds an infinity or a NaN
+ * reads back as NaN. Slot = page * page_size + place in the page; every layer
+ * has the same pages. */
 typedef struct {
     int n_layers;    /* >= 1 */
     int n_kv_heads;  /* 1..1024 */
@@ -569,7 +570,7 @@ int rabbit_cuda_kv4_read_dev(rabbit_cuda_kv4 *kv, int layer, int dtype, const in
 /* The sequences of an attention call, in DEVICE arrays that are read when the
  * call runs (so a captured graph sees their values at replay). */
 typedef struct {
-    int n_seqs;              /* 0..65535 */
+    int n_seqs;              /* 0..65535; without d_q_start at most n_tokens */
     int max_pages;           /* entries of a page_table row */
     int max_q_len;           /* at least the longest sequence's query rows; 0 means 1 */
     const int *d_q_start;    /* [n_seqs + 1] ascending: query rows of sequence i are
@@ -581,23 +582,27 @@ typedef struct {
 /* What an attention call needs while it runs (partial sums of sequences split
  * over the SMs), allocated once; it serves any layer, batch and head count of
  * `kv`. Calls, and graphs that hold them, that may run at the same time need
- * one each. */
+ * one each; after RABBIT_CUDA_ERR_TIMEOUT make a new one. */
 typedef struct rabbit_cuda_kv4_scratch rabbit_cuda_kv4_scratch;
 int rabbit_cuda_kv4_scratch_create(const rabbit_cuda_kv4 *kv, rabbit_cuda_kv4_scratch **out);
 int rabbit_cuda_kv4_scratch_free(rabbit_cuda_kv4_scratch *ws);
 
-/* Attention of n_tokens query rows (n_heads heads, a multiple of n_kv_heads;
- * query head h reads KV head h / (n_heads / n_kv_heads)) over `layer`'s cache.
- * The last query row of a sequence is its last cached position, the row before
+/* Attention of n_tokens query rows (n_heads heads, a multiple of n_kv_heads, at
+ * most 65535, n_tokens * n_heads below 2^31; query head h reads KV head
+ * h / (n_heads / n_kv_heads)) over `layer`'s cache. The last query row of a sequence is its last cached position, the row before
  * it one earlier, and so on; a row at position p sees positions 0..p, with
  * window > 0 only the last `window` of them. out = sum_j softmax_j(scale q.k_j)
  * v_j; scale 0 means 1 / sqrt(head_dim); a row that sees nothing gives 0. Rows
- * behind the last sequence are left as they were; a row past n_tokens is not
- * written. Strides in elements between rows (0: n_heads * head_dim); out may be
- * q with the same stride. Positions past max_pages pages, pages past the cache
- * and q_start not ascending read as nothing there and are reported by
- * rabbit_cuda_kv4_check. DEVICE buffers aligned to their element, asynchronous on
- * `stream`; may be captured into a graph. */
+ * behind the last sequence are left as they were. Strides in elements between
+ * rows (0: n_heads * head_dim); out may be q with the same stride. Checked on
+ * the device, and reported by rabbit_cuda_kv4_check: a kv_len below 0, past
+ * max_pages pages or past 2^30 - 1 counts as 0; a page past the cache reads as
+ * nothing there; a sequence whose q_start is out of order, past n_tokens or
+ * longer than max_q_len gets no rows. n_tokens 0 or n_seqs 0 does nothing. A
+ * visible group of 32 channels that holds an infinity or a NaN makes NaN of the
+ * rows that see it (a key's) or of their 32 channels (a value's). DEVICE
+ * buffers aligned to their element, asynchronous on `stream`; may be captured
+ * into a graph. */
 int rabbit_cuda_kv4_attention_dev(rabbit_cuda_kv4 *kv, int layer, rabbit_cuda_kv4_scratch *ws,
                                   int dtype, const void *d_q, int64_t q_stride, void *d_out,
                                   int64_t out_stride, int n_tokens, int n_heads,

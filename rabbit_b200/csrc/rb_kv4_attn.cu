@@ -31,11 +31,12 @@ static cudaError_t launch_decode(const Kv4AttnArgs &a, const rabbit_cuda_kv4 *kv
     return launch_pdl(kern, dim3(grid < kDecodeMaxGrid ? grid : kDecodeMaxGrid), dim3(C::kThreads), C::kSmem, s, a);
 }
 
-// CTAs of the chunk kernel from which it is taken: it does the work of 64 query
-// rows in the time the other takes for some 17, but only that spreads a KV head's
-// positions over the SMs (measured at 256 rows x 4 heads over 4352 positions:
-// 148 us there, 49 us here with 128 CTAs; 75 us against 84 us with 32).
-constexpr int kChunkMinCtas = 40;
+// CTAs of the chunk kernel from which it is taken. Its time goes by the rows and
+// positions of one CTA; the other's, which spreads a KV head's positions over the
+// SMs, by the whole batch. 256 rows x 4 heads a KV head over 4352 positions: 91 us
+// here with 16 to 128 CTAs; there 34 us for the work of 16 of them, 51 of 32, 85 of
+// 64, 149 of 128.
+constexpr int kChunkMinCtas = 72;
 
 template <int NG>
 static cudaError_t launch_chunk(const Kv4AttnArgs &a, int tiles, const rabbit_cuda_kv4 *kv, cudaStream_t s) {
@@ -58,8 +59,15 @@ static cudaError_t launch_rows(const Kv4AttnArgs &a, const rabbit_cuda_kv4 *kv, 
     if constexpr (NG <= 4) {
         const int64_t rows = (int64_t)a.max_q * (a.nh / a.c.nkv);
         if constexpr (!SPLIT) {
+            // Where only few sequences of a batch have many rows, the others would each take a
+            // chunk of 64 for their own one: so half a chunk a sequence on average. 64 sequences
+            // of 1024 positions, 4 heads a KV head, 1 / 4 / 16 of them with 256 rows and the rest
+            // with one (20 / 68 / 268 rows on average): 150 / 211 / 460 us here, 121 / 267 / 726
+            // us in the decode kernel; one of them with 64 rows (8): 106 and 74 us.
             const int64_t tiles = (rows + ChunkCfg<NG>::kRows - 1) / ChunkCfg<NG>::kRows;
-            if (rows > 16 && tiles * a.c.nkv * a.n_seqs >= kChunkMinCtas && tiles < (1 << 30))
+            const int64_t most = rows < ChunkCfg<NG>::kRows / 2 ? rows : ChunkCfg<NG>::kRows / 2;
+            if (rows > 16 && tiles * a.c.nkv * a.n_seqs >= kChunkMinCtas &&
+                (int64_t)a.T * (a.nh / a.c.nkv) >= most * a.n_seqs)
                 return launch_chunk<NG>(a, (int)tiles, kv, s);
         }
         if (rows > 8) return launch_decode<NG, 2, SPLIT>(a, kv, s);
@@ -136,8 +144,8 @@ int rabbit_cuda_kv4_attention_dev(rabbit_cuda_kv4 *kv, int layer, rabbit_cuda_kv
                                   const rabbit_cuda_kv4_batch *b, float scale, int window,
                                   void *stream) {
     if (!kv || !ws || !b || layer < 0 || layer >= kv->n_layers || !dtype_size(dtype) ||
-        n_tokens < 0 || n_heads < 1 || n_heads > 65535 || n_heads % kv->view.nkv || window < 0 ||
-        !isfinite(scale))
+        n_tokens < 0 || n_heads < 1 || n_heads > 65535 || n_heads % kv->view.nkv ||
+        (int64_t)n_tokens * n_heads > 0x7fffffff || window < 0 || !isfinite(scale))
         return fail(RABBIT_CUDA_ERR_ARGS,
                     "kv4_attention: NULL cache, scratch or batch, a bad layer, dtype, count, scale or "
                     "window, or n_heads not a multiple of n_kv_heads");
@@ -157,7 +165,9 @@ int rabbit_cuda_kv4_attention_dev(rabbit_cuda_kv4 *kv, int layer, rabbit_cuda_kv
     a.os = out_stride ? out_stride : row;
     if (!d_q || !d_out || !b->d_kv_len || (!b->d_page_table && b->max_pages) || a.qs < row ||
         a.os < row || (reinterpret_cast<uintptr_t>(d_q) & (size - 1)) ||
-        (reinterpret_cast<uintptr_t>(d_out) & (size - 1)) || (d_q == d_out && a.qs != a.os))
+        (reinterpret_cast<uintptr_t>(d_out) & (size - 1)) ||
+        ((reinterpret_cast<uintptr_t>(b->d_q_start) | reinterpret_cast<uintptr_t>(b->d_kv_len) |
+          reinterpret_cast<uintptr_t>(b->d_page_table)) & 3) || (d_q == d_out && a.qs != a.os))
         return fail(RABBIT_CUDA_ERR_ARGS,
                     "kv4_attention: NULL pointer, a stride below n_heads * head_dim (or different in "
                     "place), or a pointer not aligned to its element");
@@ -169,6 +179,7 @@ int rabbit_cuda_kv4_attention_dev(rabbit_cuda_kv4 *kv, int layer, rabbit_cuda_kv
     a.n_seqs = b->n_seqs;
     a.max_pages = b->max_pages;
     a.max_q = b->max_q_len ? b->max_q_len : 1;
+    if (a.max_q > n_tokens) a.max_q = n_tokens;
     a.T = n_tokens;
     a.nh = n_heads;
     a.window = window;

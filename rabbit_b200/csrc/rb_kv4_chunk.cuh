@@ -13,10 +13,12 @@
 // weights: w = 2^(x - M + ev), with the reference M as in rb_kv4_decode.cuh).
 // Only the weights are rounded.
 //
-// Bound by the matrix instructions: 64 rows x 64 positions x 128 channels are 128
-// of them a warp, 8 cycles each on a sub-partition, beside some 90 cycles a warp
-// of the making. 256 rows x 4 heads a KV head over 4352 positions of 8 KV heads:
-// 128 CTAs.
+// Bound by the latency of the two kinds of warps, not yet by the matrix
+// instructions: 64 rows x 64 positions x 128 channels are 512 of those, 1024 cycles
+// of the four sub-partitions; a tile takes some 2500. With 4 warps of either kind
+// 119 us (256 rows x 4 heads a KV head over 4352 positions of 8 KV heads, bf16, 128
+// CTAs), 8 making 130 us (the others then spilled), 8 multiplying 122 us, 8 of
+// either 91 us: 194 TFLOP/s, 0.12 of the measured cuBLAS bf16 rate.
 #pragma once
 #include <type_traits>
 
@@ -146,79 +148,79 @@ __global__ void __launch_bounds__(ChunkCfg<NG>::kThreads, 1) k_kv4_chunk(const _
             uint8_t *vt = kt + C::kTile * C::kStride;
             constexpr int NW = (NG + 1) / 2;
             auto make = [&](auto part) {
-            constexpr bool values = decltype(part)::value;
-            // the largest finite scale, and whether all are finite
-            const uint16_t *scales = reinterpret_cast<const uint16_t *>(gr + (values ? kv4_vs(NG) : kv4_ks(NG)));
-            uint32_t top = 0, any = 0;
-            if (there)
-                for (int i = lane; i < 16 * NG; i += 32) {
-                    const uint32_t x = scales[i];
-                    top = max(top, x < 0x7f80u ? x : 0u);
-                    any |= x >= 0x7f80u;
-                }
-            top = __reduce_max_sync(0xffffffffu, top);
-            const int e = min(max((int)(top >> 7) - 127, -100), 126);
-            const float down = __uint_as_float((uint32_t)(127 - e) << 23);
-            if constexpr (!values) {
-                if (lane == 0) {
-                    meta[mt][w].kscale = __uint_as_float((uint32_t)(127 + e) << 23);
-                    meta[mt][w].there = there;
-                }
+                constexpr bool values = decltype(part)::value;
+                // the largest finite scale, and whether all are finite
+                const uint16_t *scales = reinterpret_cast<const uint16_t *>(gr + (values ? kv4_vs(NG) : kv4_ks(NG)));
+                uint32_t top = 0, any = 0;
+                if (there)
+                    for (int i = lane; i < 16 * NG; i += 32) {
+                        const uint32_t x = scales[i];
+                        top = max(top, x < 0x7f80u ? x : 0u);
+                        any |= x >= 0x7f80u;
+                    }
+                top = __reduce_max_sync(0xffffffffu, top);
+                const int e = min(max((int)(top >> 7) - 127, -100), 126);
+                const float down = __uint_as_float((uint32_t)(127 - e) << 23);
+                if constexpr (!values) {
+                    if (lane == 0) {
+                        meta[mt][w].kscale = __uint_as_float((uint32_t)(127 + e) << 23);
+                        meta[mt][w].there = there;
+                    }
 #pragma unroll
-                for (int x = 0; x < 2; ++x) {  // word t of a token's groups
-                    const int j = (lane >> 2) + 8 * x, t = lane & 3;
-                    uint32_t kw[NG], sc[NW];
-                    load_piece<4 * NG>(kw, gr + j * kv4_row(NG) + t * 4 * NG);
-                    load_piece<2 * NG>(sc, scales + j * NG);
+                    for (int x = 0; x < 2; ++x) {  // word t of a token's groups
+                        const int j = (lane >> 2) + 8 * x, t = lane & 3;
+                        uint32_t kw[NG], sc[NW];
+                        load_piece<4 * NG>(kw, gr + j * kv4_row(NG) + t * 4 * NG);
+                        load_piece<2 * NG>(sc, scales + j * NG);
 #pragma unroll
-                    for (int grp = 0; grp < NG; ++grp) {
-                        uint32_t y[4];
-                        key_codes<true>(y, kw[grp]);  // nibbles (0, 4), (2, 6), (1, 5), (3, 7)
-                        const __half2 f = __float2half2_rn(piece_bf16(sc, grp) * down);
-                        *reinterpret_cast<uint4 *>(kt + j * C::kStride + 2 * (32 * grp + 8 * t)) =
-                            there ? make_uint4(mul_f16(y[0], f), mul_f16(y[2], f), mul_f16(y[1], f), mul_f16(y[3], f))
-                                  : make_uint4(0, 0, 0, 0);
+                        for (int grp = 0; grp < NG; ++grp) {
+                            uint32_t y[4];
+                            key_codes<true>(y, kw[grp]);  // nibbles (0, 4), (2, 6), (1, 5), (3, 7)
+                            const __half2 f = __float2half2_rn(piece_bf16(sc, grp) * down);
+                            *reinterpret_cast<uint4 *>(kt + j * C::kStride + 2 * (32 * grp + 8 * t)) =
+                                there ? make_uint4(mul_f16(y[0], f), mul_f16(y[2], f), mul_f16(y[1], f), mul_f16(y[3], f))
+                                      : make_uint4(0, 0, 0, 0);
+                        }
+                    }
+                } else {
+                    const bool odd = __any_sync(0xffffffffu, any);
+                    if (lane == 0) {
+                        meta[mt][w].ev = (float)e;
+                        meta[mt][w].vback = down;
+                        meta[mt][w].odd = odd;
+                    }
+                    if (odd && lane < 16) {
+                        int mask = 0;
+#pragma unroll
+                        for (int grp = 0; grp < NG; ++grp) mask |= (scales[lane * NG + grp] >= 0x7f80u) << grp;
+                        vbad[mt][16 * w + lane] = (uint8_t)mask;
+                    }
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) {  // word g of a token's groups
+                        const int j = (lane >> 3) + 4 * x, g = lane & 7;
+                        uint32_t vw[NW], sc[NW];
+                        load_piece<2 * NG>(vw, gr + kv4_v(NG) + j * kv4_row(NG) + kv4_vplace(j, g) * 2 * NG);
+                        load_piece<2 * NG>(sc, scales + j * NG);
+#pragma unroll
+                        for (int i = 0; i < NW; ++i) {  // two groups at a time, one in each half of a pair
+                            const uint32_t h = vw[i], h8 = h >> 8;
+                            // (a value that is not finite is put into the output by itself)
+                            const float s0 = piece_bf16(sc, 2 * i), s1 = 2 * i + 1 < NG ? piece_bf16(sc, 2 * i + 1) : 0.f;
+                            const __half2 f = __floats2half2_rn(s0 < INFINITY ? s0 * down : 0.f, s1 < INFINITY ? s1 * down : 0.f);
+                            uint32_t y[4];
+                            signed_codes(y[0], y[1], h);
+                            signed_codes(y[2], y[3], h8);
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) y[k] = there ? mul_f16(y[k], f) : 0u;
+                            uint8_t *to = vt + j * C::kStride + 2 * (64 * i + 4 * g);
+                            *reinterpret_cast<uint2 *>(to) =
+                                make_uint2(__byte_perm(y[0], y[1], 0x5410), __byte_perm(y[2], y[3], 0x5410));
+                            if (2 * i + 1 < NG)
+                                *reinterpret_cast<uint2 *>(to + 64) =
+                                    make_uint2(__byte_perm(y[0], y[1], 0x7632), __byte_perm(y[2], y[3], 0x7632));
+                        }
                     }
                 }
-            } else {
-                const bool odd = __any_sync(0xffffffffu, any);
-                if (lane == 0) {
-                    meta[mt][w].ev = (float)e;
-                    meta[mt][w].vback = down;
-                    meta[mt][w].odd = odd;
-                }
-                if (odd && lane < 16) {
-                    int mask = 0;
-#pragma unroll
-                    for (int grp = 0; grp < NG; ++grp) mask |= (scales[lane * NG + grp] >= 0x7f80u) << grp;
-                    vbad[mt][16 * w + lane] = (uint8_t)mask;
-                }
-#pragma unroll
-                for (int x = 0; x < 4; ++x) {  // word g of a token's groups
-                    const int j = (lane >> 3) + 4 * x, g = lane & 7;
-                    uint32_t vw[NW], sc[NW];
-                    load_piece<2 * NG>(vw, gr + kv4_v(NG) + j * kv4_row(NG) + kv4_vplace(j, g) * 2 * NG);
-                    load_piece<2 * NG>(sc, scales + j * NG);
-#pragma unroll
-                    for (int i = 0; i < NW; ++i) {  // two groups at a time, one in each half of a pair
-                        const uint32_t h = vw[i], h8 = h >> 8;
-                        // (a value that is not finite is put into the output by itself)
-                        const float s0 = piece_bf16(sc, 2 * i), s1 = 2 * i + 1 < NG ? piece_bf16(sc, 2 * i + 1) : 0.f;
-                        const __half2 f = __floats2half2_rn(s0 < INFINITY ? s0 * down : 0.f, s1 < INFINITY ? s1 * down : 0.f);
-                        uint32_t y[4];
-                        signed_codes(y[0], y[1], h);
-                        signed_codes(y[2], y[3], h8);
-#pragma unroll
-                        for (int k = 0; k < 4; ++k) y[k] = there ? mul_f16(y[k], f) : 0u;
-                        uint8_t *to = vt + j * C::kStride + 2 * (64 * i + 4 * g);
-                        *reinterpret_cast<uint2 *>(to) =
-                            make_uint2(__byte_perm(y[0], y[1], 0x5410), __byte_perm(y[2], y[3], 0x5410));
-                        if (2 * i + 1 < NG)
-                            *reinterpret_cast<uint2 *>(to + 64) =
-                                make_uint2(__byte_perm(y[0], y[1], 0x7632), __byte_perm(y[2], y[3], 0x7632));
-                    }
-                }
-            }
             };
             make(std::false_type());
             make(std::true_type());

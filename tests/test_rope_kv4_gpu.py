@@ -68,6 +68,8 @@ ROPES = [
     ("f32", 2, 3, 1024, 512, "half", 9000, 4, 0, False),
     ("bf16", 1000, 1, 64, 64, "interleaved", 40000, 0, 0, True),
     ("bf16", 2, 3, 66, 66, "interleaved", 40000, 0, 0, False),
+    ("f16", 19001, 1, 512, 512, "half", 100000, 0, 0, True),  # many tokens a CTA, the largest table
+    ("f32", 5000, 2, 64, 32, "interleaved", 9000, 0, 0, False),
 ]
 
 
@@ -268,6 +270,8 @@ def test_wrong_rope_layer_and_pointers_are_refused(torch, rc):
            lambda: kv.attention_dev(0, ws, rc.F32, p, p, 1, 0, b),
            lambda: kv.attention_dev(0, ws, rc.F32, p, p, 1, 1, b, q_stride=128),
            lambda: kv.attention_dev(0, ws, rc.F32, p, p, -1, 1, b),
+           lambda: kv.attention_dev(0, ws, rc.F32, p, p, 1 << 16, 1 << 15, b),
+           lambda: kv.attention_dev(0, ws, rc.F32, p, p, 1, 1, rc.Kv4Batch(n_seqs=1, d_kv_len=sp + 2)),
            lambda: kv.attention_dev(0, ws, rc.F32, p, p, 1, 1, rc.Kv4Batch(n_seqs=1, max_pages=1)),
            lambda: kv.attention_dev(0, ws, rc.F32, p, p, 1, 1, rc.Kv4Batch(n_seqs=-1, d_kv_len=sp))]
     for call in bad:
@@ -427,6 +431,14 @@ ATTN = [
     dict(dtype="bf16", nh=48, nkv=8, hd=128, page=64, lens=[333, 77], qs=[77, 77], gap=8, scale=0.2),
     dict(dtype="f16", nh=8, nkv=8, hd=40, page=16, lens=[700], qs=[320], q_gain=30.0),
     dict(dtype="bf16", nh=16, nkv=16, hd=8, page=16, lens=[150], qs=[150], q_gain=1e-3),
+    # few chunks among many sequences of one row
+    dict(dtype="bf16", nh=8, nkv=8, hd=64, page=16, lens=[200] + [30 + i for i in range(20)], qs=[150] + [1] * 20),
+    dict(dtype="f16", nh=8, nkv=4, hd=128, page=16, lens=[300, 200, 9, 40], qs=[150, 150, 1, 1], window=130),
+    # more sequences than a CTA has threads, among them many that have not begun
+    dict(dtype="bf16", nh=2, nkv=1, hd=32, page=16, lens=[(7 * i) % 61 * (i % 5 > 0) for i in range(700)], pad=1),
+    dict(dtype="f32", nh=1, nkv=1, hd=160, page=16, lens=[(11 * i) % 37 for i in range(300)]),
+    dict(dtype="f16", nh=4, nkv=2, hd=64, page=16, lens=[5 + i % 90 for i in range(600)],
+         qs=[1 + i % 3 for i in range(600)]),
     # a long sequence beside short ones: split over many SMs
     dict(dtype="bf16", nh=8, nkv=2, hd=128, page=64, lens=[9000, 1, 0, 200], poison=False),
     dict(dtype="f32", nh=4, nkv=1, hd=64, page=16, lens=[6000], poison=False),
