@@ -632,3 +632,37 @@ def test_a_decode_step_of_the_three_together(torch, rc):
                 # the worst case; the bar below is 2^-14 of the largest value, 16 times what
                 # such sums of random signs (sqrt(64) instead of 64 terms) come to
                 assert np.abs(got[i, h] - want[0]).max() <= 2.0 ** -14 * 5
+
+
+@pytest.mark.parametrize("page", [48, 64])
+def test_a_cache_past_32_bits_of_bytes(torch, rc, page):
+    """The last pages of a layer of more than 2^32 bytes hold what a small cache's do."""
+    nkv, hd, n = 8, 128, 3 * page - 5
+    big = 2 ** 32 // (page // 16 * nkv * 2304) + 100
+    g = torch.Generator("cuda").manual_seed(5)
+    k, v = (torch.randn(n, nkv, hd, generator=g, device="cuda") for _ in "kv")
+    outs = []
+    for n_pages in (3, big):
+        kv = rc.Kv4(n_layers=1, n_kv_heads=nkv, head_dim=hd, page_size=page, n_pages=n_pages)
+        ws, st = rc.Kv4Scratch(kv), stream(torch)
+        slots = torch.arange(n, device="cuda") + (n_pages - 3) * page
+        kv.append_dev(0, rc.F32, k.data_ptr(), v.data_ptr(), slots.data_ptr(), n, stream=st)
+        read = torch.zeros(2, n, nkv, hd, device="cuda")
+        kv.read_dev(0, rc.F32, slots.data_ptr(), n, read[0].data_ptr(), read[1].data_ptr(), stream=st)
+        got = [read]
+        table = torch.arange(n_pages - 3, n_pages, dtype=torch.int32, device="cuda")
+        length = torch.tensor([n], dtype=torch.int32, device="cuda")
+        for rows, heads in ((1, 16), (n, 40)):  # a decoding token, a chunk
+            start = torch.tensor([0, rows], dtype=torch.int32, device="cuda")
+            q = torch.randn(rows, heads, hd, generator=torch.Generator("cuda").manual_seed(6),
+                            device="cuda").half()
+            out = torch.empty_like(q)
+            b = rc.Kv4Batch(n_seqs=1, max_pages=3, max_q_len=rows, d_q_start=start.data_ptr(),
+                            d_kv_len=length.data_ptr(), d_page_table=table.data_ptr())
+            kv.attention_dev(0, ws, rc.F16, q.data_ptr(), out.data_ptr(), rows, heads, b, stream=st)
+            got.append(out)
+        kv.check(st)
+        outs.append(got)
+    assert np.array_equal(f64(outs[0][0][0]), ko.hold(f64(k))[0])
+    for small, large in zip(*outs):
+        assert torch.equal(small, large)
