@@ -497,12 +497,15 @@ __global__ void __launch_bounds__(DecodeCfg<NG, RB, SPLIT>::kThreads, 1)
         bool has = next_step(a, G, C::kRows, W, w, d, now, seq);
         if (has && d.owner < 0) load_rows<NG, RB, SPLIT>(a, d, G, x8);
         int asked_n = 0, seen_n = 0, merged_n = 0;  // steps made; steps looked at for a merge; merges
+        // A barrier may have turned for one lane's test and not yet for another's: the
+        // shuffles, votes and counters behind a test need one answer for the warp.
+        auto turned = [](uint64_t *bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_test(bar, parity)); };
         for (uint64_t t0 = 0; has || seen_n < asked_n;) {
             bool did = false;
             // Step asked_n, once its buffer's last step is done with (and merged)
             const int buf = asked_n % K;
             if (has && asked_n - seen_n < K &&
-                (asked_n < K || mbar_test(&done[buf], (asked_n / K - 1) & 1))) {
+                (asked_n < K || turned(&done[buf], (asked_n / K - 1) & 1))) {
                 did = true;
                 if (d.owner < 0)
                     make_operands<NG, RB, SPLIT>(a, queries + buf * C::kQuery, unit[buf], x8);
@@ -518,7 +521,7 @@ __global__ void __launch_bounds__(DecodeCfg<NG, RB, SPLIT>::kThreads, 1)
                 if (st.owner >= 0) {
                     ++seen_n;
                     did = true;
-                } else if (mbar_test(&left, merged_n & 1)) {
+                } else if (turned(&left, merged_n & 1)) {
                     // the warps' outputs, in their order; lane r has row r's factors
                     did = true;
                     const DecodeStep m = st;
@@ -587,6 +590,7 @@ __global__ void __launch_bounds__(DecodeCfg<NG, RB, SPLIT>::kThreads, 1)
                                 p[5] = m.rho0;
                             }
                         }
+                        __syncwarp();
                     }
                     ++merged_n;
                     ++seen_n;
