@@ -612,6 +612,10 @@ int rabbit_cuda_kv4_attention_dev(rabbit_cuda_kv4 *kv, int layer, rabbit_cuda_kv
  * of range since the last check (RABBIT_CUDA_ERR_ARGS) or a bounded wait that
  * gave up (RABBIT_CUDA_ERR_TIMEOUT). */
 int rabbit_cuda_kv4_check(rabbit_cuda_kv4 *kv, void *stream);
+/* Test hook: the next attention call on `kv` leaves out one arrival inside a CTA, so
+ * that waits in it run out; it ends with RABBIT_CUDA_ERR_TIMEOUT in the check,
+ * rows of it not written, and its scratch spoiled. */
+int rabbit_cuda_kv4_debug_withhold(rabbit_cuda_kv4 *kv);
 
 #if defined(__GNUC__)
 #pragma GCC visibility pop

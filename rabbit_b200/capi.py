@@ -152,6 +152,7 @@ SIGNATURES = {
     "rabbit_cuda_kv4_attention_dev": (_I, [_P, _I, _P, _I, _P, _L, _P, _L, _I, _I,
                                            C.POINTER(Kv4Batch), C.c_float, _I, _P]),
     "rabbit_cuda_kv4_check": (_I, [_P, _P]),
+    "rabbit_cuda_kv4_debug_withhold": (_I, [_P]),
 }
 
 _LIB: C.CDLL | None = None

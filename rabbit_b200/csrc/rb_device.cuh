@@ -151,6 +151,19 @@ __device__ __forceinline__ void wait_prerequisite() {
 __device__ __forceinline__ void named_sync(int id, int threads) {
     asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
 }
+// The same; true for all of them if `ok` is for each.
+__device__ __forceinline__ bool named_all(int id, int threads, bool ok) {
+    uint32_t all;
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t"
+        "setp.ne.u32 q, %3, 0;\n\t"
+        "bar.red.and.pred p, %1, %2, q;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(all)
+        : "r"(id), "r"(threads), "r"((uint32_t)ok)
+        : "memory");
+    return all != 0;
+}
 
 // ------------------------------------------------------- int4 dot product --
 // The 32 activations of one group are turned into a 23-bit block-floating-

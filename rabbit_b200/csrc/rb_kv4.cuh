@@ -83,6 +83,7 @@ struct rabbit_cuda_kv4 {
     rb::Kv4View view = {};      // of layer 0
     size_t layer_bytes = 0;
     int *d_err = nullptr;
+    bool withhold = false;      // test hook for the next attention
     rb::Kv4View layer(int l) const {
         rb::Kv4View v = view;
         v.base += (size_t)l * layer_bytes;

@@ -190,12 +190,20 @@ int rabbit_cuda_kv4_attention_dev(rabbit_cuda_kv4 *kv, int layer, rabbit_cuda_kv
     a.part = ws->part;
     a.count = ws->count;
     a.wait_ns = wait_limit_ns();
+    a.withhold = kv->withhold;
+    kv->withhold = false;
     DeviceScope scope(kv->device);
     if (scope.status != RABBIT_CUDA_OK) return scope.status;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     scope.launch(dtype == RABBIT_CUDA_F32 ? launch_attention<true>(a, kv, s) : launch_attention<false>(a, kv, s),
                  "kv4_attention");
     return scope.done();
+}
+
+int rabbit_cuda_kv4_debug_withhold(rabbit_cuda_kv4 *kv) {
+    if (!kv) return fail(RABBIT_CUDA_ERR_ARGS, "kv4_debug_withhold: NULL cache");
+    kv->withhold = true;
+    return ok();
 }
 
 }  // extern "C"

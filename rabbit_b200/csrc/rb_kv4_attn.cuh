@@ -21,7 +21,14 @@ struct Kv4AttnArgs {
     float *part;     // scratch: partial outputs [2 grid][rows][channels], then [2 grid][rows] pairs
     unsigned *count; // scratch: arrivals per CTA that begins a shared item, zero between calls
     uint64_t wait_ns;
+    bool withhold;   // test hook: one arrival is left out
 };
+
+// A CTA whose wait ran out leaves its work where it is: it makes no further arrival
+// (what waits for one runs out as well) and starts no further copy, and lets its copies
+// in flight, which write its shared memory, end before it does. They take
+// microseconds; this bounds that wait whatever the caller's limit is.
+constexpr uint64_t kKv4DrainNs = 2000000000ull;
 
 constexpr int kKv4MaxLen = 1 << 30;  // positions of a sequence: sums of two stay within an int
 

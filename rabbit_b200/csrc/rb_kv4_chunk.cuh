@@ -140,9 +140,10 @@ __global__ void __launch_bounds__(ChunkCfg<NG>::kThreads, 1) k_kv4_chunk(const _
         }
         for (int tile = turn; tile < tiles; tile += 2) {
             const int st = tile % C::kRaw, mt = tile % C::kMade;
-            if (ok) ok = mbar_wait(&raw_full[st], (tile / C::kRaw) & 1, a.wait_ns, c.err, 64);
+            ok = mbar_wait(&raw_full[st], (tile / C::kRaw) & 1, a.wait_ns, c.err, 64);
             if (tile >= C::kMade && ok) ok = mbar_wait(&used[mt], (tile / C::kMade - 1) & 1, a.wait_ns, c.err, 64);
-            const bool there = ok && (raw_there[st] >> w & 1);
+            ok = __all_sync(0xffffffffu, ok);
+            const bool there = raw_there[st] >> w & 1;
             const uint8_t *gr = smem + st * C::kRawBytes + w * kv4_bytes(NG);
             uint8_t *kt = smem + C::kRaw * C::kRawBytes + mt * C::kMadeBytes + (size_t)w * 16 * C::kStride;
             uint8_t *vt = kt + C::kTile * C::kStride;
@@ -222,17 +223,22 @@ __global__ void __launch_bounds__(ChunkCfg<NG>::kThreads, 1) k_kv4_chunk(const _
                     }
                 }
             };
-            make(std::false_type());
-            make(std::true_type());
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&made[mt]);
-            named_sync(3 + turn, 128);  // the raw stage is read
+            if (ok) {
+                make(std::false_type());
+                make(std::true_type());
+                __syncwarp();
+                if (lane == 0 && !(a.withhold && tile == 0 && w == 0)) mbar_arrive(&made[mt]);
+            }
+            // the raw stage is read, by all four warps, or one's wait ran out
+            ok = named_all(3 + turn, 128, ok);
+            if (!ok) {
+                if (w == 0)  // the copies of this tile and those fetched ahead of it
+                    for (int i = tile; i < min(tile + C::kRaw, tiles); i += 2)
+                        mbar_wait(&raw_full[i % C::kRaw], (i / C::kRaw) & 1, kKv4DrainNs, nullptr, 0);
+                return;
+            }
             if (w == 0 && tile + C::kRaw < tiles) fetch(tile + C::kRaw);
         }
-        if (!ok && w == 0)  // after a wait that ran out: copies in flight end before the CTA does
-            for (int i = max(0, tiles - C::kRaw); i < tiles; ++i)
-                if ((i & 1) == turn)
-                    mbar_wait(&raw_full[i % C::kRaw], (i / C::kRaw) & 1, a.wait_ns, nullptr, 0);
         return;
     }
 
@@ -291,7 +297,8 @@ __global__ void __launch_bounds__(ChunkCfg<NG>::kThreads, 1) k_kv4_chunk(const _
     const uint32_t vat = ((lane & 7) + ((lane >> 3) & 1) * 8) * C::kStride + (lane >> 4) * 16;
     for (int tile = turn; tile < tiles; tile += 2) {
         const int mt = tile % C::kMade, p0 = (g0 + 4 * tile) * kKv4Granule;
-        if (ok) ok = mbar_wait(&made[mt], (tile / C::kMade) & 1, a.wait_ns, c.err, 64);
+        ok = __all_sync(0xffffffffu, mbar_wait(&made[mt], (tile / C::kMade) & 1, a.wait_ns, c.err, 64));
+        if (!ok) break;
         const uint32_t kt = tiles_at + mt * (uint32_t)C::kMadeBytes, vt = kt + C::kTile * C::kStride;
         float sc[8][4];
 #pragma unroll
@@ -405,7 +412,7 @@ __global__ void __launch_bounds__(ChunkCfg<NG>::kThreads, 1) k_kv4_chunk(const _
         l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
     }
     // the odd tiles' part joins the even tiles'
-    named_sync(2, 32 * C::kMul);  // all fp16 tiles are read
+    if (!named_all(2, 32 * C::kMul, ok)) return;  // all fp16 tiles are read, or a wait ran out
     float *part = reinterpret_cast<float *>(smem + C::kRaw * C::kRawBytes) + wr * 32 * (4 + 16 * NG) + lane;
     if (turn == 1) {
 #pragma unroll

@@ -485,7 +485,7 @@ __global__ void __launch_bounds__(DecodeCfg<NG, RB, SPLIT>::kThreads, 1)
         }
         // copies in flight end before the CTA does, also where a wait ran out
         for (int i = max(0, issued - C::SL); i < issued; ++i)
-            mbar_wait(&full[lane + 32 * (i % C::SL)], (i / C::SL) & 1, a.wait_ns, nullptr, 0);
+            mbar_wait(&full[lane + 32 * (i % C::SL)], (i / C::SL) & 1, kKv4DrainNs, nullptr, 0);
     } else if (warp == W + 1) {
         // ---- operands of the coming steps, as far ahead as there is room, and merges
         DecodeWalk w;
@@ -511,7 +511,7 @@ __global__ void __launch_bounds__(DecodeCfg<NG, RB, SPLIT>::kThreads, 1)
                     make_operands<NG, RB, SPLIT>(a, queries + buf * C::kQuery, unit[buf], x8);
                 if (lane == 0) steps[buf] = d;
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&asked[buf]);
+                if (lane == 0 && !(a.withhold && blockIdx.x == 0 && asked_n == 0)) mbar_arrive(&asked[buf]);
                 ++asked_n;
                 has = next_step(a, G, C::kRows, W, w, d, now, seq);
                 if (has && d.owner < 0) load_rows<NG, RB, SPLIT>(a, d, G, x8);
@@ -843,7 +843,8 @@ __global__ void __launch_bounds__(DecodeCfg<NG, RB, SPLIT>::kThreads, 1)
             // warp after another, and a barrier tells only a phase from the next: a warp
             // ahead of the slot's earlier granules would take an older phase for its own.
             // So it looks for its round's tag first, which is written once the round
-            // before is over.
+            // before is over. The lanes leave with one answer: after a wait that ran out
+            // all of them have ok false.
             auto arrived = [&](int n) -> bool {
                 const volatile int *at = &tag[n % S];
                 int v = *at;
@@ -858,7 +859,8 @@ __global__ void __launch_bounds__(DecodeCfg<NG, RB, SPLIT>::kThreads, 1)
                     }
                 }
                 if (ok) ok = mbar_wait(&full[n % S], (n / S) & 1, a.wait_ns, c.err);
-                return ok && (v & 1);
+                ok = __all_sync(0xffffffffu, ok);
+                return v & 1;
             };
             // (A warp that holds a granule's slot waits only for one less than S after it:
             // the first granule that is waited for and not yet fetched never waits for a
@@ -868,11 +870,13 @@ __global__ void __launch_bounds__(DecodeCfg<NG, RB, SPLIT>::kThreads, 1)
                 Scores cur;
                 {
                     const bool there = arrived(n);
+                    if (!ok) break;
                     score(smem + n % S * kv4_bytes(NG), cur);
                     settle(cur, p00 + n * kKv4Granule, there);
                 }
                 for (int nx = n + by; nx < end; nx += by) {
                     const bool there = arrived(nx);
+                    if (!ok) break;
                     Scores nxt;
                     score(smem + nx % S * kv4_bytes(NG), nxt);
                     output(smem + n % S * kv4_bytes(NG), cur, &empty[n % S]);
@@ -880,6 +884,7 @@ __global__ void __launch_bounds__(DecodeCfg<NG, RB, SPLIT>::kThreads, 1)
                     cur = nxt;
                     n = nx;
                 }
+                if (!ok) break;
                 output(smem + n % S * kv4_bytes(NG), cur, &empty[n % S]);
             }
 #pragma unroll

@@ -1,5 +1,5 @@
-"""GPU: the paged 4-bit cache and its attention at their edges: many items a
-CTA, against float64 numpy (tests/kv4_oracle.py)."""
+"""GPU: the paged 4-bit cache and its attention at their edges: many items a CTA,
+waits that run out, against float64 numpy (tests/kv4_oracle.py)."""
 from __future__ import annotations
 
 import numpy as np
@@ -27,3 +27,30 @@ def test_many_items_of_all_lengths_in_a_cta(torch, rc, dtype, nh):
         c.call()
         assert torch.equal(c.out, first)
     c.kv.check(base.stream(torch))
+
+
+@pytest.mark.parametrize("kw", [
+    dict(dtype="bf16", nh=8, nkv=2, hd=128, page=16, lens=[9000, 40, 700], poison=False),
+    dict(dtype="f32", nh=4, nkv=4, hd=64, page=16, lens=[255]),
+    dict(dtype="f32", nh=2, nkv=1, hd=256, page=16, lens=[40] * 300),          # short items first
+    dict(dtype="bf16", nh=8, nkv=2, hd=128, page=32, lens=[400, 90], qs=[5, 7]),
+    dict(dtype="f16", nh=8, nkv=8, hd=64, page=16, lens=[1500], qs=[640]),     # chunks: more tiles than stages
+    dict(dtype="bf16", nh=16, nkv=16, hd=128, page=16, lens=[150], qs=[300]),  # and fewer
+])
+def test_a_wait_that_runs_out_is_a_status(torch, rc, kw):
+    """One arrival is withheld, so waits of a CTA run out: the launch ends, the check
+    says so once, and the next call, with a new scratch, is right."""
+    c = base.Case(torch, rc, seed=41, **kw)
+    spoiled = rc.Kv4Scratch(c.kv)
+    try:
+        rc.check(rc.lib().rabbit_cuda_set_wait_limit_us(20000))
+        rc.check(rc.lib().rabbit_cuda_kv4_debug_withhold(c.kv.handle))
+        c.call(ws=spoiled)
+        with pytest.raises(rc.RabbitCudaError) as e:
+            c.kv.check(base.stream(torch))
+        assert e.value.status == rc.ERR_TIMEOUT
+    finally:
+        rc.check(rc.lib().rabbit_cuda_set_wait_limit_ms(2000))
+    c.kv.check(base.stream(torch))  # said once
+    c.call()
+    c.check()
