@@ -479,12 +479,13 @@ int rabbit_cuda_kv4_check(rabbit_cuda_kv4 *kv, void *stream) {
     if (h == 0) return ok();
     RB_CUDA(cudaMemsetAsync(kv->d_err, 0, sizeof(int), s));
     RB_CUDA(cudaStreamSynchronize(s));
-    if (h & (RB_KV4_ERR_SLOT | RB_KV4_ERR_PAGE | RB_KV4_ERR_LEN | RB_KV4_ERR_ROWS))
-        return fail(RABBIT_CUDA_ERR_ARGS, "kv4: out of range on the device:%s%s%s%s",
-                    h & RB_KV4_ERR_SLOT ? " slot" : "", h & RB_KV4_ERR_PAGE ? " page" : "",
-                    h & RB_KV4_ERR_LEN ? " kv_len" : "", h & RB_KV4_ERR_ROWS ? " q_start" : "");
-    return h & 15 ? fail(RABBIT_CUDA_ERR_TIMEOUT, "kv4: a bounded device wait ran out")
-                  : fail(RABBIT_CUDA_ERR_DEVICE, "kv4: device error code %d", h);
+    // the timeout first: after it the caller has to replace a scratch
+    const int range = h & (RB_KV4_ERR_SLOT | RB_KV4_ERR_PAGE | RB_KV4_ERR_LEN | RB_KV4_ERR_ROWS);
+    return fail(h & RB_KV4_ERR_WAIT ? RABBIT_CUDA_ERR_TIMEOUT : RABBIT_CUDA_ERR_ARGS, "kv4: %s%s%s%s%s%s",
+                h & RB_KV4_ERR_WAIT ? "a bounded device wait ran out; " : "",
+                range ? "out of range on the device:" : "", h & RB_KV4_ERR_SLOT ? " slot" : "",
+                h & RB_KV4_ERR_PAGE ? " page" : "", h & RB_KV4_ERR_LEN ? " kv_len" : "",
+                h & RB_KV4_ERR_ROWS ? " q_start" : "");
 }
 
 }  // extern "C"

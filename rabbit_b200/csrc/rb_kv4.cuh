@@ -45,11 +45,12 @@ __host__ __device__ constexpr int kv4_bytes(int ng) { return 576 * ng; }
 // Place of V piece g of token j.
 __host__ __device__ constexpr int kv4_vplace(int j, int g) { return g ^ ((j & 2) << 1); }
 
-// Error bits of a cache's error word (RB_ERR_TIMEOUT of the bounded waits is 7).
+// Error bits of a cache's error word; set by atomicOr, so none hides another.
 #define RB_KV4_ERR_SLOT 16
 #define RB_KV4_ERR_PAGE 32
 #define RB_KV4_ERR_LEN 64
 #define RB_KV4_ERR_ROWS 128
+#define RB_KV4_ERR_WAIT 256  // a bounded wait ran out
 
 // One layer of a cache as the kernels see it.
 struct Kv4View {

@@ -5,6 +5,7 @@
 #include <cuda_fp16.h>
 #include <stdint.h>
 
+#include "rb_device.cuh"
 #include "rb_kv4.cuh"
 
 namespace rb {
@@ -29,6 +30,15 @@ struct Kv4AttnArgs {
 // in flight, which write its shared memory, end before it does. They take
 // microseconds; this bounds that wait whatever the caller's limit is.
 constexpr uint64_t kKv4DrainNs = 2000000000ull;
+
+#ifdef __CUDACC__
+// Wait for a phase of a CTA's barrier; false, and reported, after the call's limit.
+__device__ __forceinline__ bool kv4_wait(uint64_t *bar, uint32_t parity, const Kv4AttnArgs &a, uint32_t max_sleep_ns = 256) {
+    if (mbar_wait(bar, parity, a.wait_ns, nullptr, max_sleep_ns)) return true;
+    atomicOr(a.c.err, RB_KV4_ERR_WAIT);
+    return false;
+}
+#endif
 
 constexpr int kKv4MaxLen = 1 << 30;  // positions of a sequence: sums of two stay within an int
 

@@ -140,8 +140,8 @@ __global__ void __launch_bounds__(ChunkCfg<NG>::kThreads, 1) k_kv4_chunk(const _
         }
         for (int tile = turn; tile < tiles; tile += 2) {
             const int st = tile % C::kRaw, mt = tile % C::kMade;
-            ok = mbar_wait(&raw_full[st], (tile / C::kRaw) & 1, a.wait_ns, c.err, 64);
-            if (tile >= C::kMade && ok) ok = mbar_wait(&used[mt], (tile / C::kMade - 1) & 1, a.wait_ns, c.err, 64);
+            ok = kv4_wait(&raw_full[st], (tile / C::kRaw) & 1, a, 64);
+            if (tile >= C::kMade && ok) ok = kv4_wait(&used[mt], (tile / C::kMade - 1) & 1, a, 64);
             ok = __all_sync(0xffffffffu, ok);
             const bool there = raw_there[st] >> w & 1;
             const uint8_t *gr = smem + st * C::kRawBytes + w * kv4_bytes(NG);
@@ -297,7 +297,7 @@ __global__ void __launch_bounds__(ChunkCfg<NG>::kThreads, 1) k_kv4_chunk(const _
     const uint32_t vat = ((lane & 7) + ((lane >> 3) & 1) * 8) * C::kStride + (lane >> 4) * 16;
     for (int tile = turn; tile < tiles; tile += 2) {
         const int mt = tile % C::kMade, p0 = (g0 + 4 * tile) * kKv4Granule;
-        ok = __all_sync(0xffffffffu, mbar_wait(&made[mt], (tile / C::kMade) & 1, a.wait_ns, c.err, 64));
+        ok = __all_sync(0xffffffffu, kv4_wait(&made[mt], (tile / C::kMade) & 1, a, 64));
         if (!ok) break;
         const uint32_t kt = tiles_at + mt * (uint32_t)C::kMadeBytes, vt = kt + C::kTile * C::kStride;
         float sc[8][4];

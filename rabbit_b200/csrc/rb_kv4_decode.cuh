@@ -475,7 +475,7 @@ __global__ void __launch_bounds__(DecodeCfg<NG, RB, SPLIT>::kThreads, 1)
                     if (t0 == 0) t0 = globaltimer_ns();
                     __nanosleep(100);
                     if (globaltimer_ns() - t0 > a.wait_ns) {
-                        if (lane == 0) set_error(c.err, RB_ERR_TIMEOUT);
+                        if (lane == 0) atomicOr(c.err, RB_KV4_ERR_WAIT);
                         ok = false;
                     }
                     ok = __all_sync(0xffffffffu, ok);
@@ -602,7 +602,7 @@ __global__ void __launch_bounds__(DecodeCfg<NG, RB, SPLIT>::kThreads, 1)
                 if (t0 == 0) t0 = globaltimer_ns();
                 __nanosleep(64);
                 if (__any_sync(0xffffffffu, globaltimer_ns() - t0 > a.wait_ns)) {
-                    if (lane == 0) set_error(c.err, RB_ERR_TIMEOUT);
+                    if (lane == 0) atomicOr(c.err, RB_KV4_ERR_WAIT);
                     break;
                 }
             }
@@ -618,7 +618,7 @@ __global__ void __launch_bounds__(DecodeCfg<NG, RB, SPLIT>::kThreads, 1)
         int merges = 0;
         for (int step = 0;; ++step) {
             const int buf = step % K;
-            if (ok) ok = mbar_wait(&asked[buf], (step / K) & 1, a.wait_ns, c.err);
+            if (ok) ok = kv4_wait(&asked[buf], (step / K) & 1, a);
             if (!__all_sync(0xffffffffu, ok)) break;
             const DecodeStep &st = steps[buf];
             const int end = st.base + st.granules, owner = st.owner, by = owner < 0 ? W : 1;
@@ -853,12 +853,12 @@ __global__ void __launch_bounds__(DecodeCfg<NG, RB, SPLIT>::kThreads, 1)
                     while (ok && (v = *at) >> 1 != n / S) {
                         __nanosleep(64);
                         if (globaltimer_ns() - t0 > a.wait_ns) {
-                            set_error(c.err, RB_ERR_TIMEOUT);
+                            atomicOr(c.err, RB_KV4_ERR_WAIT);
                             ok = false;
                         }
                     }
                 }
-                if (ok) ok = mbar_wait(&full[n % S], (n / S) & 1, a.wait_ns, c.err);
+                if (ok) ok = kv4_wait(&full[n % S], (n / S) & 1, a);
                 ok = __all_sync(0xffffffffu, ok);
                 return v & 1;
             };
@@ -919,7 +919,7 @@ __global__ void __launch_bounds__(DecodeCfg<NG, RB, SPLIT>::kThreads, 1)
             // step has only zeros, as its factors are)
             __syncwarp();
             if (lane == 0) mbar_arrive(&done[buf]);
-            if (merges > 0 && ok) ok = mbar_wait(&merged, (merges - 1) & 1, a.wait_ns, c.err);
+            if (merges > 0 && ok) ok = kv4_wait(&merged, (merges - 1) & 1, a);
             if (!__all_sync(0xffffffffu, ok)) break;
             ++merges;
             float *out = mo + (size_t)warp * C::kRows * C::kStride;

@@ -54,3 +54,31 @@ def test_a_wait_that_runs_out_is_a_status(torch, rc, kw):
     c.kv.check(base.stream(torch))  # said once
     c.call()
     c.check()
+
+
+@pytest.mark.parametrize("order", ["page first", "slot behind"])
+def test_a_timeout_is_not_hidden_by_what_is_out_of_range(torch, rc, order):
+    """A scratch is spoiled after a timeout, so its status comes before the others'."""
+    c = base.Case(torch, rc, dtype="bf16", nh=8, nkv=2, hd=64, page=16, lens=[3000, 40], seed=42)
+    st = base.stream(torch)
+    if order == "page first":
+        bad = c.table.clone()
+        c.table[1, 0] = 100000
+        c.call()
+        c.table.copy_(bad)
+    try:
+        rc.check(rc.lib().rabbit_cuda_set_wait_limit_us(20000))
+        rc.check(rc.lib().rabbit_cuda_kv4_debug_withhold(c.kv.handle))
+        c.call(ws=rc.Kv4Scratch(c.kv))
+    finally:
+        rc.check(rc.lib().rabbit_cuda_set_wait_limit_ms(2000))
+    if order == "slot behind":
+        x = torch.zeros(1, 2, 64, device="cuda")
+        s = torch.tensor([1 << 40], device="cuda")
+        c.kv.append_dev(0, rc.F32, x.data_ptr(), x.data_ptr(), s.data_ptr(), 1, stream=st)
+    with pytest.raises(rc.RabbitCudaError, match=order.split()[0]) as e:
+        c.kv.check(st)
+    assert e.value.status == rc.ERR_TIMEOUT
+    c.kv.check(st)
+    c.call()
+    c.check()
