@@ -7,11 +7,14 @@
 // sums; scores, softmax and output stay in their registers), so tiles are made
 // while those before are multiplied. Raw granules come by bulk copies four tiles ahead.
 //
-// Exactness: a code has 3 bits and a scale 8, so code * scale is an fp16 number
-// (11 bits) once the granule's scales are brought to at most [1, 2) by a power of
-// two, 2^ek for keys (put back on the scores) and 2^ev for values (put into the
-// weights: w = 2^(x - M + ev), with the reference M as in rb_kv4_decode.cuh).
-// Only the weights are rounded.
+// Exactness: a code has 3 bits and a scale 8, so code * scale has 11, as an fp16
+// number has. Each token has a power of two of its own, 2^ek for its keys (put back on
+// its scores) and 2^ev for its values (put into its weights: 2^(x - M) is summed up,
+// 2^(x - M + ev) multiplies the values, with the reference M as in rb_kv4_decode.cuh),
+// that brings its largest scale to [2^12, 2^13). So what a row does not see, of whatever
+// size, has no part in it. Of one token the channel groups whose scale is at least
+// 2^-29 of its largest are exact; below 2^-37 they are zero. The weights are rounded to
+// fp16 (2^-11).
 //
 // Bound by the latency of the two kinds of warps, not yet by the matrix
 // instructions: 64 rows x 64 positions x 128 channels are 512 of those, 1024 cycles
@@ -43,10 +46,36 @@ struct ChunkCfg {
 };
 
 struct ChunkGranule {  // of a tile, beside its fp16 values
-    float kscale;      // 2^ek
-    float ev, vback;   // ev, 2^-ev
+    float ev;          // the largest of its tokens'
     int there, odd;    // it was read; some value scale is not finite
 };
+
+// Exponents of tokens' scales go from 2^-64 on (a scale below that, and 0, count as
+// that). A weight is at most 2^14 as its value is multiplied by it, so at most 2^90 in
+// the sum, which 2^30 positions do not overflow.
+constexpr int kChunkLeast = -64, kChunkLift = 12;
+
+// A token's exponent: of the largest finite one of its scales; and which of them
+// are not finite. (Scales are not below zero: in order as integers.)
+template <int NW>
+__device__ __forceinline__ int token_exponent(const uint32_t (&sc)[NW], int &odd) {
+    uint32_t top = sc[0];
+#pragma unroll
+    for (int i = 1; i < NW; ++i) top = __vmaxu2(top, sc[i]);
+    top = max(top & 0xffffu, top >> 16);
+    odd = 0;
+    if (top >= 0x7f80u) {
+        top = 0;
+#pragma unroll
+        for (int i = 0; i < 2 * NW; ++i) {
+            const uint32_t x = sc[i >> 1] >> (16 * (i & 1)) & 0xffffu;
+            if (x >= 0x7f80u) odd |= 1 << i;
+            else top = max(top, x);
+        }
+    }
+    return max((int)(top >> 7) - 127, kChunkLeast);
+}
+__device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }
 
 __device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t at) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
@@ -70,6 +99,7 @@ __global__ void __launch_bounds__(ChunkCfg<NG>::kThreads, 1) k_kv4_chunk(const _
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ __align__(8) uint64_t raw_full[C::kRaw], made[C::kMade], used[C::kMade];
     __shared__ ChunkGranule meta[C::kMade][4];
+    __shared__ __align__(8) float kback[C::kMade][C::kTile], vback[C::kMade][C::kTile];  // 2^(ek - lift), 2^(ev - lift) of each token
     __shared__ uint8_t vbad[C::kMade][C::kTile];  // groups of a position whose value scale is not finite
     __shared__ int raw_there[C::kRaw];
     launch_dependents();
@@ -150,29 +180,19 @@ __global__ void __launch_bounds__(ChunkCfg<NG>::kThreads, 1) k_kv4_chunk(const _
             constexpr int NW = (NG + 1) / 2;
             auto make = [&](auto part) {
                 constexpr bool values = decltype(part)::value;
-                // the largest finite scale, and whether all are finite
                 const uint16_t *scales = reinterpret_cast<const uint16_t *>(gr + (values ? kv4_vs(NG) : kv4_ks(NG)));
-                uint32_t top = 0, any = 0;
-                if (there)
-                    for (int i = lane; i < 16 * NG; i += 32) {
-                        const uint32_t x = scales[i];
-                        top = max(top, x < 0x7f80u ? x : 0u);
-                        any |= x >= 0x7f80u;
-                    }
-                top = __reduce_max_sync(0xffffffffu, top);
-                const int e = min(max((int)(top >> 7) - 127, -100), 126);
-                const float down = __uint_as_float((uint32_t)(127 - e) << 23);
                 if constexpr (!values) {
-                    if (lane == 0) {
-                        meta[mt][w].kscale = __uint_as_float((uint32_t)(127 + e) << 23);
-                        meta[mt][w].there = there;
-                    }
+                    if (lane == 0) meta[mt][w].there = there;
 #pragma unroll
                     for (int x = 0; x < 2; ++x) {  // word t of a token's groups
                         const int j = (lane >> 2) + 8 * x, t = lane & 3;
                         uint32_t kw[NG], sc[NW];
                         load_piece<4 * NG>(kw, gr + j * kv4_row(NG) + t * 4 * NG);
                         load_piece<2 * NG>(sc, scales + j * NG);
+                        int mask;
+                        const int e = token_exponent(sc, mask);
+                        const float down = pow2(kChunkLift - e);
+                        if (t == 0) kback[mt][16 * w + j] = pow2(e - kChunkLift);
 #pragma unroll
                         for (int grp = 0; grp < NG; ++grp) {
                             uint32_t y[4];
@@ -184,24 +204,22 @@ __global__ void __launch_bounds__(ChunkCfg<NG>::kThreads, 1) k_kv4_chunk(const _
                         }
                     }
                 } else {
-                    const bool odd = __any_sync(0xffffffffu, any);
-                    if (lane == 0) {
-                        meta[mt][w].ev = (float)e;
-                        meta[mt][w].vback = down;
-                        meta[mt][w].odd = odd;
-                    }
-                    if (odd && lane < 16) {
-                        int mask = 0;
-#pragma unroll
-                        for (int grp = 0; grp < NG; ++grp) mask |= (scales[lane * NG + grp] >= 0x7f80u) << grp;
-                        vbad[mt][16 * w + lane] = (uint8_t)mask;
-                    }
+                    int most = kChunkLeast, any = 0;
 #pragma unroll
                     for (int x = 0; x < 4; ++x) {  // word g of a token's groups
                         const int j = (lane >> 3) + 4 * x, g = lane & 7;
                         uint32_t vw[NW], sc[NW];
                         load_piece<2 * NG>(vw, gr + kv4_v(NG) + j * kv4_row(NG) + kv4_vplace(j, g) * 2 * NG);
                         load_piece<2 * NG>(sc, scales + j * NG);
+                        int mask;
+                        const int e = token_exponent(sc, mask);
+                        const float down = pow2(kChunkLift - e);
+                        most = max(most, e);
+                        any |= mask;
+                        if (g == 0) {
+                            vback[mt][16 * w + j] = pow2(e - kChunkLift);
+                            vbad[mt][16 * w + j] = (uint8_t)mask;
+                        }
 #pragma unroll
                         for (int i = 0; i < NW; ++i) {  // two groups at a time, one in each half of a pair
                             const uint32_t h = vw[i], h8 = h >> 8;
@@ -220,6 +238,12 @@ __global__ void __launch_bounds__(ChunkCfg<NG>::kThreads, 1) k_kv4_chunk(const _
                                 *reinterpret_cast<uint2 *>(to + 64) =
                                     make_uint2(__byte_perm(y[0], y[1], 0x7632), __byte_perm(y[2], y[3], 0x7632));
                         }
+                    }
+                    const bool odd = __any_sync(0xffffffffu, any);
+                    most = __reduce_max_sync(0xffffffffu, most);
+                    if (lane == 0) {
+                        meta[mt][w].ev = (float)(most - kChunkLift);
+                        meta[mt][w].odd = odd;
                     }
                 }
             };
@@ -331,9 +355,11 @@ __global__ void __launch_bounds__(ChunkCfg<NG>::kThreads, 1) k_kv4_chunk(const _
         const bool edge = !all || p0 + C::kTile - 1 > at_lo || (a.window > 0 && p0 <= at_hi - a.window);
         float cand[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-        for (int n = 0; n < 8; ++n)
+        for (int n = 0; n < 8; ++n) {
+            const float2 k = *reinterpret_cast<const float2 *>(&kback[mt][8 * n + 2 * t]);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) sc[n][i] *= cs[i >> 1] * m[n >> 1].kscale;
+            for (int i = 0; i < 4; ++i) sc[n][i] *= cs[i >> 1] * (i & 1 ? k.y : k.x);
+        }
         if (edge) {
 #pragma unroll
             for (int n = 0; n < 8; ++n)
@@ -343,12 +369,22 @@ __global__ void __launch_bounds__(ChunkCfg<NG>::kThreads, 1) k_kv4_chunk(const _
                     if (!m[n >> 1].there || p > r || (a.window > 0 && p <= r - a.window)) sc[n][i] = -INFINITY;
                 }
         }
+        // a bound with a granule's largest ev first, each token's own only where that fails
 #pragma unroll
         for (int n = 0; n < 8; ++n)
 #pragma unroll
             for (int i = 0; i < 2; ++i)
                 cand[i] = fmaxf(cand[i], fmaxf(sc[n][2 * i], sc[n][2 * i + 1]) + m[n >> 1].ev);
         if (__any_sync(0xffffffffu, cand[0] > M[0] + 14.f || cand[1] > M[1] + 14.f)) {
+            cand[0] = cand[1] = -INFINITY;
+#pragma unroll
+            for (int n = 0; n < 8; ++n) {
+                const float2 v = *reinterpret_cast<const float2 *>(&vback[mt][8 * n + 2 * t]);
+                const float e0 = log2_fast(v.x), e1 = log2_fast(v.y);
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+                    cand[i] = fmaxf(cand[i], fmaxf(sc[n][2 * i] + e0, sc[n][2 * i + 1] + e1));
+            }
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
                 float cd = fmaxf(cand[i], __shfl_xor_sync(0xffffffffu, cand[i], 1));
@@ -365,23 +401,18 @@ __global__ void __launch_bounds__(ChunkCfg<NG>::kThreads, 1) k_kv4_chunk(const _
         }
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            const float f0 = m[j].ev - M[0], f1 = m[j].ev - M[1];
             uint32_t w[4];
-            float sum[2] = {0.f, 0.f};
 #pragma unroll
             for (int n = 0; n < 2; ++n) {
                 float *x = sc[2 * j + n];
-                x[0] = exp2_fast(x[0] + f0);
-                x[1] = exp2_fast(x[1] + f0);
-                x[2] = exp2_fast(x[2] + f1);
-                x[3] = exp2_fast(x[3] + f1);
-                sum[0] += x[0] + x[1];
-                sum[1] += x[2] + x[3];
-                w[2 * n] = pack_f16(x[0], x[1]);
-                w[2 * n + 1] = pack_f16(x[2], x[3]);
+                const float2 v = *reinterpret_cast<const float2 *>(&vback[mt][16 * j + 8 * n + 2 * t]);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) x[i] = exp2_fast(x[i] - M[i >> 1]);
+                l[0] += x[0] + x[1];
+                l[1] += x[2] + x[3];
+                w[2 * n] = pack_f16(x[0] * v.x, x[1] * v.y);
+                w[2 * n + 1] = pack_f16(x[2] * v.x, x[3] * v.y);
             }
-            l[0] = fmaf(sum[0], m[j].vback, l[0]);
-            l[1] = fmaf(sum[1], m[j].vback, l[1]);
 #pragma unroll
             for (int b = 0; b < 4 * NG; b += 2) {
                 uint32_t v[4];

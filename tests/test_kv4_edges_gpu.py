@@ -1,10 +1,11 @@
 """GPU: the paged 4-bit cache and its attention at their edges: many items a CTA,
-waits that run out, against float64 numpy (tests/kv4_oracle.py)."""
+waits that run out, numbers of very different size, against float64 numpy (tests/kv4_oracle.py)."""
 from __future__ import annotations
 
 import numpy as np
 import pytest
 
+import kv4_oracle as ko
 import test_rope_kv4_gpu as base
 
 pytestmark = pytest.mark.gpu
@@ -80,5 +81,68 @@ def test_a_timeout_is_not_hidden_by_what_is_out_of_range(torch, rc, order):
         c.kv.check(st)
     assert e.value.status == rc.ERR_TIMEOUT
     c.kv.check(st)
+    c.call()
+    c.check()
+
+
+def rewrite(torch, rc, c, slots, k, v):
+    """Rows (fp32) into slots of a Case's cache, and of its oracle."""
+    s = torch.as_tensor(np.asarray(slots), dtype=torch.int64, device="cuda")
+    c.kv.append_dev(0, rc.F32, k.data_ptr(), v.data_ptr(), s.data_ptr(), len(s),
+                    stream=base.stream(torch))
+    (c.k[slots], c.ks[slots]), (c.v[slots], c.vs[slots]) = ko.hold(base.f64(k)), ko.hold(base.f64(v))
+
+
+# many query rows a sequence, and few
+CHUNKS = [dict(dtype="bf16", nh=16, nkv=8, hd=64, page=48, lens=[300, 90, 73], qs=[90, 90, 70]),
+          dict(dtype="f16", nh=8, nkv=8, hd=128, page=16, lens=[700], qs=[600])]
+DECODES = [dict(dtype="bf16", nh=8, nkv=2, hd=128, page=48, lens=[300, 90, 73]),
+           dict(dtype="f32", nh=8, nkv=2, hd=64, page=16, lens=[700, 33], qs=[9, 2])]
+
+
+@pytest.mark.parametrize("big", [2.0 ** 20, 2.0 ** 30, 1e30])
+@pytest.mark.parametrize("kw", CHUNKS + DECODES)
+def test_finite_rows_that_no_query_row_sees(torch, rc, kw, big):
+    """Rows of any size behind a sequence's end, as an earlier user of the page leaves
+    them, and before a window have no part in the result."""
+    for window in (0, 20):
+        c = base.Case(torch, rc, seed=43, poison=False, window=window, **kw)
+        used = np.concatenate(c.slots)
+        hidden = [np.setdiff1d(np.arange(c.kv.n_pages * c.page), used)]
+        if window:
+            hidden += [s[:max(0, n - q - window + 1)] for s, n, q in zip(c.slots, c.lens, c.qs)]
+        hidden = np.concatenate(hidden)
+        k, v = (torch.randn(len(hidden), c.nkv, c.hd, device="cuda") * big for _ in "kv")
+        rewrite(torch, rc, c, hidden, k, v)
+        c.call()
+        c.check()
+
+
+@pytest.mark.parametrize("dtype,big", [("f16", 1000.0), ("bf16", 2.0 ** 30), ("bf16", 1e30)])
+@pytest.mark.parametrize("kw", CHUNKS + DECODES[1:])
+def test_a_large_value_seen_by_some_rows_of_a_chunk(torch, rc, kw, dtype, big):
+    """The rows before its position do not see it, those behind do: each is right."""
+    c = base.Case(torch, rc, seed=44, poison=False, **{**kw, "dtype": dtype})
+    at = [(s, n - q // 2) for s, n, q in zip(c.slots, c.lens, c.qs)]
+    k, v = (torch.randn(len(at), c.nkv, c.hd, device="cuda") for _ in "kv")
+    rewrite(torch, rc, c, [s[p - 1] for s, p in at], k, v * big)
+    c.call()
+    c.check()
+
+
+@pytest.mark.parametrize("ratio", [2.0 ** 16, 2.0 ** 22, 2.0 ** 26])
+@pytest.mark.parametrize("kw", CHUNKS)
+def test_channel_groups_of_very_different_size_in_a_chunk(torch, rc, kw, ratio):
+    """32 channels of keys and values that are much larger than the others, and that
+    the queries do not look at: the scores, and the others' outputs, keep their
+    accuracy."""
+    c = base.Case(torch, rc, seed=45, poison=False, **{**kw, "dtype": "bf16"})
+    every = np.arange(c.kv.n_pages * c.page)
+    g = torch.Generator("cuda").manual_seed(46)
+    k, v = (torch.randn(len(every), c.nkv, c.hd, generator=g, device="cuda") for _ in "kv")
+    k[..., :32] *= ratio
+    v[..., :32] *= ratio
+    rewrite(torch, rc, c, every, k, v)
+    c.qbuf.view(c.rows, c.nh, c.hd)[..., :32] = 0
     c.call()
     c.check()
