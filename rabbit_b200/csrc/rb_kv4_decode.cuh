@@ -47,6 +47,9 @@ namespace rb {
 
 constexpr int kDecodeMaxGrid = 320;  // CTAs of a launch at most
 constexpr float kNoRef = -3e38f;  // M before any visible token
+// A token whose value scales are below 2^-80, or all 0, counts as one of 2^-80: its weight
+// p s is at most 2^14, so p at most 2^94, and 2^30 positions of such p have a finite sum.
+constexpr float kLeastScale = -80.f;
 
 template <int NG, int RB, bool SPLIT>
 struct DecodeCfg {
@@ -711,7 +714,7 @@ __global__ void __launch_bounds__(DecodeCfg<NG, RB, SPLIT>::kThreads, 1)
                 for (int i = 0; i < NW; ++i) vmax = __vmaxu2(vmax, __vmaxu2(s.v0[i], s.v1[i]));
                 vmax = max(vmax << 16, vmax & 0xffff0000u);
                 // a bound with it first, each token's own scale only where that one fails
-                const float vtop = fmaxf(log2_fast(__uint_as_float(vmax)), -100.f);
+                const float vtop = fmaxf(log2_fast(__uint_as_float(vmax)), kLeastScale);
                 bool odd = edge || vmax >= 0x7f800000u;
 #pragma unroll
                 for (int rb = 0; rb < RB; ++rb)
@@ -761,8 +764,8 @@ __global__ void __launch_bounds__(DecodeCfg<NG, RB, SPLIT>::kThreads, 1)
                     top0 = fmaxf(top0, piece_bf16(s.v0, grp));
                     top1 = fmaxf(top1, piece_bf16(s.v1, grp));
                 }
-                top0 = fmaxf(log2_fast(top0), -100.f);
-                top1 = fmaxf(log2_fast(top1), -100.f);
+                top0 = fmaxf(log2_fast(top0), kLeastScale);
+                top1 = fmaxf(log2_fast(top1), kLeastScale);
 #pragma unroll
                 for (int rb = 0; rb < RB; ++rb)
 #pragma unroll

@@ -146,3 +146,37 @@ def test_channel_groups_of_very_different_size_in_a_chunk(torch, rc, kw, ratio):
     c.qbuf.view(c.rows, c.nh, c.hd)[..., :32] = 0
     c.call()
     c.check()
+
+
+@pytest.mark.parametrize("dtype,nq,n", [("bf16", 64, 80000), ("bf16", 1, 480000), ("f32", 1, 480000)])
+def test_a_value_behind_many_that_are_zero(torch, rc, dtype, nq, n):
+    """The weights of zero values are as large as those of others in the sum that
+    divides, however many they are. The first positions' scores are lower, so that
+    those behind weigh 2^7.5 times as much; the last value is the only one."""
+    hd, page, sms = 32, 64, torch.cuda.get_device_properties(0).multi_processor_count
+    seqs = 80 if nq > 1 else sms  # all over the same pages; a CTA each
+    kv = rc.Kv4(n_layers=1, n_kv_heads=1, head_dim=hd, page_size=page, n_pages=n // page)
+    k, v = torch.zeros(2, n, 1, hd, device="cuda")
+    k[nq + 512:, 0, 0] = 7
+    v[-nq] = 7  # the chunk's first row's own position; the rows behind it see zeros again
+    base.filled(torch, rc, kv, (k, v))
+    dt, code = base.types(torch, rc, dtype)
+    q = torch.zeros(seqs * nq, 1, hd, dtype=dt, device="cuda")
+    q[..., 0] = 1
+    out = torch.empty_like(q)
+    i32 = dict(dtype=torch.int32, device="cuda")
+    table = torch.arange(n // page, **i32).repeat(seqs, 1)
+    lens, start = torch.full((seqs,), n, **i32), torch.arange(seqs + 1, **i32) * nq
+    b = rc.Kv4Batch(n_seqs=seqs, max_pages=n // page, max_q_len=nq, d_q_start=start.data_ptr(),
+                    d_kv_len=lens.data_ptr(), d_page_table=table.data_ptr())
+    st = base.stream(torch)
+    kv.attention_dev(0, rc.Kv4Scratch(kv), code, q.data_ptr(), out.data_ptr(), seqs * nq, 1, b,
+                     scale=7.5 * np.log(2) / 7, stream=st)
+    kv.check(st)
+    w = 2.0 ** 7.5
+    seen = n - nq + 1 + np.arange(nq)                # positions a row sees
+    want = 7 * w / ((nq + 512) + (seen - nq - 512) * w)
+    got = base.f64(out).reshape(seqs, nq, hd)
+    # exp2 and its argument 2^-20, the weight in fp16 2^-11, the division and the sum 2^-20
+    bar = 2.0 ** -11 + 2.0 ** -19 + 1.01 * ko.HALF_STEP[dtype]
+    assert np.abs(got / want[None, :, None] - 1).max() <= bar
