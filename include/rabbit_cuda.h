@@ -527,7 +527,7 @@ int rabbit_cuda_rope_dev(const rabbit_cuda_rope *r, int dtype, const void *d_x, 
  * sequence of at most 256 tokens, src/forward_v2.c:16-26). For each token, KV
  * head and 32 consecutive channels x (the last group of a head may be
  * shorter): scale s = bf16(max|x| / 7) (the fp32 product with 1/7, rounded),
- * codes rint(x / s), a channel read back as code * s; s = 0: all zero. Each
+ * codes rint(x / s) within -7..7, a channel read back as code * s; s = 0: all zero. Each
  * group has its own codes, so a token can be written without touching its
  * neighbours: 18 bytes per 32 channels. A group that holds an infinity or a NaN
  * reads back as NaN. Slot = page * page_size + place in the page; every layer

@@ -51,8 +51,11 @@ template <typename T>
 __device__ __noinline__ uint32_t exact_codes(const T *row, int ch, const double2 *table, int rot, bool halves, float s) {
     uint32_t word = 0;
 #pragma unroll 1
-    for (int n = 0; n < 8; ++n)
-        word |= ((uint32_t)(int)rint(exact_channel(row, ch + n, table, rot, halves) / (double)s) & 15u) << (4 * n);
+    for (int n = 0; n < 8; ++n) {
+        // (a scale among bf16's smallest numbers may have been rounded down by up to a half)
+        const double q = rint(exact_channel(row, ch + n, table, rot, halves) / (double)s);
+        word |= ((uint32_t)(int)fmin(fmax(q, -7.0), 7.0) & 15u) << (4 * n);
+    }
     return word;
 }
 

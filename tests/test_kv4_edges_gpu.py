@@ -180,3 +180,31 @@ def test_a_value_behind_many_that_are_zero(torch, rc, dtype, nq, n):
     # exp2 and its argument 2^-20, the weight in fp16 2^-11, the division and the sum 2^-20
     bar = 2.0 ** -11 + 2.0 ** -19 + 1.01 * ko.HALF_STEP[dtype]
     assert np.abs(got / want[None, :, None] - 1).max() <= bar
+
+
+def hold(x):
+    """The oracle's groups, their codes within -7..7: a scale among bf16's smallest
+    numbers may have been rounded down by up to a half."""
+    y, s = ko.hold(x)
+    return np.clip(y, -7 * s, 7 * s)
+
+
+@pytest.mark.parametrize("turn", [False, True])
+def test_codes_of_the_smallest_groups_stay_in_range(torch, rc, turn):
+    """Largest magnitudes from bf16's smallest scale to where its scales have all
+    their bits, of both signs, as keys, rotated keys and values."""
+    tops = np.concatenate([[9e-40, 1.5e-39, 2.2e-39, 3.3e-40, 4e-39], np.geomspace(2e-40, 2e-38, 91)])
+    T, hd = len(tops), 64
+    rng = np.random.default_rng(47)
+    x = rng.uniform(-1, 1, (T, 2, hd))
+    x[:, 0, 3], x[:, 1, 35] = 1, -1
+    x = torch.from_numpy((x * tops[:, None, None]).astype(np.float32)).cuda()
+    kv = rc.Kv4(n_layers=1, n_kv_heads=2, head_dim=hd, page_size=16, n_pages=-(-T // 16))
+    slots, pos = torch.arange(T, device="cuda"), torch.arange(T, device="cuda").int() * 1001
+    kv.append_dev(0, rc.F32, x.data_ptr(), x.data_ptr(), slots.data_ptr(), T,
+                  rope=rc.Rope(hd) if turn else None, d_positions=pos.data_ptr(),
+                  stream=base.stream(torch))
+    kx = ko.rotate(base.f64(x), pos.cpu().numpy(), ko.freqs(hd), "interleaved") if turn else base.f64(x)
+    k, v = base.read(torch, rc, kv, range(T))
+    np.testing.assert_array_equal(v, hold(base.f64(x)))
+    np.testing.assert_array_equal(k, hold(kx))
