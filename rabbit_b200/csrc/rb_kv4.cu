@@ -182,8 +182,8 @@ __global__ void __launch_bounds__(kAppendThreads, 4) k_kv4_append(const __grid_c
                 big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
                 big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
                 // cosine and sine half a step off, a product and a sum rounded: at most
-                // 4 2^-24 (|v| + |p|) of the magnitude
-                off = big * mag * 2.4e-7f;
+                // 4 2^-24 (|v| + |p|) of the magnitude, and a few of fp32's smallest steps
+                off = big > 0.f ? fmaf(big * mag, 2.4e-7f, 6e-45f) : 0.f;
                 const float a0 = __uint_as_float(top) - off, a1 = __uint_as_float(top) + off;
                 const bool open = off > 0.f && !(__bfloat162float(scale_of(fmaxf(a0, 0.f))) == __bfloat162float(scale_of(a1)));
                 if (__any_sync(0xffffffffu, open)) {

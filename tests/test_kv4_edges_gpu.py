@@ -208,3 +208,24 @@ def test_codes_of_the_smallest_groups_stay_in_range(torch, rc, turn):
     k, v = base.read(torch, rc, kv, range(T))
     np.testing.assert_array_equal(v, hold(base.f64(x)))
     np.testing.assert_array_equal(k, hold(kx))
+
+
+@pytest.mark.parametrize("steps", [1, 5, 6, 100])
+def test_rotated_keys_among_the_smallest_numbers(torch, rc, steps):
+    """Where fp32 has steps of 2^-149 an error bound relative to the value is none:
+    scales and codes are still those of the exactly rotated key. Largest magnitudes
+    within a step or two of those at which the scale's rounding turns: a seventh of them
+    is `steps` and a half steps of bf16's subnormal numbers, and half a step of fp32's."""
+    T, nkv, hd = 8192, 2, 128
+    x = np.random.default_rng(48).uniform(-1, 1, (T, nkv, hd))
+    pos, f = np.arange(T), ko.freqs(hd)
+    top = np.abs(ko.rotate(x, pos, f, "interleaved")).reshape(T, nkv, 4, 32).max(-1)
+    x = x * np.repeat(7 * ((steps + 0.5) * 2.0 ** -133 + 0.5 * 2.0 ** -149 * (-1) ** steps) / top, 32, -1)
+    x = torch.from_numpy(x.astype(np.float32)).cuda()
+    kv = rc.Kv4(n_layers=1, n_kv_heads=nkv, head_dim=hd, page_size=64, n_pages=T // 64)
+    slots, d_pos = torch.arange(T, device="cuda"), torch.from_numpy(pos).int().cuda()
+    kv.append_dev(0, rc.F32, x.data_ptr(), x.data_ptr(), slots.data_ptr(), T, rope=rc.Rope(hd),
+                  d_positions=d_pos.data_ptr(), stream=base.stream(torch))
+    want = hold(ko.rotate(base.f64(x), pos, f, "interleaved"))
+    k, _ = base.read(torch, rc, kv, range(T))
+    np.testing.assert_array_equal(k, want)
