@@ -9,8 +9,8 @@
 //
 // Exactness: a code has 3 bits and a scale 8, so code * scale has 11, as an fp16
 // number has. Each token has a power of two of its own, 2^ek for its keys (put back on
-// its scores) and 2^ev for its values (put into its weights: 2^(x - M) is summed up,
-// 2^(x - M + ev) multiplies the values, with the reference M as in rb_kv4_decode.cuh),
+// its scores) and 2^ev for its values (put into its weights: p = 2^((x - M) - D) is summed
+// up, p 2^ev multiplies the values, with the reference M, D as in rb_kv4_decode.cuh),
 // that brings its largest scale to [2^12, 2^13). So what a row does not see, of whatever
 // size, has no part in it. Of one token the channel groups whose scale is at least
 // 2^-29 of its largest are exact; below 2^-37 they are zero. The weights are rounded to
@@ -42,7 +42,7 @@ struct ChunkCfg {
     static constexpr size_t kQuery = 16 * 4 * 2 * NG * 32;  // operands of 4 x 16 rows
     static constexpr size_t kSmem = kRaw * kRawBytes + kMade * kMadeBytes + kQuery;
     // at the end the second warps' (reference, sum) and outputs, over the fp16 tiles
-    static_assert(4 * 32 * 4 * (4 + 16 * NG) <= kMade * kMadeBytes, "room for the merge");
+    static_assert(4 * 32 * 4 * (6 + 16 * NG) <= kMade * kMadeBytes, "room for the merge");
 };
 
 struct ChunkGranule {  // of a tile, beside its fp16 values
@@ -309,7 +309,7 @@ __global__ void __launch_bounds__(ChunkCfg<NG>::kThreads, 1) k_kv4_chunk(const _
         }
     }
     named_sync(2, 32 * C::kMul);
-    float M[2] = {kNoRef, kNoRef}, l[2] = {0.f, 0.f}, o[4 * NG][4];
+    float M[2] = {kNoRef, kNoRef}, D[2] = {0.f, 0.f}, l[2] = {0.f, 0.f}, o[4 * NG][4];
 #pragma unroll
     for (int b = 0; b < 4 * NG; ++b)
 #pragma unroll
@@ -353,12 +353,11 @@ __global__ void __launch_bounds__(ChunkCfg<NG>::kThreads, 1) k_kv4_chunk(const _
             odd |= m[j].there & m[j].odd;
         }
         const bool edge = !all || p0 + C::kTile - 1 > at_lo || (a.window > 0 && p0 <= at_hi - a.window);
-        float cand[2] = {-INFINITY, -INFINITY};
 #pragma unroll
         for (int n = 0; n < 8; ++n) {
             const float2 k = *reinterpret_cast<const float2 *>(&kback[mt][8 * n + 2 * t]);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) sc[n][i] *= cs[i >> 1] * (i & 1 ? k.y : k.x);
+            for (int i = 0; i < 4; ++i) sc[n][i] = __fmul_rn(sc[n][i], cs[i >> 1] * (i & 1 ? k.y : k.x));
         }
         if (edge) {
 #pragma unroll
@@ -369,28 +368,40 @@ __global__ void __launch_bounds__(ChunkCfg<NG>::kThreads, 1) k_kv4_chunk(const _
                     if (!m[n >> 1].there || p > r || (a.window > 0 && p <= r - a.window)) sc[n][i] = -INFINITY;
                 }
         }
-        // a bound with a granule's largest ev first, each token's own only where that fails
+        // a bound with the largest score and ev first, each token's own only where that fails
+        const float ev = fmaxf(fmaxf(m[0].ev, m[1].ev), fmaxf(m[2].ev, m[3].ev));
+        float mx[2] = {-INFINITY, -INFINITY};
 #pragma unroll
         for (int n = 0; n < 8; ++n)
 #pragma unroll
-            for (int i = 0; i < 2; ++i)
-                cand[i] = fmaxf(cand[i], fmaxf(sc[n][2 * i], sc[n][2 * i + 1]) + m[n >> 1].ev);
-        if (__any_sync(0xffffffffu, cand[0] > M[0] + 14.f || cand[1] > M[1] + 14.f)) {
-            cand[0] = cand[1] = -INFINITY;
+            for (int i = 0; i < 2; ++i) mx[i] = fmaxf(mx[i], fmaxf(sc[n][2 * i], sc[n][2 * i + 1]));
+        if (__any_sync(0xffffffffu, (mx[0] - M[0]) + ev > D[0] + 14.f || (mx[1] - M[1]) + ev > D[1] + 14.f)) {
+            float cand[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                mx[i] = fmaxf(mx[i], M[i]);
+                mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 1));
+                mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 2));
+            }
 #pragma unroll
             for (int n = 0; n < 8; ++n) {
                 const float2 v = *reinterpret_cast<const float2 *>(&vback[mt][8 * n + 2 * t]);
                 const float e0 = log2_fast(v.x), e1 = log2_fast(v.y);
 #pragma unroll
                 for (int i = 0; i < 2; ++i)
-                    cand[i] = fmaxf(cand[i], fmaxf(sc[n][2 * i] + e0, sc[n][2 * i + 1] + e1));
+                    cand[i] = fmaxf(cand[i], fmaxf((sc[n][2 * i] - mx[i]) + e0, (sc[n][2 * i + 1] - mx[i]) + e1));
             }
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
                 float cd = fmaxf(cand[i], __shfl_xor_sync(0xffffffffu, cand[i], 1));
                 cd = fmaxf(cd, __shfl_xor_sync(0xffffffffu, cd, 2));
-                const float mn = cd > M[i] + 14.f ? cd - 6.f : M[i], f = exp2_fast(M[i] - mn);
-                M[i] = mn;
+                const float was = (M[i] - mx[i]) + D[i];
+                const bool raise = cd > was + 14.f;
+                const float f = raise ? exp2_fast(was - (cd - 6.f)) : 1.f;
+                if (raise) {
+                    M[i] = mx[i];
+                    D[i] = cd - 6.f;
+                }
                 l[i] *= f;
 #pragma unroll
                 for (int b = 0; b < 4 * NG; ++b) {
@@ -407,7 +418,7 @@ __global__ void __launch_bounds__(ChunkCfg<NG>::kThreads, 1) k_kv4_chunk(const _
                 float *x = sc[2 * j + n];
                 const float2 v = *reinterpret_cast<const float2 *>(&vback[mt][16 * j + 8 * n + 2 * t]);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) x[i] = exp2_fast(x[i] - M[i >> 1]);
+                for (int i = 0; i < 4; ++i) x[i] = exp2_fast((x[i] - M[i >> 1]) - D[i >> 1]);
                 l[0] += x[0] + x[1];
                 l[1] += x[2] + x[3];
                 w[2 * n] = pack_f16(x[0] * v.x, x[1] * v.y);
@@ -444,30 +455,31 @@ __global__ void __launch_bounds__(ChunkCfg<NG>::kThreads, 1) k_kv4_chunk(const _
     }
     // the odd tiles' part joins the even tiles'
     if (!named_all(2, 32 * C::kMul, ok)) return;  // all fp16 tiles are read, or a wait ran out
-    float *part = reinterpret_cast<float *>(smem + C::kRaw * C::kRawBytes) + wr * 32 * (4 + 16 * NG) + lane;
+    float *part = reinterpret_cast<float *>(smem + C::kRaw * C::kRawBytes) + wr * 32 * (6 + 16 * NG) + lane;
     if (turn == 1) {
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             part[32 * i] = M[i];
-            part[32 * (2 + i)] = l[i];
+            part[32 * (2 + i)] = D[i];
+            part[32 * (4 + i)] = l[i];
         }
 #pragma unroll
         for (int b = 0; b < 4 * NG; ++b)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) part[32 * (4 + 4 * b + i)] = o[b][i];
+            for (int i = 0; i < 4; ++i) part[32 * (6 + 4 * b + i)] = o[b][i];
     }
     named_sync(2, 32 * C::kMul);
     if (turn == 1) return;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-        const float m1 = part[32 * i], l1 = part[32 * (2 + i)], mx = fmaxf(M[i], m1);
-        const float f0 = exp2_fast(M[i] - mx), f1 = exp2_fast(m1 - mx);
+        const float l1 = part[32 * (4 + i)], more = (part[32 * i] - M[i]) + (part[32 * (2 + i)] - D[i]);
+        const float f0 = exp2_fast(fminf(-more, 0.f)), f1 = exp2_fast(fminf(more, 0.f));
         l[i] = fmaf(l[i], f0, l1 * f1);
 #pragma unroll
         for (int b = 0; b < 4 * NG; ++b)
 #pragma unroll
             for (int k = 0; k < 2; ++k)
-                o[b][2 * i + k] = fmaf(o[b][2 * i + k], f0, part[32 * (4 + 4 * b + 2 * i + k)] * f1);
+                o[b][2 * i + k] = fmaf(o[b][2 * i + k], f0, part[32 * (6 + 4 * b + 2 * i + k)] * f1);
         if (!in[i]) continue;
         const float inv = l[i] != 0.f ? 1.0f / l[i] : 0.f;
         const int rho = rho0 + 16 * wr + g + 8 * i, qi = rho / G;

@@ -28,10 +28,13 @@
 //  * O^T = V^T P^T: rows are channels, columns query rows. Each group's weights
 //    are p s, s the value scale, rounded to fp16 (SPLIT: two terms) and turned
 //    from S^T's layout into the operand's by a transpose per 8 x 8 pairs.
-//  * p = 2^(x - M) with M a running reference of the row such that every weight is
-//    at most 2^14 in fp16 and the largest are far above its subnormals. M is
-//    raised only when a weight would pass 2^14, to weights of at most 2^6: after
-//    the first granules that is rare, and the output is rescaled only then.
+//  * p = 2^((x - M) - D) with a running reference of the row in two parts, a score M
+//    and an exponent D of values, such that every weight is at most 2^14 in fp16 and
+//    the largest are far above its subnormals. It is raised only when a weight
+//    would pass 2^14, to weights of at most 2^6: after the first granules that is
+//    rare, and the output is rescaled only then. (In one number a score past 2^24
+//    would leave no room for D. x is rounded to fp32 before M is taken off, so that
+//    equal scores stay equal to their reference.)
 //
 // Bound by its instructions, 387 a granule (2304 bytes at 128 channels; 16-bit
 // queries) at 55 % of the issue slots, half of them on the ALU pipe: 49 us for 1 x
@@ -645,14 +648,14 @@ __global__ void __launch_bounds__(DecodeCfg<NG, RB, SPLIT>::kThreads, 1)
             const int at_lo = st.at0 + rho0 / G, at_hi = st.at0 + (rho0 + R - 1) / G;
             const uint4 *q = reinterpret_cast<const uint4 *>(queries + buf * C::kQuery);
             const float4 *c0 = reinterpret_cast<const float4 *>(q + RB * NT * NG * 32);
-            float cs[RB][2], M[RB][2], l[RB][2], o[RB][NG][2][4];
+            float cs[RB][2], M[RB][2], D[RB][2], l[RB][2], o[RB][NG][2][4];
 #pragma unroll
             for (int rb = 0; rb < RB; ++rb)
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
                     cs[rb][i] = unit[buf][8 * rb + 2 * t + i];
                     M[rb][i] = kNoRef;
-                    l[rb][i] = 0.f;
+                    D[rb][i] = l[rb][i] = 0.f;
                 }
 #pragma unroll
             for (int rb = 0; rb < RB; ++rb)
@@ -703,6 +706,10 @@ __global__ void __launch_bounds__(DecodeCfg<NG, RB, SPLIT>::kThreads, 1)
                         }
                     }
                 }
+#pragma unroll
+                for (int rb = 0; rb < RB; ++rb)
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) s.sc[rb][x] = __fmul_rn(s.sc[rb][x], cs[rb][x & 1]);
             };
             // what only some granules need: masks at the ends of what a row sees, and a
             // higher reference
@@ -720,7 +727,7 @@ __global__ void __launch_bounds__(DecodeCfg<NG, RB, SPLIT>::kThreads, 1)
                 for (int rb = 0; rb < RB; ++rb)
 #pragma unroll
                     for (int i = 0; i < 2; ++i)
-                        odd |= fmaf(fmaxf(s.sc[rb][i], s.sc[rb][2 + i]), cs[rb][i], vtop) > M[rb][i] + 14.f;
+                        odd |= (fmaxf(s.sc[rb][i], s.sc[rb][2 + i]) - M[rb][i]) + vtop > D[rb][i] + 14.f;
                 if (!__any_sync(0xffffffffu, odd)) return;
                 if (edge) {
                     auto sees = [&](int r, int p) {  // tile row r, position p
@@ -770,12 +777,19 @@ __global__ void __launch_bounds__(DecodeCfg<NG, RB, SPLIT>::kThreads, 1)
                 for (int rb = 0; rb < RB; ++rb)
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
-                        float cd = fmaxf(fmaf(s.sc[rb][i], cs[rb][i], top0), fmaf(s.sc[rb][2 + i], cs[rb][i], top1));
+                        float mn = fmaxf(M[rb][i], fmaxf(s.sc[rb][i], s.sc[rb][2 + i]));
+#pragma unroll
+                        for (int x = 4; x < 32; x <<= 1) mn = fmaxf(mn, __shfl_xor_sync(0xffffffffu, mn, x));
+                        float cd = fmaxf((s.sc[rb][i] - mn) + top0, (s.sc[rb][2 + i] - mn) + top1);
 #pragma unroll
                         for (int x = 4; x < 32; x <<= 1) cd = fmaxf(cd, __shfl_xor_sync(0xffffffffu, cd, x));
-                        const float mn = cd > M[rb][i] + 14.f ? cd - 6.f : M[rb][i];
-                        const float f = exp2_fast(M[rb][i] - mn);
-                        M[rb][i] = mn;
+                        const float was = (M[rb][i] - mn) + D[rb][i];
+                        const bool raise = cd > was + 14.f;
+                        const float f = raise ? exp2_fast(was - (cd - 6.f)) : 1.f;
+                        if (raise) {
+                            M[rb][i] = mn;
+                            D[rb][i] = cd - 6.f;
+                        }
                         l[rb][i] *= f;
 #pragma unroll
                         for (int grp = 0; grp < NG; ++grp)
@@ -799,7 +813,7 @@ __global__ void __launch_bounds__(DecodeCfg<NG, RB, SPLIT>::kThreads, 1)
                 for (int rb = 0; rb < RB; ++rb) {
 #pragma unroll
                     for (int x = 0; x < 4; ++x)
-                        s.sc[rb][x] = exp2_fast(fmaf(s.sc[rb][x], cs[rb][x & 1], -M[rb][x & 1]));
+                        s.sc[rb][x] = exp2_fast((s.sc[rb][x] - M[rb][x & 1]) - D[rb][x & 1]);
                     l[rb][0] += s.sc[rb][0] + s.sc[rb][2];
                     l[rb][1] += s.sc[rb][1] + s.sc[rb][3];
                 }
@@ -930,15 +944,19 @@ __global__ void __launch_bounds__(DecodeCfg<NG, RB, SPLIT>::kThreads, 1)
             for (int rb = 0; rb < RB; ++rb)
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
+                    // the reference in one number again: M + D, or M where D would be lost in it
+                    const float ref = fabsf(M[rb][i]) < 1048576.f ? M[rb][i] + D[rb][i] : M[rb][i];
+                    const float f = exp2_fast((M[rb][i] - ref) + D[rb][i]);
                     if (g == 0) {
-                        wm[warp][8 * rb + 2 * t + i] = M[rb][i];
-                        wl[warp][8 * rb + 2 * t + i] = l[rb][i];
+                        wm[warp][8 * rb + 2 * t + i] = ref;
+                        wl[warp][8 * rb + 2 * t + i] = l[rb][i] * f;
                     }
                     float *row = out + (8 * rb + 2 * t + i) * C::kStride + 4 * g;
 #pragma unroll
                     for (int grp = 0; grp < NG; ++grp)
-                        *reinterpret_cast<float4 *>(row + 32 * grp) = make_float4(
-                            o[rb][grp][0][i], o[rb][grp][1][i], o[rb][grp][0][2 + i], o[rb][grp][1][2 + i]);
+                        *reinterpret_cast<float4 *>(row + 32 * grp) =
+                            make_float4(o[rb][grp][0][i] * f, o[rb][grp][1][i] * f, o[rb][grp][0][2 + i] * f,
+                                        o[rb][grp][1][2 + i] * f);
                 }
             __syncwarp();
             if (lane == 0) mbar_arrive(&left);

@@ -229,3 +229,42 @@ def test_rotated_keys_among_the_smallest_numbers(torch, rc, steps):
     want = hold(ko.rotate(base.f64(x), pos, f, "interleaved"))
     k, _ = base.read(torch, rc, kv, range(T))
     np.testing.assert_array_equal(k, want)
+
+
+@pytest.mark.parametrize("big", [1e4, 1e8, 1e18, 1e30])
+@pytest.mark.parametrize("kw", CHUNKS + DECODES)
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+def test_scores_past_the_whole_numbers_of_fp32(torch, rc, kw, dtype, big):
+    """Scores whose steps in fp32 are large beside the exponents of the weights: equal
+    ones share, a larger one has all, whatever the values' size."""
+    value = 1e3 if dtype == "f16" else 1e-20 if big < 1e9 else 1e30
+    c = base.Case(torch, rc, seed=49, poison=False, **{**kw, "dtype": dtype})
+    n = c.kv.n_pages * c.page
+    g = torch.Generator("cuda").manual_seed(50)
+    v = torch.randn(n, c.nkv, c.hd, generator=g, device="cuda") * value
+    v[::3] /= 1000
+    k = torch.zeros_like(v)
+    pick = torch.randint(1, 4, (n, c.nkv), generator=g, device="cuda") * 7.0  # scales 1, 2, 3
+    q = torch.zeros(c.rows, c.nh, c.hd, device="cuda")
+    q[..., 0] = torch.where(torch.rand(c.rows, c.nh, generator=g, device="cuda") < 0.5, -1.0, 1.0)
+    if dtype == "f16":  # the queries' type holds up to 65504
+        k[..., 0], c.scale = pick * min(big, 1e30), 1.0
+    else:
+        k[..., 0], c.scale = pick, 1.0
+        q *= big
+    c.qbuf.copy_(q.to(c.qbuf.dtype).flatten())
+    rewrite(torch, rc, c, np.arange(n), k, v)
+    c.call()
+    c.kv.check(base.stream(torch))
+    got = c.rows_of(c.out).reshape(c.rows, c.nh, c.hd)
+    q, row, G = c.rows_of(c.qbuf).reshape(got.shape), 0, c.nh // c.nkv
+    for length, nq, s in zip(c.lens, c.qs, c.slots):
+        for h in range(c.nh):
+            at = range(length - nq, length)
+            want, w = ko.attend(q[row:row + nq, h], c.k[s, h // G], c.v[s, h // G], at, c.window, 1.0)
+            size = ko.attend(q[row:row + nq, h], c.k[s, h // G], np.abs(c.v[s, h // G]), at, c.window, 1.0)[0]
+            # equal weights and weights of zero: a common factor is off, 2^-20, and each fp16
+            # weight by 2^-11, once more in its product with the value's scale
+            bar = (2.0 ** -10 + 2.0 ** -19) * size + 1.01 * ko.HALF_STEP[dtype] * np.abs(want) + 1e-30
+            assert (np.abs(got[row:row + nq, h] - want) <= bar).all()
+        row += nq
