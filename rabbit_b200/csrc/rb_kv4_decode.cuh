@@ -332,7 +332,7 @@ __global__ void __launch_bounds__(DecodeCfg<NG, RB, SPLIT>::kThreads, 1)
     __shared__ __align__(8) uint64_t left, merged;                 // outputs written; merged
     __shared__ int tag[S];                   // a slot's last granule: 2 x its round + whether it is there
     __shared__ DecodeStep steps[K];
-    __shared__ float unit[K][C::kRows];      // a step's rows: one of their scores, as a power of two
+    __shared__ __align__(8) float unit[K][C::kRows];      // a step's rows: one of their scores, as a power of two
     __shared__ int pending, pend[2][6];      // items whose last piece came from here
     __shared__ int64_t warp_sums[C::kThreads / 32];
     __shared__ int64_t found_before;
@@ -648,12 +648,11 @@ __global__ void __launch_bounds__(DecodeCfg<NG, RB, SPLIT>::kThreads, 1)
             const int at_lo = st.at0 + rho0 / G, at_hi = st.at0 + (rho0 + R - 1) / G;
             const uint4 *q = reinterpret_cast<const uint4 *>(queries + buf * C::kQuery);
             const float4 *c0 = reinterpret_cast<const float4 *>(q + RB * NT * NG * 32);
-            float cs[RB][2], M[RB][2], D[RB][2], l[RB][2], o[RB][NG][2][4];
+            float M[RB][2], D[RB][2], l[RB][2], o[RB][NG][2][4];
 #pragma unroll
             for (int rb = 0; rb < RB; ++rb)
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
-                    cs[rb][i] = unit[buf][8 * rb + 2 * t + i];
                     M[rb][i] = kNoRef;
                     D[rb][i] = l[rb][i] = 0.f;
                 }
@@ -707,9 +706,11 @@ __global__ void __launch_bounds__(DecodeCfg<NG, RB, SPLIT>::kThreads, 1)
                     }
                 }
 #pragma unroll
-                for (int rb = 0; rb < RB; ++rb)
+                for (int rb = 0; rb < RB; ++rb) {
+                    const float2 cs = *reinterpret_cast<const float2 *>(&unit[buf][8 * rb + 2 * t]);
 #pragma unroll
-                    for (int x = 0; x < 4; ++x) s.sc[rb][x] = __fmul_rn(s.sc[rb][x], cs[rb][x & 1]);
+                    for (int x = 0; x < 4; ++x) s.sc[rb][x] = __fmul_rn(s.sc[rb][x], x & 1 ? cs.y : cs.x);
+                }
             };
             // what only some granules need: masks at the ends of what a row sees, and a
             // higher reference
