@@ -608,10 +608,11 @@ int rabbit_cuda_kv4_attention_dev(rabbit_cuda_kv4 *kv, int layer, rabbit_cuda_kv
                                   int64_t out_stride, int n_tokens, int n_heads,
                                   const rabbit_cuda_kv4_batch *batch, float scale, int window,
                                   void *stream);
-/* Synchronises `stream` and reports, once, what calls on this cache found out
- * of range since the last check (RABBIT_CUDA_ERR_ARGS) or a bounded wait that
- * gave up (RABBIT_CUDA_ERR_TIMEOUT, also where something was out of range as well;
- * the text names both). */
+/* Synchronises `stream` and reports, once, what calls on this cache found out of
+ * range since the last check (RABBIT_CUDA_ERR_ARGS) or a bounded wait that gave up
+ * (RABBIT_CUDA_ERR_TIMEOUT, also where something was out of range as well; the text
+ * names both). Calls on other streams are reported as far as they have run; nothing
+ * that they find meanwhile is lost. Threads may check at the same time. */
 int rabbit_cuda_kv4_check(rabbit_cuda_kv4 *kv, void *stream);
 /* Test hook: the next attention call on `kv` leaves out one arrival inside a CTA, so
  * that waits in it run out; it ends with RABBIT_CUDA_ERR_TIMEOUT in the check,

@@ -289,6 +289,9 @@ __global__ void __launch_bounds__(kAppendThreads) k_kv4_read(const __grid_consta
     }
 }
 
+// err[0], taken and cleared in one step, into err[1].
+__global__ void k_kv4_take(int *err) { err[1] = atomicExch(err, 0); }
+
 // Tokens per CTA of the append and the read: one wave of four CTAs an SM for each
 // of keys and values, up to 8; a token's items in one CTA each 256 (blockIdx.y).
 static int tokens_per_cta(int n_tokens) {
@@ -350,8 +353,8 @@ int rabbit_cuda_kv4_create(const rabbit_cuda_kv4_desc *d, int device, rabbit_cud
                                                                                       : cudaMalloc(&base, bytes);
     if (e == cudaSuccess) {
         c->view.base = static_cast<uint8_t *>(base);
-        if ((e = cudaMalloc(&c->d_err, sizeof(int))) == cudaSuccess &&
-            (e = cudaMemset(c->d_err, 0, sizeof(int))) == cudaSuccess &&
+        if ((e = cudaMalloc(&c->d_err, 2 * sizeof(int))) == cudaSuccess &&
+            (e = cudaMemset(c->d_err, 0, 2 * sizeof(int))) == cudaSuccess &&
             (e = cudaMemset(base, 0, bytes)) == cudaSuccess)
             e = cudaStreamSynchronize(nullptr);  // zeroed before any stream uses it
     }
@@ -477,11 +480,16 @@ int rabbit_cuda_kv4_check(rabbit_cuda_kv4 *kv, void *stream) {
     if (scope.status != RABBIT_CUDA_OK) return scope.status;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     int h = 0;
-    RB_CUDA(cudaMemcpyAsync(&h, kv->d_err, sizeof(int), cudaMemcpyDeviceToHost, s));
     RB_CUDA(cudaStreamSynchronize(s));
+    {
+        // what another stream's call sets meanwhile is taken now or stays for the next check
+        std::lock_guard<std::mutex> hold(kv->taking);
+        k_kv4_take<<<1, 1, 0, s>>>(kv->d_err);
+        RB_CUDA(cudaGetLastError());
+        RB_CUDA(cudaMemcpyAsync(&h, kv->d_err + 1, sizeof(int), cudaMemcpyDeviceToHost, s));
+        RB_CUDA(cudaStreamSynchronize(s));
+    }
     if (h == 0) return ok();
-    RB_CUDA(cudaMemsetAsync(kv->d_err, 0, sizeof(int), s));
-    RB_CUDA(cudaStreamSynchronize(s));
     // the timeout first: after it the caller has to replace a scratch
     const int range = h & (RB_KV4_ERR_SLOT | RB_KV4_ERR_PAGE | RB_KV4_ERR_LEN | RB_KV4_ERR_ROWS);
     return fail(h & RB_KV4_ERR_WAIT ? RABBIT_CUDA_ERR_TIMEOUT : RABBIT_CUDA_ERR_ARGS, "kv4: %s%s%s%s%s%s",

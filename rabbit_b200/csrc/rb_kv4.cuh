@@ -83,7 +83,8 @@ struct rabbit_cuda_kv4 {
     int n_layers = 0;
     rb::Kv4View view = {};      // of layer 0
     size_t layer_bytes = 0;
-    int *d_err = nullptr;
+    int *d_err = nullptr;       // the error word, and what a check took of it
+    std::mutex taking;          // one check at a time
     bool withhold = false;      // test hook for the next attention
     rb::Kv4View layer(int l) const {
         rb::Kv4View v = view;

@@ -268,3 +268,48 @@ def test_scores_past_the_whole_numbers_of_fp32(torch, rc, kw, dtype, big):
             bar = (2.0 ** -10 + 2.0 ** -19) * size + 1.01 * ko.HALF_STEP[dtype] * np.abs(want) + 1e-30
             assert (np.abs(got[row:row + nq, h] - want) <= bar).all()
         row += nq
+
+
+def test_a_check_loses_nothing_that_another_stream_found(torch, rc):
+    """One thread makes and checks bad slots on its stream, another bad lengths on its own:
+    each length is reported by one check or the other."""
+    import threading
+    import time
+
+    kv = rc.Kv4(n_layers=1, n_kv_heads=1, head_dim=32, page_size=16, n_pages=2)
+    ws, a, b = rc.Kv4Scratch(kv), torch.cuda.Stream(), torch.cuda.Stream()
+    x = torch.zeros(1, 1, 32, device="cuda")
+    out, slot = torch.empty_like(x), torch.tensor([99], device="cuda")
+    length, table = torch.tensor([17], dtype=torch.int32, device="cuda"), torch.zeros(1, dtype=torch.int32, device="cuda")
+    batch = rc.Kv4Batch(n_seqs=1, max_pages=1, d_kv_len=length.data_ptr(), d_page_table=table.data_ptr())
+    torch.cuda.synchronize()
+    said, rounds, stop = [], [0], threading.Event()
+
+    def look(s):
+        try:
+            kv.check(s.cuda_stream)
+        except rc.RabbitCudaError as e:
+            assert e.status == rc.ERR_ARGS
+            said.append(str(e))
+
+    def slots():
+        while not stop.is_set():
+            kv.append_dev(0, rc.F32, x.data_ptr(), x.data_ptr(), slot.data_ptr(), 1, stream=a.cuda_stream)
+            look(a)
+            rounds[0] += 1
+
+    t = threading.Thread(target=slots)
+    t.start()
+    try:
+        for _ in range(400):
+            before = len(said)
+            kv.attention_dev(0, ws, rc.F32, x.data_ptr(), out.data_ptr(), 1, 1, batch, stream=b.cuda_stream)
+            look(b)
+            done = rounds[0] + 2  # a check of the other thread that was under way is over
+            while rounds[0] < done and t.is_alive():
+                time.sleep(1e-5)
+            assert any("kv_len" in m for m in said[before:])
+    finally:
+        stop.set()
+        t.join()
+    assert any("slot" in m for m in said)
