@@ -651,6 +651,8 @@ class Kv4:
                    v_stride: int = 0, stream: int = 0) -> None:
         """Rows of keys (rotated by `rope`) and values into int64 slots
         (rabbit_cuda_kv4_append_dev); negative slots are skipped."""
+        if rope is not None and not rope.handle:  # NULL would say: no rotation
+            raise RabbitCudaError(ERR_ARGS, "kv4_append: the rope was freed")
         check(lib().rabbit_cuda_kv4_append_dev(
             self.handle, layer, dtype, d_k, k_stride, d_v, v_stride, d_slots, n_tokens,
             rope.handle if rope else None, d_positions or None, stream or None))
