@@ -6,6 +6,7 @@ import numpy as np
 import pytest
 
 import kv4_oracle as ko
+import kv4_signs as ks
 import test_rope_kv4_gpu as base
 
 pytestmark = pytest.mark.gpu
@@ -313,3 +314,153 @@ def test_a_check_loses_nothing_that_another_stream_found(torch, rc):
         stop.set()
         t.join()
     assert any("slot" in m for m in said)
+
+
+# ---------------------------------------------------------------- each token, in place --
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("i", range(len(ks.CASES)))
+def test_every_token_has_its_part(torch, rc, i, dtype):
+    """Random signs whose result tells each token from the others (tests/kv4_signs.py;
+    that every one lost, doubled or misplaced passes the bar is shown there)."""
+    kw = ks.CASES[i]
+    c = base.Case(torch, rc, dtype=dtype, seed=i, poison=False, scale=ks.SCALE, **kw)
+    q, seqs = ks.inputs(i, nh=c.nh, nkv=c.nkv, hd=c.hd, lens=c.lens, qs=c.qs)
+    for s, (k, v) in zip(c.slots, seqs):
+        if len(s):
+            kx = np.zeros(v.shape, np.float32)
+            kx[..., ks.PICK] = 7 * k
+            rewrite(torch, rc, c, s, torch.from_numpy(kx).cuda(), 7 * torch.from_numpy(v).float().cuda())
+    qx = torch.zeros(c.rows, c.nh, c.hd)
+    qx[..., ks.PICK] = torch.from_numpy(q).float()
+    c.qbuf.copy_(qx.to(c.qbuf.dtype).flatten())
+    c.call()
+    c.kv.check(base.stream(torch))
+    got, row, G = c.rows_of(c.out).reshape(c.rows, c.nh, c.hd), 0, c.nh // c.nkv
+    for (k, v), n, nq in zip(seqs, c.lens, c.qs):
+        for r in range(nq):
+            for h in range(c.nh):
+                want = ks.attend(q[row + r, h], k[:, h // G], v[:, h // G], n - nq + r, c.window)[0]
+                assert (np.abs(got[row + r, h] - want) <= ks.bar(want, ko.HALF_STEP[dtype])).all(), (n, r, h)
+        row += nq
+
+
+class Close(base.Case):
+    """The same cases with bars from the keys and values at hand instead of bounds on
+    them. With T_j = scale sum_c |q_c| |k_jc|, where the 16-bit decode kernel's codes have
+    a bias of 8 scales on top:
+     * a matrix instruction adds 16 products to a sum, each cut off at 2^-23 of the largest:
+       17 2^-23 of it. A group of 32 channels takes 2 (fp32 queries: 4), whose sums are at most
+       T_j's part, in a chunk 2 in a row over all groups: e_j = (17 m + 6) 2^-23 T_j with
+       m = 2, 4 or 2 groups; the 6 are the groups' sum, the unit and the query's two terms.
+     * a weight is off by e_j, by 2^-19 (exp2 and its argument), by its rounding, r = 2^-11 or
+       2^-21, or, where that is more, by 7 2^-31 of the largest weight times scale.
+     * a granule's product is added with 17 2^-23 of the sum; a warp of a long sequence that
+       many SMs share has at most 64 of them.
+    """
+
+    def oracle(self, q):
+        scale = self.scale or self.hd ** -0.5
+        out = np.zeros((self.rows, self.nh, self.hd))
+        bar = np.zeros_like(out)
+        split, row, G = self.dtype == "f32", 0, self.nh // self.nkv
+        r, m = 2.0 ** -21 if split else 2.0 ** -11, max(4, 2 * -(-self.hd // 32))
+        for n, nq, s in zip(self.lens, self.qs, self.slots):
+            for h in range(self.nh):
+                k, v = self.k[s, h // G], self.v[s, h // G]
+                qq = q[row:row + nq, h]
+                o, w = ko.attend(qq, k, v, range(n - nq, n), self.window, scale)
+                if n:
+                    big = np.abs(k) if split else np.abs(k) + 8 * self.ks[s, h // G]
+                    e = (17 * m + 6) * 2.0 ** -23 * scale * (np.abs(qq) @ big.T) + 2.0 ** -19
+                    a = np.abs(v)
+                    bar[row:row + nq, h] = (
+                        (w * (e + r + min(n / 16, 64) * 17 * 2.0 ** -23)) @ a + np.abs(o) * (w * e).sum(1)[:, None] +
+                        n * 7 * 2.0 ** -31 * (w[:, :, None] * self.vs[s, h // G]).max(1))
+                out[row:row + nq, h] = o
+            row += nq
+        return out, bar + 1.01 * ko.HALF_STEP[self.dtype] * (np.abs(out) + bar) + 1e-30
+
+
+@pytest.mark.parametrize("i", range(len(base.ATTN)))
+def test_attention_within_close_bars(torch, rc, i):
+    c = Close(torch, rc, seed=100 + i, **base.ATTN[i])
+    c.call()
+    c.check()
+
+
+# ------------------------------------------------------------------ ways of calling --
+def test_one_scratch_for_calls_of_all_kinds_in_turn(torch, rc):
+    """On one stream, without a wait between them: other types, head counts, layers, kernels
+    and numbers of sequences. Each gives what it gives with a scratch of its own."""
+    kv = rc.Kv4(n_layers=2, n_kv_heads=4, head_dim=64, page_size=16, n_pages=400)
+    for layer in range(2):
+        g = torch.Generator("cuda").manual_seed(layer)
+        base.filled(torch, rc, kv, torch.randn(2, 6400, 4, 64, generator=g, device="cuda"), layer=layer)
+    ws, st, i32 = rc.Kv4Scratch(kv), base.stream(torch), dict(dtype=torch.int32, device="cuda")
+    table = torch.randperm(400, generator=torch.Generator().manual_seed(9)).int().cuda()
+    calls = []
+    for dtype, layer, nh, nq, lens in [("bf16", 0, 16, 1, [6400]), ("f32", 1, 4, 1, [700, 30, 5000]),
+                                       ("f16", 0, 32, 300, [2000]), ("f32", 0, 24, 4, [3000] * 3),
+                                       ("bf16", 1, 4, 1, [9] * 40), ("bf16", 1, 40, 90, [100, 90, 91]),
+                                       ("f16", 1, 8, 2, [6400, 0, 1])]:
+        dt, code = base.types(torch, rc, dtype)
+        rows = nq * len(lens)
+        q = torch.randn(rows, nh, 64, generator=torch.Generator("cuda").manual_seed(nh), device="cuda").to(dt)
+        keep = (torch.tensor(lens, **i32), torch.arange(len(lens) + 1, **i32) * nq, table.repeat(len(lens), 1))
+        b = rc.Kv4Batch(n_seqs=len(lens), max_pages=400, max_q_len=nq, d_q_start=keep[1].data_ptr(),
+                        d_kv_len=keep[0].data_ptr(), d_page_table=keep[2].data_ptr())
+        calls.append((layer, code, q, rows, nh, b, keep))
+
+    def run(own):
+        outs = []
+        for layer, code, q, rows, nh, b, _ in calls:
+            outs.append(torch.zeros_like(q))
+            w = rc.Kv4Scratch(kv) if own else ws
+            kv.attention_dev(layer, w, code, q.data_ptr(), outs[-1].data_ptr(), rows, nh, b, stream=st)
+            if own:
+                torch.cuda.synchronize()
+        kv.check(st)
+        return outs
+
+    want = run(True)
+    for _ in range(10):
+        for got, w in zip(run(False), want):
+            assert torch.equal(got, w)
+
+
+@pytest.mark.parametrize("dtype,nq", [("f32", 1), ("bf16", 1), ("bf16", 100)])
+def test_sequences_that_share_pages(torch, rc, dtype, nq):
+    """A common beginning of some pages, and the very same sequence twice."""
+    c = base.Case(torch, rc, dtype=dtype, nh=32, nkv=8, hd=64, page=32, lens=[300, 270, 300], qs=[nq] * 3,
+                  seed=51, poison=False)
+    c.table[1, :5] = c.table[0, :5]
+    c.table[2] = c.table[0]
+    c.slots[1] = np.concatenate([c.slots[0][:160], c.slots[1][160:]])
+    c.slots[2] = c.slots[0]
+    c.qbuf.view(3 * nq, -1)[2 * nq:] = c.qbuf.view(3 * nq, -1)[:nq]
+    c.call()
+    c.check()
+
+
+def test_a_cache_on_another_device_than_the_current_one(torch, rc):
+    if torch.cuda.device_count() < 2:
+        pytest.skip("one GPU")
+    kv = rc.Kv4(n_layers=1, n_kv_heads=2, head_dim=64, page_size=16, n_pages=4, device=1)
+    ws = rc.Kv4Scratch(kv)
+    assert torch.cuda.current_device() == 0
+    with torch.cuda.device(1):
+        st = torch.cuda.current_stream().cuda_stream
+        x = torch.randn(2, 40, 2, 64, device="cuda:1")
+        q, out = torch.randn(1, 4, 64, device="cuda:1"), torch.empty(1, 4, 64, device="cuda:1")
+        slots, table = torch.arange(40, device="cuda:1"), torch.arange(4, dtype=torch.int32, device="cuda:1")
+        n = torch.tensor([40], dtype=torch.int32, device="cuda:1")
+        torch.cuda.synchronize()
+    b = rc.Kv4Batch(n_seqs=1, max_pages=4, d_kv_len=n.data_ptr(), d_page_table=table.data_ptr())
+    kv.append_dev(0, rc.F32, x[0].data_ptr(), x[1].data_ptr(), slots.data_ptr(), 40, stream=st)
+    kv.attention_dev(0, ws, rc.F32, q.data_ptr(), out.data_ptr(), 1, 4, b, stream=st)
+    kv.check(st)
+    assert torch.cuda.current_device() == 0
+    k, v = (ko.hold(base.f64(y))[0] for y in x)
+    for h in range(4):
+        want, w = ko.attend(base.f64(q)[:, h], k[:, h // 2], v[:, h // 2], [39], 0, 0.125)
+        assert np.abs(base.f64(out)[0, h] - want[0]).max() <= 2.0 ** -14 * np.abs(v).max()
