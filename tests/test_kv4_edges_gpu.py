@@ -346,7 +346,7 @@ def test_every_token_has_its_part(torch, rc, i, dtype):
 
 class Close(base.Case):
     """The same cases with bars from the keys and values at hand instead of bounds on
-    them. With T_j = scale sum_c |q_c| |k_jc|, where the 16-bit decode kernel's codes have
+    them. With T_j = |scale| sum_c |q_c| |k_jc|, where the 16-bit decode kernel's codes have
     a bias of 8 scales on top:
      * a matrix instruction adds 16 products to a sum, each cut off at 2^-23 of the largest:
        17 2^-23 of it. A group of 32 channels takes 2 (fp32 queries: 4), whose sums are at most
@@ -371,7 +371,7 @@ class Close(base.Case):
                 o, w = ko.attend(qq, k, v, range(n - nq, n), self.window, scale)
                 if n:
                     big = np.abs(k) if split else np.abs(k) + 8 * self.ks[s, h // G]
-                    e = (17 * m + 6) * 2.0 ** -23 * scale * (np.abs(qq) @ big.T) + 2.0 ** -19
+                    e = (17 * m + 6) * 2.0 ** -23 * abs(scale) * (np.abs(qq) @ big.T) + 2.0 ** -19
                     a = np.abs(v)
                     bar[row:row + nq, h] = (
                         (w * (e + r + min(n / 16, 64) * 17 * 2.0 ** -23)) @ a + np.abs(o) * (w * e).sum(1)[:, None] +
@@ -464,3 +464,28 @@ def test_a_cache_on_another_device_than_the_current_one(torch, rc):
     for h in range(4):
         want, w = ko.attend(base.f64(q)[:, h], k[:, h // 2], v[:, h // 2], [39], 0, 0.125)
         assert np.abs(base.f64(out)[0, h] - want[0]).max() <= 2.0 ** -14 * np.abs(v).max()
+
+
+@pytest.mark.parametrize("kw", CHUNKS + DECODES)
+def test_a_scale_below_zero_and_the_widest_window(torch, rc, kw):
+    c = Close(torch, rc, seed=52, **{**kw, "scale": -0.2, "window": 2 ** 31 - 1})
+    c.call()
+    c.check()
+
+
+@pytest.mark.parametrize("kw", CHUNKS + DECODES)
+def test_a_query_that_is_not_finite_stays_in_its_row(torch, rc, kw):
+    """Its own head's row is NaN, every other row has the same bits as without it."""
+    c = base.Case(torch, rc, seed=53, **kw)
+    c.call()
+    want = c.rows_of(c.out).reshape(c.rows, c.nh, c.hd)
+    q = c.qbuf.view(c.rows, c.nh, c.hd)
+    q[0, 1, 3], q[c.rows - 1, 0, c.hd - 1], q[c.rows - 1, c.nh - 1, :] = float("nan"), float("inf"), float("-inf")
+    again = torch.zeros_like(c.out)
+    c.call(out=again)
+    c.kv.check(base.stream(torch))
+    got = c.rows_of(again).reshape(want.shape)
+    odd = np.zeros(want.shape[:2], bool)
+    odd[0, 1] = odd[-1, 0] = odd[-1, -1] = True
+    assert np.isnan(got[odd]).all()
+    np.testing.assert_array_equal(got[~odd], want[~odd])
