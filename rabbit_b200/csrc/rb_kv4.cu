@@ -294,8 +294,8 @@ __global__ void k_kv4_take(int *err) { err[1] = atomicExch(err, 0); }
 
 // Tokens per CTA of the append and the read: one wave of four CTAs an SM for each
 // of keys and values, up to 8; a token's items in one CTA each 256 (blockIdx.y).
-static int tokens_per_cta(int n_tokens) {
-    const int64_t n = ((int64_t)n_tokens + 591) / 592;
+static int tokens_per_cta(int n_tokens, int sms) {
+    const int64_t n = ((int64_t)n_tokens + 4 * sms - 1) / (4 * sms);
     return n > 8 ? 8 : (int)n;
 }
 
@@ -340,8 +340,8 @@ int rabbit_cuda_kv4_create(const rabbit_cuda_kv4_desc *d, int device, rabbit_cud
     c->view.ng = (d->head_dim + kKv4Group - 1) / kKv4Group;
     c->view.page = d->page_size;
     c->view.n_pages = d->n_pages;
-    c->view.head = (size_t)(d->page_size / kKv4Granule) * kv4_bytes(c->view.ng);
-    c->view.page_size = d->n_kv_heads * c->view.head;
+    c->view.head_nbytes = (size_t)(d->page_size / kKv4Granule) * kv4_bytes(c->view.ng);
+    c->view.page_nbytes = d->n_kv_heads * c->view.head_nbytes;
     c->view.n_slots = (int64_t)d->n_pages * d->page_size;
     c->view.shift = -1;
     for (int i = 4; i <= 10; ++i)
@@ -422,7 +422,7 @@ int rabbit_cuda_kv4_append_dev(rabbit_cuda_kv4 *kv, int layer, int dtype, const 
     a.slots = d_slots;
     a.pos = rope ? d_positions : nullptr;
     a.T = n_tokens;
-    a.tpc = tokens_per_cta(n_tokens);
+    a.tpc = tokens_per_cta(n_tokens, kv->ctx->sm_count);
     const bool vec = aligned(d_k, 16) && aligned(d_v, 16) && a.xs[0] * size % 16 == 0 &&
                      a.xs[1] * size % 16 == 0 && (int64_t)a.c.hd * size % 16 == 0;
     DeviceScope scope(kv->device);
@@ -458,7 +458,7 @@ int rabbit_cuda_kv4_read_dev(rabbit_cuda_kv4 *kv, int layer, int dtype, const in
     a.slots = d_slots;
     a.T = n_tokens;
     const bool vec = aligned(d_k, 16) && aligned(d_v, 16) && (int64_t)a.c.hd * size % 16 == 0;
-    a.tpc = tokens_per_cta(n_tokens);
+    a.tpc = tokens_per_cta(n_tokens, kv->ctx->sm_count);
     const int items = a.c.nkv * a.c.ng * 4;
     const dim3 grid((unsigned)(((int64_t)n_tokens + a.tpc - 1) / a.tpc), (items + kAppendThreads - 1) / kAppendThreads, 2);
     DeviceScope scope(kv->device);

@@ -58,10 +58,10 @@ struct Kv4View {
     int nkv, hd, ng, page, n_pages;
     int shift;  // page = 2^shift, or -1
     int *err;
-    size_t head, page_size;  // bytes of a page: of one KV head's part, of all
+    size_t head_nbytes, page_nbytes;  // of a page: one KV head's part, all of it
     int64_t n_slots;
-    __host__ __device__ size_t head_bytes() const { return head; }
-    __host__ __device__ size_t page_bytes() const { return page_size; }
+    __host__ __device__ size_t head_bytes() const { return head_nbytes; }
+    __host__ __device__ size_t page_bytes() const { return page_nbytes; }
     __host__ __device__ int64_t slots() const { return n_slots; }
     __device__ __forceinline__ uint8_t *granule(int64_t slot, int head) const {
         return row(slot) + (size_t)head * head_bytes();

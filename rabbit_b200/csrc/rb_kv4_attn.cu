@@ -16,6 +16,8 @@ struct rabbit_cuda_kv4_scratch {
 
 namespace rb {
 
+static_assert(kMaxDevices <= 32, "a bit for each device");
+
 template <int NG, int RB, bool SPLIT>
 static cudaError_t launch_decode(const Kv4AttnArgs &a, const rabbit_cuda_kv4 *kv, cudaStream_t s) {
     using C = DecodeCfg<NG, RB, SPLIT>;

@@ -241,7 +241,11 @@ int rabbit_cuda_rope_dev(const rabbit_cuda_rope *r, int dtype, const void *d_x, 
     // up to a CTA an SM in all. 16384 x 32 x 128 bf16: 28 tokens a CTA 55 us (4.9
     // TB/s), 2 tokens 74 us.
     const int64_t items = (int64_t)n_heads * a.per;
-    const int sms = 148;
+    int sms = 0;
+    DeviceScope scope(current_device());
+    if (scope.status == RABBIT_CUDA_OK)
+        scope.launch(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, current_device()), "rope_dev: SM count");
+    if (scope.status != RABBIT_CUDA_OK) return scope.status;
     const int64_t wave = ((int64_t)n_tokens + 4 * sms - 1) / (4 * sms);
     const int most = 48 * 1024 / (int)(sizeof(float2) * (a.tab.rot / 2));  // their angles' shared memory
     a.tpc = wave > 32 ? 32 : (int)wave;
@@ -251,8 +255,6 @@ int rabbit_cuda_rope_dev(const rabbit_cuda_rope *r, int dtype, const void *d_x, 
     if (split > sms / groups) split = sms / groups;
     const dim3 grid(groups, split < 1 ? 1 : (unsigned)split);
     const size_t smem = sizeof(float2) * (size_t)a.tpc * (a.tab.rot / 2);
-    DeviceScope scope(current_device());
-    if (scope.status != RABBIT_CUDA_OK) return scope.status;
     with_dtype(dtype, [&](auto t) {
         using T = decltype(t);
         constexpr int VT = 16 / sizeof(T);
