@@ -600,9 +600,13 @@ int rabbit_cuda_kv4_scratch_free(rabbit_cuda_kv4_scratch *ws);
  * nothing there; a sequence whose q_start is out of order, past n_tokens or
  * longer than max_q_len gets no rows. n_tokens 0 or n_seqs 0 does nothing. A
  * visible group of 32 channels that holds an infinity or a NaN makes NaN of the
- * rows that see it (a key's) or of their 32 channels (a value's). DEVICE
- * buffers aligned to their element, asynchronous on `stream`; may be captured
- * into a graph. */
+ * rows that see it (a key's) or of their 32 channels (a value's); what a row does not
+ * see has no part in it. Sums are fp32; with 16-bit queries each weight, times its value's
+ * scale, is rounded to fp16 (2^-11; with fp32 queries to 22 bits). Beside one far larger,
+ * small numbers lose bits: channels 2^22 below the largest of a 16-bit query row, weights
+ * 2^20 below the largest of a row, and in chunks of 16-bit queries channel groups 2^29 below the
+ * largest of their token. DEVICE buffers aligned to their element, asynchronous on
+ * `stream`; may be captured into a graph. */
 int rabbit_cuda_kv4_attention_dev(rabbit_cuda_kv4 *kv, int layer, rabbit_cuda_kv4_scratch *ws,
                                   int dtype, const void *d_q, int64_t q_stride, void *d_out,
                                   int64_t out_stride, int n_tokens, int n_heads,

@@ -33,11 +33,22 @@ static cudaError_t launch_decode(const Kv4AttnArgs &a, const rabbit_cuda_kv4 *kv
     return launch_pdl(kern, dim3(grid < kDecodeMaxGrid ? grid : kDecodeMaxGrid), dim3(C::kThreads), C::kSmem, s, a);
 }
 
-// CTAs of the chunk kernel from which it is taken. Its time goes by the rows and
-// positions of one CTA; the other's, which spreads a KV head's positions over the
-// SMs, by the whole batch. 256 rows x 4 heads a KV head over 4352 positions: 91 us
-// here with 16 to 128 CTAs; there 34 us for the work of 16 of them, 51 of 32, 85 of
-// 64, 149 of 128.
+// CTAs of the chunk kernel from which it is taken. Its time goes by the positions of one
+// CTA and the CTAs an SM takes in turn; the other's, which spreads a KV head's positions
+// over the SMs, by the whole batch's granules times ceil(rows / 16). us, chunk / decode kernel,
+// bf16, 8 KV heads, for equal numbers of query rows a KV head and sequence:
+//   sequences x rows      1000 positions   4096        16384
+//   4 x 64 (32 CTAs)      29 / 31          91 / 51     343 / 136
+//   4 x 128 (64)          29 / 46          92 / 83     343 / 250
+//   10 x 20 (80)          29 / 34          92 / 59     351 / 163
+//   10 x 64 (80)          29 / 50          93 / 96     353 / 307
+//   16 x 20 (128)         29 / 44          93 / 81     345 / 249
+//   16 x 64 (128)         30 / 70          93 / 140    345 / 479
+//   64 x 20 (512)         73 / 124         331 / 241   -
+//   64 x 48 (512)         76 / 188         332 / 355   -
+// The rule goes by the CTAs alone, since the host does not know the lengths. It gives away
+// 1.1 to 2.1 times for 17 to 32 rows over more than 2000 positions (decoding with drafts),
+// and up to 1.6 times elsewhere.
 constexpr int kChunkMinCtas = 72;
 
 template <int NG>

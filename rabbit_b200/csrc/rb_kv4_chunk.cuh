@@ -13,15 +13,17 @@
 // up, p 2^ev multiplies the values, with the reference M, D as in rb_kv4_decode.cuh),
 // that brings its largest scale to [2^12, 2^13). So what a row does not see, of whatever
 // size, has no part in it. Of one token the channel groups whose scale is at least
-// 2^-29 of its largest are exact; below 2^-37 they are zero. The weights are rounded to
-// fp16 (2^-11).
+// 2^-29 of its largest are exact; below 2^-37 they are zero. Query channels 2^22 below
+// their row's largest lose bits. The weights are rounded to fp16 (2^-11).
 //
 // Bound by the latency of the two kinds of warps, not yet by the matrix
-// instructions: 64 rows x 64 positions x 128 channels are 512 of those, 1024 cycles
-// of the four sub-partitions; a tile takes some 2500. With 4 warps of either kind
-// 119 us (256 rows x 4 heads a KV head over 4352 positions of 8 KV heads, bf16, 128
-// CTAs), 8 making 130 us (the others then spilled), 8 multiplying 122 us, 8 of
-// either 91 us: 194 TFLOP/s, 0.12 of the measured cuBLAS bf16 rate.
+// instructions (tensor pipe 39 %, issue slots 50 %): 64 rows x 64 positions x 128 channels
+// are 512 of those, 1024 cycles of the four sub-partitions; a tile takes some 2700.
+// 256 rows x 4 heads a KV head over 4352 positions of 8 KV heads, bf16, 128 CTAs: 97 us,
+// 183 TFLOP/s, 0.11 of the measured cuBLAS bf16 rate. Of the splits, measured with one
+// exponent a granule: 4 warps of either kind 119 us, 8 making 130 us (the others then spilled),
+// 8 multiplying 122 us, 8 of either 91 us; the tokens' own exponents take 4 us more,
+// the reference in two parts 2.
 #pragma once
 #include <type_traits>
 

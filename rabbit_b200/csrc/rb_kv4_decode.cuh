@@ -36,11 +36,16 @@
 //    would leave no room for D. x is rounded to fp32 before M is taken off, so that
 //    equal scores stay equal to their reference.)
 //
-// Bound by its instructions, 387 a granule (2304 bytes at 128 channels; 16-bit
-// queries) at 55 % of the issue slots, half of them on the ALU pipe: 49 us for 1 x
-// 131072 positions of 8 KV heads (3.05 TB/s, 0.47 of the measured copy rate), 59 us
-// for 64 x 4096 (0.45), 195 us for 128 x 8192 (0.56). fp32 queries take two terms: 65
-// us for 16 sequences of 4 rows, 6 query heads a KV head, and 2048 positions.
+// Bound by its instructions, 376 for each further granule (2304 bytes at 128 channels;
+// 16-bit queries), 46 % of a launch's issue slots with its start and merge: 49 us for 1 x
+// 131072 positions of 8 KV heads (3.06 TB/s, 0.47 of the measured copy rate), 61 us
+// for 64 x 4096 (0.44), 194 us for 128 x 8192 (0.56). fp32 queries take two terms: 67
+// us for 16 sequences of 4 rows, 6 query heads a KV head, and 2048 positions; with 16 rows
+// a tile they spill 60 / 96 bytes of stores / loads at 168 registers.
+//
+// Range: bf16 has fp32's exponents and a query operand fp16's, so channels more than 2^24
+// below their row's largest lose bits. A value's weight p s is rounded to fp16, which
+// keeps its bits down to 2^-20 of the row's largest weight and is zero from 2^-31.
 #pragma once
 #include "rb_device.cuh"
 #include "rb_kv4_attn.cuh"
