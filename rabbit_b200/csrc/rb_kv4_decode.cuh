@@ -284,7 +284,7 @@ __device__ __forceinline__ void make_operands(const Kv4AttnArgs &a, uint8_t *que
         const float up = __uint_as_float((uint32_t)(127 + 14 - e) << 23);
         const float down = __uint_as_float((uint32_t)(127 - 14 + e) << 23);
         const float sup = a.scale < 0.f ? -up : up;
-        if (t == 0) unit[8 * rb + g] = fabsf(a.scale) * down * (SPLIT ? 1.0f : 16777216.0f);
+        if (t == 0) unit[8 * rb + g] = fabsf(a.scale) * (down * 16777216.0f);
 #pragma unroll
         for (int grp = 0; grp < NG; ++grp) {
             float sum = 0.f, y[8];
@@ -686,7 +686,10 @@ __global__ void __launch_bounds__(DecodeCfg<NG, RB, SPLIT>::kThreads, 1)
                     uint32_t e0[4], e1[4];
                     key_codes<SPLIT>(e0, k0[grp]);
                     key_codes<SPLIT>(e1, k1[grp]);
-                    const float f0 = piece_bf16(s0, grp), f1 = piece_bf16(s1, grp);
+                    // signed codes are whole numbers: 2^-24 goes into their scale, so that sums with
+                    // the largest keys stay finite
+                    const float by = SPLIT ? 1.0f / 16777216.0f : 1.0f;
+                    const float f0 = piece_bf16(s0, grp) * by, f1 = piece_bf16(s1, grp) * by;
 #pragma unroll
                     for (int rb = 0; rb < RB; ++rb) {
                         float d[4];

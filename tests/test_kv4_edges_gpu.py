@@ -489,3 +489,18 @@ def test_a_query_that_is_not_finite_stays_in_its_row(torch, rc, kw):
     odd[0, 1] = odd[-1, 0] = odd[-1, -1] = True
     assert np.isnan(got[odd]).all()
     np.testing.assert_array_equal(got[~odd], want[~odd])
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("kw", CHUNKS + DECODES)
+def test_keys_of_the_largest_numbers(torch, rc, kw, dtype):
+    """Keys up to 3e38 under queries that bring the scores back to a few units."""
+    c = Close(torch, rc, seed=54, poison=False, scale=2.0 ** -115, **{**kw, "dtype": dtype})
+    g = torch.Generator("cuda").manual_seed(55)
+    n = c.kv.n_pages * c.page
+    k, v = (torch.rand(n, c.nkv, c.hd, generator=g, device="cuda") * 2 - 1 for _ in "kv")
+    rewrite(torch, rc, c, np.arange(n), k * 3e38, v)
+    q = torch.randn(c.rows, c.nh, c.hd, generator=g, device="cuda") * 2.0 ** -13
+    c.qbuf.copy_(q.to(c.qbuf.dtype).flatten())
+    c.call()
+    c.check()
