@@ -605,9 +605,9 @@ int rabbit_cuda_kv4_scratch_free(rabbit_cuda_kv4_scratch *ws);
  * scale, is rounded to fp16 (2^-11; with fp32 queries to 22 bits). Beside one far larger,
  * small numbers lose bits: channels 2^22 below the largest of a 16-bit query row, weights
  * 2^20 below the largest of a row, and in chunks of 16-bit queries channel groups 2^29 below the
- * largest of their token; beside values past 1e34 weights 2^20 below the largest are
- * lost. DEVICE buffers aligned to their element, asynchronous on
- * `stream`; may be captured into a graph. */
+ * largest of their token; beside values of 2^X, X above 114, weights 2^(134 - X) below the
+ * largest are lost. DEVICE buffers aligned to their element, asynchronous on `stream`;
+ * may be captured into a graph. */
 int rabbit_cuda_kv4_attention_dev(rabbit_cuda_kv4 *kv, int layer, rabbit_cuda_kv4_scratch *ws,
                                   int dtype, const void *d_q, int64_t q_stride, void *d_out,
                                   int64_t out_stride, int n_tokens, int n_heads,
