@@ -54,7 +54,7 @@ constexpr int kChunkMinCtas = 72;
 template <int NG>
 static cudaError_t launch_chunk(const Kv4AttnArgs &a, int tiles, const rabbit_cuda_kv4 *kv, cudaStream_t s) {
     using C = ChunkCfg<NG>;
-    static_assert(C::kSmem + 3072 <= kMaxDynSmem, "shared memory of a CTA, the static part with it");
+    static_assert(C::kSmem + 4096 <= kMaxDynSmem, "shared memory of a CTA, the static part with it");
     auto kern = k_kv4_chunk<NG>;
     static std::atomic<uint32_t> ready{0};  // devices whose limit is raised
     if (!(ready.load() >> kv->device & 1u)) {

@@ -39,7 +39,7 @@
 // Bound by its instructions, 376 for each further granule (2304 bytes at 128 channels;
 // 16-bit queries), 46 % of a launch's issue slots with its start and merge: 49 us for 1 x
 // 131072 positions of 8 KV heads (3.06 TB/s, 0.47 of the measured copy rate), 61 us
-// for 64 x 4096 (0.44), 194 us for 128 x 8192 (0.56). fp32 queries take two terms: 67
+// for 64 x 4096 (0.44), 195 us for 128 x 8192 (0.56). fp32 queries take two terms: 68
 // us for 16 sequences of 4 rows, 6 query heads a KV head, and 2048 positions; with 16 rows
 // a tile they spill 60 / 96 bytes of stores / loads at 168 registers.
 //
