@@ -378,7 +378,9 @@ class Close(base.Case):
                         n * 7 * 2.0 ** -31 * (w[:, :, None] * self.vs[s, h // G]).max(1))
                 out[row:row + nq, h] = o
             row += nq
-        return out, bar + 1.01 * ko.HALF_STEP[self.dtype] * (np.abs(out) + bar) + 1e-30
+        # half a step of the output's type: of its value, of its smallest for subnormal fp16
+        least = 2.0 ** -25 if self.dtype == "f16" else 1e-30
+        return out, bar + 1.01 * ko.HALF_STEP[self.dtype] * (np.abs(out) + bar) + least
 
 
 @pytest.mark.parametrize("i", range(len(base.ATTN)))
