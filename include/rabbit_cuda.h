@@ -624,6 +624,109 @@ int rabbit_cuda_kv4_check(rabbit_cuda_kv4 *kv, void *stream);
  * rows of it not written, and its scratch spoiled. */
 int rabbit_cuda_kv4_debug_withhold(rabbit_cuda_kv4 *kv);
 
+/* ------------------------------- 8-bit rows, products, expert batches -- */
+
+/* Models whose dense projections or experts come in e4m3 with a scale for each
+ * block of 128, or in 16 bits (the reference has int4, int8 and fp32 experts,
+ * src/forward_v2.c:297-354, one token at a time). An expert layer of any number of tokens:
+ *   rabbit_cuda_experts_route_dev      which experts, and the order by expert
+ *   rabbit_cuda_linear_grouped_dev     silu(gate) * up of each expert's rows
+ *   rabbit_cuda_f8_quantise_dev        (e4m3) its result as 8-bit rows
+ *   rabbit_cuda_linear_grouped_dev     down
+ *   rabbit_cuda_experts_combine_dev    back to the tokens, weighted and added
+ * Everything is asynchronous on `stream`, allocates nothing, may be captured into a
+ * graph, and keeps nothing between calls, so calls on different streams may run at the
+ * same time. Unless said otherwise a stride is in elements between rows and 0 means
+ * rows without a gap; pointers are aligned to their element. */
+
+/* Element type of 8-bit rows and weights: 4 exponent and 3 mantissa bits, largest value 448. */
+#define RABBIT_CUDA_E4M3 3
+
+/* Rows (block_rows 1) or blocks of 128 rows (block_rows 128) of x [n_rows][n_cols] (f32, f16 or
+ * bf16) as e4m3 codes with a scale for each 128 consecutive columns (the last block of columns
+ * or rows may be shorter):
+ *   s = fp32(max|x| / 448),  q = e4m3(x / s), to nearest, ties to even; held at +-448
+ * both as of the exact quotient; s = 0: all zero. A block that holds an infinity or a NaN has
+ * s = NaN and codes NaN. q [n_rows] rows of q_stride bytes; d_scale [n_rows or its blocks][n_cols /
+ * 128 rounded up]. With d_rows (block_rows 1 only) row i is row d_rows[i] of the x_rows rows
+ * of x; where that is outside of them, row i of q and of d_scale is left as it was. x_rows is
+ * not read without d_rows. n_rows 0 does nothing. On the calling thread's device. */
+int rabbit_cuda_f8_quantise_dev(int dtype, const void *d_x, int64_t x_stride, int x_rows,
+                                const int *d_rows, void *d_q, int64_t q_stride, float *d_scale,
+                                int n_rows, int n_cols, int block_rows, void *stream);
+
+/* The weights of products y = x W^T: one matrix, or one for each expert. */
+typedef struct {
+    int dtype;             /* of W and x: RABBIT_CUDA_E4M3, _F16 or _BF16 */
+    int n_experts;         /* 1..1024 */
+    int gated;             /* 0: y = x W^T; 1: each W is gate, then up, and y = silu(x gate^T) * (x up^T) */
+    int n_out, n_in;       /* rows and columns of W (of gate, and of up), 1..2^20 */
+    const void *d_w;       /* [n_experts][1 or, gated, 2][n_out] rows, 16-byte aligned */
+    int64_t w_stride;      /* elements between rows, a multiple of 16 bytes; 0 means n_in */
+    const float *d_scale;  /* E4M3: [n_experts][1 or 2][n_out / 128][n_in / 128], rounded up */
+} rabbit_cuda_linear_desc;
+
+typedef struct rabbit_cuda_linear rabbit_cuda_linear;
+
+/* Checks `desc` and prepares its loads on `device`. The weights stay the caller's, are
+ * not copied, and may be rewritten between calls; calls read them while they run. Several objects may share
+ * weights. */
+int rabbit_cuda_linear_create(const rabbit_cuda_linear_desc *desc, int device,
+                              rabbit_cuda_linear **out);
+/* After the calls that use it have run. */
+int rabbit_cuda_linear_free(rabbit_cuda_linear *lin);
+/* y [n_rows][n_out] (f32, f16 or bf16) = x [n_rows][n_in] times the one matrix. x of the weights'
+ * type, 16-byte aligned, its stride a multiple of 16 bytes. E4M3: d_x_scale, rows of x_scale_stride
+ * floats, n_in / 128 rounded up of them, and
+ *   y = sum_b sx[row][b] sw[n / 128][b] sum_{k in block b} x[row][k] w[n][k].
+ * Sums are fp32 (a block's on the tensor cores, then over the blocks in order), rounded to
+ * out_dtype once; silu in fp32. Infinities and NaN go where the formula takes them, and to
+ * no other row. y must not overlap an input. n_rows 0 does nothing. */
+int rabbit_cuda_linear_dev(rabbit_cuda_linear *lin, const void *d_x, int64_t x_stride,
+                           const float *d_x_scale, int64_t x_scale_stride, int out_dtype, void *d_y,
+                           int64_t y_stride, int n_rows, void *stream);
+/* Rows d_offsets[e] .. d_offsets[e + 1] - 1 of y [n_rows] from expert e; d_offsets [n_experts + 1]
+ * ascending within 0..n_rows, read when the call runs. Row i of y comes from row i of x or, with
+ * d_rows [n_rows], from row d_rows[i] of its x_rows rows (without: x_rows >= n_rows). Rows outside of
+ * every expert's, and rows whose d_rows entry is outside of x, are left as they were. Reported by
+ * rabbit_cuda_linear_check: offsets out of order or range (the call then writes
+ * nothing), an entry of d_rows within an expert's rows that is outside of x. */
+int rabbit_cuda_linear_grouped_dev(rabbit_cuda_linear *lin, const void *d_x, int64_t x_stride,
+                                   int x_rows, const float *d_x_scale, int64_t x_scale_stride,
+                                   const int *d_rows, const int *d_offsets, int out_dtype,
+                                   void *d_y, int64_t y_stride, int n_rows, void *stream);
+/* Synchronises `stream` and reports, once, what calls with this object found out of range
+ * since the last check (RABBIT_CUDA_ERR_ARGS) or a bounded wait that gave up
+ * (RABBIT_CUDA_ERR_TIMEOUT; rows of that call are not written, or wrong). */
+int rabbit_cuda_linear_check(rabbit_cuda_linear *lin, void *stream);
+
+/* k experts for each of n_tokens tokens, and the order by expert. With d_scores [n_tokens]
+ * rows of n_experts (stride score_stride): the k largest scores, the lower id first among
+ * equals (select_top_k, src/forward_v2.c:248-278), into d_ids [n_tokens][k], and d_weights
+ * [n_tokens][k] = softmax over the k taken (the reference's) or, over_all = 1, over all
+ * scores. A score of -inf or NaN is never taken: where fewer are left, id -1 and weight 0. Without
+ * d_scores (NULL) d_ids is read (any order, repeats allowed; an id outside of 0..n_experts - 1 has no
+ * expert) and d_weights is not used. Then, over the pairs p = t * k + j that have an expert, by
+ * expert and within it by p:
+ *   d_offsets [n_experts + 1]  places of expert e: d_offsets[e] .. d_offsets[e + 1] - 1
+ *   d_rows [n_tokens * k]      token of each place; -1 behind the last
+ *   d_place [n_tokens][k]      place of each pair; -1 without an expert
+ * 1 <= n_experts <= 1024, 1 <= k <= min(n_experts, 32), n_tokens * k below 2^30; n_tokens 0 writes
+ * d_offsets. On the calling thread's device. */
+int rabbit_cuda_experts_route_dev(const float *d_scores, int64_t score_stride, int n_tokens,
+                                  int n_experts, int k, int over_all, int *d_ids, float *d_weights,
+                                  int *d_offsets, int *d_rows, int *d_place, void *stream);
+
+/* out[t] = base[t] + sum_j weights[t][j] y[place[t][j]], in the order of j, in fp32, rounded
+ * once: y [y_rows] rows of n_cols in dtype, base (may be NULL: 0; may be out, with the same stride)
+ * and out in out_dtype. A place outside of 0..y_rows - 1 adds nothing. out must not
+ * overlap y. 1 <= k <= 32. n_tokens 0 does nothing. On the calling thread's device. */
+int rabbit_cuda_experts_combine_dev(int dtype, const void *d_y, int64_t y_stride, int y_rows,
+                                    const int *d_place, const float *d_weights, int n_tokens, int k,
+                                    int n_cols, int out_dtype, const void *d_base,
+                                    int64_t base_stride, void *d_out, int64_t out_stride,
+                                    void *stream);
+
 #if defined(__GNUC__)
 #pragma GCC visibility pop
 #endif

@@ -64,6 +64,13 @@ class Kv4Batch(C.Structure):
                 ("d_q_start", C.c_void_p), ("d_kv_len", C.c_void_p), ("d_page_table", C.c_void_p)]
 
 
+class LinearDesc(C.Structure):
+    """rabbit_cuda_linear_desc"""
+    _fields_ = [("dtype", C.c_int), ("n_experts", C.c_int), ("gated", C.c_int),
+                ("n_out", C.c_int), ("n_in", C.c_int), ("d_w", C.c_void_p),
+                ("w_stride", C.c_int64), ("d_scale", C.c_void_p)]
+
+
 _P = C.c_void_p
 _I = C.c_int
 _L = C.c_int64
@@ -153,6 +160,15 @@ SIGNATURES = {
                                            C.POINTER(Kv4Batch), C.c_float, _I, _P]),
     "rabbit_cuda_kv4_check": (_I, [_P, _P]),
     "rabbit_cuda_kv4_debug_withhold": (_I, [_P]),
+    "rabbit_cuda_f8_quantise_dev": (_I, [_I, _P, _L, _I, _P, _P, _L, _P, _I, _I, _I, _P]),
+    "rabbit_cuda_linear_create": (_I, [C.POINTER(LinearDesc), _I, C.POINTER(_P)]),
+    "rabbit_cuda_linear_free": (_I, [_P]),
+    "rabbit_cuda_linear_dev": (_I, [_P, _P, _L, _P, _L, _I, _P, _L, _I, _P]),
+    "rabbit_cuda_linear_grouped_dev": (_I, [_P, _P, _L, _I, _P, _L, _P, _P, _I, _P, _L, _I, _P]),
+    "rabbit_cuda_linear_check": (_I, [_P, _P]),
+    "rabbit_cuda_experts_route_dev": (_I, [_P, _L, _I, _I, _I, _I, _P, _P, _P, _P, _P, _P]),
+    "rabbit_cuda_experts_combine_dev": (_I, [_I, _P, _L, _I, _P, _P, _I, _I, _I, _I, _P, _L, _P,
+                                             _L, _P]),
 }
 
 _LIB: C.CDLL | None = None
@@ -583,7 +599,7 @@ class Cache:
             self.handle = None
 
 
-F32, F16, BF16 = range(3)  # RABBIT_CUDA_F32 ...
+F32, F16, BF16, E4M3 = range(4)  # RABBIT_CUDA_F32 ...
 ROPE_INTERLEAVED, ROPE_HALF = range(2)
 (ROPE_SCALE_NONE, ROPE_SCALE_LINEAR, ROPE_SCALE_NTK, ROPE_SCALE_BANDS,
  ROPE_SCALE_YARN) = range(5)
@@ -706,3 +722,79 @@ class Kv4Scratch:
             self.free()
         except Exception:
             pass
+
+
+def f8_quantise_dev(dtype: int, d_x: int, d_q: int, d_scale: int, n_rows: int, n_cols: int, *,
+                    block_rows: int = 1, d_rows: int = 0, x_rows: int = 0, x_stride: int = 0,
+                    q_stride: int = 0, stream: int = 0) -> None:
+    """Rows or 128 x 128 blocks as e4m3 codes with a scale for each 128 columns
+    (rabbit_cuda_f8_quantise_dev). Device pointers as ints."""
+    check(lib().rabbit_cuda_f8_quantise_dev(dtype, d_x, x_stride, x_rows, d_rows or None, d_q,
+                                            q_stride, d_scale, n_rows, n_cols, block_rows,
+                                            stream or None))
+
+
+class Linear:
+    """Weights of products y = x W^T in e4m3 with a scale for each 128 x 128 block,
+    fp16 or bf16; one matrix or one for each expert (rabbit_cuda_linear). The
+    weights stay the caller's. Device pointers as ints."""
+
+    def __init__(self, dtype: int, n_out: int, n_in: int, d_w: int, *, n_experts: int = 1,
+                 gated: bool = False, w_stride: int = 0, d_scale: int = 0, device: int = 0):
+        d = LinearDesc(dtype, n_experts, int(gated), n_out, n_in, d_w, w_stride, d_scale or None)
+        h = C.c_void_p()
+        check(lib().rabbit_cuda_linear_create(C.byref(d), device, C.byref(h)))
+        self.handle = h
+        self.dtype, self.n_out, self.n_in, self.n_experts = dtype, n_out, n_in, n_experts
+
+    def apply_dev(self, d_x: int, out_dtype: int, d_y: int, n_rows: int, *, x_stride: int = 0,
+                  d_x_scale: int = 0, x_scale_stride: int = 0, y_stride: int = 0,
+                  stream: int = 0) -> None:
+        """y = x W^T, gated silu(x gate^T) * (x up^T) (rabbit_cuda_linear_dev)."""
+        check(lib().rabbit_cuda_linear_dev(self.handle, d_x, x_stride, d_x_scale or None,
+                                           x_scale_stride, out_dtype, d_y, y_stride, n_rows,
+                                           stream or None))
+
+    def grouped_dev(self, d_x: int, x_rows: int, d_offsets: int, out_dtype: int, d_y: int,
+                    n_rows: int, *, d_rows: int = 0, x_stride: int = 0, d_x_scale: int = 0,
+                    x_scale_stride: int = 0, y_stride: int = 0, stream: int = 0) -> None:
+        """Rows d_offsets[e] .. d_offsets[e + 1] - 1 of y from expert e, of x or of its rows
+        d_rows (rabbit_cuda_linear_grouped_dev)."""
+        check(lib().rabbit_cuda_linear_grouped_dev(
+            self.handle, d_x, x_stride, x_rows, d_x_scale or None, x_scale_stride, d_rows or None,
+            d_offsets, out_dtype, d_y, y_stride, n_rows, stream or None))
+
+    def check(self, stream: int = 0) -> None:
+        check(lib().rabbit_cuda_linear_check(self.handle, stream or None))
+
+    def free(self) -> None:
+        if self.handle:
+            check(lib().rabbit_cuda_linear_free(self.handle))
+            self.handle = C.c_void_p()
+
+    def __del__(self):
+        try:
+            self.free()
+        except Exception:
+            pass
+
+
+def experts_route_dev(d_scores: int, n_tokens: int, n_experts: int, k: int, d_ids: int,
+                      d_weights: int, d_offsets: int, d_rows: int, d_place: int, *,
+                      score_stride: int = 0, over_all: bool = False, stream: int = 0) -> None:
+    """k experts for each token and the order by expert; with d_scores 0 the ids are given
+    (rabbit_cuda_experts_route_dev). Device pointers as ints."""
+    check(lib().rabbit_cuda_experts_route_dev(d_scores or None, score_stride, n_tokens, n_experts,
+                                              k, int(over_all), d_ids, d_weights or None,
+                                              d_offsets, d_rows, d_place, stream or None))
+
+
+def experts_combine_dev(dtype: int, d_y: int, y_rows: int, d_place: int, d_weights: int,
+                        n_tokens: int, k: int, n_cols: int, out_dtype: int, d_out: int, *,
+                        d_base: int = 0, y_stride: int = 0, base_stride: int = 0,
+                        out_stride: int = 0, stream: int = 0) -> None:
+    """out[t] = base[t] + sum_j weights[t, j] y[place[t, j]] (rabbit_cuda_experts_combine_dev).
+    Device pointers as ints."""
+    check(lib().rabbit_cuda_experts_combine_dev(dtype, d_y, y_stride, y_rows, d_place, d_weights,
+                                                n_tokens, k, n_cols, out_dtype, d_base or None,
+                                                base_stride, d_out, out_stride, stream or None))

@@ -1,0 +1,246 @@
+// rb_f8.cu -- C ABI: rows and blocks as e4m3 codes with a scale for each 128
+// columns.
+//
+// Bound by memory: x is read and its codes are written once. The codes are those of the
+// exact quotient x / s without a division for each value: with r = fp32(1 / s),
+//   |x| r (1 - 2^-22) <= |x| / s <= |x| r (1 + 2^-22)
+// holds for the computed products (r and two products round by 2^-24 each), rounding to
+// e4m3 is monotone, so where both ends give one code it is the quotient's. Where they give two
+// neighbours, the sign of x - m s, m the middle between them, decides; one fma has it exactly.
+// 16384 rows of 4096 bf16: see the launch below.
+#include <cuda_fp8.h>
+
+#include "rb_device.cuh"
+#include "rb_launch.h"
+#include "rb_runtime.h"
+#include "rb_types.cuh"
+
+namespace rb {
+
+struct F8Args {
+    const void *x;
+    int64_t xs;
+    const int *rows;  // [n_rows] or NULL
+    int x_rows;
+    uint8_t *q;
+    int64_t qs;
+    float *scale;
+    int n_rows, n_cols, nb;  // nb: blocks of 128 columns
+};
+
+constexpr int kF8Threads = 256;
+constexpr uint32_t kInfBits = 0x7F800000u;
+
+// e4m3 codes of two values, to nearest even, held at +-448 (a in the low byte).
+__device__ __forceinline__ uint32_t e4m3x2(float a, float b) {
+    return __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
+}
+__device__ __forceinline__ float e4m3_value(uint32_t code) {
+    return __half2float(__half(__nv_cvt_fp8_to_halfraw((__nv_fp8_storage_t)code, __NV_E4M3)));
+}
+
+// A block's scale from the bits of its largest |x|, and what its codes are made with.
+struct F8Scale {
+    float s, lo, hi, grow;  // grow: x and s are multiplied by it for tiny scales
+    bool zero, bad;
+};
+__device__ __forceinline__ F8Scale f8_scale(uint32_t top) {
+    F8Scale f;
+    f.bad = top >= kInfBits;
+    f.s = __fdiv_rn(__uint_as_float(top), 448.f);
+    f.zero = f.s == 0.f;
+    // below 2^-60: by 2^64 on, where 1 / s and the remainders are far from fp32's smallest
+    f.grow = f.s < 8.67361738e-19f ? 18446744073709551616.f : 1.f;
+    const float r = __frcp_rn(f.s * f.grow);
+    f.lo = r * (1.f - 0x1p-22f);
+    f.hi = r * (1.f + 0x1p-22f);
+    if (f.bad) f.s = __uint_as_float(0x7FC00000u);
+    return f;
+}
+
+__device__ __noinline__ uint32_t f8_between(float x, float s, uint32_t a, uint32_t b) {
+    // codes a and b (of one sign, b = a + 1 in magnitude)
+    const float m = 0.5f * (fabsf(e4m3_value(a)) + fabsf(e4m3_value(b)));
+    const float d = fmaf(-m, s, fabsf(x));
+    return d < 0.f ? a : d > 0.f ? b : (a & 1) ? b : a;
+}
+
+// Codes of four values, the first in the low byte.
+__device__ __forceinline__ uint32_t f8_codes(const float (&x)[4], const F8Scale &f) {
+    if (f.bad) return 0x7F7F7F7Fu;
+    if (f.zero) return 0u;
+    float v[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = x[i] * f.grow;
+    const uint32_t a = e4m3x2(v[0] * f.lo, v[1] * f.lo) | e4m3x2(v[2] * f.lo, v[3] * f.lo) << 16;
+    const uint32_t b = e4m3x2(v[0] * f.hi, v[1] * f.hi) | e4m3x2(v[2] * f.hi, v[3] * f.hi) << 16;
+    if (a == b) return a;
+    uint32_t c = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const uint32_t ai = a >> (8 * i) & 255, bi = b >> (8 * i) & 255;
+        c |= (ai == bi ? ai : f8_between(v[i], f.s * f.grow, ai, bi)) << (8 * i);
+    }
+    return c;
+}
+
+// Eight values of a row from column c on; past the row zeros.
+template <typename T, bool VEC>
+__device__ __forceinline__ void f8_load(float (&d)[8], const T *row, int c, int n_cols) {
+    if (c + 8 <= n_cols) {
+        load8<VEC>(d, row + c);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) d[i] = c + i < n_cols ? to_f32(row[c + i]) : 0.f;
+    }
+}
+__device__ __forceinline__ uint32_t f8_top(const float (&d)[8]) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(d[i]) & 0x7FFFFFFFu);
+    return m;
+}
+template <bool VEC>
+__device__ __forceinline__ void f8_store(uint8_t *row, int c, int n_cols, const float (&d)[8],
+                                         const F8Scale &f) {
+    const float lo[4] = {d[0], d[1], d[2], d[3]}, hi[4] = {d[4], d[5], d[6], d[7]};
+    const uint2 w = make_uint2(f8_codes(lo, f), f8_codes(hi, f));
+    if (VEC && c + 8 <= n_cols) {
+        *reinterpret_cast<uint2 *>(row + c) = w;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (c + i < n_cols) row[c + i] = (uint8_t)((i < 4 ? w.x : w.y) >> (8 * (i & 3)));
+    }
+}
+
+// One scale for each row's block: 16 lanes hold a block, eight values each; BATCH
+// blocks of each half warp are in flight.
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(kF8Threads) k_f8_rows(const __grid_constant__ F8Args a) {
+    constexpr int BATCH = 4;
+    launch_dependents();
+    wait_prerequisite();
+    const int64_t items = (int64_t)a.n_rows * a.nb;
+    const int lane = threadIdx.x & 15;
+    const int64_t teams = (int64_t)gridDim.x * (kF8Threads / 16);
+    for (int64_t i0 = ((int64_t)blockIdx.x * kF8Threads + threadIdx.x) / 32 * 2; i0 < items;
+         i0 += teams * BATCH) {
+        float d[BATCH][8];
+        int64_t at[BATCH];
+        int col[BATCH];
+#pragma unroll
+        for (int b = 0; b < BATCH; ++b) {  // a warp's two blocks side by side, then `teams` on
+            const int64_t i = i0 + (threadIdx.x >> 4 & 1) + b * teams;
+            at[b] = -1;
+            if (i < items) {
+                const int64_t r = items >> 31 ? i / a.nb : (int)i / a.nb;
+                col[b] = (int)(i - r * a.nb) * 128 + lane * 8;
+                const int64_t src = a.rows ? __ldg(a.rows + r) : r;
+                if (!a.rows || (src >= 0 && src < a.x_rows)) {
+                    at[b] = r;
+                    f8_load<T, VEC>(d[b], static_cast<const T *>(a.x) + src * a.xs, col[b], a.n_cols);
+                }
+            }
+            if (at[b] < 0) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) d[b][j] = 0.f;
+            }
+        }
+#pragma unroll
+        for (int b = 0; b < BATCH; ++b) {
+            uint32_t top = f8_top(d[b]);
+#pragma unroll
+            for (int m = 8; m; m >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, m));
+            if (at[b] < 0) continue;
+            const F8Scale f = f8_scale(top);
+            f8_store<VEC>(a.q + at[b] * a.qs, col[b], a.n_cols, d[b], f);
+            if (lane == 0) a.scale[at[b] * a.nb + col[b] / 128] = f.s;
+        }
+    }
+}
+
+// One scale for each 128 rows x 128 columns: a CTA holds the block in registers.
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(kF8Threads) k_f8_blocks(const __grid_constant__ F8Args a) {
+    __shared__ uint32_t warp_top[kF8Threads / 32];
+    launch_dependents();
+    wait_prerequisite();
+    const int r0 = blockIdx.x * 128, c = blockIdx.y * 128 + (threadIdx.x & 15) * 8;
+    float d[8][8];
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const int r = r0 + (threadIdx.x >> 4) + 16 * i;
+        if (r < a.n_rows) {
+            f8_load<T, VEC>(d[i], static_cast<const T *>(a.x) + r * a.xs, c, a.n_cols);
+            top = max(top, f8_top(d[i]));
+        }
+    }
+    top = __reduce_max_sync(0xffffffffu, top);
+    if ((threadIdx.x & 31) == 0) warp_top[threadIdx.x >> 5] = top;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kF8Threads / 32; ++i) top = max(top, warp_top[i]);
+    const F8Scale f = f8_scale(top);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const int r = r0 + (threadIdx.x >> 4) + 16 * i;
+        if (r < a.n_rows) f8_store<VEC>(a.q + r * a.qs, c, a.n_cols, d[i], f);
+    }
+    if (threadIdx.x == 0) a.scale[(int64_t)blockIdx.x * a.nb + blockIdx.y] = f.s;
+}
+
+}  // namespace rb
+
+using namespace rb;
+
+extern "C" int rabbit_cuda_f8_quantise_dev(int dtype, const void *d_x, int64_t x_stride, int x_rows,
+                                           const int *d_rows, void *d_q, int64_t q_stride,
+                                           float *d_scale, int n_rows, int n_cols, int block_rows,
+                                           void *stream) {
+    const int size = dtype_size(dtype);
+    if (!size || n_rows < 0 || n_cols < 1 || n_cols > 1 << 20 || (block_rows != 1 && block_rows != 128))
+        return fail(RABBIT_CUDA_ERR_ARGS,
+                    "f8_quantise: unknown dtype, n_rows below 0, n_cols not in 1..2^20 or block_rows "
+                    "not 1 or 128");
+    if (n_rows == 0) return ok();
+    if (!d_x || !d_q || !d_scale) return fail(RABBIT_CUDA_ERR_ARGS, "f8_quantise: NULL pointer");
+    if (d_rows && (block_rows != 1 || x_rows < 1))
+        return fail(RABBIT_CUDA_ERR_ARGS, "f8_quantise: d_rows needs block_rows 1 and x_rows above 0");
+    F8Args a;
+    a.x = d_x;
+    a.xs = x_stride ? x_stride : n_cols;
+    a.rows = d_rows;
+    a.x_rows = x_rows;
+    a.q = static_cast<uint8_t *>(d_q);
+    a.qs = q_stride ? q_stride : n_cols;
+    a.scale = d_scale;
+    a.n_rows = n_rows;
+    a.n_cols = n_cols;
+    a.nb = (n_cols + 127) / 128;
+    const uintptr_t x = reinterpret_cast<uintptr_t>(d_x), q = reinterpret_cast<uintptr_t>(d_q);
+    if (a.xs < n_cols || a.qs < n_cols || (x & (size - 1)) ||
+        (reinterpret_cast<uintptr_t>(d_scale) & 3) || (reinterpret_cast<uintptr_t>(d_rows) & 3))
+        return fail(RABBIT_CUDA_ERR_ARGS,
+                    "f8_quantise: a stride below n_cols, or a pointer not aligned to its element");
+    const bool vec = (x & 15) == 0 && a.xs * size % 16 == 0 && (q & 7) == 0 && a.qs % 8 == 0;
+    int sms = 0;
+    DeviceScope scope(current_device());
+    if (scope.status == RABBIT_CUDA_OK)
+        scope.launch(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, current_device()), "f8_quantise: SM count");
+    if (scope.status != RABBIT_CUDA_OK) return scope.status;
+    // Rows: blocks are handed out warp by warp, in one wave of the SMs at most.
+    const int64_t ctas = ((int64_t)n_rows * a.nb + kF8Threads / 16 - 1) / (kF8Threads / 16);
+    const dim3 grid = block_rows == 1 ? dim3((unsigned)(ctas < 8 * sms ? ctas : 8 * sms))
+                                      : dim3((n_rows + 127) / 128, a.nb);
+    with_dtype(dtype, [&](auto t) {
+        using T = decltype(t);
+        auto k = block_rows == 1 ? (vec ? k_f8_rows<T, true> : k_f8_rows<T, false>)
+                                 : (vec ? k_f8_blocks<T, true> : k_f8_blocks<T, false>);
+        scope.launch(launch_pdl(k, grid, dim3(kF8Threads), 0, static_cast<cudaStream_t>(stream), a),
+                     "f8_quantise");
+        return 0;
+    });
+    return scope.done();
+}

@@ -1,0 +1,267 @@
+// rb_linear.cu -- C ABI: products with e4m3 (a scale for each block of 128) or
+// 16-bit weights, one matrix or one for each expert (rb_linear.cuh).
+#include <cuda.h>
+#include <cudaTypedefs.h>
+
+#include <new>
+
+#include "rb_launch.h"
+#include "rb_linear.cuh"
+
+struct rabbit_cuda_linear {
+    int device = -1;
+    rb::DevCtx *ctx = nullptr;
+    rabbit_cuda_linear_desc d = {};
+    CUtensorMap map = {};
+    PFN_cuTensorMapEncodeTiled_v12000 encode = nullptr;
+    int *d_err = nullptr;  // the error word, and what a check took of it
+    std::mutex taking;     // one check at a time
+};
+
+namespace rb {
+
+__global__ void k_linear_take(int *err) { err[1] = atomicExch(err, 0); }
+
+static bool aligned(const void *p, uintptr_t n) {
+    return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0;
+}
+
+static int operand_size(int dtype) {
+    return dtype == RABBIT_CUDA_E4M3 ? 1
+           : dtype == RABBIT_CUDA_F16 || dtype == RABBIT_CUDA_BF16 ? 2 : 0;
+}
+
+using LinKernel = void (*)(LinArgs, CUtensorMap, CUtensorMap);
+
+static LinKernel lin_kernel(const rabbit_cuda_linear_desc &d) {
+    const bool f8 = d.dtype == RABBIT_CUDA_E4M3;
+    return d.gated ? (f8 ? k_linear<true, true> : k_linear<false, true>)
+                   : (f8 ? k_linear<true, false> : k_linear<false, false>);
+}
+
+// A map of rows of `cols` elements, `stride` elements apart: boxes of 128 bytes of
+// `box` rows, swizzled by 128 bytes; past the rows and columns reads zero.
+static bool rows_map(const rabbit_cuda_linear *lin, CUtensorMap *map, const void *base, int rank,
+                     const cuuint64_t *dims, const cuuint64_t *strides, int box) {
+    const bool f8 = lin->d.dtype == RABBIT_CUDA_E4M3;
+    const cuuint32_t boxes[4] = {f8 ? 128u : 64u, (cuuint32_t)box, 1, 1}, one[4] = {1, 1, 1, 1};
+    return lin->encode(map, f8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_UINT16,
+                       rank, const_cast<void *>(base), dims, strides, boxes, one,
+                       CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                       CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                       CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+static int up_to(int64_t n, int unit) { return (int)((n + unit - 1) / unit * unit); }
+
+// The launch's shape from the sizes alone (the groups' rows are on the device).
+static void lin_plan(LinArgs &a, const rabbit_cuda_linear_desc &d, int sms, int64_t *tiles) {
+    const int most = d.gated ? 128 : 256;
+    const int64_t mean = (a.R + a.E - 1) / a.E;
+    const int64_t want = a.E == 1 ? mean : 4 * mean;
+    // a multiple of 16 or, with more than one box, of the box's rows
+    auto tokens = [&](int64_t n) { return n <= 16 ? 16 : n >= most ? most : up_to(n, 32); };
+    a.bn = tokens(want < a.R ? want : a.R);
+    const int64_t groups = a.E < a.R ? a.E : a.R;
+    const int64_t token_tiles = a.E == 1 ? (a.R + a.bn - 1) / a.bn : groups + a.R / a.bn;
+    *tiles = token_tiles * a.mt;
+    a.split = 1;
+    while (a.split < 8 && *tiles * a.split * 2 <= sms && a.steps / (a.split * 2) >= 2) a.split *= 2;
+    a.box = a.bn < 32 ? a.bn : 32;
+    a.band = d.gated ? 16 : 8;
+    const size_t room = kMaxDynSmem - lin_smem(d.gated, a.bn, 0);
+    a.stages = (int)(room / lin_stage_bytes(d.gated, a.bn));
+    if (a.stages > kLinStages) a.stages = kLinStages;
+}
+
+static int lin_run(rabbit_cuda_linear *lin, const char *what, const void *d_x, int64_t x_stride,
+                   int x_rows, const float *d_x_scale, int64_t x_scale_stride, const int *d_rows,
+                   const int *d_offsets, int out_dtype, void *d_y, int64_t y_stride, int n_rows,
+                   void *stream) {
+    const rabbit_cuda_linear_desc &d = lin->d;
+    const int size = operand_size(d.dtype), out = dtype_size(out_dtype);
+    const bool f8 = d.dtype == RABBIT_CUDA_E4M3;
+    if (!out || n_rows < 0)
+        return fail(RABBIT_CUDA_ERR_ARGS, "%s: unknown out_dtype or a negative count", what);
+    if (n_rows == 0) return ok();
+    LinArgs a = {};
+    a.N = d.n_out;
+    a.E = d.n_experts;
+    a.R = n_rows;
+    a.x_rows = x_rows;
+    a.steps = (int)(((int64_t)d.n_in * size + 127) / 128);
+    a.mt = (d.n_out + 127) / 128;
+    const int64_t xs = x_stride ? x_stride : d.n_in;
+    a.xs_stride = x_scale_stride ? x_scale_stride : a.steps;
+    a.y_stride = y_stride ? y_stride : d.n_out;
+    if (!d_x || !d_y || (f8 && !d_x_scale))
+        return fail(RABBIT_CUDA_ERR_ARGS, "%s: NULL pointer", what);
+    if (!aligned(d_x, 16) || xs < d.n_in || xs > (1 << 30) || xs * size % 16 || !aligned(d_y, out) ||
+        a.y_stride < d.n_out || !aligned(d_rows, 4) || !aligned(d_offsets, 4))
+        return fail(RABBIT_CUDA_ERR_ARGS,
+                    "%s: x not aligned to 16 bytes, a stride below its row or (x) not a multiple of "
+                    "16 bytes, or a pointer not aligned to its element", what);
+    if (f8 && (a.xs_stride < a.steps || !aligned(d_x_scale, 4)))
+        return fail(RABBIT_CUDA_ERR_ARGS, "%s: x_scale_stride below its row, or scales not aligned", what);
+    if (x_rows < 1 || (!d_rows && x_rows < n_rows))
+        return fail(RABBIT_CUDA_ERR_ARGS, "%s: x_rows of %d for %d rows", what, x_rows, n_rows);
+    int64_t tiles;
+    lin_plan(a, d, lin->ctx->sm_count, &tiles);
+    if (tiles * a.split >= (int64_t)1 << 31)
+        return fail(RABBIT_CUDA_ERR_ARGS, "%s: more than 2^31 tiles", what);
+    a.offsets = d_offsets;
+    a.rows = d_rows;
+    a.xs = d_x_scale;
+    a.ws = d.d_scale;
+    a.y = d_y;
+    a.out_dtype = out_dtype;
+    a.format = d.dtype == RABBIT_CUDA_BF16;
+    a.err = lin->d_err;
+    a.wait_ns = wait_limit_ns();
+    CUtensorMap mx;
+    const cuuint64_t dims[2] = {(cuuint64_t)d.n_in, (cuuint64_t)x_rows};
+    const cuuint64_t strides[1] = {(cuuint64_t)xs * size};
+    if (!rows_map(lin, &mx, d_x, 2, dims, strides, d_rows ? 1 : a.box))
+        return fail(RABBIT_CUDA_ERR_DEVICE, "%s: the driver could not encode the rows' tensor map", what);
+    DeviceScope scope(lin->device);
+    if (scope.status != RABBIT_CUDA_OK) return scope.status;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = a.split;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(a.split > 1 ? tiles * a.split
+                                  : tiles < lin->ctx->sm_count ? tiles : lin->ctx->sm_count));
+    cfg.blockDim = dim3(kLinThreads);
+    cfg.dynamicSmemBytes = lin_smem(d.gated, a.bn, a.stages);
+    cfg.stream = static_cast<cudaStream_t>(stream);
+    cfg.attrs = attr;
+    cfg.numAttrs = a.split > 1 ? 2 : 1;
+    scope.launch(cudaLaunchKernelEx(&cfg, lin_kernel(d), a, lin->map, mx), what);
+    return scope.done();
+}
+
+}  // namespace rb
+
+using namespace rb;
+
+extern "C" {
+
+int rabbit_cuda_linear_create(const rabbit_cuda_linear_desc *d, int device,
+                              rabbit_cuda_linear **out) {
+    if (!d || !out) return fail(RABBIT_CUDA_ERR_ARGS, "linear_create: NULL argument");
+    *out = nullptr;
+    const int size = operand_size(d->dtype);
+    if (!size || d->n_experts < 1 || d->n_experts > kLinMaxExperts || (d->gated & ~1) ||
+        d->n_out < 1 || d->n_out > 1 << 20 || d->n_in < 1 || d->n_in > 1 << 20)
+        return fail(RABBIT_CUDA_ERR_ARGS,
+                    "linear_create: need dtype E4M3, F16 or BF16, n_experts in 1..%d, gated 0 or 1, "
+                    "n_out and n_in in 1..2^20", kLinMaxExperts);
+    const int64_t ws = d->w_stride ? d->w_stride : d->n_in;
+    if (!d->d_w || !aligned(d->d_w, 16) || ws < d->n_in || ws > 1 << 30 || ws * size % 16)
+        return fail(RABBIT_CUDA_ERR_ARGS,
+                    "linear_create: weights NULL or not aligned to 16 bytes, or a stride below n_in "
+                    "or not a multiple of 16 bytes");
+    if ((size == 1) != (d->d_scale != nullptr) || !aligned(d->d_scale, 4))
+        return fail(RABBIT_CUDA_ERR_ARGS, "linear_create: E4M3 weights, and no others, have scales");
+    const uint64_t row = (uint64_t)ws * size, matrix = row * d->n_out;
+    if (matrix * (1 + d->gated) >= (uint64_t)1 << 40)
+        return fail(RABBIT_CUDA_ERR_ARGS, "linear_create: an expert of 2^40 bytes or more");
+    int prev = 0;
+    cudaGetDevice(&prev);
+    int st;
+    DevCtx *ctx = dev_ctx(device, &st);
+    if (!ctx) {
+        cudaSetDevice(prev);
+        return st;
+    }
+    auto *lin = new (std::nothrow) rabbit_cuda_linear();
+    if (!lin) {
+        cudaSetDevice(prev);
+        return fail(RABBIT_CUDA_ERR_MEM, "linear_create: out of host memory");
+    }
+    lin->device = device;
+    lin->ctx = ctx;
+    lin->d = *d;
+    cudaDriverEntryPointQueryResult found;
+    void *fn = nullptr;
+    cudaError_t e = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &found);
+    lin->encode = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(fn);
+    if (e == cudaSuccess && (e = cudaMalloc(&lin->d_err, 2 * sizeof(int))) == cudaSuccess &&
+        (e = cudaMemset(lin->d_err, 0, 2 * sizeof(int))) == cudaSuccess &&
+        (e = cudaStreamSynchronize(nullptr)) == cudaSuccess)  // zeroed before any stream uses it
+        e = cudaFuncSetAttribute(reinterpret_cast<const void *>(lin_kernel(*d)),
+                                 cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxDynSmem);
+    const cuuint64_t dims[4] = {(cuuint64_t)d->n_in, (cuuint64_t)d->n_out, (cuuint64_t)1 + d->gated,
+                                (cuuint64_t)d->n_experts};
+    const cuuint64_t strides[3] = {row, matrix, matrix * (1 + d->gated)};
+    const bool mapped = e == cudaSuccess && found == cudaDriverEntryPointSuccess &&
+                        rows_map(lin, &lin->map, d->d_w, 4, dims, strides, 128);
+    if (!mapped) {
+        rabbit_cuda_linear_free(lin);
+        cudaSetDevice(prev);
+        cudaGetLastError();
+        return e != cudaSuccess ? cuda_fail(e, "linear_create")
+                                : fail(RABBIT_CUDA_ERR_DEVICE,
+                                       "linear_create: the driver could not encode the weights' tensor map");
+    }
+    cudaSetDevice(prev);
+    *out = lin;
+    return ok();
+}
+
+int rabbit_cuda_linear_free(rabbit_cuda_linear *lin) {
+    if (!lin) return ok();
+    {
+        DeviceScope scope(lin->device);
+        if (lin->d_err) cudaFree(lin->d_err);
+    }
+    delete lin;
+    return ok();
+}
+
+int rabbit_cuda_linear_dev(rabbit_cuda_linear *lin, const void *d_x, int64_t x_stride,
+                           const float *d_x_scale, int64_t x_scale_stride, int out_dtype, void *d_y,
+                           int64_t y_stride, int n_rows, void *stream) {
+    if (!lin) return fail(RABBIT_CUDA_ERR_ARGS, "linear: NULL object");
+    if (lin->d.n_experts != 1)
+        return fail(RABBIT_CUDA_ERR_ARGS, "linear: the object has %d experts: rabbit_cuda_linear_grouped_dev",
+                    lin->d.n_experts);
+    return lin_run(lin, "linear", d_x, x_stride, n_rows, d_x_scale, x_scale_stride, nullptr, nullptr,
+                   out_dtype, d_y, y_stride, n_rows, stream);
+}
+
+int rabbit_cuda_linear_grouped_dev(rabbit_cuda_linear *lin, const void *d_x, int64_t x_stride,
+                                   int x_rows, const float *d_x_scale, int64_t x_scale_stride,
+                                   const int *d_rows, const int *d_offsets, int out_dtype,
+                                   void *d_y, int64_t y_stride, int n_rows, void *stream) {
+    if (!lin) return fail(RABBIT_CUDA_ERR_ARGS, "linear_grouped: NULL object");
+    if (!d_offsets) return fail(RABBIT_CUDA_ERR_ARGS, "linear_grouped: NULL offsets");
+    return lin_run(lin, "linear_grouped", d_x, x_stride, x_rows, d_x_scale, x_scale_stride, d_rows,
+                   d_offsets, out_dtype, d_y, y_stride, n_rows, stream);
+}
+
+int rabbit_cuda_linear_check(rabbit_cuda_linear *lin, void *stream) {
+    if (!lin) return fail(RABBIT_CUDA_ERR_ARGS, "linear_check: NULL object");
+    DeviceScope scope(lin->device);
+    if (scope.status != RABBIT_CUDA_OK) return scope.status;
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    int h = 0;
+    RB_CUDA(cudaStreamSynchronize(s));
+    {
+        std::lock_guard<std::mutex> hold(lin->taking);
+        k_linear_take<<<1, 1, 0, s>>>(lin->d_err);
+        RB_CUDA(cudaGetLastError());
+        RB_CUDA(cudaMemcpyAsync(&h, lin->d_err + 1, sizeof(int), cudaMemcpyDeviceToHost, s));
+        RB_CUDA(cudaStreamSynchronize(s));
+    }
+    if (h == 0) return ok();
+    return fail(h & RB_LIN_ERR_WAIT ? RABBIT_CUDA_ERR_TIMEOUT : RABBIT_CUDA_ERR_ARGS, "linear: %s%s%s%s",
+                h & RB_LIN_ERR_WAIT ? "a bounded device wait ran out; " : "",
+                h & ~RB_LIN_ERR_WAIT ? "out of range on the device:" : "",
+                h & RB_LIN_ERR_OFFSETS ? " offsets" : "", h & RB_LIN_ERR_ROWS ? " rows" : "");
+}
+
+}  // extern "C"

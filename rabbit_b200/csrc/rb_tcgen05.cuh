@@ -1,7 +1,8 @@
 // rb_tcgen05.cuh -- sm_100a tensor-core building blocks: tensor memory
 // (TMEM) allocation, tcgen05.mma of kind::i8 with A in TMEM and B in shared
-// memory, its commit to an mbarrier, TMEM loads / stores, and the tiled TMA
-// copy (cp.async.bulk.tensor, no multicast) that stages weight rows.
+// memory and of kind::f8f6f4 / kind::f16 with both in shared memory, the commit
+// to an mbarrier, TMEM loads / stores, and the tiled TMA copies
+// (cp.async.bulk.tensor, no multicast) that stage their operands.
 //
 // Conventions used throughout (PTX ISA, tcgen05 chapter):
 //  * a TMEM address is (lane << 16) | column; a warp may touch only the 32
@@ -117,6 +118,44 @@ __device__ __forceinline__ void mma_commit(uint64_t *bar) {
                  : "memory");
 }
 
+// Instruction descriptor of kind::f8f6f4 (e4m3: format 0) and kind::f16 (f16 0,
+// bf16 1): f32 accumulator, A and B of one format, both K-major, M = 128, N a
+// multiple of 16 up to 256.
+__host__ __device__ constexpr uint32_t float_idesc(int format, int N) {
+    return (1u << 4) | ((uint32_t)format << 7) | ((uint32_t)format << 10) |
+           ((uint32_t)(N >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
+}
+
+// Shared-memory matrix descriptor of a K-major tile of 128-byte rows in the
+// 128-byte swizzle (the layout in which a TMA box with that swizzle arrives at a
+// 1024-byte aligned address): 8-row groups 1024 bytes apart. A K step of 32
+// bytes further on is 2 added to the descriptor.
+__device__ __forceinline__ uint64_t swizzled_desc(uint32_t smem_addr) {
+    return (uint64_t)((smem_addr & 0x3FFFFu) >> 4) | (1ull << 16) |
+           ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
+}
+
+// D[128 x N] (+)= A[128 x 32 bytes] * B[N x 32 bytes]^T, f32 accumulator, both
+// operands in shared memory. Issued by one thread.
+template <bool F8>
+__device__ __forceinline__ void mma_float_ss(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc,
+                                             uint32_t idesc, uint32_t accumulate) {
+    if constexpr (F8)
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "setp.ne.b32 p, %4, 0;\n\t"
+            "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
+            ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+            : "memory");
+    else
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "setp.ne.b32 p, %4, 0;\n\t"
+            "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+            ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+            : "memory");
+}
+
 // ----------------------------------------------------------- tiled TMA --
 // Box of a 4-D / 5-D tensor map into shared memory, completing on `bar`.
 // The innermost coordinate c0 is a byte offset and a multiple of 16 at every
@@ -138,6 +177,24 @@ __device__ __forceinline__ void tma_load_5d(void *smem_dst, const CUtensorMap *m
         ".L2::cache_hint [%0], [%1, {%2, %3, %4, %5, %6}], [%7], %8;" ::"r"(smem_u32(smem_dst)),
         "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(c4),
         "r"(smem_u32(bar)), "l"(policy)
+        : "memory");
+}
+__device__ __forceinline__ void tma_load_2d(void *smem_dst, const CUtensorMap *map, int c0, int c1,
+                                            uint64_t *bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%2, %3}], [%4];" ::"r"(smem_u32(smem_dst)),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(smem_u32(bar))
+        : "memory");
+}
+// Four rows r0 .. r3 of a 2-D map whose box is one row high, one after the other.
+__device__ __forceinline__ void tma_gather4(void *smem_dst, const CUtensorMap *map, int c0, int r0,
+                                            int r1, int r2, int r3, uint64_t *bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cta.global.tile::gather4.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%2, %3, %4, %5, %6}], [%7];" ::"r"(smem_u32(smem_dst)),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(r0), "r"(r1), "r"(r2), "r"(r3),
+        "r"(smem_u32(bar))
         : "memory");
 }
 __device__ __forceinline__ void tma_prefetch_map(const CUtensorMap *map) {
