@@ -33,10 +33,26 @@ static int operand_size(int dtype) {
 
 using LinKernel = void (*)(LinArgs, CUtensorMap, CUtensorMap);
 
-static LinKernel lin_kernel(const rabbit_cuda_linear_desc &d) {
-    const bool f8 = d.dtype == RABBIT_CUDA_E4M3;
-    return d.gated ? (f8 ? k_linear<true, true> : k_linear<false, true>)
-                   : (f8 ? k_linear<true, false> : k_linear<false, false>);
+static LinKernel lin_kernel(int mode, bool pair) {
+    if (mode == kLinF8) return pair ? k_linear<kLinF8, true> : k_linear<kLinF8, false>;
+    if (mode == kLinParts) return pair ? k_linear<kLinParts, true> : k_linear<kLinParts, false>;
+    return pair ? k_linear<kLinWhole, true> : k_linear<kLinWhole, false>;
+}
+
+// The current device's kernels for an object: their shared memory; `fits`: those that share
+// out registers were built to be launched with the 128 a thread that the shares add up to.
+static cudaError_t lin_prepare_kernels(bool f8, bool *fits) {
+    for (int mode = f8 ? kLinF8 : kLinWhole; mode <= (f8 ? kLinF8 : kLinParts); ++mode)
+        for (int pair = 0; pair < 2; ++pair) {
+            const void *k = reinterpret_cast<const void *>(lin_kernel(mode, pair));
+            cudaFuncAttributes at;
+            cudaError_t e = cudaFuncGetAttributes(&at, k);
+            if (e == cudaSuccess)
+                e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxDynSmem);
+            if (e != cudaSuccess) return e;
+            if (mode != kLinWhole && at.numRegs != 128) *fits = false;
+        }
+    return cudaSuccess;
 }
 
 // A map of rows of `cols` elements, `stride` elements apart: boxes of 128 bytes of
@@ -55,23 +71,28 @@ static bool rows_map(const rabbit_cuda_linear *lin, CUtensorMap *map, const void
 static int up_to(int64_t n, int unit) { return (int)((n + unit - 1) / unit * unit); }
 
 // The launch's shape from the sizes alone (the groups' rows are on the device).
-static void lin_plan(LinArgs &a, const rabbit_cuda_linear_desc &d, int sms, int64_t *tiles) {
-    const int most = d.gated ? 128 : 256;
-    const int64_t mean = (a.R + a.E - 1) / a.E;
-    const int64_t want = a.E == 1 ? mean : 4 * mean;
+static bool lin_plan(LinArgs &a, bool f8, int sms, int64_t *tiles) {
+    const int64_t mean = ((int64_t)a.R + a.E - 1) / a.E;
+    const bool pair = mean >= 128;
+    const int outputs = (a.gated ? 64 : 128) * (pair ? 2 : 1);
+    a.mt = (a.N + outputs - 1) / outputs;
+    a.unit = pair ? 64 : 16;
+    const int64_t want = a.E == 1 ? mean : 4 * mean, rows = want < a.R ? want : a.R;
     // a multiple of 16 or, with more than one box, of the box's rows
-    auto tokens = [&](int64_t n) { return n <= 16 ? 16 : n >= most ? most : up_to(n, 32); };
-    a.bn = tokens(want < a.R ? want : a.R);
+    a.bn = rows >= 256 ? 256 : rows <= 16 ? 16 : up_to(rows, 32);
+    if (pair) a.bn = up_to(a.bn, a.unit);
+    a.bufs = 512 / a.bn < kLinBufs ? 512 / a.bn : kLinBufs;
     const int64_t groups = a.E < a.R ? a.E : a.R;
     const int64_t token_tiles = a.E == 1 ? (a.R + a.bn - 1) / a.bn : groups + a.R / a.bn;
     *tiles = token_tiles * a.mt;
     a.split = 1;
-    while (a.split < 8 && *tiles * a.split * 2 <= sms && a.steps / (a.split * 2) >= 2) a.split *= 2;
+    while (!pair && a.split < 8 && *tiles * a.split * 2 <= sms && a.steps / (a.split * 2) >= 2) a.split *= 2;
     a.box = a.bn < 32 ? a.bn : 32;
-    a.band = d.gated ? 16 : 8;
-    const size_t room = kMaxDynSmem - lin_smem(d.gated, a.bn, 0);
-    a.stages = (int)(room / lin_stage_bytes(d.gated, a.bn));
+    a.band = 8;
+    const uint32_t stage = lin_stage_bytes(pair, a.bn);
+    a.stages = (int)((kMaxDynSmem - lin_fixed(f8, a.gated, a.bn, a.bufs, a.E)) / stage);
     if (a.stages > kLinStages) a.stages = kLinStages;
+    return pair;
 }
 
 static int lin_run(rabbit_cuda_linear *lin, const char *what, const void *d_x, int64_t x_stride,
@@ -90,7 +111,7 @@ static int lin_run(rabbit_cuda_linear *lin, const char *what, const void *d_x, i
     a.R = n_rows;
     a.x_rows = x_rows;
     a.steps = (int)(((int64_t)d.n_in * size + 127) / 128);
-    a.mt = (d.n_out + 127) / 128;
+    a.gated = d.gated;
     const int64_t xs = x_stride ? x_stride : d.n_in;
     a.xs_stride = x_scale_stride ? x_scale_stride : a.steps;
     a.y_stride = y_stride ? y_stride : d.n_out;
@@ -106,11 +127,20 @@ static int lin_run(rabbit_cuda_linear *lin, const char *what, const void *d_x, i
     if (x_rows < 1 || (!d_rows && x_rows < n_rows))
         return fail(RABBIT_CUDA_ERR_ARGS, "%s: x_rows of %d for %d rows", what, x_rows, n_rows);
     int64_t tiles;
-    lin_plan(a, d, lin->ctx->sm_count, &tiles);
-    if (tiles * a.split >= (int64_t)1 << 31)
-        return fail(RABBIT_CUDA_ERR_ARGS, "%s: more than 2^31 tiles", what);
+    const int sms = lin->ctx->sm_count;
+    const bool pair = lin_plan(a, f8, sms, &tiles);
+    if (tiles * a.split >= (int64_t)1 << 30)
+        return fail(RABBIT_CUDA_ERR_ARGS, "%s: 2^30 tiles or more", what);
+    // The tensor cores' sums of 16-bit products lose up to 2^-25 of the result at each of K / 16
+    // steps: nothing beside a 16-bit output's half step up to K 16384 (2^-15), parts beyond
+    // and for fp32 outputs.
+    const int mode = f8 ? kLinF8 : out == 4 || d.n_in > 16384 ? kLinParts : kLinWhole;
     a.offsets = d_offsets;
     a.rows = d_rows;
+    a.x = static_cast<const uint8_t *>(d_x);
+    a.x_bytes = xs * size;
+    a.k_bytes = d.n_in * size;
+    a.vec = aligned(d_y, 16) && a.y_stride * out % 16 == 0;
     a.xs = d_x_scale;
     a.ws = d.d_scale;
     a.y = d_y;
@@ -121,25 +151,26 @@ static int lin_run(rabbit_cuda_linear *lin, const char *what, const void *d_x, i
     CUtensorMap mx;
     const cuuint64_t dims[2] = {(cuuint64_t)d.n_in, (cuuint64_t)x_rows};
     const cuuint64_t strides[1] = {(cuuint64_t)xs * size};
-    if (!rows_map(lin, &mx, d_x, 2, dims, strides, d_rows ? 1 : a.box))
+    if (!rows_map(lin, &mx, d_x, 2, dims, strides, a.box))
         return fail(RABBIT_CUDA_ERR_DEVICE, "%s: the driver could not encode the rows' tensor map", what);
     DeviceScope scope(lin->device);
     if (scope.status != RABBIT_CUDA_OK) return scope.status;
+    const int team = pair ? 2 : a.split;
+    const int64_t teams = a.split == 1 && tiles > sms / team ? sms / team : tiles;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     attr[1].id = cudaLaunchAttributeClusterDimension;
-    attr[1].val.clusterDim.x = a.split;
+    attr[1].val.clusterDim.x = team;
     attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(a.split > 1 ? tiles * a.split
-                                  : tiles < lin->ctx->sm_count ? tiles : lin->ctx->sm_count));
+    cfg.gridDim = dim3((unsigned)(teams * team));
     cfg.blockDim = dim3(kLinThreads);
-    cfg.dynamicSmemBytes = lin_smem(d.gated, a.bn, a.stages);
+    cfg.dynamicSmemBytes = lin_fixed(f8, a.gated, a.bn, a.bufs, a.E) + (size_t)a.stages * lin_stage_bytes(pair, a.bn);
     cfg.stream = static_cast<cudaStream_t>(stream);
     cfg.attrs = attr;
-    cfg.numAttrs = a.split > 1 ? 2 : 1;
-    scope.launch(cudaLaunchKernelEx(&cfg, lin_kernel(d), a, lin->map, mx), what);
+    cfg.numAttrs = team > 1 ? 2 : 1;
+    scope.launch(cudaLaunchKernelEx(&cfg, lin_kernel(mode, pair), a, lin->map, mx), what);
     return scope.done();
 }
 
@@ -186,19 +217,19 @@ int rabbit_cuda_linear_create(const rabbit_cuda_linear_desc *d, int device,
     lin->ctx = ctx;
     lin->d = *d;
     cudaDriverEntryPointQueryResult found;
+    bool fits = true;
     void *fn = nullptr;
     cudaError_t e = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &found);
     lin->encode = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(fn);
     if (e == cudaSuccess && (e = cudaMalloc(&lin->d_err, 2 * sizeof(int))) == cudaSuccess &&
         (e = cudaMemset(lin->d_err, 0, 2 * sizeof(int))) == cudaSuccess &&
         (e = cudaStreamSynchronize(nullptr)) == cudaSuccess)  // zeroed before any stream uses it
-        e = cudaFuncSetAttribute(reinterpret_cast<const void *>(lin_kernel(*d)),
-                                 cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxDynSmem);
+        e = lin_prepare_kernels(d->dtype == RABBIT_CUDA_E4M3, &fits);
     const cuuint64_t dims[4] = {(cuuint64_t)d->n_in, (cuuint64_t)d->n_out, (cuuint64_t)1 + d->gated,
                                 (cuuint64_t)d->n_experts};
     const cuuint64_t strides[3] = {row, matrix, matrix * (1 + d->gated)};
-    const bool mapped = e == cudaSuccess && found == cudaDriverEntryPointSuccess &&
-                        rows_map(lin, &lin->map, d->d_w, 4, dims, strides, 128);
+    const bool mapped = e == cudaSuccess && fits && found == cudaDriverEntryPointSuccess &&
+                        rows_map(lin, &lin->map, d->d_w, 4, dims, strides, d->gated ? 64 : 128);
     if (!mapped) {
         rabbit_cuda_linear_free(lin);
         cudaSetDevice(prev);

@@ -2,27 +2,36 @@
 // sm_100a tensor cores: the kernel behind rabbit_cuda_linear_dev and
 // rabbit_cuda_linear_grouped_dev.
 //
-// The weights are the MMA's A operand (128 rows, so a tile of them is one row of
-// 128 x 128 scale blocks), the tokens its B operand: a tile takes as many tokens as
-// its expert has for it, in steps of 16, so ragged groups and single tokens do not pay for
-// 128 rows. A tile of y is 128 outputs x up to `bn` tokens; gated, the
-// gate's and the up matrix's 128 rows are two MMAs over the same tokens.
+// The weights are the MMA's A operand, the tokens its B operand: a tile takes as many
+// tokens as its expert has for it, so ragged groups and single tokens do not pay
+// for 128 rows, and a CTA's 128 weight rows are in one row of 128 x 128 scale
+// blocks. Gated, the 128 rows are 64 of the gate and the same 64 of the up matrix.
 //
-// Roles of a CTA's 12 warps, over the same sequence of tiles and of steps of 128 bytes of K:
-//   warp 0      TMA: the step's weight rows (one box of each matrix) and token rows
-//               (boxes, or gather4 through d_rows) into a ring of stages;
-//   warp 1      tensor memory; one lane issues the step's MMAs and commits;
-//   warp 2      (e4m3) the step's scales, sw * sx for each token, into shared memory;
-//   warps 4..11 readout: warp w reads lanes 32 (w % 4) .. + 31 (outputs), and the even or odd
-//               blocks of 16 tokens.
-// 16-bit: the accumulator stays in tensor memory over all of K and is read once.
-// e4m3: a step is one scale block. Its product is read out and added to 32-bit registers as
-// acc += (sw sx) * product, while the MMAs of the next steps fill other buffers of tensor
-// memory (512 columns / the tile's width, at least two).
-//
-// Short products (few tiles) are split over K by a cluster of `split` CTAs: each leaves its
-// part in its own shared memory and sums a share of the tokens over the cluster in the order
-// of the ranks, so there is no workspace and the same bits come each time.
+// Roles of a CTA's 16 warps, over the same sequence of tiles and of steps of 128 bytes of K:
+//   warp 0       TMA: the step's weight rows and, without a list, token rows into a ring of
+//                stages (128-byte rows, 128-byte swizzle);
+//   warp 1       tensor memory; one thread issues the step's MMAs and commits;
+//   warp 2       (e4m3) the step's scales, sw * sx for each token, into shared memory;
+//   warps 4..11  readout: warp w reads lanes 32 (w % 4) .. + 31 (weight rows), and the
+//                even or odd blocks of 16 tokens; outputs go through shared memory, so that
+//                they leave in rows of 16 bytes a thread;
+//   warps 12..15 with a list: the token rows by cp.async, 16 bytes a thread (a gather by
+//                TMA, four rows an instruction, took 80 cycles for 512 bytes).
+// Accumulation (MODE):
+//   kLinWhole  16-bit: in tensor memory over all of K, read once;
+//   kLinParts  16-bit, for fp32 outputs or a very long K: the tensor cores' sum is cut off,
+//              not rounded, at each MMA, an error that grows with their number (K 2048: 2e-6 of
+//              the result, K 14336: 1.4e-5); so each 256 channels are read out and added
+//              in 32-bit registers;
+//   kLinF8     e4m3: each step is a scale block, read out and added to 32-bit registers as
+//              acc += (sw sx) * product, while the MMAs of the next steps fill other buffers
+//              of tensor memory.
+// PAIR: two CTAs share a tile of 256 weight rows: each has its rows of A and half the
+// tokens' rows of B, and CTA 0 issues one MMA of M = 256 for both (cta_group::2), so a step
+// brings 32 KB instead of 48 KB to each SM for the same work.
+// Otherwise, short products (few tiles) are split over K by a cluster of `split` CTAs: each
+// leaves its part in its own shared memory and sums a share of the outputs over the cluster in
+// the order of the ranks, so there is no workspace and the same bits come each time.
 #pragma once
 #include <cuda_runtime.h>
 #include <stdint.h>
@@ -34,11 +43,17 @@
 
 namespace rb {
 
-constexpr int kLinThreads = 384;
+enum { kLinWhole, kLinParts, kLinF8 };
+
+constexpr int kLinThreads = 512;
+constexpr int kLinReaders = 256;          // threads of the readout warps
 constexpr int kLinMaxExperts = 1024;
-constexpr int kLinBufs = 8;      // buffers of tensor memory, at most
-constexpr int kLinStages = 12;   // stages of the ring, at most
-constexpr uint32_t kLinTile = 128 * 128;  // bytes of 128 weight rows of a step
+constexpr int kLinBufs = 8;               // buffers of tensor memory, at most
+constexpr int kLinStages = 12;            // stages of the ring, at most
+constexpr int kLinPart = 4;               // steps of a part (kLinParts)
+constexpr int kLinLag = 2;                // steps by which a gathered row's arrival is told later
+constexpr uint32_t kLinTile = 128 * 128;  // bytes of a step's 128 weight rows
+constexpr uint32_t kLinOut = 32 * 128 * 4;  // outputs on their way: 32 tokens
 
 // Error bits of an object's error word.
 #define RB_LIN_ERR_OFFSETS 16
@@ -48,96 +63,171 @@ constexpr uint32_t kLinTile = 128 * 128;  // bytes of 128 weight rows of a step
 struct LinArgs {
     const int *offsets;   // [E + 1], or NULL: one expert with all rows
     const int *rows;      // [R] rows of x, or NULL
+    const uint8_t *x;     // with a list: x, its row in bytes, and the bytes of n_in
+    int64_t x_bytes;
+    int k_bytes;
     const float *xs, *ws; // e4m3: scales
     int64_t xs_stride;
     void *y;
     int64_t y_stride;
     int out_dtype;
+    bool vec;             // y takes rows of 16 bytes
+    int gated;
     int N, E, R, x_rows;
     int steps;            // of 128 bytes, over K
-    int mt;               // tiles of 128 outputs
-    int bn;               // tokens of a tile, at most; a multiple of 16
+    int mt;               // tiles of outputs
+    int bn;               // tokens of a tile, at most: 16 or a multiple of 32
+    int unit;             // tokens of a tile come in multiples of it
     int box;              // token rows of a box
-    int stages;
-    int split;            // CTAs of a cluster
+    int stages, bufs;
+    int split;            // CTAs of a cluster that splits K
     int band;             // token tiles that go together, for the L2
     uint32_t format;      // operand format of the instruction descriptor
     int *err;
     uint64_t wait_ns;
 };
 
+// Shared memory: the ring (aligned to 1024), the outputs on their way, then LinShared,
+// the scales [bufs][1 or 2][bn, at least 32], off [E + 1] and pre [E + 1].
 struct LinShared {
     uint64_t full[kLinStages], empty[kLinStages];
-    uint64_t dfull[kLinBufs], sfull[kLinBufs], dempty[kLinBufs];
+    uint64_t dfull[kLinBufs], dempty[kLinBufs], mfree[kLinBufs];
     uint64_t mdone;
     uint32_t tmem;
     int abort;
-    alignas(16) float sc[kLinBufs][256];  // scales of a step: tokens (gated: gate's, then up's)
-    int off[kLinMaxExperts], cnt[kLinMaxExperts];  // first row and rows of each expert
-    int pre[kLinMaxExperts + 1];                   // token tiles of the experts before
+    int src[256];  // with a list: the tile's rows of x, -1 for none
 };
-
-// Bytes of shared memory: the ring (aligned to 1024), then LinShared.
-__host__ __device__ constexpr uint32_t lin_stage_bytes(bool gated, int bn) {
-    return (gated ? 2 : 1) * kLinTile + (uint32_t)bn * 128;
+static_assert(sizeof(LinShared) % 16 == 0, "the scales behind it are read 16 bytes at a time");
+__host__ __device__ constexpr int lin_sc(int bn) { return bn < 32 ? 32 : bn; }
+__host__ __device__ constexpr uint32_t lin_stage_bytes(bool pair, int bn) {
+    return kLinTile + (uint32_t)bn * (pair ? 64 : 128);
 }
-__host__ __device__ constexpr size_t lin_smem(bool gated, int bn, int stages) {
-    return 1024 + (size_t)stages * lin_stage_bytes(gated, bn) + sizeof(LinShared);
+// All but the ring.
+__host__ __device__ constexpr size_t lin_fixed(bool f8, int gated, int bn, int bufs, int E) {
+    return 1024 + kLinOut + sizeof(LinShared) +
+           (f8 ? (size_t)bufs * (1 + gated) * lin_sc(bn) * 4 : 0) + 8 * (size_t)(E + 1);
 }
 
 struct LinTile {
-    int e, mt, row0, n, n16;  // expert, tile of outputs, first row of y, tokens, in steps of 16
+    int e, mt, row0, n, cols;  // expert, tile of outputs, first row of y, tokens, in units
 };
 
 // Tile `i` of the launch; false past the last.
-__device__ __forceinline__ bool lin_tile(const LinArgs &a, const LinShared &s, int i, LinTile &t) {
-    if (i >= s.pre[a.E] * a.mt) return false;
+__device__ __forceinline__ bool lin_tile(const LinArgs &a, const int *off, const int *pre, int i,
+                                         LinTile &t) {
+    if (i >= pre[a.E] * a.mt) return false;
     int lo = 0, hi = a.E;  // the expert: pre[lo] * mt <= i < pre[lo + 1] * mt
     while (hi - lo > 1) {
         const int m = (lo + hi) / 2;
-        if (s.pre[m] * a.mt <= i) lo = m;
+        if (pre[m] * a.mt <= i) lo = m;
         else hi = m;
     }
-    const int l = i - s.pre[lo] * a.mt, nt = s.pre[lo + 1] - s.pre[lo];
-    const int rows = s.cnt[lo];
+    const int l = i - pre[lo] * a.mt, nt = pre[lo + 1] - pre[lo];
+    const int rows = off[lo + 1] - off[lo];
     // bands of token tiles; in a band the outputs' tiles one after the other
     const int b = l / (a.band * a.mt), r = l - b * a.band * a.mt;
     const int w = min(a.band, nt - b * a.band);
     const int mt = r / w, ti = b * a.band + (r - mt * w);
-    const int per = ((rows + nt - 1) / nt + 15) & ~15;  // equal tiles: at most bn, none empty
+    // equal tiles: at most bn, none empty
+    const int per = ((rows + nt - 1) / nt + a.unit - 1) / a.unit * a.unit;
     t.e = lo;
     t.mt = mt;
-    t.row0 = s.off[lo] + ti * per;
+    t.row0 = off[lo] + ti * per;
     t.n = min(per, rows - ti * per);
-    t.n16 = (t.n + 15) & ~15;
+    t.cols = (t.n + a.unit - 1) / a.unit * a.unit;
     return true;
 }
 
-__device__ __forceinline__ bool lin_wait(uint64_t *bar, uint32_t parity, const LinArgs &a,
-                                         volatile int *abort) {
-    bool ok = mbar_try_wait(bar, parity);
-    if (!ok) {
-        const uint64_t t0 = globaltimer_ns();
-        for (uint32_t it = 1; !ok; ++it) {
-            ok = mbar_try_wait(bar, parity);
-            if (!ok && (it & 15u) == 0) {
-                if (*abort) break;
-                if (globaltimer_ns() - t0 > a.wait_ns) {
-                    atomicOr(a.err, RB_LIN_ERR_WAIT);
-                    *abort = 1;
-                    break;
-                }
+// A place in a ring and the parity of its use.
+struct LinRing {
+    int at = 0;
+    uint32_t phase = 0;
+    __device__ __forceinline__ void next(int n) {
+        if (++at == n) {
+            at = 0;
+            phase ^= 1;
+        }
+    }
+};
+
+// Bounded wait of one thread; what the other CTA of a pair wrote before its arrival
+// is seen after it.
+__device__ __forceinline__ bool lin_try(uint64_t *bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(smem_u32(bar)), "r"(parity)
+        : "memory");
+    return ok != 0;
+}
+__device__ __forceinline__ bool lin_wait1(uint64_t *bar, uint32_t parity, const LinArgs &a,
+                                          volatile int *abort) {
+    if (lin_try(bar, parity)) return true;
+    const uint64_t t0 = globaltimer_ns();
+    for (uint32_t it = 1;; ++it) {
+        if (lin_try(bar, parity)) return true;
+        if ((it & 15u) == 0) {
+            if (*abort) return false;
+            if (globaltimer_ns() - t0 > a.wait_ns) {
+                atomicOr(a.err, RB_LIN_ERR_WAIT);
+                *abort = 1;
+                return false;
             }
         }
     }
-    return __all_sync(0xffffffffu, ok);  // the warp goes one way
+}
+// Of a warp: it goes one way.
+__device__ __forceinline__ bool lin_wait(uint64_t *bar, uint32_t parity, const LinArgs &a,
+                                         volatile int *abort) {
+    return __all_sync(0xffffffffu, lin_wait1(bar, parity, a, abort));
 }
 
-// 16 consecutive columns of this thread's lane.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t one;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "elect.sync _|p, 0xffffffff;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(one));
+    return one != 0;
+}
+// Address in the cluster's window of `p` (this CTA's shared memory) in CTA `rank`.
+__device__ __forceinline__ uint32_t cluster_addr(const void *p, uint32_t rank) {
+    uint32_t at;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(p)), "r"(rank));
+    return at;
+}
+__device__ __forceinline__ void cluster_bar_arrive(uint32_t bar) {
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void cluster_sync_all() {
+    asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t cluster_rank() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ float4 cluster_ld4(uint32_t at) {
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                 : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+                 : "r"(at)
+                 : "memory");
+    return v;
+}
+// 16 bytes (n of them read, the rest zero) into shared memory.
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void *src, int n) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+}
+
+// 16 consecutive columns of this thread's lane, and the wait before their first use.
 __device__ __forceinline__ void lin_ld16(uint32_t taddr, float (&v)[16]) {
     tmem_ld16(taddr, reinterpret_cast<int(&)[16]>(v), 0);
 }
-// Wait for it; the values are not used before.
 __device__ __forceinline__ void lin_ld_done(float (&v)[16]) {
     asm volatile("tcgen05.wait::ld.sync.aligned;"
                  : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]),
@@ -147,366 +237,452 @@ __device__ __forceinline__ void lin_ld_done(float (&v)[16]) {
 
 __device__ __forceinline__ float lin_silu(float g) { return g / (1.f + expf(-g)); }
 
-__device__ __forceinline__ void lin_store(const LinArgs &a, int64_t at, float v) {
-    if (a.out_dtype == RABBIT_CUDA_F32) static_cast<float *>(a.y)[at] = v;
-    else if (a.out_dtype == RABBIT_CUDA_F16) static_cast<__half *>(a.y)[at] = from_f32<__half>(v);
-    else static_cast<__nv_bfloat16 *>(a.y)[at] = from_f32<__nv_bfloat16>(v);
-}
-
-// Which of 32 tokens of a tile, from c on, are written: bit j for token c + j.
-__device__ __forceinline__ uint32_t lin_written(const LinArgs &a, const LinTile &t, int c, int lane) {
-    bool w = c + lane < t.n;
-    if (w && a.rows) {
-        const int r = __ldg(a.rows + t.row0 + c + lane);
-        w = r >= 0 && r < a.x_rows;
+// Eight outputs of a row from column c on.
+template <typename T>
+__device__ __forceinline__ void lin_put8(const LinArgs &a, int64_t row, int c, const float (&v)[8]) {
+    T *y = static_cast<T *>(a.y) + row * a.y_stride + c;
+    if (a.vec && c + 8 <= a.N) {
+        store8<true>(y, v);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (c + i < a.N) y[i] = from_f32<T>(v[i]);
     }
-    return __ballot_sync(0xffffffffu, w);
+}
+// Piece `seg` of 8 of a token's row of 128 sums, which `get(i)` reads four at a time, to
+// row `row` of y, whose columns from `n0` on they are.
+template <typename F>
+__device__ __forceinline__ void lin_put(const LinArgs &a, int64_t row, int n0, int seg, F &&get) {
+#pragma unroll
+    for (int p = 0; p < 2; ++p) {
+        const int c = a.gated ? seg * 8 : (p * 8 + seg) * 8;
+        if (a.gated && p) break;
+        const float4 l = get(c), h = get(c + 4);
+        float v[8] = {l.x, l.y, l.z, l.w, h.x, h.y, h.z, h.w};
+        if (a.gated) {
+            const float4 ul = get(64 + c), uh = get(64 + c + 4);
+            const float u[8] = {ul.x, ul.y, ul.z, ul.w, uh.x, uh.y, uh.z, uh.w};
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = lin_silu(v[i]) * u[i];
+        }
+        if (a.out_dtype == RABBIT_CUDA_F32) lin_put8<float>(a, row, n0 + c, v);
+        else if (a.out_dtype == RABBIT_CUDA_F16) lin_put8<__half>(a, row, n0 + c, v);
+        else lin_put8<__nv_bfloat16>(a, row, n0 + c, v);
+    }
+}
+// Whether token c of a tile is written.
+__device__ __forceinline__ bool lin_written(const LinArgs &a, const LinTile &t, int c) {
+    if (c >= t.n) return false;
+    if (!a.rows) return true;
+    const int r = __ldg(a.rows + t.row0 + c);
+    return r >= 0 && r < a.x_rows;
 }
 
-__device__ __forceinline__ void cluster_arrive() {
-    asm volatile("barrier.cluster.arrive.release;" ::: "memory");
-}
-__device__ __forceinline__ void cluster_wait() {
-    asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
-}
-__device__ __forceinline__ uint32_t cluster_rank() {
-    uint32_t r;
-    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-    return r;
-}
-// Word at `p` (this CTA's shared memory) of the cluster's CTA `rank`.
-__device__ __forceinline__ float cluster_ld(const float *p, uint32_t rank) {
-    uint32_t at;
-    float v;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(p)), "r"(rank));
-    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
-    return v;
-}
-
-template <bool F8, bool GATED>
+template <int MODE, bool PAIR>
 __global__ void __launch_bounds__(kLinThreads, 1)
     k_linear(const __grid_constant__ LinArgs a, const __grid_constant__ CUtensorMap mw,
              const __grid_constant__ CUtensorMap mx) {
     extern __shared__ uint8_t lin_raw[];
+    constexpr bool F8 = MODE == kLinF8;
+    constexpr int PART = MODE == kLinF8 ? 1 : MODE == kLinParts ? kLinPart : 1 << 30;
     uint8_t *ring = lin_raw + ((1024u - (smem_u32(lin_raw) & 1023u)) & 1023u);
-    constexpr int G = GATED ? 2 : 1;
-    const uint32_t stage_bytes = lin_stage_bytes(GATED, a.bn);
-    LinShared &s = *reinterpret_cast<LinShared *>(ring + (size_t)a.stages * stage_bytes);
+    const uint32_t stage_bytes = lin_stage_bytes(PAIR, a.bn);
+    float *outs = reinterpret_cast<float *>(ring + (size_t)a.stages * stage_bytes);
+    LinShared &s = *reinterpret_cast<LinShared *>(reinterpret_cast<uint8_t *>(outs) + kLinOut);
+    float *scales = reinterpret_cast<float *>(&s + 1);
+    const int sc_row = lin_sc(a.bn), sc_buf = (1 + a.gated) * sc_row;
+    int *off = reinterpret_cast<int *>(scales + (F8 ? a.bufs * sc_buf : 0)), *pre = off + a.E + 1;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int width = G * a.bn;                       // columns of a buffer
-    const int bufs = min(512 / width, kLinBufs);
     volatile int *abort = &s.abort;
+    const uint32_t rank = PAIR || a.split > 1 ? cluster_rank() : 0;
+    const bool leader = !PAIR || rank == 0;
 
     if (threadIdx.x == 0) {
+        const int rows_from = a.rows ? (PAIR ? 8 : 4) : 0;  // gathering warps that arrive
         for (int i = 0; i < a.stages; ++i) {
-            mbar_init(&s.full[i], 1);
+            mbar_init(&s.full[i], 1 + rows_from);
             mbar_init(&s.empty[i], 1);
         }
-        for (int i = 0; i < bufs; ++i) {
-            mbar_init(&s.dfull[i], 1);
-            mbar_init(&s.sfull[i], 1);
-            mbar_init(&s.dempty[i], 8);
+        for (int i = 0; i < a.bufs; ++i) {
+            mbar_init(&s.dfull[i], F8 ? 2 : 1);  // the MMAs and the scales
+            mbar_init(&s.dempty[i], 8);          // this CTA's readout
+            mbar_init(&s.mfree[i], 16);          // the pair's
         }
         mbar_init(&s.mdone, 1);
         s.abort = 0;
         mbar_init_fence();
     }
-    if (warp == 1) tmem_alloc(&s.tmem, 512);
+    if (warp == 1) {
+        if (PAIR) tmem_alloc_pair(&s.tmem, 512);
+        else tmem_alloc(&s.tmem, 512);
+    }
     launch_dependents();
     wait_prerequisite();
     // The experts' rows; with offsets out of order or range the call has none at all (tiles
     // of ranges that overlap could be more than the launch was made for).
     bool bad = false;
-    for (int e = threadIdx.x; e < a.E; e += kLinThreads) {
-        int lo = 0, hi = a.R;
-        if (a.offsets) {
-            lo = a.offsets[e];
-            hi = a.offsets[e + 1];
-            bad |= lo < 0 || hi < lo || hi > a.R;
-        }
-        s.off[e] = lo;
-        s.cnt[e] = hi - lo;
+    for (int e = threadIdx.x; e <= a.E; e += kLinThreads) {
+        const int o = a.offsets ? a.offsets[e] : e ? a.R : 0;
+        off[e] = o;
+        bad |= o < 0 || o > a.R || (a.offsets && e && a.offsets[e - 1] > o);
     }
     bad = __syncthreads_or(bad);
     if (bad && threadIdx.x == 0) atomicOr(a.err, RB_LIN_ERR_OFFSETS);
     if (warp == 0) {
         int before = 0;
         for (int e0 = 0; e0 < a.E; e0 += 32) {
-            int n = e0 + lane < a.E && !bad ? (s.cnt[e0 + lane] + a.bn - 1) / a.bn : 0;
+            const int e = e0 + lane;
+            int n = e < a.E && !bad ? (off[e + 1] - off[e] + a.bn - 1) / a.bn : 0;
 #pragma unroll
             for (int d = 1; d < 32; d <<= 1) {
                 const int m = __shfl_up_sync(0xffffffffu, n, d);
                 if (lane >= d) n += m;
             }
-            if (e0 + lane < a.E) s.pre[e0 + lane + 1] = before + n;
+            if (e < a.E) pre[e + 1] = before + n;
             before += __shfl_sync(0xffffffffu, n, 31);
         }
-        if (lane == 0) s.pre[0] = 0;
+        if (lane == 0) pre[0] = 0;
     }
     tc_fence_before();
     __syncthreads();
+    if (PAIR) cluster_sync_all();  // both CTAs' barriers are ready
     tc_fence_after();
     const uint32_t tmem = s.tmem;
-    const uint32_t rank = a.split > 1 ? cluster_rank() : 0;
-    // a cluster has one tile; a CTA by itself each gridDim.x-th
-    const int first = blockIdx.x / a.split, stride = a.split > 1 ? 1 << 30 : gridDim.x;
-    const int k0 = (int)((int64_t)a.steps * rank / a.split);
-    const int k1 = (int)((int64_t)a.steps * (rank + 1) / a.split);
+    // a pair has every (CTAs / 2)-th tile, a CTA by itself each gridDim.x-th, a cluster that
+    // splits K one
+    const int team = PAIR ? 2 : a.split;
+    const int first = blockIdx.x / team, stride = !PAIR && a.split > 1 ? 1 << 30 : gridDim.x / team;
+    const int k0 = PAIR ? 0 : (int)((int64_t)a.steps * rank / a.split);
+    const int k1 = PAIR ? a.steps : (int)((int64_t)a.steps * (rank + 1) / a.split);
+    const int outputs = a.gated ? 64 : 128;  // of a CTA's tile
     LinTile t;
 
+    // Registers: 512 x 128 at the launch (linear_create checks it); 128 x 64 + 128 x 48 +
+    // 256 x 200 from here.
+    if (warp < 4) {
+        if constexpr (MODE != kLinWhole) asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
     if (warp == 0) {  // ------------------------------------------------ TMA
-        const uint64_t keep = policy_evict_last(), once = policy_evict_first();
-        int it = 0;
-        bool ok = true;
-        for (int i = first; ok && lin_tile(a, s, i, t); i += stride) {
-            int src[2][4];  // with a list: the rows of x of quads lane and lane + 32
-            if (a.rows) {
-#pragma unroll
-                for (int h = 0; h < 2; ++h)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const int c = (lane + 32 * h) * 4 + j;
-                        int r = c < t.n ? __ldg(a.rows + t.row0 + c) : 0;
-                        if (r < 0 || r >= a.x_rows) {
-                            atomicOr(a.err, RB_LIN_ERR_ROWS);
-                            r = 0;  // read for nothing: lin_written leaves the row out
-                        }
-                        src[h][j] = r;
+        if (elect_one()) {
+            const uint64_t keep = policy_evict_last(), once = policy_evict_first();
+            LinRing st;
+            int issued = 0;
+            bool ok = true;
+            for (int i = first; ok && lin_tile(a, off, pre, i, t); i += stride) {
+                const int n0 = (PAIR ? 2 * t.mt + rank : t.mt) * outputs;
+                const int here = PAIR ? t.cols / 2 : t.cols;  // token rows of this CTA
+                const int boxes = a.rows ? 0 : (here + a.box - 1) / a.box;
+                const uint32_t bytes = (PAIR ? 2 : 1) * (kLinTile + boxes * a.box * 128);
+                const int r0 = t.row0 + (PAIR ? rank * here : 0);
+                // weights that no other tile of tokens reads leave the L2 first
+                const uint64_t pol = pre[t.e + 1] - pre[t.e] > 1 ? keep : once;
+                for (int k = k0; k < k1; ++k, ++issued) {
+                    if (!(ok = lin_wait1(&s.empty[st.at], st.phase ^ 1, a, abort))) break;
+                    uint8_t *base = ring + (size_t)st.at * stage_bytes, *xb = base + kLinTile;
+                    const int c0 = k * (F8 ? 128 : 64);
+                    if (leader) mbar_arrive_expect_tx(&s.full[st.at], bytes);
+                    if constexpr (PAIR) {
+                        const uint32_t bar = cluster_addr(&s.full[st.at], 0);
+                        tma_load_4d_pair(base, &mw, c0, n0, 0, t.e, bar, pol);
+                        if (a.gated) tma_load_4d_pair(base + kLinTile / 2, &mw, c0, n0, 1, t.e, bar, pol);
+                        for (int b = 0; b < boxes; ++b)
+                            tma_load_2d_pair(xb + b * a.box * 128, &mx, c0, r0 + b * a.box, bar);
+                    } else {
+                        tma_load_4d(base, &mw, c0, n0, 0, t.e, &s.full[st.at], pol);
+                        if (a.gated) tma_load_4d(base + kLinTile / 2, &mw, c0, n0, 1, t.e, &s.full[st.at], pol);
+                        for (int b = 0; b < boxes; ++b)
+                            tma_load_2d(xb + b * a.box * 128, &mx, c0, r0 + b * a.box, &s.full[st.at]);
                     }
-            }
-            const int boxes = (t.n16 + a.box - 1) / a.box;
-            const uint32_t bytes = G * kLinTile + (a.rows ? t.n16 : boxes * a.box) * 128;
-            // weights that no other tile of tokens reads leave the L2 first
-            const uint64_t pol = s.pre[t.e + 1] - s.pre[t.e] > 1 ? keep : once;
-            for (int k = k0; k < k1; ++k, ++it) {
-                const int st = it % a.stages;
-                if (!(ok = lin_wait(&s.empty[st], ((it / a.stages) & 1) ^ 1, a, abort))) break;
-                uint8_t *base = ring + (size_t)st * stage_bytes, *xb = base + G * kLinTile;
-                const int c0 = k * (F8 ? 128 : 64);
-                if (lane == 0) {
-                    mbar_arrive_expect_tx(&s.full[st], bytes);
-#pragma unroll
-                    for (int g = 0; g < G; ++g)
-                        tma_load_4d(base + g * kLinTile, &mw, c0, t.mt * 128, g, t.e, &s.full[st],
-                                    pol);
-                }
-                __syncwarp();
-                if (a.rows) {
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        const int q = lane + 32 * h;
-                        if (4 * q < t.n16)
-                            tma_gather4(xb + q * 512, &mx, c0, src[h][0], src[h][1], src[h][2],
-                                        src[h][3], &s.full[st]);
-                    }
-                } else if (lane < boxes) {
-                    tma_load_2d(xb + lane * a.box * 128, &mx, c0, t.row0 + lane * a.box,
-                                &s.full[st]);
+                    st.next(a.stages);
                 }
             }
+            // copies under way (the pair's complete on the leader's barriers) end before
+            // the block does
+            if (!ok && leader)
+                for (int j = max(0, issued - a.stages); j < issued; ++j)
+                    mbar_wait(&s.full[j % a.stages], (j / a.stages) & 1, a.wait_ns, nullptr, 0);
         }
-        if (!ok)  // copies under way end before the block does
-            for (int j = max(0, it - a.stages); j < it; ++j)
-                if (lane == 0) mbar_wait(&s.full[j % a.stages], (j / a.stages) & 1, a.wait_ns, nullptr, 0);
+        __syncwarp();
     } else if (warp == 1) {  // ------------------------------------------ MMA
-        int it = 0, db = 0;
-        bool ok = true;
-        for (int i = first; ok && lin_tile(a, s, i, t); i += stride) {
-            const uint32_t idesc = float_idesc(a.format, t.n16);
-            for (int k = k0; k < k1; ++k, ++it) {
-                const int st = it % a.stages, buf = db % bufs;
-                if (F8 || k == k0)
-                    if (!(ok = lin_wait(&s.dempty[buf], ((db / bufs) & 1) ^ 1, a, abort))) break;
-                if (!(ok = lin_wait(&s.full[st], (it / a.stages) & 1, a, abort))) break;
-                tc_fence_after();
-                if (lane == 0) {
-                    uint8_t *base = ring + (size_t)st * stage_bytes;
-                    const uint64_t xd = swizzled_desc(smem_u32(base + G * kLinTile));
+        if (leader && elect_one()) {
+            LinRing st, db;
+            bool ok = true;
+            const uint64_t wd0 = swizzled_desc(smem_u32(ring)), xd0 = swizzled_desc(smem_u32(ring + kLinTile));
+            for (int i = first; ok && lin_tile(a, off, pre, i, t); i += stride) {
+                const uint32_t idesc = float_idesc(a.format, PAIR ? 256 : 128, t.cols);
+                int part = 0;
+                for (int k = k0; k < k1; ++k) {
+                    if (part == 0)
+                        if (!(ok = lin_wait1(PAIR ? &s.mfree[db.at] : &s.dempty[db.at], db.phase ^ 1, a, abort))) break;
+                    if (!(ok = lin_wait1(&s.full[st.at], st.phase, a, abort))) break;
+                    tc_fence_after();
+                    const uint64_t step = (uint64_t)(st.at * stage_bytes) >> 4;
+                    const uint32_t d = tmem + db.at * a.bn;
 #pragma unroll
-                    for (int g = 0; g < G; ++g) {
-                        const uint64_t wd = swizzled_desc(smem_u32(base + g * kLinTile));
-                        const uint32_t d = tmem + buf * width + g * a.bn;
-#pragma unroll
-                        for (int j = 0; j < 4; ++j)
-                            mma_float_ss<F8>(d, wd + 2 * j, xd + 2 * j, idesc,
-                                             j > 0 || (!F8 && k > k0));
+                    for (int j = 0; j < 4; ++j)
+                        mma_float_ss<F8, PAIR>(d, wd0 + step + 2 * j, xd0 + step + 2 * j, idesc, j > 0 || part > 0);
+                    if (PAIR) mma_commit_pair(&s.empty[st.at]);
+                    else mma_commit(&s.empty[st.at]);
+                    st.next(a.stages);
+                    if (++part == PART || k == k1 - 1) {
+                        if (PAIR) mma_commit_pair(&s.dfull[db.at]);
+                        else mma_commit(&s.dfull[db.at]);
+                        db.next(a.bufs);
+                        part = 0;
                     }
-                    mma_commit(&s.empty[st]);
-                    if (F8 || k == k1 - 1) mma_commit(&s.dfull[buf]);
                 }
-                __syncwarp();
-                if (F8 || k == k1 - 1) ++db;
             }
-        }
-        if (!ok && lane == 0) {  // products under way end before their memory is given back
-            mma_commit(&s.mdone);
-            mbar_wait(&s.mdone, 0, a.wait_ns, nullptr, 0);
+            if (!ok) {  // products under way end before their memory is given back
+                if (PAIR) mma_commit_pair(&s.mdone);
+                else mma_commit(&s.mdone);
+                mbar_wait(&s.mdone, 0, a.wait_ns, nullptr, 0);
+            }
         }
         __syncwarp();
     } else if (F8 && warp == 2) {  // --------------------------------- scales
-        constexpr int NT = GATED ? 4 : 8;  // tokens of a lane
-        const int nb = a.mt;               // rows of scale blocks of a matrix
-        int db = 0;
+        constexpr int NT = 8;                 // tokens of a lane
+        const int nb = (a.N + 127) / 128;     // rows of scale blocks of a matrix
+        LinRing db;
         bool ok = true;
-        for (int i = first; ok && lin_tile(a, s, i, t); i += stride) {
-            const float *xs[NT];
+        for (int i = first; ok && lin_tile(a, off, pre, i, t); i += stride) {
+            int r[NT];
 #pragma unroll
             for (int j = 0; j < NT; ++j) {
                 const int c = lane + 32 * j;
-                int64_t r = t.row0 + c;
+                r[j] = t.row0 + c;
                 if (c < t.n && a.rows) {
-                    r = __ldg(a.rows + r);
-                    if (r < 0 || r >= a.x_rows) r = 0;
+                    r[j] = __ldg(a.rows + r[j]);
+                    if (r[j] >= a.x_rows) r[j] = -1;
                 }
-                xs[j] = c < t.n ? a.xs + r * a.xs_stride : nullptr;
+                if (c >= t.n) r[j] = -1;
             }
-            const float *ws = a.ws + ((int64_t)t.e * G * nb + t.mt) * a.steps;
-            float v[NT], w[G];
-            auto fetch = [&](int k) {
+            const int n0 = (PAIR ? 2 * t.mt + rank : t.mt) * outputs;
+            const float *ws = a.ws + ((int64_t)t.e * (1 + a.gated) * nb + min(n0 / 128, nb - 1)) * a.steps;
+            const int64_t up = (int64_t)nb * a.steps;
+            float v[2][NT], w[2][2];  // two steps ahead
+            auto fetch = [&](int k, int h) {
+                if (k >= k1) return;
 #pragma unroll
-                for (int j = 0; j < NT; ++j) v[j] = xs[j] ? __ldg(xs[j] + k) : 0.f;
-#pragma unroll
-                for (int g = 0; g < G; ++g) w[g] = __ldg(ws + (int64_t)g * nb * a.steps + k);
+                for (int j = 0; j < NT; ++j)
+                    if (32 * j < t.cols) v[h][j] = r[j] >= 0 ? __ldg(a.xs + r[j] * a.xs_stride + k) : 0.f;
+                w[h][0] = __ldg(ws + k);
+                w[h][1] = a.gated ? __ldg(ws + up + k) : 0.f;
             };
-            fetch(k0);
-            for (int k = k0; k < k1; ++k, ++db) {
-                const int buf = db % bufs;
-                if (!(ok = lin_wait(&s.dempty[buf], ((db / bufs) & 1) ^ 1, a, abort))) break;
+            fetch(k0, 0);
+            fetch(k0 + 1, 1);
+            auto give = [&](int k, int h) {
+                if (k >= k1 || !ok) return;
+                if (!(ok = lin_wait(&s.dempty[db.at], db.phase ^ 1, a, abort))) return;
+                float *sc = scales + db.at * sc_buf;
 #pragma unroll
-                for (int g = 0; g < G; ++g)
-#pragma unroll
-                    for (int j = 0; j < NT; ++j)
-                        if (lane + 32 * j < t.n16) s.sc[buf][g * a.bn + lane + 32 * j] = v[j] * w[g];
+                for (int j = 0; j < NT; ++j)
+                    if (32 * j < t.cols && lane + 32 * j < sc_row) {
+                        sc[lane + 32 * j] = v[h][j] * w[h][0];
+                        if (a.gated) sc[sc_row + lane + 32 * j] = v[h][j] * w[h][1];
+                    }
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&s.sfull[buf]);
-                if (k + 1 < k1) fetch(k + 1);
+                if (lane == 0) mbar_arrive(&s.dfull[db.at]);
+                db.next(a.bufs);
+                fetch(k + 2, h);
+            };
+            for (int k = k0; k < k1; k += 2) {
+                give(k, 0);
+                give(k + 1, 1);
             }
         }
-    } else if (warp >= 4) {  // ------------------------------------- readout
-        const int q = warp & 3, h = (warp - 4) >> 2;
-        const int nl = q * 32 + lane;  // output of the tile
-        float *part = reinterpret_cast<float *>(ring);
-        int db = 0;
-        bool ok = true;
-        for (int i = first; ok && lin_tile(a, s, i, t); i += stride) {
-            const int n = t.mt * 128 + nl;
-            const int64_t y0 = (int64_t)t.row0 * a.y_stride + n;
-            // values of the 16 tokens from c on (gated: gate's and up's): to y, or to the
-            // cluster's sum
-            auto put = [&](int c, const float (&v)[16], const float (&u)[16]) {
-                if (a.split > 1) {
-#pragma unroll
-                    for (int j = 0; j < 16; ++j) {
-                        part[(c + j) * 128 + nl] = v[j];
-                        if (GATED) part[(a.bn + c + j) * 128 + nl] = u[j];
-                    }
-                    return;
+    }
+    } else if (warp >= 12) {  // ------------------------------------- gather
+        if constexpr (MODE != kLinWhole) asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
+        if (a.rows) {
+            const int tid = threadIdx.x - 384, piece = tid & 7, part = tid >> 3;
+            LinRing st, told;
+            int open = 0;  // steps whose arrival is not told yet
+            bool ok = true;
+            auto tell = [&]() {
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) {
+                    if (PAIR) cluster_bar_arrive(cluster_addr(&s.full[told.at], 0));
+                    else mbar_arrive(&s.full[told.at]);
                 }
-                uint32_t to = lin_written(a, t, c, lane);
-                if (n >= a.N) to = 0;
+                told.next(a.stages);
+                --open;
+            };
+            for (int i = first; lin_tile(a, off, pre, i, t); i += stride) {
+                const int here = PAIR ? t.cols / 2 : t.cols, c0 = PAIR ? rank * here : 0;
+                // the rows of the tile before were used, and no warp's wait ran out
+                if (!named_all(2, 128, ok)) break;
+                for (int c = tid; c < here; c += 128) {
+                    int r = -1;
+                    if (c0 + c < t.n) {
+                        r = __ldg(a.rows + t.row0 + c0 + c);
+                        if (r < 0 || r >= a.x_rows) {
+                            atomicOr(a.err, RB_LIN_ERR_ROWS);
+                            r = -1;
+                        }
+                    }
+                    s.src[c] = r;
+                }
+                named_sync(2, 128);
+                for (int k = k0; k < k1; ++k) {
+                    if (!(ok = lin_wait(&s.empty[st.at], st.phase ^ 1, a, abort))) break;
+                    const uint32_t xb = smem_u32(ring) + st.at * stage_bytes + kLinTile;
+                    const int at = k * 128 + piece * 16;
+                    const int n = min(max(a.k_bytes - at, 0), 16);
+                    for (int c = part; c < here; c += 16) {
+                        const int r = s.src[c];
+                        const bool some = r >= 0 && n > 0;
+                        cp_async16(xb + c * 128 + ((piece ^ (c & 7)) << 4),
+                                   some ? a.x + r * a.x_bytes + at : a.x, some ? n : 0);
+                    }
+                    asm volatile("cp.async.commit_group;" ::: "memory");
+                    st.next(a.stages);
+                    if (++open > kLinLag) {
+                        asm volatile("cp.async.wait_group %0;" ::"n"(kLinLag) : "memory");
+                        tell();
+                    }
+                }
+            }
+            asm volatile("cp.async.wait_group 0;" ::: "memory");
+            while (open) tell();
+        }
+    } else {  // ---------------------------------------------------- readout
+        if constexpr (MODE != kLinWhole) asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
+        const int q = warp & 3, h = (warp - 4) >> 2;
+        const int nl = q * 32 + lane;  // weight row of the tile
+        const int tid = threadIdx.x - 128, seg = tid & 7;
+        const uint32_t lanes = (uint32_t)(q * 32) << 16;
+        float *part = reinterpret_cast<float *>(ring);
+        LinRing db;
+        bool ok = true;
+        const uint32_t mfree = PAIR ? cluster_addr(&s.mfree[0], 0) : 0;
+        auto release = [&]() {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) {
+                if (!PAIR || F8) mbar_arrive(&s.dempty[db.at]);
+                if (PAIR) cluster_bar_arrive(mfree + db.at * 8);
+            }
+            db.next(a.bufs);
+        };
+        // sums of this warp's 16 tokens of block pair b: to y, or to the cluster's sum
+        auto put = [&](int b, const float (&v)[16]) {
+            const int c = 32 * b + 16 * h;
+            if (!PAIR && a.split > 1) {
 #pragma unroll
                 for (int j = 0; j < 16; ++j)
-                    if (to >> j & 1)
-                        lin_store(a, y0 + (c + j) * a.y_stride,
-                                  GATED ? lin_silu(v[j]) * u[j] : v[j]);
-                __syncwarp();
-            };
-            if constexpr (F8) {
-                constexpr int NC = GATED ? 4 : 8;  // blocks of 16 tokens
-                float acc[G][NC][16];
+                    if (c < t.cols) part[(c + j) * 128 + nl] = v[j];
+                return;
+            }
+            named_sync(1, kLinReaders);  // the outputs before have left
 #pragma unroll
-                for (int g = 0; g < G; ++g)
+            for (int j = 0; j < 16; ++j) outs[(16 * h + j) * 128 + nl] = v[j];
+            named_sync(1, kLinReaders);
+            const int token = tid >> 3;
+            if (lin_written(a, t, 32 * b + token))
+                lin_put(a, t.row0 + 32 * b + token, (PAIR ? 2 * t.mt + (int)rank : t.mt) * outputs, seg,
+                        [&](int i) { return *reinterpret_cast<const float4 *>(outs + token * 128 + i); });
+        };
+        for (int i = first; ok && lin_tile(a, off, pre, i, t); i += stride) {
+            if constexpr (MODE != kLinWhole) {
+                float acc[8][16];
 #pragma unroll
-                    for (int c = 0; c < NC; ++c)
+                for (int c = 0; c < 8; ++c)
 #pragma unroll
-                        for (int j = 0; j < 16; ++j) acc[g][c][j] = 0.f;
-                for (int k = k0; k < k1; ++k, ++db) {
-                    const int buf = db % bufs, ph = (db / bufs) & 1;
-                    if (!(ok = lin_wait(&s.sfull[buf], ph, a, abort))) break;
-                    if (!(ok = lin_wait(&s.dfull[buf], ph, a, abort))) break;
+                    for (int j = 0; j < 16; ++j) acc[c][j] = 0.f;
+                for (int k = k0; k < k1; k += PART) {
+                    if (!(ok = lin_wait(&s.dfull[db.at], db.phase, a, abort))) break;
                     tc_fence_after();
-                    const uint32_t d = tmem + ((uint32_t)(q * 32) << 16) + buf * width;
+                    const uint32_t d = tmem + lanes + db.at * a.bn + 16 * h;
+                    const float *sc = scales + db.at * sc_buf + (a.gated && q >= 2 ? sc_row : 0) + 16 * h;
+                    float v[2][16];
+                    if (16 * h < t.cols) lin_ld16(d, v[0]);
 #pragma unroll
-                    for (int g = 0; g < G; ++g)
+                    for (int c = 0; c < 8; ++c) {
+                        if (32 * c + 16 * h >= t.cols) break;
+                        float4 f[4];
+                        if (F8) {
 #pragma unroll
-                        for (int c = 0; c < NC; ++c) {
-                            const int col = (2 * c + h) * 16;
-                            if (col >= t.n16) break;
-                            float v[16];
-                            lin_ld16(d + g * a.bn + col, v);
-                            const float4 *sc = reinterpret_cast<const float4 *>(&s.sc[buf][g * a.bn + col]);
-                            float4 f[4];
+                            for (int j = 0; j < 4; ++j) f[j] = reinterpret_cast<const float4 *>(sc + 32 * c)[j];
+                        }
+                        lin_ld_done(v[c & 1]);
+                        if (c < 7 && 32 * (c + 1) + 16 * h < t.cols) lin_ld16(d + 32 * (c + 1), v[(c + 1) & 1]);
+                        const float(&u)[16] = v[c & 1];
 #pragma unroll
-                            for (int j = 0; j < 4; ++j) f[j] = sc[j];
-                            lin_ld_done(v);
+                        for (int j = 0; j < 4; ++j) {
+                            if (F8) {
+                                acc[c][4 * j] = fmaf(u[4 * j], f[j].x, acc[c][4 * j]);
+                                acc[c][4 * j + 1] = fmaf(u[4 * j + 1], f[j].y, acc[c][4 * j + 1]);
+                                acc[c][4 * j + 2] = fmaf(u[4 * j + 2], f[j].z, acc[c][4 * j + 2]);
+                                acc[c][4 * j + 3] = fmaf(u[4 * j + 3], f[j].w, acc[c][4 * j + 3]);
+                            } else {
 #pragma unroll
-                            for (int j = 0; j < 4; ++j) {
-                                acc[g][c][4 * j] = fmaf(v[4 * j], f[j].x, acc[g][c][4 * j]);
-                                acc[g][c][4 * j + 1] = fmaf(v[4 * j + 1], f[j].y, acc[g][c][4 * j + 1]);
-                                acc[g][c][4 * j + 2] = fmaf(v[4 * j + 2], f[j].z, acc[g][c][4 * j + 2]);
-                                acc[g][c][4 * j + 3] = fmaf(v[4 * j + 3], f[j].w, acc[g][c][4 * j + 3]);
+                                for (int l = 0; l < 4; ++l) acc[c][4 * j + l] += u[4 * j + l];
                             }
                         }
-                    tc_fence_before();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(&s.dempty[buf]);
+                    }
+                    release();
                 }
+                // (a wait that ran out ends it for every warp of the block before a barrier
+                // among them)
+                ok = named_all(1, kLinReaders, ok);
                 if (!ok) break;
 #pragma unroll
-                for (int c = 0; c < NC; ++c)
-                    if ((2 * c + h) * 16 < t.n16)
-                        put((2 * c + h) * 16, acc[0][c], acc[G - 1][c]);
-            } else {
-                const int buf = db % bufs;
-                if (!(ok = lin_wait(&s.dfull[buf], (db / bufs) & 1, a, abort))) break;
-                tc_fence_after();
-                const uint32_t d = tmem + ((uint32_t)(q * 32) << 16) + buf * width;
-                for (int c = 16 * h; c < t.n16; c += 32) {
-                    float v[16], u[16];
-                    lin_ld16(d + c, v);
-                    if (GATED) lin_ld16(d + a.bn + c, u);
-                    lin_ld_done(v);
-                    if (GATED) lin_ld_done(u);
-                    put(c, v, GATED ? u : v);
+                for (int c = 0; c < 8; ++c) {
+                    if (32 * c >= t.cols) break;
+                    put(c, acc[c]);
                 }
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&s.dempty[buf]);
-                ++db;
+            } else {
+                ok = named_all(1, kLinReaders, lin_wait(&s.dfull[db.at], db.phase, a, abort));
+                if (!ok) break;
+                tc_fence_after();
+                const uint32_t d = tmem + lanes + db.at * a.bn + 16 * h;
+                for (int c = 0; 32 * c < t.cols; ++c) {
+                    float v[16];
+                    lin_ld16(d + 32 * c, v);
+                    lin_ld_done(v);
+                    put(c, v);
+                    __syncwarp();
+                }
+                release();
             }
         }
     }
     __syncwarp();
-    if (a.split > 1) {  // one tile a cluster: its parts summed in the order of the ranks
-        cluster_arrive();
-        cluster_wait();
-        if (warp >= 4 && !*abort && lin_tile(a, s, first, t)) {
-            const int nl = (warp & 3) * 32 + lane, h = (warp - 4) >> 2;
-            const int n = t.mt * 128 + nl;
-            const float *part = reinterpret_cast<const float *>(ring);
-            for (int c = 0; c < t.n; c += 32) {
-                const uint32_t to = lin_written(a, t, c, lane);
-                for (int j = 0; j < 32; ++j) {
-                    const int tok = c + j, turn = tok / a.split;
-                    if (!(to >> j & 1) || tok - turn * a.split != (int)rank || (turn & 1) != h) continue;
-                    float v = 0.f, u = 0.f;
+    if (!PAIR && a.split > 1) {  // one tile a cluster: its parts summed in the order of the ranks
+        cluster_sync_all();
+        if (warp >= 4 && warp < 12 && !*abort && lin_tile(a, off, pre, first, t)) {
+            const uint32_t part = smem_u32(ring);
+            for (int j = threadIdx.x - 128;; j += kLinReaders) {
+                const int item = j * a.split + rank, token = item >> 3;
+                if (token >= t.n) break;
+                if (!lin_written(a, t, token)) continue;
+                lin_put(a, t.row0 + token, t.mt * outputs, item & 7, [&](int i) {
+                    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
                     for (int r = 0; r < a.split; ++r) {
-                        v += cluster_ld(part + tok * 128 + nl, r);
-                        if (GATED) u += cluster_ld(part + (a.bn + tok) * 128 + nl, r);
+                        uint32_t at;
+                        asm volatile("mapa.shared::cluster.u32 %0, %1, %2;"
+                                     : "=r"(at) : "r"(part + (uint32_t)(token * 128 + i) * 4), "r"(r));
+                        const float4 u = cluster_ld4(at);
+                        v.x += u.x;
+                        v.y += u.y;
+                        v.z += u.z;
+                        v.w += u.w;
                     }
-                    if (n < a.N)
-                        lin_store(a, (int64_t)(t.row0 + tok) * a.y_stride + n,
-                                  GATED ? lin_silu(v) * u : v);
-                }
+                    return v;
+                });
             }
         }
-        cluster_arrive();  // nobody leaves while its part is read
-        cluster_wait();
+        cluster_sync_all();  // nobody leaves while its part is read
     }
     tc_fence_before();
     __syncthreads();
+    if (PAIR) cluster_sync_all();  // both have read their products
     tc_fence_after();
-    if (warp == 1) tmem_dealloc(tmem, 512);
+    if (warp == 1) {
+        if (PAIR) tmem_dealloc_pair(tmem, 512);
+        else tmem_dealloc(tmem, 512);
+    }
+    if (PAIR) cluster_sync_all();
 }
 
 }  // namespace rb

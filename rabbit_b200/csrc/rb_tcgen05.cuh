@@ -54,6 +54,19 @@ __device__ __forceinline__ void tmem_dealloc(uint32_t taddr, uint32_t cols) {
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(cols)
                  : "memory");
 }
+// The same for a pair of CTAs (ranks 2 i and 2 i + 1 of a cluster): a warp of each
+// calls it.
+__device__ __forceinline__ void tmem_alloc_pair(uint32_t *dst, uint32_t cols) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                     smem_u32(dst)),
+                 "r"(cols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void tmem_dealloc_pair(uint32_t taddr, uint32_t cols) {
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(cols)
+                 : "memory");
+}
 __device__ __forceinline__ void tc_fence_before() {
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
 }
@@ -119,11 +132,11 @@ __device__ __forceinline__ void mma_commit(uint64_t *bar) {
 }
 
 // Instruction descriptor of kind::f8f6f4 (e4m3: format 0) and kind::f16 (f16 0,
-// bf16 1): f32 accumulator, A and B of one format, both K-major, M = 128, N a
-// multiple of 16 up to 256.
-__host__ __device__ constexpr uint32_t float_idesc(int format, int N) {
+// bf16 1): f32 accumulator, A and B of one format, both K-major, M = 128 (256 for
+// a pair of CTAs), N a multiple of 16 up to 256.
+__host__ __device__ constexpr uint32_t float_idesc(int format, int M, int N) {
     return (1u << 4) | ((uint32_t)format << 7) | ((uint32_t)format << 10) |
-           ((uint32_t)(N >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
+           ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
 }
 
 // Shared-memory matrix descriptor of a K-major tile of 128-byte rows in the
@@ -135,25 +148,33 @@ __device__ __forceinline__ uint64_t swizzled_desc(uint32_t smem_addr) {
            ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
 }
 
-// D[128 x N] (+)= A[128 x 32 bytes] * B[N x 32 bytes]^T, f32 accumulator, both
-// operands in shared memory. Issued by one thread.
-template <bool F8>
+// D[M x N] (+)= A[M x 32 bytes] * B[N x 32 bytes]^T, f32 accumulator, both
+// operands in shared memory; issued by one thread. PAIR: M = 256, CTA r of the pair has
+// rows 128 r .. of A and D and the r-th half of B's rows, at the same offsets;
+// issued by rank 0 for both.
+template <bool F8, bool PAIR>
 __device__ __forceinline__ void mma_float_ss(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc,
                                              uint32_t idesc, uint32_t accumulate) {
-    if constexpr (F8)
-        asm volatile(
-            "{\n\t.reg .pred p;\n\t"
-            "setp.ne.b32 p, %4, 0;\n\t"
-            "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
-            ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
-            : "memory");
-    else
-        asm volatile(
-            "{\n\t.reg .pred p;\n\t"
-            "setp.ne.b32 p, %4, 0;\n\t"
-            "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
-            ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
-            : "memory");
+#define RB_MMA(GROUP, KIND)                                                     \
+    asm volatile(                                                               \
+        "{\n\t.reg .pred p;\n\t"                                               \
+        "setp.ne.b32 p, %4, 0;\n\t"                                             \
+        "tcgen05.mma.cta_group::" GROUP ".kind::" KIND " [%0], %1, %2, %3, p;\n\t}" \
+        ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)    \
+        : "memory")
+    if constexpr (F8 && PAIR) RB_MMA("2", "f8f6f4");
+    else if constexpr (F8) RB_MMA("1", "f8f6f4");
+    else if constexpr (PAIR) RB_MMA("2", "f16");
+    else RB_MMA("1", "f16");
+#undef RB_MMA
+}
+// mma_commit of a pair's products: one arrival on the barrier at this offset in both CTAs.
+__device__ __forceinline__ void mma_commit_pair(uint64_t *bar) {
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 "
+        "[%0], %1;" ::"r"(smem_u32(bar)),
+        "h"((uint16_t)3)
+        : "memory");
 }
 
 // ----------------------------------------------------------- tiled TMA --
@@ -187,14 +208,24 @@ __device__ __forceinline__ void tma_load_2d(void *smem_dst, const CUtensorMap *m
         "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(smem_u32(bar))
         : "memory");
 }
-// Four rows r0 .. r3 of a 2-D map whose box is one row high, one after the other.
-__device__ __forceinline__ void tma_gather4(void *smem_dst, const CUtensorMap *map, int c0, int r0,
-                                            int r1, int r2, int r3, uint64_t *bar) {
+// For a CTA of a pair: into its own shared memory, completing on a barrier of either
+// CTA (`bar`: a shared::cluster address). No multicast.
+__device__ __forceinline__ void tma_load_2d_pair(void *smem_dst, const CUtensorMap *map, int c0,
+                                                 int c1, uint32_t bar) {
     asm volatile(
-        "cp.async.bulk.tensor.2d.shared::cta.global.tile::gather4.mbarrier::complete_tx::bytes"
-        " [%0], [%1, {%2, %3, %4, %5, %6}], [%7];" ::"r"(smem_u32(smem_dst)),
-        "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(r0), "r"(r1), "r"(r2), "r"(r3),
-        "r"(smem_u32(bar))
+        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%2, %3}], [%4];" ::"r"(smem_u32(smem_dst)),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(bar)
+        : "memory");
+}
+__device__ __forceinline__ void tma_load_4d_pair(void *smem_dst, const CUtensorMap *map, int c0,
+                                                 int c1, int c2, int c3, uint32_t bar,
+                                                 uint64_t policy) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+        ".L2::cache_hint [%0], [%1, {%2, %3, %4, %5}], [%6], %7;" ::"r"(smem_u32(smem_dst)),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(bar),
+        "l"(policy)
         : "memory");
 }
 __device__ __forceinline__ void tma_prefetch_map(const CUtensorMap *map) {
