@@ -33,18 +33,29 @@ static int operand_size(int dtype) {
 
 using LinKernel = void (*)(LinArgs, CUtensorMap, CUtensorMap);
 
-static LinKernel lin_kernel(int mode, bool pair) {
-    if (mode == kLinF8) return pair ? k_linear<kLinF8, true> : k_linear<kLinF8, false>;
-    if (mode == kLinParts) return pair ? k_linear<kLinParts, true> : k_linear<kLinParts, false>;
-    return pair ? k_linear<kLinWhole, true> : k_linear<kLinWhole, false>;
+template <int MODE, bool PAIR>
+static LinKernel lin_kernel_of(bool gated, int out_dtype) {
+    LinKernel k = nullptr;
+    with_dtype(out_dtype, [&](auto t) {
+        k = gated ? k_linear<MODE, PAIR, true, decltype(t)> : k_linear<MODE, PAIR, false, decltype(t)>;
+        return 0;
+    });
+    return k;
+}
+static LinKernel lin_kernel(int mode, bool pair, bool gated, int out_dtype) {
+    if (mode == kLinF8)
+        return pair ? lin_kernel_of<kLinF8, true>(gated, out_dtype) : lin_kernel_of<kLinF8, false>(gated, out_dtype);
+    if (mode == kLinParts)
+        return pair ? lin_kernel_of<kLinParts, true>(gated, out_dtype) : lin_kernel_of<kLinParts, false>(gated, out_dtype);
+    return pair ? lin_kernel_of<kLinWhole, true>(gated, out_dtype) : lin_kernel_of<kLinWhole, false>(gated, out_dtype);
 }
 
 // The current device's kernels for an object: their shared memory; `fits`: those that share
 // out registers were built to be launched with the 128 a thread that the shares add up to.
-static cudaError_t lin_prepare_kernels(bool f8, bool *fits) {
+static cudaError_t lin_prepare_kernels(bool f8, bool gated, bool *fits) {
     for (int mode = f8 ? kLinF8 : kLinWhole; mode <= (f8 ? kLinF8 : kLinParts); ++mode)
-        for (int pair = 0; pair < 2; ++pair) {
-            const void *k = reinterpret_cast<const void *>(lin_kernel(mode, pair));
+        for (int i = 0; i < 6; ++i) {
+            const void *k = reinterpret_cast<const void *>(lin_kernel(mode, i & 1, gated, i >> 1));
             cudaFuncAttributes at;
             cudaError_t e = cudaFuncGetAttributes(&at, k);
             if (e == cudaSuccess)
@@ -113,7 +124,8 @@ static int lin_run(rabbit_cuda_linear *lin, const char *what, const void *d_x, i
     a.steps = (int)(((int64_t)d.n_in * size + 127) / 128);
     a.gated = d.gated;
     const int64_t xs = x_stride ? x_stride : d.n_in;
-    a.xs_stride = x_scale_stride ? x_scale_stride : a.steps;
+    const int64_t scale_stride = x_scale_stride ? x_scale_stride : a.steps;
+    a.xs_stride = (uint32_t)scale_stride;
     a.y_stride = y_stride ? y_stride : d.n_out;
     if (!d_x || !d_y || (f8 && !d_x_scale))
         return fail(RABBIT_CUDA_ERR_ARGS, "%s: NULL pointer", what);
@@ -122,8 +134,8 @@ static int lin_run(rabbit_cuda_linear *lin, const char *what, const void *d_x, i
         return fail(RABBIT_CUDA_ERR_ARGS,
                     "%s: x not aligned to 16 bytes, a stride below its row or (x) not a multiple of "
                     "16 bytes, or a pointer not aligned to its element", what);
-    if (f8 && (a.xs_stride < a.steps || !aligned(d_x_scale, 4)))
-        return fail(RABBIT_CUDA_ERR_ARGS, "%s: x_scale_stride below its row, or scales not aligned", what);
+    if (f8 && (scale_stride < a.steps || scale_stride > 1 << 30 || !aligned(d_x_scale, 4)))
+        return fail(RABBIT_CUDA_ERR_ARGS, "%s: x_scale_stride below its row or above 2^30, or scales not aligned", what);
     if (x_rows < 1 || (!d_rows && x_rows < n_rows))
         return fail(RABBIT_CUDA_ERR_ARGS, "%s: x_rows of %d for %d rows", what, x_rows, n_rows);
     int64_t tiles;
@@ -138,7 +150,7 @@ static int lin_run(rabbit_cuda_linear *lin, const char *what, const void *d_x, i
     a.offsets = d_offsets;
     a.rows = d_rows;
     a.x = static_cast<const uint8_t *>(d_x);
-    a.x_bytes = xs * size;
+    a.x_bytes = (uint32_t)(xs * size);
     a.k_bytes = d.n_in * size;
     a.vec = aligned(d_y, 16) && a.y_stride * out % 16 == 0;
     a.xs = d_x_scale;
@@ -170,7 +182,7 @@ static int lin_run(rabbit_cuda_linear *lin, const char *what, const void *d_x, i
     cfg.stream = static_cast<cudaStream_t>(stream);
     cfg.attrs = attr;
     cfg.numAttrs = team > 1 ? 2 : 1;
-    scope.launch(cudaLaunchKernelEx(&cfg, lin_kernel(mode, pair), a, lin->map, mx), what);
+    scope.launch(cudaLaunchKernelEx(&cfg, lin_kernel(mode, pair, d.gated, out_dtype), a, lin->map, mx), what);
     return scope.done();
 }
 
@@ -224,7 +236,7 @@ int rabbit_cuda_linear_create(const rabbit_cuda_linear_desc *d, int device,
     if (e == cudaSuccess && (e = cudaMalloc(&lin->d_err, 2 * sizeof(int))) == cudaSuccess &&
         (e = cudaMemset(lin->d_err, 0, 2 * sizeof(int))) == cudaSuccess &&
         (e = cudaStreamSynchronize(nullptr)) == cudaSuccess)  // zeroed before any stream uses it
-        e = lin_prepare_kernels(d->dtype == RABBIT_CUDA_E4M3, &fits);
+        e = lin_prepare_kernels(d->dtype == RABBIT_CUDA_E4M3, d->gated, &fits);
     const cuuint64_t dims[4] = {(cuuint64_t)d->n_in, (cuuint64_t)d->n_out, (cuuint64_t)1 + d->gated,
                                 (cuuint64_t)d->n_experts};
     const cuuint64_t strides[3] = {row, matrix, matrix * (1 + d->gated)};

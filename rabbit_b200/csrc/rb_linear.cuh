@@ -11,7 +11,7 @@
 //   warp 0       TMA: the step's weight rows and, without a list, token rows into a ring of
 //                stages (128-byte rows, 128-byte swizzle);
 //   warp 1       tensor memory; one thread issues the step's MMAs and commits;
-//   warp 2       (e4m3) the step's scales, sw * sx for each token, into shared memory;
+//   warps 2, 3   (e4m3) the step's scales, sw * sx for each token, into shared memory;
 //   warps 4..11  readout: warp w reads lanes 32 (w % 4) .. + 31 (weight rows), and the
 //                even or odd blocks of 16 tokens; outputs go through shared memory, so that
 //                they leave in rows of 16 bytes a thread;
@@ -51,7 +51,6 @@ constexpr int kLinMaxExperts = 1024;
 constexpr int kLinBufs = 8;               // buffers of tensor memory, at most
 constexpr int kLinStages = 12;            // stages of the ring, at most
 constexpr int kLinPart = 4;               // steps of a part (kLinParts)
-constexpr int kLinLag = 2;                // steps by which a gathered row's arrival is told later
 constexpr uint32_t kLinTile = 128 * 128;  // bytes of a step's 128 weight rows
 constexpr uint32_t kLinOut = 32 * 128 * 4;  // outputs on their way: 32 tokens
 
@@ -64,10 +63,10 @@ struct LinArgs {
     const int *offsets;   // [E + 1], or NULL: one expert with all rows
     const int *rows;      // [R] rows of x, or NULL
     const uint8_t *x;     // with a list: x, its row in bytes, and the bytes of n_in
-    int64_t x_bytes;
+    uint32_t x_bytes;
     int k_bytes;
     const float *xs, *ws; // e4m3: scales
-    int64_t xs_stride;
+    uint32_t xs_stride;
     void *y;
     int64_t y_stride;
     int out_dtype;
@@ -91,11 +90,11 @@ struct LinArgs {
 // the scales [bufs][1 or 2][bn, at least 32], off [E + 1] and pre [E + 1].
 struct LinShared {
     uint64_t full[kLinStages], empty[kLinStages];
+    uint64_t rows[kLinStages];  // with a list: this CTA's token rows have arrived
     uint64_t dfull[kLinBufs], dempty[kLinBufs], mfree[kLinBufs];
     uint64_t mdone;
     uint32_t tmem;
     int abort;
-    int src[256];  // with a list: the tile's rows of x, -1 for none
 };
 static_assert(sizeof(LinShared) % 16 == 0, "the scales behind it are read 16 bytes at a time");
 __host__ __device__ constexpr int lin_sc(int bn) { return bn < 32 ? 32 : bn; }
@@ -137,6 +136,11 @@ __device__ __forceinline__ bool lin_tile(const LinArgs &a, const int *off, const
     t.cols = (t.n + a.unit - 1) / a.unit * a.unit;
     return true;
 }
+
+template <int N>
+struct LinInt {
+    static constexpr int value = N;
+};
 
 // A place in a ring and the parity of its use.
 struct LinRing {
@@ -219,6 +223,11 @@ __device__ __forceinline__ float4 cluster_ld4(uint32_t at) {
                  : "memory");
     return v;
 }
+// Writes of the generic proxy (cp.async) that this thread waited for are seen by the
+// asynchronous one (the MMAs issued after).
+__device__ __forceinline__ void fence_async() {
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+}
 // 16 bytes (n of them read, the rest zero) into shared memory.
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void *src, int n) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
@@ -235,39 +244,32 @@ __device__ __forceinline__ void lin_ld_done(float (&v)[16]) {
                    "+f"(v[12]), "+f"(v[13]), "+f"(v[14]), "+f"(v[15])::"memory");
 }
 
-__device__ __forceinline__ float lin_silu(float g) { return g / (1.f + expf(-g)); }
+// g / (1 + exp(-g)); the division to 2 units in the last place.
+__device__ __forceinline__ float lin_silu(float g) { return __fdividef(g, 1.f + expf(-g)); }
 
-// Eight outputs of a row from column c on.
-template <typename T>
-__device__ __forceinline__ void lin_put8(const LinArgs &a, int64_t row, int c, const float (&v)[8]) {
-    T *y = static_cast<T *>(a.y) + row * a.y_stride + c;
-    if (a.vec && c + 8 <= a.N) {
-        store8<true>(y, v);
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-            if (c + i < a.N) y[i] = from_f32<T>(v[i]);
-    }
-}
 // Piece `seg` of 8 of a token's row of 128 sums, which `get(i)` reads four at a time, to
 // row `row` of y, whose columns from `n0` on they are.
-template <typename F>
+template <bool GATED, typename T, typename F>
 __device__ __forceinline__ void lin_put(const LinArgs &a, int64_t row, int n0, int seg, F &&get) {
 #pragma unroll
-    for (int p = 0; p < 2; ++p) {
-        const int c = a.gated ? seg * 8 : (p * 8 + seg) * 8;
-        if (a.gated && p) break;
+    for (int p = 0; p < (GATED ? 1 : 2); ++p) {
+        const int c = (p * 8 + seg) * 8;
         const float4 l = get(c), h = get(c + 4);
         float v[8] = {l.x, l.y, l.z, l.w, h.x, h.y, h.z, h.w};
-        if (a.gated) {
+        if constexpr (GATED) {
             const float4 ul = get(64 + c), uh = get(64 + c + 4);
             const float u[8] = {ul.x, ul.y, ul.z, ul.w, uh.x, uh.y, uh.z, uh.w};
 #pragma unroll
             for (int i = 0; i < 8; ++i) v[i] = lin_silu(v[i]) * u[i];
         }
-        if (a.out_dtype == RABBIT_CUDA_F32) lin_put8<float>(a, row, n0 + c, v);
-        else if (a.out_dtype == RABBIT_CUDA_F16) lin_put8<__half>(a, row, n0 + c, v);
-        else lin_put8<__nv_bfloat16>(a, row, n0 + c, v);
+        T *y = static_cast<T *>(a.y) + row * a.y_stride + n0 + c;
+        if (a.vec && n0 + c + 8 <= a.N) {
+            store8<true>(y, v);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (n0 + c + i < a.N) y[i] = from_f32<T>(v[i]);
+        }
     }
 }
 // Whether token c of a tile is written.
@@ -278,7 +280,7 @@ __device__ __forceinline__ bool lin_written(const LinArgs &a, const LinTile &t, 
     return r >= 0 && r < a.x_rows;
 }
 
-template <int MODE, bool PAIR>
+template <int MODE, bool PAIR, bool GATED, typename OUT>
 __global__ void __launch_bounds__(kLinThreads, 1)
     k_linear(const __grid_constant__ LinArgs a, const __grid_constant__ CUtensorMap mw,
              const __grid_constant__ CUtensorMap mx) {
@@ -290,7 +292,7 @@ __global__ void __launch_bounds__(kLinThreads, 1)
     float *outs = reinterpret_cast<float *>(ring + (size_t)a.stages * stage_bytes);
     LinShared &s = *reinterpret_cast<LinShared *>(reinterpret_cast<uint8_t *>(outs) + kLinOut);
     float *scales = reinterpret_cast<float *>(&s + 1);
-    const int sc_row = lin_sc(a.bn), sc_buf = (1 + a.gated) * sc_row;
+    const int sc_row = lin_sc(a.bn), sc_buf = (1 + GATED) * sc_row;
     int *off = reinterpret_cast<int *>(scales + (F8 ? a.bufs * sc_buf : 0)), *pre = off + a.E + 1;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     volatile int *abort = &s.abort;
@@ -298,13 +300,13 @@ __global__ void __launch_bounds__(kLinThreads, 1)
     const bool leader = !PAIR || rank == 0;
 
     if (threadIdx.x == 0) {
-        const int rows_from = a.rows ? (PAIR ? 8 : 4) : 0;  // gathering warps that arrive
         for (int i = 0; i < a.stages; ++i) {
-            mbar_init(&s.full[i], 1 + rows_from);
+            mbar_init(&s.full[i], PAIR && a.rows ? 2 : 1);  // the TMA, and word of CTA 1's rows
             mbar_init(&s.empty[i], 1);
+            mbar_init(&s.rows[i], 128);
         }
         for (int i = 0; i < a.bufs; ++i) {
-            mbar_init(&s.dfull[i], F8 ? 2 : 1);  // the MMAs and the scales
+            mbar_init(&s.dfull[i], F8 ? 3 : 1);  // the MMAs, and two warps of scales
             mbar_init(&s.dempty[i], 8);          // this CTA's readout
             mbar_init(&s.mfree[i], 16);          // the pair's
         }
@@ -354,13 +356,13 @@ __global__ void __launch_bounds__(kLinThreads, 1)
     const int first = blockIdx.x / team, stride = !PAIR && a.split > 1 ? 1 << 30 : gridDim.x / team;
     const int k0 = PAIR ? 0 : (int)((int64_t)a.steps * rank / a.split);
     const int k1 = PAIR ? a.steps : (int)((int64_t)a.steps * (rank + 1) / a.split);
-    const int outputs = a.gated ? 64 : 128;  // of a CTA's tile
+    const int outputs = GATED ? 64 : 128;  // of a CTA's tile
     LinTile t;
 
-    // Registers: 512 x 128 at the launch (linear_create checks it); 128 x 64 + 128 x 48 +
-    // 256 x 200 from here.
+    // Registers: 512 x 128 at the launch (linear_create checks it); 128 x 72 + 128 x 56 +
+    // 256 x 192 from here.
     if (warp < 4) {
-        if constexpr (MODE != kLinWhole) asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+        if constexpr (MODE != kLinWhole) asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
     if (warp == 0) {  // ------------------------------------------------ TMA
         if (elect_one()) {
             const uint64_t keep = policy_evict_last(), once = policy_evict_first();
@@ -383,12 +385,12 @@ __global__ void __launch_bounds__(kLinThreads, 1)
                     if constexpr (PAIR) {
                         const uint32_t bar = cluster_addr(&s.full[st.at], 0);
                         tma_load_4d_pair(base, &mw, c0, n0, 0, t.e, bar, pol);
-                        if (a.gated) tma_load_4d_pair(base + kLinTile / 2, &mw, c0, n0, 1, t.e, bar, pol);
+                        if (GATED) tma_load_4d_pair(base + kLinTile / 2, &mw, c0, n0, 1, t.e, bar, pol);
                         for (int b = 0; b < boxes; ++b)
                             tma_load_2d_pair(xb + b * a.box * 128, &mx, c0, r0 + b * a.box, bar);
                     } else {
                         tma_load_4d(base, &mw, c0, n0, 0, t.e, &s.full[st.at], pol);
-                        if (a.gated) tma_load_4d(base + kLinTile / 2, &mw, c0, n0, 1, t.e, &s.full[st.at], pol);
+                        if (GATED) tma_load_4d(base + kLinTile / 2, &mw, c0, n0, 1, t.e, &s.full[st.at], pol);
                         for (int b = 0; b < boxes; ++b)
                             tma_load_2d(xb + b * a.box * 128, &mx, c0, r0 + b * a.box, &s.full[st.at]);
                     }
@@ -414,6 +416,10 @@ __global__ void __launch_bounds__(kLinThreads, 1)
                     if (part == 0)
                         if (!(ok = lin_wait1(PAIR ? &s.mfree[db.at] : &s.dempty[db.at], db.phase ^ 1, a, abort))) break;
                     if (!(ok = lin_wait1(&s.full[st.at], st.phase, a, abort))) break;
+                    if (a.rows) {
+                        if (!(ok = lin_wait1(&s.rows[st.at], st.phase, a, abort))) break;
+                        fence_async();
+                    }
                     tc_fence_after();
                     const uint64_t step = (uint64_t)(st.at * stage_bytes) >> 4;
                     const uint32_t d = tmem + db.at * a.bn;
@@ -437,17 +443,32 @@ __global__ void __launch_bounds__(kLinThreads, 1)
                 mbar_wait(&s.mdone, 0, a.wait_ns, nullptr, 0);
             }
         }
+        if (PAIR && !leader && a.rows && elect_one()) {  // word of this CTA's rows to the leader
+            LinRing st;
+            bool ok = true;
+            for (int i = first; ok && lin_tile(a, off, pre, i, t); i += stride)
+                for (int k = k0; k < k1; ++k) {
+                    if (!(ok = lin_wait1(&s.rows[st.at], st.phase, a, abort))) break;
+                    fence_async();
+                    cluster_bar_arrive(cluster_addr(&s.full[st.at], 0));
+                    st.next(a.stages);
+                }
+        }
         __syncwarp();
-    } else if (F8 && warp == 2) {  // --------------------------------- scales
-        constexpr int NT = 8;                 // tokens of a lane
-        const int nb = (a.N + 127) / 128;     // rows of scale blocks of a matrix
+    } else if (F8) {  // ---------------------------------------------- scales
+        const int nb = (a.N + 127) / 128;  // rows of scale blocks of a matrix
+        const int64_t up = (int64_t)nb * a.steps;
         LinRing db;
         bool ok = true;
-        for (int i = first; ok && lin_tile(a, off, pre, i, t); i += stride) {
+        const int c1 = (warp - 2) * 128 + lane;  // tokens c1, c1 + 32, ..
+        // NT tokens a lane, the scales of the next AHEAD steps on their way (a step of a few
+        // tokens takes 0.4 us, as long as half a read from HBM)
+        auto tile = [&](auto nt, auto ahead) {
+            constexpr int NT = decltype(nt)::value, AHEAD = decltype(ahead)::value;
             int r[NT];
 #pragma unroll
             for (int j = 0; j < NT; ++j) {
-                const int c = lane + 32 * j;
+                const int c = c1 + 32 * j;
                 r[j] = t.row0 + c;
                 if (c < t.n && a.rows) {
                     r[j] = __ldg(a.rows + r[j]);
@@ -456,97 +477,84 @@ __global__ void __launch_bounds__(kLinThreads, 1)
                 if (c >= t.n) r[j] = -1;
             }
             const int n0 = (PAIR ? 2 * t.mt + rank : t.mt) * outputs;
-            const float *ws = a.ws + ((int64_t)t.e * (1 + a.gated) * nb + min(n0 / 128, nb - 1)) * a.steps;
-            const int64_t up = (int64_t)nb * a.steps;
-            float v[2][NT], w[2][2];  // two steps ahead
+            const float *ws = a.ws + ((int64_t)t.e * (1 + GATED) * nb + min(n0 / 128, nb - 1)) * a.steps;
+            float v[AHEAD][NT], w[AHEAD][2];
             auto fetch = [&](int k, int h) {
                 if (k >= k1) return;
 #pragma unroll
                 for (int j = 0; j < NT; ++j)
-                    if (32 * j < t.cols) v[h][j] = r[j] >= 0 ? __ldg(a.xs + r[j] * a.xs_stride + k) : 0.f;
+                    v[h][j] = r[j] >= 0 ? __ldg(a.xs + (uint64_t)r[j] * a.xs_stride + k) : 0.f;
                 w[h][0] = __ldg(ws + k);
-                w[h][1] = a.gated ? __ldg(ws + up + k) : 0.f;
+                w[h][1] = GATED ? __ldg(ws + up + k) : 0.f;
             };
-            fetch(k0, 0);
-            fetch(k0 + 1, 1);
-            auto give = [&](int k, int h) {
-                if (k >= k1 || !ok) return;
-                if (!(ok = lin_wait(&s.dempty[db.at], db.phase ^ 1, a, abort))) return;
-                float *sc = scales + db.at * sc_buf;
 #pragma unroll
-                for (int j = 0; j < NT; ++j)
-                    if (32 * j < t.cols && lane + 32 * j < sc_row) {
-                        sc[lane + 32 * j] = v[h][j] * w[h][0];
-                        if (a.gated) sc[sc_row + lane + 32 * j] = v[h][j] * w[h][1];
-                    }
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&s.dfull[db.at]);
-                db.next(a.bufs);
-                fetch(k + 2, h);
-            };
-            for (int k = k0; k < k1; k += 2) {
-                give(k, 0);
-                give(k + 1, 1);
+            for (int h = 0; h < AHEAD; ++h) fetch(k0 + h, h);
+            for (int k = k0; k < k1; k += AHEAD) {
+#pragma unroll
+                for (int h = 0; h < AHEAD; ++h) {
+                    if (k + h >= k1 || !ok) break;
+                    if (!(ok = lin_wait(&s.dempty[db.at], db.phase ^ 1, a, abort))) break;
+                    float *sc = scales + db.at * sc_buf;
+#pragma unroll
+                    for (int j = 0; j < NT; ++j)
+                        if (c1 + 32 * j < sc_row) {
+                            sc[c1 + 32 * j] = v[h][j] * w[h][0];
+                            if (GATED) sc[sc_row + c1 + 32 * j] = v[h][j] * w[h][1];
+                        }
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&s.dfull[db.at]);
+                    db.next(a.bufs);
+                    fetch(k + h + AHEAD, h);
+                }
             }
+        };
+        for (int i = first; ok && lin_tile(a, off, pre, i, t); i += stride) {
+            if (t.cols <= 32) tile(LinInt<1>(), LinInt<GATED ? 5 : 8>());
+            else tile(LinInt<4>(), LinInt<2>());
         }
     }
     } else if (warp >= 12) {  // ------------------------------------- gather
-        if constexpr (MODE != kLinWhole) asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
+        if constexpr (MODE != kLinWhole) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
         if (a.rows) {
+            constexpr int ROWS = PAIR ? 8 : 16;  // of a thread: part, part + 16, ..
             const int tid = threadIdx.x - 384, piece = tid & 7, part = tid >> 3;
-            LinRing st, told;
-            int open = 0;  // steps whose arrival is not told yet
+            const uint32_t to = smem_u32(ring) + kLinTile + part * 128 + ((piece ^ (part & 7)) << 4);
+            LinRing st;
             bool ok = true;
-            auto tell = [&]() {
-                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                __syncwarp();
-                if (lane == 0) {
-                    if (PAIR) cluster_bar_arrive(cluster_addr(&s.full[told.at], 0));
-                    else mbar_arrive(&s.full[told.at]);
-                }
-                told.next(a.stages);
-                --open;
-            };
-            for (int i = first; lin_tile(a, off, pre, i, t); i += stride) {
+            for (int i = first; ok && lin_tile(a, off, pre, i, t); i += stride) {
                 const int here = PAIR ? t.cols / 2 : t.cols, c0 = PAIR ? rank * here : 0;
-                // the rows of the tile before were used, and no warp's wait ran out
-                if (!named_all(2, 128, ok)) break;
-                for (int c = tid; c < here; c += 128) {
-                    int r = -1;
-                    if (c0 + c < t.n) {
-                        r = __ldg(a.rows + t.row0 + c0 + c);
-                        if (r < 0 || r >= a.x_rows) {
+                int r[ROWS];  // of x; -1: none, zeros
+#pragma unroll
+                for (int j = 0; j < ROWS; ++j) {
+                    const int c = part + 16 * j;
+                    r[j] = -1;
+                    if (c < here && c0 + c < t.n) {
+                        r[j] = __ldg(a.rows + t.row0 + c0 + c);
+                        if (r[j] < 0 || r[j] >= a.x_rows) {
                             atomicOr(a.err, RB_LIN_ERR_ROWS);
-                            r = -1;
+                            r[j] = -1;
                         }
                     }
-                    s.src[c] = r;
                 }
-                named_sync(2, 128);
                 for (int k = k0; k < k1; ++k) {
                     if (!(ok = lin_wait(&s.empty[st.at], st.phase ^ 1, a, abort))) break;
-                    const uint32_t xb = smem_u32(ring) + st.at * stage_bytes + kLinTile;
-                    const int at = k * 128 + piece * 16;
-                    const int n = min(max(a.k_bytes - at, 0), 16);
-                    for (int c = part; c < here; c += 16) {
-                        const int r = s.src[c];
-                        const bool some = r >= 0 && n > 0;
-                        cp_async16(xb + c * 128 + ((piece ^ (c & 7)) << 4),
-                                   some ? a.x + r * a.x_bytes + at : a.x, some ? n : 0);
-                    }
-                    asm volatile("cp.async.commit_group;" ::: "memory");
+                    const uint32_t dst = to + st.at * stage_bytes;
+                    const int at = k * 128 + piece * 16, n = min(max(a.k_bytes - at, 0), 16);
+                    const uint8_t *x = a.x + (n > 0 ? at : 0);
+#pragma unroll
+                    for (int j = 0; j < ROWS; ++j)
+                        if (16 * j < here)
+                            cp_async16(dst + j * 2048, x + (int64_t)max(r[j], 0) * a.x_bytes, r[j] >= 0 ? n : 0);
+                    // (the fence that lets the tensor cores see them is the waiting thread's: here it
+                    // would wait for every copy under way)
+                    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(&s.rows[st.at])) : "memory");
                     st.next(a.stages);
-                    if (++open > kLinLag) {
-                        asm volatile("cp.async.wait_group %0;" ::"n"(kLinLag) : "memory");
-                        tell();
-                    }
                 }
             }
-            asm volatile("cp.async.wait_group 0;" ::: "memory");
-            while (open) tell();
+            asm volatile("cp.async.wait_all;" ::: "memory");
         }
     } else {  // ---------------------------------------------------- readout
-        if constexpr (MODE != kLinWhole) asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
+        if constexpr (MODE != kLinWhole) asm volatile("setmaxnreg.inc.sync.aligned.u32 192;");
         const int q = warp & 3, h = (warp - 4) >> 2;
         const int nl = q * 32 + lane;  // weight row of the tile
         const int tid = threadIdx.x - 128, seg = tid & 7;
@@ -579,7 +587,7 @@ __global__ void __launch_bounds__(kLinThreads, 1)
             named_sync(1, kLinReaders);
             const int token = tid >> 3;
             if (lin_written(a, t, 32 * b + token))
-                lin_put(a, t.row0 + 32 * b + token, (PAIR ? 2 * t.mt + (int)rank : t.mt) * outputs, seg,
+                lin_put<GATED, OUT>(a, t.row0 + 32 * b + token, (PAIR ? 2 * t.mt + (int)rank : t.mt) * outputs, seg,
                         [&](int i) { return *reinterpret_cast<const float4 *>(outs + token * 128 + i); });
         };
         for (int i = first; ok && lin_tile(a, off, pre, i, t); i += stride) {
@@ -593,7 +601,7 @@ __global__ void __launch_bounds__(kLinThreads, 1)
                     if (!(ok = lin_wait(&s.dfull[db.at], db.phase, a, abort))) break;
                     tc_fence_after();
                     const uint32_t d = tmem + lanes + db.at * a.bn + 16 * h;
-                    const float *sc = scales + db.at * sc_buf + (a.gated && q >= 2 ? sc_row : 0) + 16 * h;
+                    const float *sc = scales + db.at * sc_buf + (GATED && q >= 2 ? sc_row : 0) + 16 * h;
                     float v[2][16];
                     if (16 * h < t.cols) lin_ld16(d, v[0]);
 #pragma unroll
@@ -656,7 +664,7 @@ __global__ void __launch_bounds__(kLinThreads, 1)
                 const int item = j * a.split + rank, token = item >> 3;
                 if (token >= t.n) break;
                 if (!lin_written(a, t, token)) continue;
-                lin_put(a, t.row0 + token, t.mt * outputs, item & 7, [&](int i) {
+                lin_put<GATED, OUT>(a, t.row0 + token, t.mt * outputs, item & 7, [&](int i) {
                     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
                     for (int r = 0; r < a.split; ++r) {
                         uint32_t at;
