@@ -6,7 +6,7 @@
 #include <new>
 
 #include "rb_launch.h"
-#include "rb_linear.cuh"
+#include "rb_linear_rows.cuh"
 
 struct rabbit_cuda_linear {
     int device = -1;
@@ -43,8 +43,15 @@ static LinKernel lin_kernel_of(bool gated, int out_dtype) {
     return k;
 }
 static LinKernel lin_kernel(int mode, bool pair, bool gated, int out_dtype) {
-    if (mode == kLinF8)
-        return pair ? lin_kernel_of<kLinF8, true>(gated, out_dtype) : lin_kernel_of<kLinF8, false>(gated, out_dtype);
+    if (mode == kLinF8 && pair) {
+        LinKernel k = nullptr;
+        with_dtype(out_dtype, [&](auto t) {
+            k = gated ? k_linear_rows<true, decltype(t)> : k_linear_rows<false, decltype(t)>;
+            return 0;
+        });
+        return k;
+    }
+    if (mode == kLinF8) return lin_kernel_of<kLinF8, false>(gated, out_dtype);
     if (mode == kLinParts)
         return pair ? lin_kernel_of<kLinParts, true>(gated, out_dtype) : lin_kernel_of<kLinParts, false>(gated, out_dtype);
     return pair ? lin_kernel_of<kLinWhole, true>(gated, out_dtype) : lin_kernel_of<kLinWhole, false>(gated, out_dtype);
@@ -82,27 +89,32 @@ static bool rows_map(const rabbit_cuda_linear *lin, CUtensorMap *map, const void
 static int up_to(int64_t n, int unit) { return (int)((n + unit - 1) / unit * unit); }
 
 // The launch's shape from the sizes alone (the groups' rows are on the device).
-static bool lin_plan(LinArgs &a, bool f8, int sms, int64_t *tiles) {
+static bool lin_plan(LinArgs &a, int mode, int sms, int64_t *tiles, size_t *smem) {
     const int64_t mean = ((int64_t)a.R + a.E - 1) / a.E;
-    const bool pair = mean >= 128;
+    const bool pair = mean >= 128, as_rows = pair && mode == kLinF8;
     const int outputs = (a.gated ? 64 : 128) * (pair ? 2 : 1);
     a.mt = (a.N + outputs - 1) / outputs;
-    a.unit = pair ? 64 : 16;
+    a.unit = as_rows ? 256 : pair ? 64 : 16;
     const int64_t want = a.E == 1 ? mean : 4 * mean, rows = want < a.R ? want : a.R;
     // a multiple of 16 or, with more than one box, of the box's rows
     a.bn = rows >= 256 ? 256 : rows <= 16 ? 16 : up_to(rows, 32);
     if (pair) a.bn = up_to(a.bn, a.unit);
-    a.bufs = 512 / a.bn < kLinBufs ? 512 / a.bn : kLinBufs;
+    a.buf_shift = 1;
+    while (a.buf_shift < 3 && (2 << a.buf_shift) * a.bn <= 512) ++a.buf_shift;
+    a.bufs = 1 << a.buf_shift;
+    static_assert(kLinBufs == 1 << 3, "buffers of tensor memory");
     const int64_t groups = a.E < a.R ? a.E : a.R;
     const int64_t token_tiles = a.E == 1 ? (a.R + a.bn - 1) / a.bn : groups + a.R / a.bn;
     *tiles = token_tiles * a.mt;
     a.split = 1;
     while (!pair && a.split < 8 && *tiles * a.split * 2 <= sms && a.steps / (a.split * 2) >= 2) a.split *= 2;
-    a.box = a.bn < 32 ? a.bn : 32;
+    a.box = as_rows ? 128 : a.bn < 32 ? a.bn : 32;
     a.band = 8;
-    const uint32_t stage = lin_stage_bytes(pair, a.bn);
-    a.stages = (int)((kMaxDynSmem - lin_fixed(f8, a.gated, a.bn, a.bufs, a.E)) / stage);
+    const size_t stage = as_rows ? kRowsStage : lin_stage_bytes(pair, a.bn);
+    const size_t fixed = as_rows ? lin_rows_fixed(a.E) : lin_fixed(mode == kLinF8, a.gated, a.bn, a.bufs, a.E);
+    a.stages = (int)((kMaxDynSmem - fixed) / stage);
     if (a.stages > kLinStages) a.stages = kLinStages;
+    *smem = fixed + a.stages * stage;
     return pair;
 }
 
@@ -138,15 +150,16 @@ static int lin_run(rabbit_cuda_linear *lin, const char *what, const void *d_x, i
         return fail(RABBIT_CUDA_ERR_ARGS, "%s: x_scale_stride below its row or above 2^30, or scales not aligned", what);
     if (x_rows < 1 || (!d_rows && x_rows < n_rows))
         return fail(RABBIT_CUDA_ERR_ARGS, "%s: x_rows of %d for %d rows", what, x_rows, n_rows);
-    int64_t tiles;
-    const int sms = lin->ctx->sm_count;
-    const bool pair = lin_plan(a, f8, sms, &tiles);
-    if (tiles * a.split >= (int64_t)1 << 30)
-        return fail(RABBIT_CUDA_ERR_ARGS, "%s: 2^30 tiles or more", what);
     // The tensor cores' sums of 16-bit products lose up to 2^-25 of the result at each of K / 16
     // steps: nothing beside a 16-bit output's half step up to K 16384 (2^-15), parts beyond
     // and for fp32 outputs.
     const int mode = f8 ? kLinF8 : out == 4 || d.n_in > 16384 ? kLinParts : kLinWhole;
+    int64_t tiles;
+    size_t smem;
+    const int sms = lin->ctx->sm_count;
+    const bool pair = lin_plan(a, mode, sms, &tiles, &smem);
+    if (tiles * a.split >= (int64_t)1 << 30)
+        return fail(RABBIT_CUDA_ERR_ARGS, "%s: 2^30 tiles or more", what);
     a.offsets = d_offsets;
     a.rows = d_rows;
     a.x = static_cast<const uint8_t *>(d_x);
@@ -178,7 +191,7 @@ static int lin_run(rabbit_cuda_linear *lin, const char *what, const void *d_x, i
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(teams * team));
     cfg.blockDim = dim3(kLinThreads);
-    cfg.dynamicSmemBytes = lin_fixed(f8, a.gated, a.bn, a.bufs, a.E) + (size_t)a.stages * lin_stage_bytes(pair, a.bn);
+    cfg.dynamicSmemBytes = smem;
     cfg.stream = static_cast<cudaStream_t>(stream);
     cfg.attrs = attr;
     cfg.numAttrs = team > 1 ? 2 : 1;

@@ -25,7 +25,7 @@
 //              in 32-bit registers;
 //   kLinF8     e4m3: each step is a scale block, read out and added to 32-bit registers as
 //              acc += (sw sx) * product, while the MMAs of the next steps fill other buffers
-//              of tensor memory.
+//              of tensor memory (512 columns / the tile's, at least two).
 // PAIR: two CTAs share a tile of 256 weight rows: each has its rows of A and half the
 // tokens' rows of B, and CTA 0 issues one MMA of M = 256 for both (cta_group::2), so a step
 // brings 32 KB instead of 48 KB to each SM for the same work.
@@ -78,7 +78,8 @@ struct LinArgs {
     int bn;               // tokens of a tile, at most: 16 or a multiple of 32
     int unit;             // tokens of a tile come in multiples of it
     int box;              // token rows of a box
-    int stages, bufs;
+    int stages;
+    int bufs, buf_shift;  // buffers: 2^buf_shift
     int split;            // CTAs of a cluster that splits K
     int band;             // token tiles that go together, for the L2
     uint32_t format;      // operand format of the instruction descriptor
@@ -91,6 +92,7 @@ struct LinArgs {
 struct LinShared {
     uint64_t full[kLinStages], empty[kLinStages];
     uint64_t rows[kLinStages];  // with a list: this CTA's token rows have arrived
+    uint64_t told[kLinStages];  // and the other CTA's, in the leader
     uint64_t dfull[kLinBufs], dempty[kLinBufs], mfree[kLinBufs];
     uint64_t mdone;
     uint32_t tmem;
@@ -154,25 +156,16 @@ struct LinRing {
     }
 };
 
-// Bounded wait of one thread; what the other CTA of a pair wrote before its arrival
-// is seen after it.
-__device__ __forceinline__ bool lin_try(uint64_t *bar, uint32_t parity) {
-    uint32_t ok;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(ok)
-        : "r"(smem_u32(bar)), "r"(parity)
-        : "memory");
-    return ok != 0;
-}
+// Bounded wait of one thread. (Arrivals and waits between the CTAs of a pair have the
+// default scope: with the cluster's on every barrier a step took 0.2 us more. What crosses
+// from one to the other is either read by the tensor cores of its own CTA after a proxy
+// fence there, or no memory at all.)
 __device__ __forceinline__ bool lin_wait1(uint64_t *bar, uint32_t parity, const LinArgs &a,
                                           volatile int *abort) {
-    if (lin_try(bar, parity)) return true;
+    if (mbar_try_wait(bar, parity)) return true;
     const uint64_t t0 = globaltimer_ns();
     for (uint32_t it = 1;; ++it) {
-        if (lin_try(bar, parity)) return true;
+        if (mbar_try_wait(bar, parity)) return true;
         if ((it & 15u) == 0) {
             if (*abort) return false;
             if (globaltimer_ns() - t0 > a.wait_ns) {
@@ -205,7 +198,7 @@ __device__ __forceinline__ uint32_t cluster_addr(const void *p, uint32_t rank) {
     return at;
 }
 __device__ __forceinline__ void cluster_bar_arrive(uint32_t bar) {
-    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 __device__ __forceinline__ void cluster_sync_all() {
     asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
@@ -214,6 +207,21 @@ __device__ __forceinline__ uint32_t cluster_rank() {
     uint32_t r;
     asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
     return r;
+}
+// Two fp32 numbers in a register pair; acc += v * f and acc += v on both.
+__device__ __forceinline__ uint64_t pack2(float a, float b) {
+    uint64_t p;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(p) : "f"(a), "f"(b));
+    return p;
+}
+__device__ __forceinline__ void unpack2(uint64_t p, float &a, float &b) {
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(p));
+}
+__device__ __forceinline__ void fma2(uint64_t &acc, uint64_t v, uint64_t f) {
+    asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(acc) : "l"(v), "l"(f));
+}
+__device__ __forceinline__ void add2(uint64_t &acc, uint64_t v) {
+    asm("add.rn.f32x2 %0, %0, %1;" : "+l"(acc) : "l"(v));
 }
 __device__ __forceinline__ float4 cluster_ld4(uint32_t at) {
     float4 v;
@@ -280,6 +288,73 @@ __device__ __forceinline__ bool lin_written(const LinArgs &a, const LinTile &t, 
     return r >= 0 && r < a.x_rows;
 }
 
+// off and pre from the offsets, by the whole block (a barrier has to follow). With offsets out
+// of order or range the call has no tile at all: tiles of ranges that overlap could be more than
+// the launch was made for.
+__device__ __forceinline__ void lin_experts(const LinArgs &a, int *off, int *pre, int per) {
+    bool bad = false;
+    for (int e = threadIdx.x; e <= a.E; e += kLinThreads) {
+        const int o = a.offsets ? a.offsets[e] : e ? a.R : 0;
+        off[e] = o;
+        bad |= o < 0 || o > a.R || (a.offsets && e && a.offsets[e - 1] > o);
+    }
+    bad = __syncthreads_or(bad);
+    if (bad && threadIdx.x == 0) atomicOr(a.err, RB_LIN_ERR_OFFSETS);
+    if (threadIdx.x >= 32) return;
+    const int lane = threadIdx.x;
+    int before = 0;
+    for (int e0 = 0; e0 < a.E; e0 += 32) {
+        const int e = e0 + lane;
+        int n = e < a.E && !bad ? (off[e + 1] - off[e] + per - 1) / per : 0;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const int m = __shfl_up_sync(0xffffffffu, n, d);
+            if (lane >= d) n += m;
+        }
+        if (e < a.E) pre[e + 1] = before + n;
+        before += __shfl_sync(0xffffffffu, n, 31);
+    }
+    if (lane == 0) pre[0] = 0;
+}
+
+// The gathering warps' part of a tile: tokens c0 .. c0 + here - 1 of it into rows 0.. of the
+// token rows `at` bytes into each stage, ROWS of them a thread (part, part + 16, ..).
+template <int ROWS>
+__device__ __forceinline__ bool lin_gather(const LinArgs &a, LinShared &s, uint32_t at, uint32_t stage_bytes,
+                                           const LinTile &t, int c0, int here, int k0, int k1,
+                                           LinRing &st, volatile int *abort) {
+    const int tid = threadIdx.x - 384, piece = tid & 7, part = tid >> 3;
+    const uint32_t to = at + part * 128 + ((piece ^ (part & 7)) << 4);
+    int r[ROWS];  // of x; -1: none, zeros
+#pragma unroll
+    for (int j = 0; j < ROWS; ++j) {
+        const int c = c0 + part + 16 * j;
+        r[j] = -1;
+        if (part + 16 * j < here && c < t.n) {
+            r[j] = __ldg(a.rows + t.row0 + c);
+            if (r[j] < 0 || r[j] >= a.x_rows) {
+                atomicOr(a.err, RB_LIN_ERR_ROWS);
+                r[j] = -1;
+            }
+        }
+    }
+    for (int k = k0; k < k1; ++k) {
+        if (!lin_wait(&s.empty[st.at], st.phase ^ 1, a, abort)) return false;
+        const uint32_t dst = to + st.at * stage_bytes;
+        const int b = k * 128 + piece * 16, n = min(max(a.k_bytes - b, 0), 16);
+        const uint8_t *x = a.x + (n > 0 ? b : 0);
+#pragma unroll
+        for (int j = 0; j < ROWS; ++j)
+            if (16 * j < here)
+                cp_async16(dst + j * 2048, x + (int64_t)max(r[j], 0) * a.x_bytes, r[j] >= 0 ? n : 0);
+        // (the fence that lets the tensor cores see them is the waiting thread's: here it
+        // would wait for every copy under way)
+        asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(&s.rows[st.at])) : "memory");
+        st.next(a.stages);
+    }
+    return true;
+}
+
 template <int MODE, bool PAIR, bool GATED, typename OUT>
 __global__ void __launch_bounds__(kLinThreads, 1)
     k_linear(const __grid_constant__ LinArgs a, const __grid_constant__ CUtensorMap mw,
@@ -301,12 +376,13 @@ __global__ void __launch_bounds__(kLinThreads, 1)
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < a.stages; ++i) {
-            mbar_init(&s.full[i], PAIR && a.rows ? 2 : 1);  // the TMA, and word of CTA 1's rows
+            mbar_init(&s.full[i], 1);
             mbar_init(&s.empty[i], 1);
             mbar_init(&s.rows[i], 128);
+            mbar_init(&s.told[i], 1);
         }
         for (int i = 0; i < a.bufs; ++i) {
-            mbar_init(&s.dfull[i], F8 ? 3 : 1);  // the MMAs, and two warps of scales
+            mbar_init(&s.dfull[i], F8 ? 3 : 1);  // the MMAs, and the scales' two warps
             mbar_init(&s.dempty[i], 8);          // this CTA's readout
             mbar_init(&s.mfree[i], 16);          // the pair's
         }
@@ -320,31 +396,7 @@ __global__ void __launch_bounds__(kLinThreads, 1)
     }
     launch_dependents();
     wait_prerequisite();
-    // The experts' rows; with offsets out of order or range the call has none at all (tiles
-    // of ranges that overlap could be more than the launch was made for).
-    bool bad = false;
-    for (int e = threadIdx.x; e <= a.E; e += kLinThreads) {
-        const int o = a.offsets ? a.offsets[e] : e ? a.R : 0;
-        off[e] = o;
-        bad |= o < 0 || o > a.R || (a.offsets && e && a.offsets[e - 1] > o);
-    }
-    bad = __syncthreads_or(bad);
-    if (bad && threadIdx.x == 0) atomicOr(a.err, RB_LIN_ERR_OFFSETS);
-    if (warp == 0) {
-        int before = 0;
-        for (int e0 = 0; e0 < a.E; e0 += 32) {
-            const int e = e0 + lane;
-            int n = e < a.E && !bad ? (off[e + 1] - off[e] + a.bn - 1) / a.bn : 0;
-#pragma unroll
-            for (int d = 1; d < 32; d <<= 1) {
-                const int m = __shfl_up_sync(0xffffffffu, n, d);
-                if (lane >= d) n += m;
-            }
-            if (e < a.E) pre[e + 1] = before + n;
-            before += __shfl_sync(0xffffffffu, n, 31);
-        }
-        if (lane == 0) pre[0] = 0;
-    }
+    lin_experts(a, off, pre, a.bn);
     tc_fence_before();
     __syncthreads();
     if (PAIR) cluster_sync_all();  // both CTAs' barriers are ready
@@ -374,7 +426,6 @@ __global__ void __launch_bounds__(kLinThreads, 1)
                 const int here = PAIR ? t.cols / 2 : t.cols;  // token rows of this CTA
                 const int boxes = a.rows ? 0 : (here + a.box - 1) / a.box;
                 const uint32_t bytes = (PAIR ? 2 : 1) * (kLinTile + boxes * a.box * 128);
-                const int r0 = t.row0 + (PAIR ? rank * here : 0);
                 // weights that no other tile of tokens reads leave the L2 first
                 const uint64_t pol = pre[t.e + 1] - pre[t.e] > 1 ? keep : once;
                 for (int k = k0; k < k1; ++k, ++issued) {
@@ -387,12 +438,13 @@ __global__ void __launch_bounds__(kLinThreads, 1)
                         tma_load_4d_pair(base, &mw, c0, n0, 0, t.e, bar, pol);
                         if (GATED) tma_load_4d_pair(base + kLinTile / 2, &mw, c0, n0, 1, t.e, bar, pol);
                         for (int b = 0; b < boxes; ++b)
-                            tma_load_2d_pair(xb + b * a.box * 128, &mx, c0, r0 + b * a.box, bar);
+                            tma_load_2d_pair(xb + b * a.box * 128, &mx, c0,
+                                             t.row0 + rank * here + b * a.box, bar);
                     } else {
                         tma_load_4d(base, &mw, c0, n0, 0, t.e, &s.full[st.at], pol);
                         if (GATED) tma_load_4d(base + kLinTile / 2, &mw, c0, n0, 1, t.e, &s.full[st.at], pol);
                         for (int b = 0; b < boxes; ++b)
-                            tma_load_2d(xb + b * a.box * 128, &mx, c0, r0 + b * a.box, &s.full[st.at]);
+                            tma_load_2d(xb + b * a.box * 128, &mx, c0, t.row0 + b * a.box, &s.full[st.at]);
                     }
                     st.next(a.stages);
                 }
@@ -413,15 +465,16 @@ __global__ void __launch_bounds__(kLinThreads, 1)
                 const uint32_t idesc = float_idesc(a.format, PAIR ? 256 : 128, t.cols);
                 int part = 0;
                 for (int k = k0; k < k1; ++k) {
-                    if (part == 0)
-                        if (!(ok = lin_wait1(PAIR ? &s.mfree[db.at] : &s.dempty[db.at], db.phase ^ 1, a, abort))) break;
                     if (!(ok = lin_wait1(&s.full[st.at], st.phase, a, abort))) break;
                     if (a.rows) {
-                        if (!(ok = lin_wait1(&s.rows[st.at], st.phase, a, abort))) break;
+                        if (PAIR) ok = lin_wait1(&s.told[st.at], st.phase, a, abort);
+                        if (!ok || !(ok = lin_wait1(&s.rows[st.at], st.phase, a, abort))) break;
                         fence_async();
                     }
-                    tc_fence_after();
                     const uint64_t step = (uint64_t)(st.at * stage_bytes) >> 4;
+                    if (part == 0)
+                        if (!(ok = lin_wait1(PAIR ? &s.mfree[db.at] : &s.dempty[db.at], db.phase ^ 1, a, abort))) break;
+                    tc_fence_after();
                     const uint32_t d = tmem + db.at * a.bn;
 #pragma unroll
                     for (int j = 0; j < 4; ++j)
@@ -450,7 +503,7 @@ __global__ void __launch_bounds__(kLinThreads, 1)
                 for (int k = k0; k < k1; ++k) {
                     if (!(ok = lin_wait1(&s.rows[st.at], st.phase, a, abort))) break;
                     fence_async();
-                    cluster_bar_arrive(cluster_addr(&s.full[st.at], 0));
+                    cluster_bar_arrive(cluster_addr(&s.told[st.at], 0));
                     st.next(a.stages);
                 }
         }
@@ -458,13 +511,17 @@ __global__ void __launch_bounds__(kLinThreads, 1)
     } else if (F8) {  // ---------------------------------------------- scales
         const int nb = (a.N + 127) / 128;  // rows of scale blocks of a matrix
         const int64_t up = (int64_t)nb * a.steps;
-        LinRing db;
         bool ok = true;
-        const int c1 = (warp - 2) * 128 + lane;  // tokens c1, c1 + 32, ..
+        // Of a tile of more than 128 tokens, one warp has the first 128 and the other the rest of
+        // each buffer; else each has every other one, whole.
+        uint32_t count = 0;  // buffers before the tile
         // NT tokens a lane, the scales of the next AHEAD steps on their way (a step of a few
         // tokens takes 0.4 us, as long as half a read from HBM)
         auto tile = [&](auto nt, auto ahead) {
             constexpr int NT = decltype(nt)::value, AHEAD = decltype(ahead)::value;
+            const bool both = t.cols > 128;
+            const int mine = both ? 0 : (warp - 2) ^ (count & 1);  // the tile's first buffer that is
+            const int c1 = lane + (both ? (warp - 2) * 128 : 0), by = both ? 1 : 2;
             int r[NT];
 #pragma unroll
             for (int j = 0; j < NT; ++j) {
@@ -487,14 +544,19 @@ __global__ void __launch_bounds__(kLinThreads, 1)
                 w[h][0] = __ldg(ws + k);
                 w[h][1] = GATED ? __ldg(ws + up + k) : 0.f;
             };
+            const int ks = k0 + mine;
+            uint32_t use = count + mine;  // of the buffers, in order
+            count += k1 - k0;
 #pragma unroll
-            for (int h = 0; h < AHEAD; ++h) fetch(k0 + h, h);
-            for (int k = k0; k < k1; k += AHEAD) {
+            for (int h = 0; h < AHEAD; ++h) fetch(ks + h * by, h);
+            int k = ks;
+            while (ok && k < k1) {
 #pragma unroll
                 for (int h = 0; h < AHEAD; ++h) {
-                    if (k + h >= k1 || !ok) break;
-                    if (!(ok = lin_wait(&s.dempty[db.at], db.phase ^ 1, a, abort))) break;
-                    float *sc = scales + db.at * sc_buf;
+                    if (k >= k1) break;
+                    const int at = use & (a.bufs - 1);
+                    if (!(ok = lin_wait(&s.dempty[at], (use >> a.buf_shift & 1) ^ 1, a, abort))) break;
+                    float *sc = scales + at * sc_buf;
 #pragma unroll
                     for (int j = 0; j < NT; ++j)
                         if (c1 + 32 * j < sc_row) {
@@ -502,9 +564,10 @@ __global__ void __launch_bounds__(kLinThreads, 1)
                             if (GATED) sc[sc_row + c1 + 32 * j] = v[h][j] * w[h][1];
                         }
                     __syncwarp();
-                    if (lane == 0) mbar_arrive(&s.dfull[db.at]);
-                    db.next(a.bufs);
-                    fetch(k + h + AHEAD, h);
+                    if (lane == 0) mbar_arrive_cnt(&s.dfull[at], both ? 1 : 2);
+                    use += by;
+                    fetch(k + AHEAD * by, h);
+                    k += by;
                 }
             }
         };
@@ -516,40 +579,12 @@ __global__ void __launch_bounds__(kLinThreads, 1)
     } else if (warp >= 12) {  // ------------------------------------- gather
         if constexpr (MODE != kLinWhole) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
         if (a.rows) {
-            constexpr int ROWS = PAIR ? 8 : 16;  // of a thread: part, part + 16, ..
-            const int tid = threadIdx.x - 384, piece = tid & 7, part = tid >> 3;
-            const uint32_t to = smem_u32(ring) + kLinTile + part * 128 + ((piece ^ (part & 7)) << 4);
             LinRing st;
             bool ok = true;
             for (int i = first; ok && lin_tile(a, off, pre, i, t); i += stride) {
-                const int here = PAIR ? t.cols / 2 : t.cols, c0 = PAIR ? rank * here : 0;
-                int r[ROWS];  // of x; -1: none, zeros
-#pragma unroll
-                for (int j = 0; j < ROWS; ++j) {
-                    const int c = part + 16 * j;
-                    r[j] = -1;
-                    if (c < here && c0 + c < t.n) {
-                        r[j] = __ldg(a.rows + t.row0 + c0 + c);
-                        if (r[j] < 0 || r[j] >= a.x_rows) {
-                            atomicOr(a.err, RB_LIN_ERR_ROWS);
-                            r[j] = -1;
-                        }
-                    }
-                }
-                for (int k = k0; k < k1; ++k) {
-                    if (!(ok = lin_wait(&s.empty[st.at], st.phase ^ 1, a, abort))) break;
-                    const uint32_t dst = to + st.at * stage_bytes;
-                    const int at = k * 128 + piece * 16, n = min(max(a.k_bytes - at, 0), 16);
-                    const uint8_t *x = a.x + (n > 0 ? at : 0);
-#pragma unroll
-                    for (int j = 0; j < ROWS; ++j)
-                        if (16 * j < here)
-                            cp_async16(dst + j * 2048, x + (int64_t)max(r[j], 0) * a.x_bytes, r[j] >= 0 ? n : 0);
-                    // (the fence that lets the tensor cores see them is the waiting thread's: here it
-                    // would wait for every copy under way)
-                    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(&s.rows[st.at])) : "memory");
-                    st.next(a.stages);
-                }
+                const int here = PAIR ? t.cols / 2 : t.cols;
+                ok = lin_gather<PAIR ? 8 : 16>(a, s, smem_u32(ring) + kLinTile, stage_bytes, t,
+                                               PAIR ? rank * here : 0, here, k0, k1, st, abort);
             }
             asm volatile("cp.async.wait_all;" ::: "memory");
         }
@@ -592,41 +627,43 @@ __global__ void __launch_bounds__(kLinThreads, 1)
         };
         for (int i = first; ok && lin_tile(a, off, pre, i, t); i += stride) {
             if constexpr (MODE != kLinWhole) {
-                float acc[8][16];
+                uint64_t acc[8][8];  // block pair, two tokens
 #pragma unroll
                 for (int c = 0; c < 8; ++c)
 #pragma unroll
-                    for (int j = 0; j < 16; ++j) acc[c][j] = 0.f;
+                    for (int j = 0; j < 8; ++j) acc[c][j] = 0;
+                const int n = t.cols - 16 * h;  // columns from this warp's first on
                 for (int k = k0; k < k1; k += PART) {
                     if (!(ok = lin_wait(&s.dfull[db.at], db.phase, a, abort))) break;
                     tc_fence_after();
                     const uint32_t d = tmem + lanes + db.at * a.bn + 16 * h;
                     const float *sc = scales + db.at * sc_buf + (GATED && q >= 2 ? sc_row : 0) + 16 * h;
-                    float v[2][16];
-                    if (16 * h < t.cols) lin_ld16(d, v[0]);
-#pragma unroll
-                    for (int c = 0; c < 8; ++c) {
-                        if (32 * c + 16 * h >= t.cols) break;
-                        float4 f[4];
-                        if (F8) {
-#pragma unroll
-                            for (int j = 0; j < 4; ++j) f[j] = reinterpret_cast<const float4 *>(sc + 32 * c)[j];
-                        }
-                        lin_ld_done(v[c & 1]);
-                        if (c < 7 && 32 * (c + 1) + 16 * h < t.cols) lin_ld16(d + 32 * (c + 1), v[(c + 1) & 1]);
-                        const float(&u)[16] = v[c & 1];
+                    auto add = [&](int c, const float(&v)[16]) {
 #pragma unroll
                         for (int j = 0; j < 4; ++j) {
+                            const uint64_t v0 = pack2(v[4 * j], v[4 * j + 1]), v1 = pack2(v[4 * j + 2], v[4 * j + 3]);
                             if (F8) {
-                                acc[c][4 * j] = fmaf(u[4 * j], f[j].x, acc[c][4 * j]);
-                                acc[c][4 * j + 1] = fmaf(u[4 * j + 1], f[j].y, acc[c][4 * j + 1]);
-                                acc[c][4 * j + 2] = fmaf(u[4 * j + 2], f[j].z, acc[c][4 * j + 2]);
-                                acc[c][4 * j + 3] = fmaf(u[4 * j + 3], f[j].w, acc[c][4 * j + 3]);
+                                const ulonglong2 f = reinterpret_cast<const ulonglong2 *>(sc + 32 * c)[j];
+                                fma2(acc[c][2 * j], v0, f.x);
+                                fma2(acc[c][2 * j + 1], v1, f.y);
                             } else {
-#pragma unroll
-                                for (int l = 0; l < 4; ++l) acc[c][4 * j + l] += u[4 * j + l];
+                                add2(acc[c][2 * j], v0);
+                                add2(acc[c][2 * j + 1], v1);
                             }
                         }
+                    };
+                    // 32 columns in flight at a time (16: a step of 256 tokens took half as long again)
+#pragma unroll
+                    for (int c = 0; c < 8; c += 2) {
+                        if (32 * c >= n) break;
+                        float v[2][16];
+                        lin_ld16(d + 32 * c, v[0]);
+                        const bool two = 32 * (c + 1) < n;
+                        if (two) lin_ld16(d + 32 * (c + 1), v[1]);
+                        lin_ld_done(v[0]);
+                        if (two) lin_ld_done(v[1]);
+                        add(c, v[0]);
+                        if (two) add(c + 1, v[1]);
                     }
                     release();
                 }
@@ -637,7 +674,10 @@ __global__ void __launch_bounds__(kLinThreads, 1)
 #pragma unroll
                 for (int c = 0; c < 8; ++c) {
                     if (32 * c >= t.cols) break;
-                    put(c, acc[c]);
+                    float v[16];
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) unpack2(acc[c][j], v[2 * j], v[2 * j + 1]);
+                    put(c, v);
                 }
             } else {
                 ok = named_all(1, kLinReaders, lin_wait(&s.dfull[db.at], db.phase, a, abort));

@@ -223,7 +223,7 @@ def test_linear(torch, rc, name, R, N, K, gated, out, wg, xg, yg):
 
 SIZES = {  # rows of each expert
     "even": [3, 3, 3, 3], "one": [40], "empty": [0, 0, 0], "holes": [0, 5, 0, 0, 130, 1, 0],
-    "ragged": [1, 17, 0, 300, 33, 16, 2, 129], "last": [0, 0, 0, 7], "many": [1, 0, 2] * 341 + [5],
+    "large": [300, 0, 260, 129, 1, 384], "ragged": [1, 17, 0, 300, 33, 16, 2, 129], "last": [0, 0, 0, 7], "many": [1, 0, 2] * 341 + [5],
 }
 
 
