@@ -2,9 +2,9 @@
 // columns.
 //
 // Bound by memory: x is read and its codes are written once. The codes are those of the
-// exact quotient x / s without a division for each value: with r = fp32(1 / s),
-//   |x| r (1 - 2^-22) <= |x| / s <= |x| r (1 + 2^-22)
-// holds for the computed products (r and two products round by 2^-24 each), rounding to
+// exact quotient x / s without a division for each value: with r within 2^-22 of 1 / s,
+//   |x| r (1 - 2^-21) <= |x| / s <= |x| r (1 + 2^-21)
+// holds for the computed products (they round by 2^-24 each), rounding to
 // e4m3 is monotone, so where both ends give one code it is the quotient's. Where they give two
 // neighbours, the sign of x - m s, m the middle between them, decides; one fma has it exactly.
 // 16384 rows of 4096 bf16: see the launch below.
@@ -26,6 +26,8 @@ struct F8Args {
     int64_t qs;
     float *scale;
     int n_rows, n_cols, nb;  // nb: blocks of 128 columns
+    uint32_t magic;          // i / nb = umulhi(i, magic) >> shift for i below 2^31
+    int shift;
 };
 
 constexpr int kF8Threads = 256;
@@ -41,19 +43,21 @@ __device__ __forceinline__ float e4m3_value(uint32_t code) {
 
 // A block's scale from the bits of its largest |x|, and what its codes are made with.
 struct F8Scale {
-    float s, lo, hi, grow;  // grow: x and s are multiplied by it for tiny scales
-    bool zero, bad;
+    float s, lo, hi;
+    bool zero, bad, tiny;
 };
+constexpr float kF8Tiny = 0x1p-60f, kF8Grow = 0x1p64f;
 __device__ __forceinline__ F8Scale f8_scale(uint32_t top) {
     F8Scale f;
     f.bad = top >= kInfBits;
     f.s = __fdiv_rn(__uint_as_float(top), 448.f);
     f.zero = f.s == 0.f;
-    // below 2^-60: by 2^64 on, where 1 / s and the remainders are far from fp32's smallest
-    f.grow = f.s < 8.67361738e-19f ? 18446744073709551616.f : 1.f;
-    const float r = __frcp_rn(f.s * f.grow);
-    f.lo = r * (1.f - 0x1p-22f);
-    f.hi = r * (1.f + 0x1p-22f);
+    // below 2^-60 x and s are multiplied by 2^64, where 1 / s and the remainders are far from
+    // fp32's smallest numbers
+    f.tiny = f.s < kF8Tiny;
+    const float r = __fdividef(1.f, f.tiny ? f.s * kF8Grow : f.s);
+    f.lo = r * (1.f - 0x1p-21f);
+    f.hi = r * (1.f + 0x1p-21f);
     if (f.bad) f.s = __uint_as_float(0x7FC00000u);
     return f;
 }
@@ -65,46 +69,84 @@ __device__ __noinline__ uint32_t f8_between(float x, float s, uint32_t a, uint32
     return d < 0.f ? a : d > 0.f ? b : (a & 1) ? b : a;
 }
 
-// Codes of four values, the first in the low byte.
-__device__ __forceinline__ uint32_t f8_codes(const float (&x)[4], const F8Scale &f) {
-    if (f.bad) return 0x7F7F7F7Fu;
-    if (f.zero) return 0u;
-    float v[4];
+// Codes of eight values, the first in the low byte.
+__device__ __forceinline__ uint2 f8_codes(float (&x)[8], const F8Scale &f) {
+    if (f.bad | f.zero) return f.bad ? make_uint2(0x7F7F7F7Fu, 0x7F7F7F7Fu) : make_uint2(0u, 0u);
+    float s = f.s;
+    if (f.tiny) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = x[i] * f.grow;
-    const uint32_t a = e4m3x2(v[0] * f.lo, v[1] * f.lo) | e4m3x2(v[2] * f.lo, v[3] * f.lo) << 16;
-    const uint32_t b = e4m3x2(v[0] * f.hi, v[1] * f.hi) | e4m3x2(v[2] * f.hi, v[3] * f.hi) << 16;
-    if (a == b) return a;
-    uint32_t c = 0;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const uint32_t ai = a >> (8 * i) & 255, bi = b >> (8 * i) & 255;
-        c |= (ai == bi ? ai : f8_between(v[i], f.s * f.grow, ai, bi)) << (8 * i);
+        for (int i = 0; i < 8; ++i) x[i] *= kF8Grow;
+        s *= kF8Grow;
     }
-    return c;
+    uint32_t a[2], b[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const float *v = x + 4 * i;
+        a[i] = e4m3x2(v[0] * f.lo, v[1] * f.lo) | e4m3x2(v[2] * f.lo, v[3] * f.lo) << 16;
+        b[i] = e4m3x2(v[0] * f.hi, v[1] * f.hi) | e4m3x2(v[2] * f.hi, v[3] * f.hi) << 16;
+    }
+    if (a[0] != b[0] || a[1] != b[1]) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const uint32_t ai = a[i / 4] >> (8 * (i & 3)) & 255, bi = b[i / 4] >> (8 * (i & 3)) & 255;
+            if (ai != bi) a[i / 4] ^= (ai ^ f8_between(x[i], s, ai, bi)) << (8 * (i & 3));
+        }
+    }
+    return make_uint2(a[0], a[1]);
 }
 
-// Eight values of a row from column c on; past the row zeros.
+// Eight values of a row as they lie in memory, from column c on; past the row zeros.
+template <typename T>
+struct F8Raw {
+    uint4 w[sizeof(T) / 2];
+};
 template <typename T, bool VEC>
-__device__ __forceinline__ void f8_load(float (&d)[8], const T *row, int c, int n_cols) {
-    if (c + 8 <= n_cols) {
-        load8<VEC>(d, row + c);
-    } else {
+__device__ __forceinline__ F8Raw<T> f8_load(const T *row, int c, int n_cols) {
+    F8Raw<T> d;
+    if (VEC && c + 8 <= n_cols) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) d[i] = c + i < n_cols ? to_f32(row[c + i]) : 0.f;
+        for (int i = 0; i < (int)sizeof(T) / 2; ++i) d.w[i] = reinterpret_cast<const uint4 *>(row + c)[i];
+    } else {
+        T *e = reinterpret_cast<T *>(&d);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) e[i] = c + i < n_cols ? row[c + i] : from_f32<T>(0.f);
+    }
+    return d;
+}
+template <typename T>
+__device__ __forceinline__ void f8_values(const F8Raw<T> &d, float (&v)[8]) {
+    const T *e = reinterpret_cast<const T *>(&d);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = to_f32(e[i]);
+}
+// The largest |value|'s bits, in T's own format (they order as the values do, infinity and
+// NaN above); two 16-bit numbers at a time.
+template <typename T>
+__device__ __forceinline__ uint32_t f8_top(const F8Raw<T> &d) {
+    const uint32_t *w = reinterpret_cast<const uint32_t *>(&d);
+    if constexpr (sizeof(T) == 2) {
+        uint32_t m = w[0] & 0x7FFF7FFFu;
+#pragma unroll
+        for (int i = 1; i < 4; ++i) m = __vmaxu2(m, w[i] & 0x7FFF7FFFu);
+        return max(m & 0xFFFFu, m >> 16);
+    } else {
+        uint32_t m = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) m = max(m, w[i] & 0x7FFFFFFFu);
+        return m;
     }
 }
-__device__ __forceinline__ uint32_t f8_top(const float (&d)[8]) {
-    uint32_t m = 0;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(d[i]) & 0x7FFFFFFFu);
-    return m;
+template <typename T>
+__device__ __forceinline__ uint32_t f8_top_f32(uint32_t top) {
+    if constexpr (sizeof(T) == 2) {
+        const unsigned short h = (unsigned short)top;
+        return __float_as_uint(to_f32(*reinterpret_cast<const T *>(&h)));
+    } else {
+        return top;
+    }
 }
 template <bool VEC>
-__device__ __forceinline__ void f8_store(uint8_t *row, int c, int n_cols, const float (&d)[8],
-                                         const F8Scale &f) {
-    const float lo[4] = {d[0], d[1], d[2], d[3]}, hi[4] = {d[4], d[5], d[6], d[7]};
-    const uint2 w = make_uint2(f8_codes(lo, f), f8_codes(hi, f));
+__device__ __forceinline__ void f8_store(uint8_t *row, int c, int n_cols, uint2 w) {
     if (VEC && c + 8 <= n_cols) {
         *reinterpret_cast<uint2 *>(row + c) = w;
     } else {
@@ -126,36 +168,35 @@ __global__ void __launch_bounds__(kF8Threads) k_f8_rows(const __grid_constant__ 
     const int64_t teams = (int64_t)gridDim.x * (kF8Threads / 16);
     for (int64_t i0 = ((int64_t)blockIdx.x * kF8Threads + threadIdx.x) / 32 * 2; i0 < items;
          i0 += teams * BATCH) {
-        float d[BATCH][8];
+        F8Raw<T> d[BATCH];
         int64_t at[BATCH];
-        int col[BATCH];
+        int block[BATCH];
 #pragma unroll
         for (int b = 0; b < BATCH; ++b) {  // a warp's two blocks side by side, then `teams` on
             const int64_t i = i0 + (threadIdx.x >> 4 & 1) + b * teams;
             at[b] = -1;
             if (i < items) {
-                const int64_t r = items >> 31 ? i / a.nb : (int)i / a.nb;
-                col[b] = (int)(i - r * a.nb) * 128 + lane * 8;
+                const int64_t r = items >> 31 ? i / a.nb : a.nb == 1 ? i : __umulhi((uint32_t)i, a.magic) >> a.shift;
+                block[b] = (int)(i - r * a.nb);
                 const int64_t src = a.rows ? __ldg(a.rows + r) : r;
                 if (!a.rows || (src >= 0 && src < a.x_rows)) {
                     at[b] = r;
-                    f8_load<T, VEC>(d[b], static_cast<const T *>(a.x) + src * a.xs, col[b], a.n_cols);
+                    d[b] = f8_load<T, VEC>(static_cast<const T *>(a.x) + src * a.xs, block[b] * 128 + lane * 8,
+                                           a.n_cols);
                 }
-            }
-            if (at[b] < 0) {
-#pragma unroll
-                for (int j = 0; j < 8; ++j) d[b][j] = 0.f;
             }
         }
 #pragma unroll
         for (int b = 0; b < BATCH; ++b) {
-            uint32_t top = f8_top(d[b]);
+            uint32_t top = at[b] >= 0 ? f8_top(d[b]) : 0u;
 #pragma unroll
             for (int m = 8; m; m >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, m));
             if (at[b] < 0) continue;
-            const F8Scale f = f8_scale(top);
-            f8_store<VEC>(a.q + at[b] * a.qs, col[b], a.n_cols, d[b], f);
-            if (lane == 0) a.scale[at[b] * a.nb + col[b] / 128] = f.s;
+            const F8Scale f = f8_scale(f8_top_f32<T>(top));
+            float v[8];
+            f8_values(d[b], v);
+            f8_store<VEC>(a.q + at[b] * a.qs, block[b] * 128 + lane * 8, a.n_cols, f8_codes(v, f));
+            if (lane == 0) a.scale[at[b] * a.nb + block[b]] = f.s;
         }
     }
 }
@@ -167,13 +208,13 @@ __global__ void __launch_bounds__(kF8Threads) k_f8_blocks(const __grid_constant_
     launch_dependents();
     wait_prerequisite();
     const int r0 = blockIdx.x * 128, c = blockIdx.y * 128 + (threadIdx.x & 15) * 8;
-    float d[8][8];
+    F8Raw<T> d[8];
     uint32_t top = 0;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
         const int r = r0 + (threadIdx.x >> 4) + 16 * i;
         if (r < a.n_rows) {
-            f8_load<T, VEC>(d[i], static_cast<const T *>(a.x) + r * a.xs, c, a.n_cols);
+            d[i] = f8_load<T, VEC>(static_cast<const T *>(a.x) + r * a.xs, c, a.n_cols);
             top = max(top, f8_top(d[i]));
         }
     }
@@ -182,11 +223,14 @@ __global__ void __launch_bounds__(kF8Threads) k_f8_blocks(const __grid_constant_
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < kF8Threads / 32; ++i) top = max(top, warp_top[i]);
-    const F8Scale f = f8_scale(top);
+    const F8Scale f = f8_scale(f8_top_f32<T>(top));
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
         const int r = r0 + (threadIdx.x >> 4) + 16 * i;
-        if (r < a.n_rows) f8_store<VEC>(a.q + r * a.qs, c, a.n_cols, d[i], f);
+        if (r >= a.n_rows) break;
+        float v[8];
+        f8_values(d[i], v);
+        f8_store<VEC>(a.q + r * a.qs, c, a.n_cols, f8_codes(v, f));
     }
     if (threadIdx.x == 0) a.scale[(int64_t)blockIdx.x * a.nb + blockIdx.y] = f.s;
 }
@@ -224,6 +268,11 @@ extern "C" int rabbit_cuda_f8_quantise_dev(int dtype, const void *d_x, int64_t x
         (reinterpret_cast<uintptr_t>(d_scale) & 3) || (reinterpret_cast<uintptr_t>(d_rows) & 3))
         return fail(RABBIT_CUDA_ERR_ARGS,
                     "f8_quantise: a stride below n_cols, or a pointer not aligned to its element");
+    // i / nb as a product: with 2^(31 + l) / nb rounded up, 2^l >= nb, exact below 2^31
+    int l = 0;
+    while ((1 << l) < a.nb) ++l;
+    a.magic = a.nb == 1 ? 0 : (uint32_t)((((uint64_t)1 << (31 + l)) + a.nb - 1) / a.nb);
+    a.shift = l - 1;
     const bool vec = (x & 15) == 0 && a.xs * size % 16 == 0 && (q & 7) == 0 && a.qs % 8 == 0;
     int sms = 0;
     DeviceScope scope(current_device());

@@ -162,6 +162,7 @@ static int lin_run(rabbit_cuda_linear *lin, const char *what, const void *d_x, i
         return fail(RABBIT_CUDA_ERR_ARGS, "%s: 2^30 tiles or more", what);
     a.offsets = d_offsets;
     a.rows = d_rows;
+    a.gather = d_rows && a.bn > 32;
     a.x = static_cast<const uint8_t *>(d_x);
     a.x_bytes = (uint32_t)(xs * size);
     a.k_bytes = d.n_in * size;
@@ -176,7 +177,7 @@ static int lin_run(rabbit_cuda_linear *lin, const char *what, const void *d_x, i
     CUtensorMap mx;
     const cuuint64_t dims[2] = {(cuuint64_t)d.n_in, (cuuint64_t)x_rows};
     const cuuint64_t strides[1] = {(cuuint64_t)xs * size};
-    if (!rows_map(lin, &mx, d_x, 2, dims, strides, a.box))
+    if (!rows_map(lin, &mx, d_x, 2, dims, strides, d_rows && !a.gather ? 1 : a.box))
         return fail(RABBIT_CUDA_ERR_DEVICE, "%s: the driver could not encode the rows' tensor map", what);
     DeviceScope scope(lin->device);
     if (scope.status != RABBIT_CUDA_OK) return scope.status;

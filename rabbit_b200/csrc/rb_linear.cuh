@@ -15,8 +15,10 @@
 //   warps 4..11  readout: warp w reads lanes 32 (w % 4) .. + 31 (weight rows), and the
 //                even or odd blocks of 16 tokens; outputs go through shared memory, so that
 //                they leave in rows of 16 bytes a thread;
-//   warps 12..15 with a list: the token rows by cp.async, 16 bytes a thread (a gather by
-//                TMA, four rows an instruction, took 80 cycles for 512 bytes).
+//   warps 12..15 with a list and tiles of more than 32 tokens: the token rows by cp.async, 16
+//                bytes a thread. (A gather by TMA takes 80 cycles for four rows of 128 bytes: too
+//                long for many; of few rows it spares the MMAs' thread the fence between the
+//                proxies, some 0.3 us a step.)
 // Accumulation (MODE):
 //   kLinWhole  16-bit: in tensor memory over all of K, read once;
 //   kLinParts  16-bit, for fp32 outputs or a very long K: the tensor cores' sum is cut off,
@@ -62,7 +64,8 @@ constexpr uint32_t kLinOut = 32 * 128 * 4;  // outputs on their way: 32 tokens
 struct LinArgs {
     const int *offsets;   // [E + 1], or NULL: one expert with all rows
     const int *rows;      // [R] rows of x, or NULL
-    const uint8_t *x;     // with a list: x, its row in bytes, and the bytes of n_in
+    bool gather;          // by warps 12..15; with a list and without: by TMA
+    const uint8_t *x;     // to gather: x, its row in bytes, and the bytes of n_in
     uint32_t x_bytes;
     int k_bytes;
     const float *xs, *ws; // e4m3: scales
@@ -97,6 +100,7 @@ struct LinShared {
     uint64_t mdone;
     uint32_t tmem;
     int abort;
+    int4 src[8];  // a list's rows of x, gathered by TMA
 };
 static_assert(sizeof(LinShared) % 16 == 0, "the scales behind it are read 16 bytes at a time");
 __host__ __device__ constexpr int lin_sc(int bn) { return bn < 32 ? 32 : bn; }
@@ -425,7 +429,17 @@ __global__ void __launch_bounds__(kLinThreads, 1)
                 const int n0 = (PAIR ? 2 * t.mt + rank : t.mt) * outputs;
                 const int here = PAIR ? t.cols / 2 : t.cols;  // token rows of this CTA
                 const int boxes = a.rows ? 0 : (here + a.box - 1) / a.box;
-                const uint32_t bytes = (PAIR ? 2 : 1) * (kLinTile + boxes * a.box * 128);
+                const int quads = !PAIR && a.rows && !a.gather ? t.cols / 4 : 0;
+                const uint32_t bytes = (PAIR ? 2 : 1) * (kLinTile + boxes * a.box * 128) + quads * 512;
+                if (!PAIR)
+                    for (int c = 0; c < 4 * quads; ++c) {
+                        int r = c < t.n ? __ldg(a.rows + t.row0 + c) : 0;
+                        if (r < 0 || r >= a.x_rows) {
+                            atomicOr(a.err, RB_LIN_ERR_ROWS);
+                            r = 0;  // read for nothing: lin_written leaves the row out
+                        }
+                        reinterpret_cast<int *>(s.src)[c] = r;
+                    }
                 // weights that no other tile of tokens reads leave the L2 first
                 const uint64_t pol = pre[t.e + 1] - pre[t.e] > 1 ? keep : once;
                 for (int k = k0; k < k1; ++k, ++issued) {
@@ -445,6 +459,10 @@ __global__ void __launch_bounds__(kLinThreads, 1)
                         if (GATED) tma_load_4d(base + kLinTile / 2, &mw, c0, n0, 1, t.e, &s.full[st.at], pol);
                         for (int b = 0; b < boxes; ++b)
                             tma_load_2d(xb + b * a.box * 128, &mx, c0, t.row0 + b * a.box, &s.full[st.at]);
+                        for (int j = 0; j < quads; ++j) {
+                            const int4 r = s.src[j];
+                            tma_gather4(xb + j * 512, &mx, c0, r.x, r.y, r.z, r.w, &s.full[st.at]);
+                        }
                     }
                     st.next(a.stages);
                 }
@@ -466,7 +484,7 @@ __global__ void __launch_bounds__(kLinThreads, 1)
                 int part = 0;
                 for (int k = k0; k < k1; ++k) {
                     if (!(ok = lin_wait1(&s.full[st.at], st.phase, a, abort))) break;
-                    if (a.rows) {
+                    if (a.gather) {
                         if (PAIR) ok = lin_wait1(&s.told[st.at], st.phase, a, abort);
                         if (!ok || !(ok = lin_wait1(&s.rows[st.at], st.phase, a, abort))) break;
                         fence_async();
@@ -496,7 +514,7 @@ __global__ void __launch_bounds__(kLinThreads, 1)
                 mbar_wait(&s.mdone, 0, a.wait_ns, nullptr, 0);
             }
         }
-        if (PAIR && !leader && a.rows && elect_one()) {  // word of this CTA's rows to the leader
+        if (PAIR && !leader && a.gather && elect_one()) {  // word of this CTA's rows to the leader
             LinRing st;
             bool ok = true;
             for (int i = first; ok && lin_tile(a, off, pre, i, t); i += stride)
@@ -578,7 +596,7 @@ __global__ void __launch_bounds__(kLinThreads, 1)
     }
     } else if (warp >= 12) {  // ------------------------------------- gather
         if constexpr (MODE != kLinWhole) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
-        if (a.rows) {
+        if (a.gather) {
             LinRing st;
             bool ok = true;
             for (int i = first; ok && lin_tile(a, off, pre, i, t); i += stride) {

@@ -208,6 +208,16 @@ __device__ __forceinline__ void tma_load_2d(void *smem_dst, const CUtensorMap *m
         "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(smem_u32(bar))
         : "memory");
 }
+// Four rows r0 .. r3 of a 2-D map whose box is one row high, one after the other.
+__device__ __forceinline__ void tma_gather4(void *smem_dst, const CUtensorMap *map, int c0, int r0,
+                                            int r1, int r2, int r3, uint64_t *bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cta.global.tile::gather4.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%2, %3, %4, %5, %6}], [%7];" ::"r"(smem_u32(smem_dst)),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(r0), "r"(r1), "r"(r2), "r"(r3),
+        "r"(smem_u32(bar))
+        : "memory");
+}
 // For a CTA of a pair: into its own shared memory, completing on a barrier of either
 // CTA (`bar`: a shared::cluster address). No multicast.
 __device__ __forceinline__ void tma_load_2d_pair(void *smem_dst, const CUtensorMap *map, int c0,
