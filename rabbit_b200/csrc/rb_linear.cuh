@@ -643,60 +643,71 @@ __global__ void __launch_bounds__(kLinThreads, 1)
                 lin_put<GATED, OUT>(a, t.row0 + 32 * b + token, (PAIR ? 2 * t.mt + (int)rank : t.mt) * outputs, seg,
                         [&](int i) { return *reinterpret_cast<const float4 *>(outs + token * 128 + i); });
         };
+        // A tile's sums in registers, NC blocks of 16 tokens a warp (with those of 256 tokens in
+        // the way, a step of 16 took 0.2 us more)
+        auto sums = [&](auto blocks) {
+            constexpr int NC = decltype(blocks)::value;
+            uint64_t acc[NC][8];  // block pair, two tokens
+#pragma unroll
+            for (int c = 0; c < NC; ++c)
+#pragma unroll
+                for (int j = 0; j < 8; ++j) acc[c][j] = 0;
+            const int n = t.cols - 16 * h;  // columns from this warp's first on
+            for (int k = k0; k < k1; k += PART) {
+                if (!(ok = lin_wait(&s.dfull[db.at], db.phase, a, abort))) break;
+                tc_fence_after();
+                const uint32_t d = tmem + lanes + db.at * a.bn + 16 * h;
+                const float *sc = scales + db.at * sc_buf + (GATED && q >= 2 ? sc_row : 0) + 16 * h;
+                auto add = [&](int c, const float(&v)[16]) {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const uint64_t v0 = pack2(v[4 * j], v[4 * j + 1]), v1 = pack2(v[4 * j + 2], v[4 * j + 3]);
+                        if (F8) {
+                            const ulonglong2 f = reinterpret_cast<const ulonglong2 *>(sc + 32 * c)[j];
+                            fma2(acc[c][2 * j], v0, f.x);
+                            fma2(acc[c][2 * j + 1], v1, f.y);
+                        } else {
+                            add2(acc[c][2 * j], v0);
+                            add2(acc[c][2 * j + 1], v1);
+                        }
+                    }
+                };
+                // 32 columns in flight at a time
+#pragma unroll
+                for (int c = 0; c < NC; c += 2) {
+                    float v[2][16];
+                    const bool one = 32 * c < n, two = c + 1 < NC && 32 * (c + 1) < n;
+                    if (one) lin_ld16(d + 32 * c, v[0]);
+                    if (two) lin_ld16(d + 32 * (c + 1), v[1]);
+                    if (one) {
+                        lin_ld_done(v[0]);
+                        add(c, v[0]);
+                    }
+                    if (two) {
+                        lin_ld_done(v[1]);
+                        if (c + 1 < NC) add(c + 1, v[1]);
+                    }
+                }
+                release();
+            }
+            // (a wait that ran out ends it for every warp of the block before a barrier
+            // among them)
+            ok = named_all(1, kLinReaders, ok);
+            if (!ok) return;
+#pragma unroll
+            for (int c = 0; c < NC; ++c) {
+                if (32 * c >= t.cols) break;
+                float v[16];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) unpack2(acc[c][j], v[2 * j], v[2 * j + 1]);
+                put(c, v);
+            }
+        };
         for (int i = first; ok && lin_tile(a, off, pre, i, t); i += stride) {
             if constexpr (MODE != kLinWhole) {
-                uint64_t acc[8][8];  // block pair, two tokens
-#pragma unroll
-                for (int c = 0; c < 8; ++c)
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) acc[c][j] = 0;
-                const int n = t.cols - 16 * h;  // columns from this warp's first on
-                for (int k = k0; k < k1; k += PART) {
-                    if (!(ok = lin_wait(&s.dfull[db.at], db.phase, a, abort))) break;
-                    tc_fence_after();
-                    const uint32_t d = tmem + lanes + db.at * a.bn + 16 * h;
-                    const float *sc = scales + db.at * sc_buf + (GATED && q >= 2 ? sc_row : 0) + 16 * h;
-                    auto add = [&](int c, const float(&v)[16]) {
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            const uint64_t v0 = pack2(v[4 * j], v[4 * j + 1]), v1 = pack2(v[4 * j + 2], v[4 * j + 3]);
-                            if (F8) {
-                                const ulonglong2 f = reinterpret_cast<const ulonglong2 *>(sc + 32 * c)[j];
-                                fma2(acc[c][2 * j], v0, f.x);
-                                fma2(acc[c][2 * j + 1], v1, f.y);
-                            } else {
-                                add2(acc[c][2 * j], v0);
-                                add2(acc[c][2 * j + 1], v1);
-                            }
-                        }
-                    };
-                    // 32 columns in flight at a time (16: a step of 256 tokens took half as long again)
-#pragma unroll
-                    for (int c = 0; c < 8; c += 2) {
-                        if (32 * c >= n) break;
-                        float v[2][16];
-                        lin_ld16(d + 32 * c, v[0]);
-                        const bool two = 32 * (c + 1) < n;
-                        if (two) lin_ld16(d + 32 * (c + 1), v[1]);
-                        lin_ld_done(v[0]);
-                        if (two) lin_ld_done(v[1]);
-                        add(c, v[0]);
-                        if (two) add(c + 1, v[1]);
-                    }
-                    release();
-                }
-                // (a wait that ran out ends it for every warp of the block before a barrier
-                // among them)
-                ok = named_all(1, kLinReaders, ok);
-                if (!ok) break;
-#pragma unroll
-                for (int c = 0; c < 8; ++c) {
-                    if (32 * c >= t.cols) break;
-                    float v[16];
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) unpack2(acc[c][j], v[2 * j], v[2 * j + 1]);
-                    put(c, v);
-                }
+                if (t.cols <= 32) sums(LinInt<1>());
+                else if (t.cols <= 64) sums(LinInt<2>());
+                else sums(LinInt<8>());
             } else {
                 ok = named_all(1, kLinReaders, lin_wait(&s.dfull[db.at], db.phase, a, abort));
                 if (!ok) break;
