@@ -88,30 +88,58 @@ static bool rows_map(const rabbit_cuda_linear *lin, CUtensorMap *map, const void
 
 static int up_to(int64_t n, int unit) { return (int)((n + unit - 1) / unit * unit); }
 
+// Microseconds that a step of 128 bytes of K takes with tiles of `cols` tokens, and that a
+// cluster takes to sum the parts of a tile, from 2048 and 8192 x 1024 .. 14336 at 40 to 512 rows
+// (us, one CTA a tile / pairs; n_out 14336 shows the steps, 1024 the sums):
+//   bf16 8192 x 14336   64 rows 40 / 39    128 rows 43 / 42    256 rows 58 / 54    512 rows 107 / 95
+//   bf16 8192 x 1024    64 rows 14 / 27    128 rows 17 / 30    256 rows 27 / 44    512 rows 50 / 44
+//   e4m3 8192 x 14336   64 rows 31 / 40    128 rows 74 / 41    256 rows 110 / 42   512 rows 215 / 75
+//   e4m3 8192 x 1024    64 rows 15 / 36    128 rows 24 / 37    256 rows 36 / 37    512 rows 68 / 37
+static double lin_step_us(bool f8, bool pair, int64_t cols) {
+    if (pair) return f8 ? 0.44 : 0.16 + 0.0005 * cols;
+    if (f8) return cols <= 64 ? 0.3 : 0.4 + 0.0047 * cols;
+    return 0.2 + 0.0006 * cols;
+}
+static double lin_sum_us(int64_t cols) { return 0.058 * cols; }
+
 // The launch's shape from the sizes alone (the groups' rows are on the device).
 static bool lin_plan(LinArgs &a, int mode, int sms, int64_t *tiles, size_t *smem) {
-    const int64_t mean = ((int64_t)a.R + a.E - 1) / a.E;
-    const bool pair = mean >= 128, as_rows = pair && mode == kLinF8;
-    const int outputs = (a.gated ? 64 : 128) * (pair ? 2 : 1);
-    a.mt = (a.N + outputs - 1) / outputs;
+    const bool f8 = mode == kLinF8;
+    const int64_t mean = ((int64_t)a.R + a.E - 1) / a.E, groups = a.E < a.R ? a.E : a.R;
+    const int outputs = a.gated ? 64 : 128;
+    auto div_up = [](int64_t n, int64_t d) { return (n + d - 1) / d; };
+    // a pair of CTAs a tile, or one CTA and a split of K: by the estimate above, every
+    // expert with the mean's rows
+    const int64_t cols = mean < 256 ? mean : 256, token_tiles_est = (a.E == 1 ? 1 : groups) * div_up(mean, 256);
+    const double by_pairs = lin_step_us(f8, true, cols) * a.steps *
+                            div_up(token_tiles_est * div_up(a.N, 2 * outputs), sms / 2);
+    const int64_t one_tiles = token_tiles_est * div_up(a.N, outputs);
+    double by_one = 0;
+    for (int split = 1; split <= 8 && (split == 1 || (one_tiles * split <= sms && a.steps / split >= 2)); split *= 2) {
+        const double us = lin_step_us(f8, false, cols) * div_up(a.steps, split) * div_up(one_tiles * split, sms) +
+                          (split > 1 ? lin_sum_us(cols) : 0.0);
+        if (split == 1 || us < by_one) {
+            by_one = us;
+            a.split = split;
+        }
+    }
+    const bool pair = by_pairs < by_one, as_rows = pair && f8;
+    if (pair) a.split = 1;
+    a.mt = (int)div_up(a.N, pair ? 2 * outputs : outputs);
     a.unit = as_rows ? 256 : pair ? 64 : 16;
+    // tokens of a tile: a multiple of 16 or, with more than one box, of the box's rows; room
+    // for four times the mean where the experts' rows differ
     const int64_t want = a.E == 1 ? mean : 4 * mean, rows = want < a.R ? want : a.R;
-    // a multiple of 16 or, with more than one box, of the box's rows
-    a.bn = rows >= 256 ? 256 : rows <= 16 ? 16 : up_to(rows, 32);
-    if (pair) a.bn = up_to(a.bn, a.unit);
+    a.bn = as_rows || rows >= 256 ? 256 : pair ? up_to(rows, 64) : rows <= 16 ? 16 : up_to(rows, 32);
     a.buf_shift = 1;
     while (a.buf_shift < 3 && (2 << a.buf_shift) * a.bn <= 512) ++a.buf_shift;
     a.bufs = 1 << a.buf_shift;
     static_assert(kLinBufs == 1 << 3, "buffers of tensor memory");
-    const int64_t groups = a.E < a.R ? a.E : a.R;
-    const int64_t token_tiles = a.E == 1 ? (a.R + a.bn - 1) / a.bn : groups + a.R / a.bn;
-    *tiles = token_tiles * a.mt;
-    a.split = 1;
-    while (!pair && a.split < 8 && *tiles * a.split * 2 <= sms && a.steps / (a.split * 2) >= 2) a.split *= 2;
+    *tiles = (a.E == 1 ? div_up(a.R, a.bn) : groups + a.R / a.bn) * a.mt;
     a.box = as_rows ? 128 : a.bn < 32 ? a.bn : 32;
     a.band = 8;
     const size_t stage = as_rows ? kRowsStage : lin_stage_bytes(pair, a.bn);
-    const size_t fixed = as_rows ? lin_rows_fixed(a.E) : lin_fixed(mode == kLinF8, a.gated, a.bn, a.bufs, a.E);
+    const size_t fixed = as_rows ? lin_rows_fixed(a.E) : lin_fixed(f8, a.gated, a.bn, a.bufs, a.E);
     a.stages = (int)((kMaxDynSmem - fixed) / stage);
     if (a.stages > kLinStages) a.stages = kLinStages;
     *smem = fixed + a.stages * stage;
