@@ -50,7 +50,12 @@ constexpr float kF8Tiny = 0x1p-60f, kF8Grow = 0x1p64f;
 __device__ __forceinline__ F8Scale f8_scale(uint32_t top) {
     F8Scale f;
     f.bad = top >= kInfBits;
-    f.s = __fdiv_rn(__uint_as_float(top), 448.f);
+    // top / 448 to nearest: a product and one correction (equal to the division for every
+    // mantissa while nothing falls below fp32's normal numbers)
+    const float t = __uint_as_float(top), q = t * (1.f / 448.f);
+    f.s = fmaf(fmaf(-q, 448.f, t), 1.f / 448.f, q);
+    if (t < 0x1p-100f) f.s = __fdiv_rn(t, 448.f);
+    if (f.bad) f.s = __uint_as_float(0x7FC00000u);
     f.zero = f.s == 0.f;
     // below 2^-60 x and s are multiplied by 2^64, where 1 / s and the remainders are far from
     // fp32's smallest numbers
@@ -58,15 +63,7 @@ __device__ __forceinline__ F8Scale f8_scale(uint32_t top) {
     const float r = __fdividef(1.f, f.tiny ? f.s * kF8Grow : f.s);
     f.lo = r * (1.f - 0x1p-21f);
     f.hi = r * (1.f + 0x1p-21f);
-    if (f.bad) f.s = __uint_as_float(0x7FC00000u);
     return f;
-}
-
-__device__ __noinline__ uint32_t f8_between(float x, float s, uint32_t a, uint32_t b) {
-    // codes a and b (of one sign, b = a + 1 in magnitude)
-    const float m = 0.5f * (fabsf(e4m3_value(a)) + fabsf(e4m3_value(b)));
-    const float d = fmaf(-m, s, fabsf(x));
-    return d < 0.f ? a : d > 0.f ? b : (a & 1) ? b : a;
 }
 
 // Codes of eight values, the first in the low byte.
@@ -85,12 +82,20 @@ __device__ __forceinline__ uint2 f8_codes(float (&x)[8], const F8Scale &f) {
         a[i] = e4m3x2(v[0] * f.lo, v[1] * f.lo) | e4m3x2(v[2] * f.lo, v[3] * f.lo) << 16;
         b[i] = e4m3x2(v[0] * f.hi, v[1] * f.hi) | e4m3x2(v[2] * f.hi, v[3] * f.hi) << 16;
     }
-    if (a[0] != b[0] || a[1] != b[1]) {
+    // one at a time: of 16-bit values, whose quotients are often ties, a lane has one or two
+    uint64_t d = (uint64_t)(a[1] ^ b[1]) << 32 | (a[0] ^ b[0]);
+    while (d) {
+        const int i = (__ffsll((long long)d) - 1) >> 3, sh = 8 * (i & 3);
+        d &= ~(0xFFull << (8 * i));
+        float v = x[0];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const uint32_t ai = a[i / 4] >> (8 * (i & 3)) & 255, bi = b[i / 4] >> (8 * (i & 3)) & 255;
-            if (ai != bi) a[i / 4] ^= (ai ^ f8_between(x[i], s, ai, bi)) << (8 * (i & 3));
-        }
+        for (int j = 1; j < 8; ++j) v = i == j ? x[j] : v;
+        const uint32_t word = i < 4 ? a[0] : a[1], c = word >> sh & 255;  // below m; above it c + 1
+        const float m = 0.5f * (fabsf(e4m3_value(c)) + fabsf(e4m3_value(c + 1)));
+        const float r = fmaf(-m, s, fabsf(v));
+        const uint32_t up = (r > 0.f || (r == 0.f && (c & 1))) ? 1u << sh : 0u;
+        if (i < 4) a[0] += up;
+        else a[1] += up;
     }
     return make_uint2(a[0], a[1]);
 }
@@ -156,24 +161,24 @@ __device__ __forceinline__ void f8_store(uint8_t *row, int c, int n_cols, uint2 
     }
 }
 
-// One scale for each row's block: 16 lanes hold a block, eight values each; BATCH
-// blocks of each half warp are in flight.
+// One scale for each row's block: eight lanes hold a block, a lane columns 8 l .. and
+// 64 + 8 l .. of it; BATCH blocks of each eight lanes are in flight.
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(kF8Threads) k_f8_rows(const __grid_constant__ F8Args a) {
-    constexpr int BATCH = 4;
+    constexpr int BATCH = 2;
     launch_dependents();
     wait_prerequisite();
     const int64_t items = (int64_t)a.n_rows * a.nb;
-    const int lane = threadIdx.x & 15;
-    const int64_t teams = (int64_t)gridDim.x * (kF8Threads / 16);
-    for (int64_t i0 = ((int64_t)blockIdx.x * kF8Threads + threadIdx.x) / 32 * 2; i0 < items;
+    const int lane = threadIdx.x & 7;
+    const int64_t teams = (int64_t)gridDim.x * (kF8Threads / 8);
+    for (int64_t i0 = ((int64_t)blockIdx.x * kF8Threads + threadIdx.x) / 32 * 4; i0 < items;
          i0 += teams * BATCH) {
-        F8Raw<T> d[BATCH];
+        F8Raw<T> d[BATCH][2];
         int64_t at[BATCH];
         int block[BATCH];
 #pragma unroll
-        for (int b = 0; b < BATCH; ++b) {  // a warp's two blocks side by side, then `teams` on
-            const int64_t i = i0 + (threadIdx.x >> 4 & 1) + b * teams;
+        for (int b = 0; b < BATCH; ++b) {  // a warp's four blocks side by side, then `teams` on
+            const int64_t i = i0 + (threadIdx.x >> 3 & 3) + b * teams;
             at[b] = -1;
             if (i < items) {
                 const int64_t r = items >> 31 ? i / a.nb : a.nb == 1 ? i : __umulhi((uint32_t)i, a.magic) >> a.shift;
@@ -181,21 +186,27 @@ __global__ void __launch_bounds__(kF8Threads) k_f8_rows(const __grid_constant__ 
                 const int64_t src = a.rows ? __ldg(a.rows + r) : r;
                 if (!a.rows || (src >= 0 && src < a.x_rows)) {
                     at[b] = r;
-                    d[b] = f8_load<T, VEC>(static_cast<const T *>(a.x) + src * a.xs, block[b] * 128 + lane * 8,
-                                           a.n_cols);
+                    const T *row = static_cast<const T *>(a.x) + src * a.xs;
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+                        d[b][h] = f8_load<T, VEC>(row, block[b] * 128 + h * 64 + lane * 8, a.n_cols);
                 }
             }
         }
 #pragma unroll
         for (int b = 0; b < BATCH; ++b) {
-            uint32_t top = at[b] >= 0 ? f8_top(d[b]) : 0u;
+            uint32_t top = at[b] >= 0 ? max(f8_top(d[b][0]), f8_top(d[b][1])) : 0u;
 #pragma unroll
-            for (int m = 8; m; m >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, m));
+            for (int m = 4; m; m >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, m));
             if (at[b] < 0) continue;
             const F8Scale f = f8_scale(f8_top_f32<T>(top));
-            float v[8];
-            f8_values(d[b], v);
-            f8_store<VEC>(a.q + at[b] * a.qs, block[b] * 128 + lane * 8, a.n_cols, f8_codes(v, f));
+            uint8_t *q = a.q + at[b] * a.qs;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                float v[8];
+                f8_values(d[b][h], v);
+                f8_store<VEC>(q, block[b] * 128 + h * 64 + lane * 8, a.n_cols, f8_codes(v, f));
+            }
             if (lane == 0) a.scale[at[b] * a.nb + block[b]] = f.s;
         }
     }
@@ -280,7 +291,7 @@ extern "C" int rabbit_cuda_f8_quantise_dev(int dtype, const void *d_x, int64_t x
         scope.launch(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, current_device()), "f8_quantise: SM count");
     if (scope.status != RABBIT_CUDA_OK) return scope.status;
     // Rows: blocks are handed out warp by warp, in one wave of the SMs at most.
-    const int64_t ctas = ((int64_t)n_rows * a.nb + kF8Threads / 16 - 1) / (kF8Threads / 16);
+    const int64_t ctas = ((int64_t)n_rows * a.nb + kF8Threads / 8 - 1) / (kF8Threads / 8);
     const dim3 grid = block_rows == 1 ? dim3((unsigned)(ctas < 8 * sms ? ctas : 8 * sms))
                                       : dim3((n_rows + 127) / 128, a.nb);
     with_dtype(dtype, [&](auto t) {
