@@ -650,7 +650,8 @@ int rabbit_cuda_kv4_debug_withhold(rabbit_cuda_kv4 *kv);
  * s = NaN and codes NaN. q [n_rows] rows of q_stride bytes; d_scale [n_rows or its blocks][n_cols /
  * 128 rounded up]. With d_rows (block_rows 1 only) row i is row d_rows[i] of the x_rows rows
  * of x; where that is outside of them, row i of q and of d_scale is left as it was. x_rows is
- * not read without d_rows. n_rows 0 does nothing. On the calling thread's device. */
+ * not read without d_rows. n_rows 0 does nothing; n_rows * blocks of columns below 2^31. On the calling
+ * thread's device. */
 int rabbit_cuda_f8_quantise_dev(int dtype, const void *d_x, int64_t x_stride, int x_rows,
                                 const int *d_rows, void *d_q, int64_t q_stride, float *d_scale,
                                 int n_rows, int n_cols, int block_rows, void *stream);
@@ -720,7 +721,7 @@ int rabbit_cuda_experts_route_dev(const float *d_scores, int64_t score_stride, i
 /* out[t] = base[t] + sum_j weights[t][j] y[place[t][j]], in the order of j, in fp32, rounded
  * once: y [y_rows] rows of n_cols in dtype, base (may be NULL: 0; may be out, with the same stride)
  * and out in out_dtype. A place outside of 0..y_rows - 1 adds nothing. out must not
- * overlap y. 1 <= k <= 32. n_tokens 0 does nothing. On the calling thread's device. */
+ * overlap y. 1 <= k <= 32, n_tokens below 2^23. n_tokens 0 does nothing. On the calling thread's device. */
 int rabbit_cuda_experts_combine_dev(int dtype, const void *d_y, int64_t y_stride, int y_rows,
                                     const int *d_place, const float *d_weights, int n_tokens, int k,
                                     int n_cols, int out_dtype, const void *d_base,

@@ -3,6 +3,8 @@
 // experts' rows (:356-357, 398-399).
 #include <math.h>
 
+#include <type_traits>
+
 #include "rb_device.cuh"
 #include "rb_launch.h"
 #include "rb_runtime.h"
@@ -89,28 +91,33 @@ __device__ void route_token(const RouteArgs &a, int t, int lane) {
     }
 }
 
-__device__ __forceinline__ void route_any(const RouteArgs &a, int t, int lane) {
-    if (a.E <= 32) route_token<1>(a, t, lane);
-    else if (a.E <= 64) route_token<2>(a, t, lane);
-    else if (a.E <= 128) route_token<4>(a, t, lane);
-    else if (a.E <= 256) route_token<8>(a, t, lane);
-    else route_token<32>(a, t, lane);
-}
-
+template <int V>
 __global__ void __launch_bounds__(256) k_route(const __grid_constant__ RouteArgs a) {
     launch_dependents();
     wait_prerequisite();
     for (int t = blockIdx.x * 8 + (threadIdx.x >> 5); t < a.T; t += gridDim.x * 8)
-        route_any(a, t, threadIdx.x & 31);
+        route_token<V>(a, t, threadIdx.x & 31);
+}
+
+// Lanes with the same low `bits` bits of e (a vote for each: of 32 values that mostly differ,
+// match.any takes several times as long).
+__device__ __forceinline__ uint32_t lanes_alike(int e, int bits) {
+    uint32_t same = 0xffffffffu;
+    for (int b = 0; b < bits; ++b) {
+        const bool set = e >> b & 1;
+        const uint32_t v = __ballot_sync(0xffffffffu, set);
+        same &= set ? v : ~v;
+    }
+    return same;
 }
 
 // A counting sort of the pairs by expert that keeps their order, one cluster of CTAs: CTA r
 // and in it warp w have the r-th and w-th part of the pairs. Each warp counts its pairs of
 // each expert in its own column of shared memory; the counts become places (experts, CTAs, warps in
 // turn); then each warp takes its pairs again, 32 at a time, a pair's place its
-// column's plus the equal experts on lower lanes. No atomics: same places each time.
-// PICK: the tokens' experts are chosen here, too.
-template <bool PICK>
+// column's plus the equal experts on lower lanes: the same places each time.
+// PICK above 0: the tokens' experts are chosen here, too, PICK scores a lane.
+template <int PICK>
 __global__ void __launch_bounds__(kRouteThreads, 1) k_route_order(const __grid_constant__ RouteArgs a) {
     extern __shared__ int route_smem[];
     int *count = route_smem;                       // [warps][E]
@@ -123,8 +130,8 @@ __global__ void __launch_bounds__(kRouteThreads, 1) k_route_order(const __grid_c
     wait_prerequisite();
     const int warps = ctas * kRouteWarps, w = cta * kRouteWarps + warp;
     const int t0 = (int)((int64_t)a.T * w / warps), t1 = (int)((int64_t)a.T * (w + 1) / warps);
-    if (PICK)
-        for (int t = t0; t < t1; ++t) route_any(a, t, lane);
+    if constexpr (PICK > 0)
+        for (int t = t0; t < t1; ++t) route_token<PICK>(a, t, lane);
     __syncwarp();
     int *mine = count + warp * a.E;
     for (int e = lane; e < a.E; e += 32) mine[e] = 0;
@@ -134,19 +141,29 @@ __global__ void __launch_bounds__(kRouteThreads, 1) k_route_order(const __grid_c
         const int e = p < p1 ? a.ids[p] : -1;
         return e >= 0 && e < a.E ? e : -1;
     };
-    for (int p = p0; p < p1; p += 32) {
-        const int e = expert(p + lane);
-        const uint32_t same = __match_any_sync(0xffffffffu, e);
-        if (e >= 0 && (same >> lane) == 1) mine[e] += __popc(same);  // its highest lane
-        __syncwarp();
+    const int bits = 32 - __clz(a.E);  // of an expert and of -1's low bits
+    constexpr int B = 8;  // pairs of a lane read at a time: one after the other they took 8 us
+    for (int p = p0; p < p1; p += 32 * B) {
+        int es[B];
+#pragma unroll
+        for (int b = 0; b < B; ++b) es[b] = expert(p + 32 * b + lane);
+#pragma unroll
+        for (int b = 0; b < B; ++b)
+            if (es[b] >= 0) atomicAdd(&mine[es[b]], 1);  // (a sum of whole numbers: in any order)
     }
     __syncthreads();
     for (int e = threadIdx.x; e < a.E; e += kRouteThreads) {  // columns: first place in the CTA
         int n = 0;
-        for (int i = 0; i < kRouteWarps; ++i) {
-            const int c = count[i * a.E + e];
-            count[i * a.E + e] = n;
-            n += c;
+#pragma unroll
+        for (int i0 = 0; i0 < kRouteWarps; i0 += 16) {
+            int c[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) c[i] = count[(i0 + i) * a.E + e];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                count[(i0 + i) * a.E + e] = n;
+                n += c[i];
+            }
         }
         total[e] = n;
     }
@@ -198,18 +215,25 @@ __global__ void __launch_bounds__(kRouteThreads, 1) k_route_order(const __grid_c
         }
     }
     __syncthreads();
-    for (int p = p0; p < p1; p += 32) {
-        const int e = expert(p + lane);
-        const uint32_t same = __match_any_sync(0xffffffffu, e);
-        int at = -1;
-        if (e >= 0) {
-            at = base[e] + mine[e] + __popc(same & ((1u << lane) - 1));
-            a.rows[at] = (p + lane) / a.k;
+    for (int p = p0; p < p1; p += 32 * B) {
+        int es[B];
+#pragma unroll
+        for (int b = 0; b < B; ++b) es[b] = expert(p + 32 * b + lane);
+#pragma unroll
+        for (int b = 0; b < B; ++b) {
+            const int q = p + 32 * b + lane, e = es[b];
+            if (p + 32 * b >= p1) break;
+            const uint32_t same = lanes_alike(e, bits);
+            int at = -1;
+            if (e >= 0) {
+                at = base[e] + mine[e] + __popc(same & ((1u << lane) - 1));
+                a.rows[at] = q / a.k;
+            }
+            if (q < p1) a.place[q] = at;
+            __syncwarp();
+            if (e >= 0 && (same >> lane) == 1) mine[e] += __popc(same);
+            __syncwarp();
         }
-        if (p + lane < p1) a.place[p + lane] = at;
-        __syncwarp();
-        if (e >= 0 && (same >> lane) == 1) mine[e] += __popc(same);
-        __syncwarp();
     }
     // behind the last place
     const int n = a.T * a.k;
@@ -225,7 +249,7 @@ struct CombineArgs {
     int y_rows;
     const int *place;
     const float *weights;
-    int T, k, cols;
+    int T, k, cols, shift;
     const void *base;
     int64_t bs;
     void *out;
@@ -234,40 +258,64 @@ struct CombineArgs {
 
 constexpr int kCombineThreads = 256;
 
-// Bound by memory: each row of y is read once. A thread has eight columns of a token
-// (scalar form: one).
+// Eight elements as they lie in memory (VEC), or one.
+template <typename T, bool VEC>
+struct Piece {
+    using W = typename std::conditional<VEC, uint4, T>::type;
+    W w[VEC ? sizeof(T) / 2 : 1];
+    __device__ __forceinline__ void load(const T *p) {
+#pragma unroll
+        for (int i = 0; i < (VEC ? (int)sizeof(T) / 2 : 1); ++i) w[i] = reinterpret_cast<const W *>(p)[i];
+    }
+    __device__ __forceinline__ void values(float (&v)[VEC ? 8 : 1]) const {
+        const T *e = reinterpret_cast<const T *>(w);
+#pragma unroll
+        for (int i = 0; i < (VEC ? 8 : 1); ++i) v[i] = to_f32(e[i]);
+    }
+};
+
+// Bound by memory: each row of y is read once. 2^shift threads have a token, a thread eight
+// columns at a time (scalar form: one).
 template <typename Y, typename O, bool VEC>
-__global__ void __launch_bounds__(kCombineThreads) k_combine(const __grid_constant__ CombineArgs a) {
-    constexpr int V = VEC ? 8 : 1;
+__global__ void __launch_bounds__(kCombineThreads, 4) k_combine(const __grid_constant__ CombineArgs a) {
+    constexpr int V = VEC ? 8 : 1, B = 2;  // B rows of y in flight
     launch_dependents();
     wait_prerequisite();
-    const int per = a.cols / V;
-    const int64_t items = (int64_t)a.T * per;
-    for (int64_t i = (int64_t)blockIdx.x * kCombineThreads + threadIdx.x; i < items;
-         i += (int64_t)gridDim.x * kCombineThreads) {
-        const int64_t t = items >> 31 ? i / per : (int)i / per;
-        const int c = (int)(i - t * per) * V;
-        float acc[V];
+    const int t = (blockIdx.x * kCombineThreads + threadIdx.x) >> a.shift;
+    if (t >= a.T) return;
+    const int *place = a.place + (int64_t)t * a.k;
+    const float *weights = a.weights + (int64_t)t * a.k;
+    for (int c = (threadIdx.x & ((1 << a.shift) - 1)) * V; c < a.cols; c += V << a.shift) {
+        Piece<O, VEC> base;
+        if (a.base) base.load(static_cast<const O *>(a.base) + t * a.bs + c);
+        float acc[V], v[V];
 #pragma unroll
-        for (int v = 0; v < V; ++v) acc[v] = 0.f;
-        for (int j = 0; j < a.k; ++j) {
-            const int p = __ldg(a.place + t * a.k + j);
-            if (p < 0 || p >= a.y_rows) continue;
-            const float w = __ldg(a.weights + t * a.k + j);
-            const Y *y = static_cast<const Y *>(a.y) + p * a.ys + c;
-            float d[V];
-            if constexpr (VEC) load8<true>(d, y);
-            else d[0] = to_f32(*y);
+        for (int e = 0; e < V; ++e) acc[e] = 0.f;
+        for (int j0 = 0; j0 < a.k; j0 += B) {
+            Piece<Y, VEC> d[B];
+            float w[B];
+            bool some[B];
 #pragma unroll
-            for (int v = 0; v < V; ++v) acc[v] = fmaf(w, d[v], acc[v]);
+            for (int b = 0; b < B; ++b) {
+                const int p = j0 + b < a.k ? __ldg(place + j0 + b) : -1;
+                some[b] = p >= 0 && p < a.y_rows;
+                if (some[b]) {
+                    w[b] = __ldg(weights + j0 + b);
+                    d[b].load(static_cast<const Y *>(a.y) + p * a.ys + c);
+                }
+            }
+#pragma unroll
+            for (int b = 0; b < B; ++b)
+                if (some[b]) {
+                    d[b].values(v);
+#pragma unroll
+                    for (int e = 0; e < V; ++e) acc[e] = fmaf(w[b], v[e], acc[e]);
+                }
         }
         if (a.base) {
-            const O *b = static_cast<const O *>(a.base) + t * a.bs + c;
-            float d[V];
-            if constexpr (VEC) load8<true>(d, b);
-            else d[0] = to_f32(*b);
+            base.values(v);
 #pragma unroll
-            for (int v = 0; v < V; ++v) acc[v] = d[v] + acc[v];
+            for (int e = 0; e < V; ++e) acc[e] = v[e] + acc[e];
         }
         O *o = static_cast<O *>(a.out) + t * a.os + c;
         if constexpr (VEC) store8<true>(o, acc);
@@ -309,22 +357,25 @@ int rabbit_cuda_experts_route_dev(const float *d_scores, int64_t score_stride, i
     a.offsets = d_offsets;
     a.rows = d_rows;
     a.place = d_place;
+    if (!device_sms()) return fail(RABBIT_CUDA_ERR_DEVICE, "experts_route: no device %d", current_device());
     DeviceScope scope(current_device());
     if (scope.status != RABBIT_CUDA_OK) return scope.status;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     const size_t smem = sizeof(int) * (size_t)a.E * (kRouteWarps + 2);
     // Up to a token a warp of the cluster the picks are made by the kernel that orders: one launch.
-    const bool pick = d_scores && n_tokens <= kRouteCluster * kRouteWarps;
+    // (With more than 256 experts a lane has too many for that kernel's registers.)
+    const int v = n_experts <= 32 ? 1 : n_experts <= 64 ? 2 : n_experts <= 128 ? 4 : n_experts <= 256 ? 8 : 32;
+    const bool pick = d_scores && n_tokens <= kRouteCluster * kRouteWarps && v <= 8;
     const unsigned ctas = n_tokens <= kRouteWarps ? 1 : kRouteCluster;
     if (d_scores && !pick) {
-        int sms = 0;
-        scope.launch(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, current_device()), "experts_route: SM count");
-        if (scope.status != RABBIT_CUDA_OK) return scope.status;
+        const int sms = device_sms();
         const int64_t want = ((int64_t)n_tokens + 7) / 8;
-        scope.launch(launch_pdl(k_route, dim3((unsigned)(want < 8 * sms ? want : 8 * sms)), dim3(256), 0, s, a),
+        auto k = v == 1 ? k_route<1> : v == 2 ? k_route<2> : v == 4 ? k_route<4> : v == 8 ? k_route<8> : k_route<32>;
+        scope.launch(launch_pdl(k, dim3((unsigned)(want < 8 * sms ? want : 8 * sms)), dim3(256), 0, s, a),
                      "experts_route");
     }
-    auto kern = pick ? k_route_order<true> : k_route_order<false>;
+    auto kern = !pick ? k_route_order<0> : v == 1 ? k_route_order<1> : v == 2 ? k_route_order<2>
+                : v == 4 ? k_route_order<4> : k_route_order<8>;
     if (smem > 48 * 1024 - 256)
         scope.launch(cudaFuncSetAttribute(reinterpret_cast<const void *>(kern),
                                           cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem),
@@ -352,10 +403,10 @@ int rabbit_cuda_experts_combine_dev(int dtype, const void *d_y, int64_t y_stride
                                     int64_t base_stride, void *d_out, int64_t out_stride,
                                     void *stream) {
     const int ys = dtype_size(dtype), os = dtype_size(out_dtype);
-    if (!ys || !os || y_rows < 0 || n_tokens < 0 || k < 1 || k > kRouteK || n_cols < 1 || n_cols > 1 << 20)
+    if (!ys || !os || y_rows < 0 || n_tokens < 0 || n_tokens >= 1 << 23 || k < 1 || k > kRouteK || n_cols < 1 || n_cols > 1 << 20)
         return fail(RABBIT_CUDA_ERR_ARGS,
-                    "experts_combine: unknown dtype, a negative count, k not in 1..%d or n_cols not in "
-                    "1..2^20", kRouteK);
+                    "experts_combine: unknown dtype, a negative count, 2^23 tokens or more, k not in 1..%d or "
+                    "n_cols not in 1..2^20", kRouteK);
     if (n_tokens == 0) return ok();
     if (!d_y || !d_place || !d_weights || !d_out)
         return fail(RABBIT_CUDA_ERR_ARGS, "experts_combine: NULL pointer");
@@ -382,13 +433,12 @@ int rabbit_cuda_experts_combine_dev(int dtype, const void *d_y, int64_t y_stride
                     "aligned to its element");
     const bool vec = (y & 15) == 0 && (o & 15) == 0 && a.ys * ys % 16 == 0 && a.os * os % 16 == 0 &&
                      (!d_base || a.bs * os % 16 == 0) && n_cols % 8 == 0;
-    int sms = 0;
+    a.shift = 0;  // up to a CTA's threads to a token
+    while (a.shift < 8 && (1 << a.shift) * (vec ? 8 : 1) < n_cols) ++a.shift;
+    const int64_t threads = (int64_t)n_tokens << a.shift;  // below 2^31
     DeviceScope scope(current_device());
-    if (scope.status == RABBIT_CUDA_OK)
-        scope.launch(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, current_device()), "experts_combine: SM count");
     if (scope.status != RABBIT_CUDA_OK) return scope.status;
-    const int64_t ctas = ((int64_t)n_tokens * (n_cols / (vec ? 8 : 1)) + kCombineThreads - 1) / kCombineThreads;
-    const dim3 grid((unsigned)(ctas < 64 * sms ? ctas : 64 * sms));
+    const dim3 grid((unsigned)((threads + kCombineThreads - 1) / kCombineThreads));
     with_dtype(dtype, [&](auto yt) {
         return with_dtype(out_dtype, [&](auto ot) {
             using Y = decltype(yt);

@@ -2,12 +2,19 @@
 // columns.
 //
 // Bound by memory: x is read and its codes are written once. The codes are those of the
-// exact quotient x / s without a division for each value: with r within 2^-22 of 1 / s,
-//   |x| r (1 - 2^-21) <= |x| / s <= |x| r (1 + 2^-21)
-// holds for the computed products (they round by 2^-24 each), rounding to
-// e4m3 is monotone, so where both ends give one code it is the quotient's. Where they give two
-// neighbours, the sign of x - m s, m the middle between them, decides; one fma has it exactly.
-// 16384 rows of 4096 bf16: see the launch below.
+// exact quotient x / s, without a division for each value, from r within 2^-22 of 1 / s:
+//  * fp32: |x| r (1 - 2^-21) <= |x| / s <= |x| r (1 + 2^-21) holds for the computed products
+//    (they round by 2^-24 each). Rounding to e4m3 is monotone, so where both ends give one
+//    code it is the quotient's. Where they give two neighbours, the sign of x - m s, m the middle
+//    between them, decides; one fma has it exactly.
+//  * 16 bits: x, the block's largest value t and a middle m have at most 11, 11 and 5
+//    bits, so 448 x / t and m are 2^-16 apart or equal; x / s differs from 448 x / t by s's rounding
+//    alone. So x / s is on the side of m on which 448 x / t is or, where that equals m (such x are
+//    not rare: x = 3/4 t is one), on the side that the sign of t - 448 s tells, one for the
+//    block: the product with r (1 +- 2^-20) has the quotient's code. With 448 s = t the quotient itself is
+//    made exact by a correction, and a tie goes to the even code.
+// Each rounding and tie is equal to the 64-bit oracle's. 16384 rows of 4096 bf16 took 124 us with the ends
+// of the interval and a call for each value between them.
 #include <cuda_fp8.h>
 
 #include "rb_device.cuh"
@@ -30,7 +37,7 @@ struct F8Args {
     int shift;
 };
 
-constexpr int kF8Threads = 256;
+constexpr int kF8Threads = 256, kF8Resident = 4;  // CTAs of an SM
 constexpr uint32_t kInfBits = 0x7F800000u;
 
 // e4m3 codes of two values, to nearest even, held at +-448 (a in the low byte).
@@ -43,59 +50,91 @@ __device__ __forceinline__ float e4m3_value(uint32_t code) {
 
 // A block's scale from the bits of its largest |x|, and what its codes are made with.
 struct F8Scale {
-    float s, lo, hi;
-    bool zero, bad, tiny;
+    float s, r, lo, hi;  // s, near 1 / s; fp32: the interval's ends; 16 bits: lo, towards the block's side
+    bool even;           // 448 s is the block's largest value
+    bool rare;           // s is zero, NaN, or below kF8Tiny
 };
 constexpr float kF8Tiny = 0x1p-60f, kF8Grow = 0x1p64f;
+template <bool SHORT>
 __device__ __forceinline__ F8Scale f8_scale(uint32_t top) {
     F8Scale f;
-    f.bad = top >= kInfBits;
     // top / 448 to nearest: a product and one correction (equal to the division for every
     // mantissa while nothing falls below fp32's normal numbers)
     const float t = __uint_as_float(top), q = t * (1.f / 448.f);
     f.s = fmaf(fmaf(-q, 448.f, t), 1.f / 448.f, q);
-    if (t < 0x1p-100f) f.s = __fdiv_rn(t, 448.f);
-    if (f.bad) f.s = __uint_as_float(0x7FC00000u);
-    f.zero = f.s == 0.f;
-    // below 2^-60 x and s are multiplied by 2^64, where 1 / s and the remainders are far from
-    // fp32's smallest numbers
-    f.tiny = f.s < kF8Tiny;
-    const float r = __fdividef(1.f, f.tiny ? f.s * kF8Grow : f.s);
-    f.lo = r * (1.f - 0x1p-21f);
-    f.hi = r * (1.f + 0x1p-21f);
+    f.rare = !(f.s >= kF8Tiny) || top >= kInfBits;
+    f.r = __fdividef(1.f, f.s);
+    if constexpr (SHORT) {
+        const float rest = fmaf(-f.s, 448.f, t);
+        f.even = rest == 0.f;
+        f.lo = f.r * (rest > 0.f ? 1.f + 0x1p-20f : 1.f - 0x1p-20f);
+    } else {
+        f.lo = f.r * (1.f - 0x1p-21f);
+        f.hi = f.r * (1.f + 0x1p-21f);
+    }
+    if (f.rare) f.s = top >= kInfBits ? __uint_as_float(0x7FC00000u) : __fdiv_rn(t, 448.f);
     return f;
 }
 
-// Codes of eight values, the first in the low byte.
-__device__ __forceinline__ uint2 f8_codes(float (&x)[8], const F8Scale &f) {
-    if (f.bad | f.zero) return f.bad ? make_uint2(0x7F7F7F7Fu, 0x7F7F7F7Fu) : make_uint2(0u, 0u);
-    float s = f.s;
-    if (f.tiny) {
+// Code of v where the ends of its quotient's interval give c and c + 1.
+__device__ __forceinline__ uint32_t f8_between(float v, float s, uint32_t c) {
+    const float m = 0.5f * (fabsf(e4m3_value(c)) + fabsf(e4m3_value(c + 1)));
+    const float r = fmaf(-m, s, fabsf(v));
+    return r > 0.f || (r == 0.f && (c & 1)) ? c + 1 : c;
+}
+// Codes of a block without a number (NaN), of zeros, or with a scale below kF8Tiny: x and s are
+// multiplied by 2^64, where 1 / s and the remainders are far from fp32's smallest numbers.
+__device__ __noinline__ uint32_t f8_rare(float v, float s) {
+    if (!(s > 0.f)) return s == 0.f ? 0u : 0x7Fu;
+    s *= kF8Grow;
+    v *= kF8Grow;
+    const float r = __fdividef(1.f, s);
+    const uint32_t ab = e4m3x2(v * (r * (1.f - 0x1p-21f)), v * (r * (1.f + 0x1p-21f)));
+    const uint32_t a = ab & 255, b = ab >> 8 & 255;
+    return a == b ? a : f8_between(v, s, a);
+}
+
+// Codes of eight values, the first in the low byte. SHORT: they have at most 11 significant
+// bits.
+template <bool SHORT>
+__device__ __forceinline__ uint2 f8_codes(const float (&x)[8], const F8Scale &f) {
+    uint32_t a[2];
+    if constexpr (SHORT) {
+        float t[8];
+        if (f.even) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] *= kF8Grow;
-        s *= kF8Grow;
+            for (int i = 0; i < 8; ++i) {
+                t[i] = x[i] * f.r;
+                t[i] = fmaf(-fmaf(t[i], f.s, -x[i]), f.r, t[i]);  // (a zero keeps its sign)
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) t[i] = x[i] * f.lo;
+        }
+        a[0] = e4m3x2(t[0], t[1]) | e4m3x2(t[2], t[3]) << 16;
+        a[1] = e4m3x2(t[4], t[5]) | e4m3x2(t[6], t[7]) << 16;
+        return make_uint2(a[0], a[1]);
     }
-    uint32_t a[2], b[2];
+    uint32_t m[2];  // 1 in the bytes whose upper end has the next code
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
         const float *v = x + 4 * i;
         a[i] = e4m3x2(v[0] * f.lo, v[1] * f.lo) | e4m3x2(v[2] * f.lo, v[3] * f.lo) << 16;
-        b[i] = e4m3x2(v[0] * f.hi, v[1] * f.hi) | e4m3x2(v[2] * f.hi, v[3] * f.hi) << 16;
+        m[i] = (e4m3x2(v[0] * f.hi, v[1] * f.hi) | e4m3x2(v[2] * f.hi, v[3] * f.hi) << 16) - a[i];
     }
-    // one at a time: of 16-bit values, whose quotients are often ties, a lane has one or two
-    uint64_t d = (uint64_t)(a[1] ^ b[1]) << 32 | (a[0] ^ b[0]);
-    while (d) {
-        const int i = (__ffsll((long long)d) - 1) >> 3, sh = 8 * (i & 3);
-        d &= ~(0xFFull << (8 * i));
-        float v = x[0];
+    if (m[0] | m[1]) {
+#pragma unroll 1
+        for (int i = 0; i < 8; ++i) {
+            const int sh = 8 * (i & 3);
+            if (((i < 4 ? m[0] : m[1]) >> sh & 1) == 0) continue;
+            float v = x[0];
 #pragma unroll
-        for (int j = 1; j < 8; ++j) v = i == j ? x[j] : v;
-        const uint32_t word = i < 4 ? a[0] : a[1], c = word >> sh & 255;  // below m; above it c + 1
-        const float m = 0.5f * (fabsf(e4m3_value(c)) + fabsf(e4m3_value(c + 1)));
-        const float r = fmaf(-m, s, fabsf(v));
-        const uint32_t up = (r > 0.f || (r == 0.f && (c & 1))) ? 1u << sh : 0u;
-        if (i < 4) a[0] += up;
-        else a[1] += up;
+            for (int j = 1; j < 8; ++j) v = i == j ? x[j] : v;
+            const uint32_t c = (i < 4 ? a[0] : a[1]) >> sh & 255;
+            const uint32_t up = (f8_between(v, f.s, c) - c) << sh;
+            if (i < 4) a[0] += up;
+            else a[1] += up;
+        }
     }
     return make_uint2(a[0], a[1]);
 }
@@ -106,15 +145,15 @@ struct F8Raw {
     uint4 w[sizeof(T) / 2];
 };
 template <typename T, bool VEC>
-__device__ __forceinline__ F8Raw<T> f8_load(const T *row, int c, int n_cols) {
+__device__ __forceinline__ F8Raw<T> f8_load(const T *at, int left) {  // `left` columns from there on
     F8Raw<T> d;
-    if (VEC && c + 8 <= n_cols) {
+    if (VEC && left >= 8) {
 #pragma unroll
-        for (int i = 0; i < (int)sizeof(T) / 2; ++i) d.w[i] = reinterpret_cast<const uint4 *>(row + c)[i];
+        for (int i = 0; i < (int)sizeof(T) / 2; ++i) d.w[i] = reinterpret_cast<const uint4 *>(at)[i];
     } else {
         T *e = reinterpret_cast<T *>(&d);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) e[i] = c + i < n_cols ? row[c + i] : from_f32<T>(0.f);
+        for (int i = 0; i < 8; ++i) e[i] = i < left ? at[i] : from_f32<T>(0.f);
     }
     return d;
 }
@@ -150,64 +189,71 @@ __device__ __forceinline__ uint32_t f8_top_f32(uint32_t top) {
         return top;
     }
 }
-template <bool VEC>
-__device__ __forceinline__ void f8_store(uint8_t *row, int c, int n_cols, uint2 w) {
-    if (VEC && c + 8 <= n_cols) {
-        *reinterpret_cast<uint2 *>(row + c) = w;
+// The codes of eight values to q, `left` columns from there on.
+template <typename T, bool VEC>
+__device__ __forceinline__ void f8_store(uint8_t *q, int left, const F8Raw<T> &d, const F8Scale &f) {
+    float v[8];
+    f8_values(d, v);
+    if (!f.rare) {
+        const uint2 w = f8_codes<sizeof(T) == 2>(v, f);
+        if (VEC && left >= 8) {
+            *reinterpret_cast<uint2 *>(q) = w;
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (i < left) q[i] = (uint8_t)((i < 4 ? w.x : w.y) >> (8 * (i & 3)));
+        }
     } else {
 #pragma unroll
         for (int i = 0; i < 8; ++i)
-            if (c + i < n_cols) row[c + i] = (uint8_t)((i < 4 ? w.x : w.y) >> (8 * (i & 3)));
+            if (i < left) q[i] = (uint8_t)f8_rare(v[i], f.s);
     }
 }
 
 // One scale for each row's block: eight lanes hold a block, a lane columns 8 l .. and
 // 64 + 8 l .. of it; BATCH blocks of each eight lanes are in flight.
 template <typename T, bool VEC>
-__global__ void __launch_bounds__(kF8Threads) k_f8_rows(const __grid_constant__ F8Args a) {
+__global__ void __launch_bounds__(kF8Threads, kF8Resident) k_f8_rows(const __grid_constant__ F8Args a) {
     constexpr int BATCH = 2;
     launch_dependents();
     wait_prerequisite();
-    const int64_t items = (int64_t)a.n_rows * a.nb;
+    const uint32_t items = (uint32_t)a.n_rows * a.nb, teams = gridDim.x * (kF8Threads / 8);
     const int lane = threadIdx.x & 7;
-    const int64_t teams = (int64_t)gridDim.x * (kF8Threads / 8);
-    for (int64_t i0 = ((int64_t)blockIdx.x * kF8Threads + threadIdx.x) / 32 * 4; i0 < items;
-         i0 += teams * BATCH) {
+    for (uint32_t i0 = (blockIdx.x * kF8Threads + threadIdx.x) / 32 * 4; i0 < items; i0 += teams * BATCH) {
         F8Raw<T> d[BATCH][2];
-        int64_t at[BATCH];
-        int block[BATCH];
+        int row[BATCH], block[BATCH];
 #pragma unroll
         for (int b = 0; b < BATCH; ++b) {  // a warp's four blocks side by side, then `teams` on
-            const int64_t i = i0 + (threadIdx.x >> 3 & 3) + b * teams;
-            at[b] = -1;
+            const uint32_t i = i0 + (threadIdx.x >> 3 & 3) + b * teams;
+            row[b] = -1;
             if (i < items) {
-                const int64_t r = items >> 31 ? i / a.nb : a.nb == 1 ? i : __umulhi((uint32_t)i, a.magic) >> a.shift;
-                block[b] = (int)(i - r * a.nb);
-                const int64_t src = a.rows ? __ldg(a.rows + r) : r;
-                if (!a.rows || (src >= 0 && src < a.x_rows)) {
-                    at[b] = r;
-                    const T *row = static_cast<const T *>(a.x) + src * a.xs;
-#pragma unroll
-                    for (int h = 0; h < 2; ++h)
-                        d[b][h] = f8_load<T, VEC>(row, block[b] * 128 + h * 64 + lane * 8, a.n_cols);
+                int r = a.nb == 1 ? i : __umulhi(i, a.magic) >> a.shift;
+                block[b] = i - r * a.nb;
+                row[b] = r;
+                if (a.rows) {
+                    r = __ldg(a.rows + r);
+                    if (r < 0 || r >= a.x_rows) row[b] = -1;
+                }
+                if (row[b] >= 0) {
+                    const int c = block[b] * 128 + lane * 8;
+                    const T *x = static_cast<const T *>(a.x) + r * a.xs + c;
+                    d[b][0] = f8_load<T, VEC>(x, a.n_cols - c);
+                    d[b][1] = f8_load<T, VEC>(x + 64, a.n_cols - c - 64);
                 }
             }
         }
 #pragma unroll
         for (int b = 0; b < BATCH; ++b) {
-            uint32_t top = at[b] >= 0 ? max(f8_top(d[b][0]), f8_top(d[b][1])) : 0u;
+            uint32_t top = row[b] >= 0 ? max(f8_top(d[b][0]), f8_top(d[b][1])) : 0u;
 #pragma unroll
             for (int m = 4; m; m >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, m));
-            if (at[b] < 0) continue;
-            const F8Scale f = f8_scale(f8_top_f32<T>(top));
-            uint8_t *q = a.q + at[b] * a.qs;
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                float v[8];
-                f8_values(d[b][h], v);
-                f8_store<VEC>(q, block[b] * 128 + h * 64 + lane * 8, a.n_cols, f8_codes(v, f));
-            }
-            if (lane == 0) a.scale[at[b] * a.nb + block[b]] = f.s;
+            if (row[b] < 0) continue;
+            const F8Scale f = f8_scale<sizeof(T) == 2>(f8_top_f32<T>(top));
+            const int c = block[b] * 128 + lane * 8;
+            uint8_t *q = a.q + row[b] * a.qs + c;
+            f8_store<T, VEC>(q, a.n_cols - c, d[b][0], f);
+            f8_store<T, VEC>(q + 64, a.n_cols - c - 64, d[b][1], f);
+            if (lane == 0) a.scale[(int64_t)row[b] * a.nb + block[b]] = f.s;
         }
     }
 }
@@ -225,7 +271,7 @@ __global__ void __launch_bounds__(kF8Threads) k_f8_blocks(const __grid_constant_
     for (int i = 0; i < 8; ++i) {
         const int r = r0 + (threadIdx.x >> 4) + 16 * i;
         if (r < a.n_rows) {
-            d[i] = f8_load<T, VEC>(static_cast<const T *>(a.x) + r * a.xs, c, a.n_cols);
+            d[i] = f8_load<T, VEC>(static_cast<const T *>(a.x) + r * a.xs + c, a.n_cols - c);
             top = max(top, f8_top(d[i]));
         }
     }
@@ -234,14 +280,12 @@ __global__ void __launch_bounds__(kF8Threads) k_f8_blocks(const __grid_constant_
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < kF8Threads / 32; ++i) top = max(top, warp_top[i]);
-    const F8Scale f = f8_scale(f8_top_f32<T>(top));
+    const F8Scale f = f8_scale<sizeof(T) == 2>(f8_top_f32<T>(top));
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
         const int r = r0 + (threadIdx.x >> 4) + 16 * i;
         if (r >= a.n_rows) break;
-        float v[8];
-        f8_values(d[i], v);
-        f8_store<VEC>(a.q + r * a.qs, c, a.n_cols, f8_codes(v, f));
+        f8_store<T, VEC>(a.q + r * a.qs + c, a.n_cols - c, d[i], f);
     }
     if (threadIdx.x == 0) a.scale[(int64_t)blockIdx.x * a.nb + blockIdx.y] = f.s;
 }
@@ -274,6 +318,8 @@ extern "C" int rabbit_cuda_f8_quantise_dev(int dtype, const void *d_x, int64_t x
     a.n_rows = n_rows;
     a.n_cols = n_cols;
     a.nb = (n_cols + 127) / 128;
+    if ((int64_t)n_rows * a.nb >= (int64_t)1 << 31)
+        return fail(RABBIT_CUDA_ERR_ARGS, "f8_quantise: 2^31 blocks or more");
     const uintptr_t x = reinterpret_cast<uintptr_t>(d_x), q = reinterpret_cast<uintptr_t>(d_q);
     if (a.xs < n_cols || a.qs < n_cols || (x & (size - 1)) ||
         (reinterpret_cast<uintptr_t>(d_scale) & 3) || (reinterpret_cast<uintptr_t>(d_rows) & 3))
@@ -285,14 +331,13 @@ extern "C" int rabbit_cuda_f8_quantise_dev(int dtype, const void *d_x, int64_t x
     a.magic = a.nb == 1 ? 0 : (uint32_t)((((uint64_t)1 << (31 + l)) + a.nb - 1) / a.nb);
     a.shift = l - 1;
     const bool vec = (x & 15) == 0 && a.xs * size % 16 == 0 && (q & 7) == 0 && a.qs % 8 == 0;
-    int sms = 0;
+    const int sms = device_sms();
+    if (!sms) return fail(RABBIT_CUDA_ERR_DEVICE, "f8_quantise: no device %d", current_device());
     DeviceScope scope(current_device());
-    if (scope.status == RABBIT_CUDA_OK)
-        scope.launch(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, current_device()), "f8_quantise: SM count");
     if (scope.status != RABBIT_CUDA_OK) return scope.status;
     // Rows: blocks are handed out warp by warp, in one wave of the SMs at most.
     const int64_t ctas = ((int64_t)n_rows * a.nb + kF8Threads / 8 - 1) / (kF8Threads / 8);
-    const dim3 grid = block_rows == 1 ? dim3((unsigned)(ctas < 8 * sms ? ctas : 8 * sms))
+    const dim3 grid = block_rows == 1 ? dim3((unsigned)(ctas < kF8Resident * sms ? ctas : kF8Resident * sms))
                                       : dim3((n_rows + 127) / 128, a.nb);
     with_dtype(dtype, [&](auto t) {
         using T = decltype(t);

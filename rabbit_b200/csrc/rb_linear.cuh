@@ -420,28 +420,29 @@ __global__ void __launch_bounds__(kLinThreads, 1)
     if (warp < 4) {
         if constexpr (MODE != kLinWhole) asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
     if (warp == 0) {  // ------------------------------------------------ TMA
-        if (elect_one()) {
-            const uint64_t keep = policy_evict_last(), once = policy_evict_first();
-            LinRing st;
-            int issued = 0;
-            bool ok = true;
-            for (int i = first; ok && lin_tile(a, off, pre, i, t); i += stride) {
-                const int n0 = (PAIR ? 2 * t.mt + rank : t.mt) * outputs;
-                const int here = PAIR ? t.cols / 2 : t.cols;  // token rows of this CTA
-                const int boxes = a.rows ? 0 : (here + a.box - 1) / a.box;
-                const int quads = !PAIR && a.rows && !a.gather ? t.cols / 4 : 0;
-                const uint32_t bytes = (PAIR ? 2 : 1) * (kLinTile + boxes * a.box * 128) + quads * 512;
-                if (!PAIR)
-                    for (int c = 0; c < 4 * quads; ++c) {
-                        int r = c < t.n ? __ldg(a.rows + t.row0 + c) : 0;
-                        if (r < 0 || r >= a.x_rows) {
-                            atomicOr(a.err, RB_LIN_ERR_ROWS);
-                            r = 0;  // read for nothing: lin_written leaves the row out
-                        }
-                        reinterpret_cast<int *>(s.src)[c] = r;
-                    }
-                // weights that no other tile of tokens reads leave the L2 first
-                const uint64_t pol = pre[t.e + 1] - pre[t.e] > 1 ? keep : once;
+        const uint64_t keep = policy_evict_last(), once = policy_evict_first();
+        LinRing st;
+        int issued = 0;
+        bool ok = true;
+        const bool chosen = elect_one();
+        for (int i = first; ok && lin_tile(a, off, pre, i, t); i += stride) {
+            const int n0 = (PAIR ? 2 * t.mt + rank : t.mt) * outputs;
+            const int here = PAIR ? t.cols / 2 : t.cols;  // token rows of this CTA
+            const int boxes = a.rows ? 0 : (here + a.box - 1) / a.box;
+            const int quads = !PAIR && a.rows && !a.gather ? t.cols / 4 : 0;
+            const uint32_t bytes = (PAIR ? 2 : 1) * (kLinTile + boxes * a.box * 128) + quads * 512;
+            if (lane < 4 * quads) {
+                int r = lane < t.n ? __ldg(a.rows + t.row0 + lane) : 0;
+                if (r < 0 || r >= a.x_rows) {
+                    atomicOr(a.err, RB_LIN_ERR_ROWS);
+                    r = 0;  // read for nothing: lin_written leaves the row out
+                }
+                reinterpret_cast<int *>(s.src)[lane] = r;
+            }
+            __syncwarp();
+            // weights that no other tile of tokens reads leave the L2 first
+            const uint64_t pol = pre[t.e + 1] - pre[t.e] > 1 ? keep : once;
+            if (chosen) {
                 for (int k = k0; k < k1; ++k, ++issued) {
                     if (!(ok = lin_wait1(&s.empty[st.at], st.phase ^ 1, a, abort))) break;
                     uint8_t *base = ring + (size_t)st.at * stage_bytes, *xb = base + kLinTile;
@@ -452,8 +453,7 @@ __global__ void __launch_bounds__(kLinThreads, 1)
                         tma_load_4d_pair(base, &mw, c0, n0, 0, t.e, bar, pol);
                         if (GATED) tma_load_4d_pair(base + kLinTile / 2, &mw, c0, n0, 1, t.e, bar, pol);
                         for (int b = 0; b < boxes; ++b)
-                            tma_load_2d_pair(xb + b * a.box * 128, &mx, c0,
-                                             t.row0 + rank * here + b * a.box, bar);
+                            tma_load_2d_pair(xb + b * a.box * 128, &mx, c0, t.row0 + rank * here + b * a.box, bar);
                     } else {
                         tma_load_4d(base, &mw, c0, n0, 0, t.e, &s.full[st.at], pol);
                         if (GATED) tma_load_4d(base + kLinTile / 2, &mw, c0, n0, 1, t.e, &s.full[st.at], pol);
@@ -467,12 +467,13 @@ __global__ void __launch_bounds__(kLinThreads, 1)
                     st.next(a.stages);
                 }
             }
-            // copies under way (the pair's complete on the leader's barriers) end before
-            // the block does
-            if (!ok && leader)
-                for (int j = max(0, issued - a.stages); j < issued; ++j)
-                    mbar_wait(&s.full[j % a.stages], (j / a.stages) & 1, a.wait_ns, nullptr, 0);
+            ok = __all_sync(0xffffffffu, ok);
         }
+        // copies under way (the pair's complete on the leader's barriers) end before
+        // the block does
+        if (chosen && !ok && leader)
+            for (int j = max(0, issued - a.stages); j < issued; ++j)
+                mbar_wait(&s.full[j % a.stages], (j / a.stages) & 1, a.wait_ns, nullptr, 0);
         __syncwarp();
     } else if (warp == 1) {  // ------------------------------------------ MMA
         if (leader && elect_one()) {

@@ -37,6 +37,15 @@ int cuda_fail(cudaError_t e, const char *what) {
 
 int current_device() { return t_device; }
 
+int device_sms() {
+    static std::atomic<int> known[kMaxDevices];
+    const int d = t_device;
+    int n = known[d].load(std::memory_order_relaxed);
+    if (n == 0 && cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, d) == cudaSuccess)
+        known[d].store(n, std::memory_order_relaxed);
+    return n;
+}
+
 uint64_t wait_limit_ns() { return g_wait_ns.load(); }
 
 DevCtx *dev_ctx(int device, int *status) {

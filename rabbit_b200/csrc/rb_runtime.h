@@ -46,6 +46,8 @@ struct DevCtx {
 int current_device();
 // Lazily created context for `device`; nullptr + error text on failure.
 DevCtx *dev_ctx(int device, int *status);
+// SMs of the current thread's device, asked for once each; 0 without such a device.
+int device_sms();
 // Grow pinned / device scratch of ctx (caller holds ctx->mu).
 int ensure_pinned(DevCtx *c, size_t bytes);
 int ensure_dscratch(DevCtx *c, size_t bytes);
