@@ -256,8 +256,8 @@ __device__ __forceinline__ void lin_ld_done(float (&v)[16]) {
                    "+f"(v[12]), "+f"(v[13]), "+f"(v[14]), "+f"(v[15])::"memory");
 }
 
-// g / (1 + exp(-g)); the division to 2 units in the last place.
-__device__ __forceinline__ float lin_silu(float g) { return __fdividef(g, 1.f + expf(-g)); }
+// g / (1 + exp(-g)): the exponential to |g| 2^-24 + 2^-22 of itself, the division to 2^-22.
+__device__ __forceinline__ float lin_silu(float g) { return __fdividef(g, 1.f + __expf(-g)); }
 
 // Piece `seg` of 8 of a token's row of 128 sums, which `get(i)` reads four at a time, to
 // row `row` of y, whose columns from `n0` on they are.

@@ -161,33 +161,39 @@ __global__ void __launch_bounds__(kLinThreads, 1)
         constexpr int AHEAD = 4;  // steps whose scales are on their way
         LinRing db;
         bool ok = true;
-        for (int i = first; ok && lin_tile(a, off, pre, i, t); i += stride) {
-            const int c = rank * 128 + mine;  // token of the tile
+        const float *xs, *w0, *w1;  // scales of this thread's token and of columns 0..127, 128..255
+        float sx[AHEAD], s0[AHEAD], s1[AHEAD];
+        auto fetch = [&](int k, int j) {
+            if (k >= a.steps) return;
+            sx[j] = __ldg(xs + k);
+            s0[j] = __ldg(w0 + k);
+            s1[j] = __ldg(w1 + k);
+        };
+        auto begin = [&](const LinTile &t) {  // a tile's scales and the first of them
+            const int c = rank * 128 + mine;
             int r = t.row0 + c;
             if (c < t.n && a.rows) {
                 r = __ldg(a.rows + r);
                 if (r >= a.x_rows) r = -1;
             }
             if (c >= t.n) r = -1;
-            const float *xs = a.xs + (uint64_t)max(r, 0) * a.xs_stride;
-            // scale blocks of columns 0..127 and 128..255
+            xs = a.xs + (uint64_t)max(r, 0) * a.xs_stride;
             const int b0 = GATED ? t.mt : 2 * t.mt, b1 = GATED ? nb + t.mt : min(2 * t.mt + 1, nb - 1);
-            const float *w0 = a.ws + ((int64_t)t.e * (1 + GATED) * nb + b0) * a.steps;
-            const float *w1 = w0 + (int64_t)(b1 - b0) * a.steps;
-            float sx[AHEAD], s0[AHEAD], s1[AHEAD];
-            auto fetch = [&](int k, int j) {
-                if (k >= a.steps) return;
-                sx[j] = __ldg(xs + k);
-                s0[j] = __ldg(w0 + k);
-                s1[j] = __ldg(w1 + k);
-            };
+            w0 = a.ws + ((int64_t)t.e * (1 + GATED) * nb + b0) * a.steps;
+            w1 = w0 + (int64_t)(b1 - b0) * a.steps;
+#pragma unroll
+            for (int j = 0; j < AHEAD; ++j) fetch(j, j);
+        };
+        LinTile next;
+        bool more = lin_tile(a, off, pre, first, next);
+        if (more) begin(next);
+        for (int i = first; ok && more; i += stride) {
+            t = next;
             float acc[8][16];  // block 2 j + h
 #pragma unroll
             for (int j = 0; j < 8; ++j)
 #pragma unroll
                 for (int l = 0; l < 16; ++l) acc[j][l] = 0.f;
-#pragma unroll
-            for (int j = 0; j < AHEAD; ++j) fetch(j, j);
             for (int k = 0; ok && k < a.steps; k += AHEAD) {
 #pragma unroll
                 for (int p = 0; p < AHEAD; ++p) {
@@ -216,6 +222,9 @@ __global__ void __launch_bounds__(kLinThreads, 1)
                     }
                 }
             }
+            // the next tile's first scales come while this one's outputs leave
+            more = lin_tile(a, off, pre, i + stride, next);
+            if (more) begin(next);
             // (a wait that ran out ends it for every warp of the block before a barrier among them)
             ok = named_all(1, kLinReaders, ok);
             if (!ok) break;
