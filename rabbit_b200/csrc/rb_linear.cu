@@ -3,6 +3,7 @@
 #include <cuda.h>
 #include <cudaTypedefs.h>
 
+#include <atomic>
 #include <new>
 
 #include "rb_launch.h"
@@ -57,9 +58,12 @@ static LinKernel lin_kernel(int mode, bool pair, bool gated, int out_dtype) {
     return pair ? lin_kernel_of<kLinWhole, true>(gated, out_dtype) : lin_kernel_of<kLinWhole, false>(gated, out_dtype);
 }
 
-// The current device's kernels for an object: their shared memory; `fits`: those that share
-// out registers were built to be launched with the 128 a thread that the shares add up to.
-static cudaError_t lin_prepare_kernels(bool f8, bool gated, bool *fits) {
+// The current device's kernels for an object, once: their shared memory; `fits`: those that
+// share out registers were built to be launched with the 128 a thread that the shares add up to.
+static cudaError_t lin_prepare_kernels(int device, bool f8, bool gated, bool *fits) {
+    static std::atomic<bool> done[kMaxDevices][4];
+    std::atomic<bool> &mine = done[device][2 * f8 + gated];
+    if (mine.load()) return cudaSuccess;
     for (int mode = f8 ? kLinF8 : kLinWhole; mode <= (f8 ? kLinF8 : kLinParts); ++mode)
         for (int i = 0; i < 6; ++i) {
             const void *k = reinterpret_cast<const void *>(lin_kernel(mode, i & 1, gated, i >> 1));
@@ -70,6 +74,7 @@ static cudaError_t lin_prepare_kernels(bool f8, bool gated, bool *fits) {
             if (e != cudaSuccess) return e;
             if (mode != kLinWhole && at.numRegs != 128) *fits = false;
         }
+    if (*fits) mine.store(true);
     return cudaSuccess;
 }
 
@@ -195,6 +200,7 @@ static int lin_run(rabbit_cuda_linear *lin, const char *what, const void *d_x, i
     a.x_bytes = (uint32_t)(xs * size);
     a.k_bytes = d.n_in * size;
     a.vec = aligned(d_y, 16) && a.y_stride * out % 16 == 0;
+    a.pairs = aligned(d_y, 2 * out) && a.y_stride % 2 == 0;
     a.xs = d_x_scale;
     a.ws = d.d_scale;
     a.y = d_y;
@@ -278,7 +284,7 @@ int rabbit_cuda_linear_create(const rabbit_cuda_linear_desc *d, int device,
     if (e == cudaSuccess && (e = cudaMalloc(&lin->d_err, 2 * sizeof(int))) == cudaSuccess &&
         (e = cudaMemset(lin->d_err, 0, 2 * sizeof(int))) == cudaSuccess &&
         (e = cudaStreamSynchronize(nullptr)) == cudaSuccess)  // zeroed before any stream uses it
-        e = lin_prepare_kernels(d->dtype == RABBIT_CUDA_E4M3, d->gated, &fits);
+        e = lin_prepare_kernels(device, d->dtype == RABBIT_CUDA_E4M3, d->gated, &fits);
     const cuuint64_t dims[4] = {(cuuint64_t)d->n_in, (cuuint64_t)d->n_out, (cuuint64_t)1 + d->gated,
                                 (cuuint64_t)d->n_experts};
     const cuuint64_t strides[3] = {row, matrix, matrix * (1 + d->gated)};
@@ -289,8 +295,10 @@ int rabbit_cuda_linear_create(const rabbit_cuda_linear_desc *d, int device,
         cudaSetDevice(prev);
         cudaGetLastError();
         return e != cudaSuccess ? cuda_fail(e, "linear_create")
-                                : fail(RABBIT_CUDA_ERR_DEVICE,
-                                       "linear_create: the driver could not encode the weights' tensor map");
+               : !fits ? fail(RABBIT_CUDA_ERR_UNSUPPORTED,
+                              "linear_create: kernels built without 128 registers a thread")
+                       : fail(RABBIT_CUDA_ERR_DEVICE,
+                              "linear_create: the driver could not encode the weights' tensor map");
     }
     cudaSetDevice(prev);
     *out = lin;

@@ -73,7 +73,7 @@ struct LinArgs {
     void *y;
     int64_t y_stride;
     int out_dtype;
-    bool vec;             // y takes rows of 16 bytes
+    bool vec, pairs;      // y's rows take pieces of 16 bytes, of two elements
     int gated;
     int N, E, R, x_rows;
     int steps;            // of 128 bytes, over K
@@ -101,6 +101,7 @@ struct LinShared {
     uint32_t tmem;
     int abort;
     int4 src[8];  // a list's rows of x, gathered by TMA
+    uint32_t written[2][8];  // of the tile, and of the one before: a bit for each token to write
 };
 static_assert(sizeof(LinShared) % 16 == 0, "the scales behind it are read 16 bytes at a time");
 __host__ __device__ constexpr int lin_sc(int bn) { return bn < 32 ? 32 : bn; }
@@ -259,12 +260,27 @@ __device__ __forceinline__ void lin_ld_done(float (&v)[16]) {
 // g / (1 + exp(-g)): the exponential to |g| 2^-24 + 2^-22 of itself, the division to 2^-22.
 __device__ __forceinline__ float lin_silu(float g) { return __fdividef(g, 1.f + __expf(-g)); }
 
+// Two outputs of a row from column c on.
+template <typename T>
+__device__ __forceinline__ void lin_put2(const LinArgs &a, int64_t row, int c, float v0, float v1) {
+    T *y = static_cast<T *>(a.y) + row * a.y_stride + c;
+    if (a.pairs && c + 2 <= a.N) {
+        struct alignas(2 * sizeof(T)) Two {
+            T a, b;
+        };
+        *reinterpret_cast<Two *>(y) = Two{from_f32<T>(v0), from_f32<T>(v1)};
+    } else {
+        if (c < a.N) y[0] = from_f32<T>(v0);
+        if (c + 1 < a.N) y[1] = from_f32<T>(v1);
+    }
+}
 // Piece `seg` of 8 of a token's row of 128 sums, which `get(i)` reads four at a time, to
-// row `row` of y, whose columns from `n0` on they are.
-template <bool GATED, typename T, typename F>
+// row `row` of y, whose columns from `n0` on they are. FAR: reads that take long.
+template <bool GATED, bool FAR, typename T, typename F>
 __device__ __forceinline__ void lin_put(const LinArgs &a, int64_t row, int n0, int seg, F &&get) {
 #pragma unroll
     for (int p = 0; p < (GATED ? 1 : 2); ++p) {
+        if (!a.vec) break;
         const int c = (p * 8 + seg) * 8;
         const float4 l = get(c), h = get(c + 4);
         float v[8] = {l.x, l.y, l.z, l.w, h.x, h.y, h.z, h.w};
@@ -275,13 +291,25 @@ __device__ __forceinline__ void lin_put(const LinArgs &a, int64_t row, int n0, i
             for (int i = 0; i < 8; ++i) v[i] = lin_silu(v[i]) * u[i];
         }
         T *y = static_cast<T *>(a.y) + row * a.y_stride + n0 + c;
-        if (a.vec && n0 + c + 8 <= a.N) {
+        if (n0 + c + 8 <= a.N) {
             store8<true>(y, v);
         } else {
 #pragma unroll
             for (int i = 0; i < 8; ++i)
                 if (n0 + c + i < a.N) y[i] = from_f32<T>(v[i]);
         }
+    }
+    if (a.vec) return;
+    // rows that do not lie on 16 bytes: four columns at a time, the eight threads' side by side
+#pragma unroll FAR ? 4 : 1
+    for (int c = 4 * seg; c < (GATED ? 64 : 128); c += 32) {
+        float4 f = get(c);
+        if constexpr (GATED) {
+            const float4 u = get(64 + c);
+            f = make_float4(lin_silu(f.x) * u.x, lin_silu(f.y) * u.y, lin_silu(f.z) * u.z, lin_silu(f.w) * u.w);
+        }
+        lin_put2<T>(a, row, n0 + c, f.x, f.y);
+        lin_put2<T>(a, row, n0 + c + 2, f.z, f.w);
     }
 }
 // Whether token c of a tile is written.
@@ -616,6 +644,7 @@ __global__ void __launch_bounds__(kLinThreads, 1)
         float *part = reinterpret_cast<float *>(ring);
         LinRing db;
         bool ok = true;
+        uint32_t tile = 0;
         const uint32_t mfree = PAIR ? cluster_addr(&s.mfree[0], 0) : 0;
         auto release = [&]() {
             tc_fence_before();
@@ -640,8 +669,8 @@ __global__ void __launch_bounds__(kLinThreads, 1)
             for (int j = 0; j < 16; ++j) outs[(16 * h + j) * 128 + nl] = v[j];
             named_sync(1, kLinReaders);
             const int token = tid >> 3;
-            if (lin_written(a, t, 32 * b + token))
-                lin_put<GATED, OUT>(a, t.row0 + 32 * b + token, (PAIR ? 2 * t.mt + (int)rank : t.mt) * outputs, seg,
+            if (s.written[tile & 1][b] >> token & 1)
+                lin_put<GATED, false, OUT>(a, t.row0 + 32 * b + token, (PAIR ? 2 * t.mt + (int)rank : t.mt) * outputs, seg,
                         [&](int i) { return *reinterpret_cast<const float4 *>(outs + token * 128 + i); });
         };
         // A tile's sums in registers, NC blocks of 16 tokens a warp (with those of 256 tokens in
@@ -705,6 +734,9 @@ __global__ void __launch_bounds__(kLinThreads, 1)
             }
         };
         for (int i = first; ok && lin_tile(a, off, pre, i, t); i += stride) {
+            ++tile;
+            const uint32_t w = __ballot_sync(0xffffffffu, lin_written(a, t, tid));
+            if (lane == 0) s.written[tile & 1][warp - 4] = w;
             if constexpr (MODE != kLinWhole) {
                 if (t.cols <= 32) sums(LinInt<1>());
                 else if (t.cols <= 64) sums(LinInt<2>());
@@ -734,7 +766,7 @@ __global__ void __launch_bounds__(kLinThreads, 1)
                 const int item = j * a.split + rank, token = item >> 3;
                 if (token >= t.n) break;
                 if (!lin_written(a, t, token)) continue;
-                lin_put<GATED, OUT>(a, t.row0 + token, t.mt * outputs, item & 7, [&](int i) {
+                lin_put<GATED, true, OUT>(a, t.row0 + token, t.mt * outputs, item & 7, [&](int i) {
                     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
                     for (int r = 0; r < a.split; ++r) {
                         uint32_t at;

@@ -161,6 +161,7 @@ __global__ void __launch_bounds__(kLinThreads, 1)
         constexpr int AHEAD = 4;  // steps whose scales are on their way
         LinRing db;
         bool ok = true;
+        uint32_t tile = 0;
         const float *xs, *w0, *w1;  // scales of this thread's token and of columns 0..127, 128..255
         float sx[AHEAD], s0[AHEAD], s1[AHEAD];
         auto fetch = [&](int k, int j) {
@@ -177,6 +178,9 @@ __global__ void __launch_bounds__(kLinThreads, 1)
                 if (r >= a.x_rows) r = -1;
             }
             if (c >= t.n) r = -1;
+            // (the tile before the last is behind every warp, by the barrier)
+            const uint32_t w = __ballot_sync(0xffffffffu, r >= 0);
+            if (h == 0 && lane == 0) s.written[(tile + 1) & 1][q] = w;
             xs = a.xs + (uint64_t)max(r, 0) * a.xs_stride;
             const int b0 = GATED ? t.mt : 2 * t.mt, b1 = GATED ? nb + t.mt : min(2 * t.mt + 1, nb - 1);
             w0 = a.ws + ((int64_t)t.e * (1 + GATED) * nb + b0) * a.steps;
@@ -189,6 +193,7 @@ __global__ void __launch_bounds__(kLinThreads, 1)
         if (more) begin(next);
         for (int i = first; ok && more; i += stride) {
             t = next;
+            ++tile;
             float acc[8][16];  // block 2 j + h
 #pragma unroll
             for (int j = 0; j < 8; ++j)
@@ -222,12 +227,12 @@ __global__ void __launch_bounds__(kLinThreads, 1)
                     }
                 }
             }
-            // the next tile's first scales come while this one's outputs leave
-            more = lin_tile(a, off, pre, i + stride, next);
-            if (more) begin(next);
             // (a wait that ran out ends it for every warp of the block before a barrier among them)
             ok = named_all(1, kLinReaders, ok);
             if (!ok) break;
+            // the next tile's first scales come while this one's outputs leave
+            more = lin_tile(a, off, pre, i + stride, next);
+            if (more) begin(next);
             // Out in rows: W columns of the 128 tokens at a time, through shared memory
             constexpr int W = 128 / (int)sizeof(OUT), NB = W / 32;  // columns, a thread's blocks of 16
             const int n0 = t.mt * (GATED ? 128 : 256);
@@ -248,21 +253,31 @@ __global__ void __launch_bounds__(kLinThreads, 1)
                     }
                 }
                 named_sync(1, kLinReaders);
-                const int col = n0 + o * W + (tid & 7) * (16 / (int)sizeof(OUT));
+                const int col = n0 + o * W, piece = tid & 7;
                 constexpr int V = 16 / (int)sizeof(OUT);
 #pragma unroll
                 for (int p = 0; p < 4; ++p) {
                     const int tok = p * 32 + (tid >> 3);
-                    if (!lin_written(a, t, rank * 128 + tok)) continue;
-                    const uint4 v = *reinterpret_cast<const uint4 *>(outs + tok * kRowsPitch + (tid & 7) * 16);
+                    if (!(s.written[tile & 1][p] >> (tid >> 3) & 1)) continue;
+                    const uint8_t *row = outs + tok * kRowsPitch;
                     OUT *y = static_cast<OUT *>(a.y) + (int64_t)(t.row0 + rank * 128 + tok) * a.y_stride + col;
-                    if (a.vec && col + V <= a.N) {
-                        *reinterpret_cast<uint4 *>(y) = v;
-                    } else {
-                        const OUT *e = reinterpret_cast<const OUT *>(&v);
-#pragma unroll
-                        for (int l = 0; l < V; ++l)
-                            if (col + l < a.N) y[l] = e[l];
+                    if (a.vec && col + (piece + 1) * V <= a.N) {
+                        reinterpret_cast<uint4 *>(y)[piece] = reinterpret_cast<const uint4 *>(row)[piece];
+                        continue;
+                    }
+                    // rows that do not lie on 16 bytes, or the last columns: 4 bytes at a time, the
+                    // eight threads' side by side (without them: this thread's piece)
+#pragma unroll 1
+                    for (int e = 0; e < 4; ++e) {
+                        const int w = a.vec ? 4 * piece + e : 8 * e + piece, c = w * (4 / (int)sizeof(OUT));
+                        const uint32_t v = reinterpret_cast<const uint32_t *>(row)[w];
+                        if (sizeof(OUT) == 4 || (a.pairs && col + c + 2 <= a.N)) {
+                            if (col + c < a.N) *reinterpret_cast<uint32_t *>(y + c) = v;
+                        } else {
+                            const OUT *two = reinterpret_cast<const OUT *>(&v);
+                            if (col + c < a.N) y[c] = two[0];
+                            if (col + c + 1 < a.N) y[c + 1] = two[1];
+                        }
                     }
                 }
             }
