@@ -700,6 +700,9 @@ int rabbit_cuda_linear_grouped_dev(rabbit_cuda_linear *lin, const void *d_x, int
  * since the last check (RABBIT_CUDA_ERR_ARGS) or a bounded wait that gave up
  * (RABBIT_CUDA_ERR_TIMEOUT; rows of that call are not written, or wrong). */
 int rabbit_cuda_linear_check(rabbit_cuda_linear *lin, void *stream);
+/* Test hook: in the next call with `lin` the copies end one step early, so that waits in it run
+ * out; it ends with RABBIT_CUDA_ERR_TIMEOUT in the check, rows of it not written. */
+int rabbit_cuda_linear_debug_withhold(rabbit_cuda_linear *lin);
 
 /* k experts for each of n_tokens tokens, and the order by expert. With d_scores [n_tokens]
  * rows of n_experts (stride score_stride): the k largest scores, the lower id first among

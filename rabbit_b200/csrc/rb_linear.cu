@@ -17,6 +17,7 @@ struct rabbit_cuda_linear {
     PFN_cuTensorMapEncodeTiled_v12000 encode = nullptr;
     int *d_err = nullptr;  // the error word, and what a check took of it
     std::mutex taking;     // one check at a time
+    std::atomic<bool> withhold{false};  // test hook for the next call
 };
 
 namespace rb {
@@ -208,6 +209,7 @@ static int lin_run(rabbit_cuda_linear *lin, const char *what, const void *d_x, i
     a.format = d.dtype == RABBIT_CUDA_BF16;
     a.err = lin->d_err;
     a.wait_ns = wait_limit_ns();
+    a.withhold = lin->withhold.exchange(false);
     CUtensorMap mx;
     const cuuint64_t dims[2] = {(cuuint64_t)d.n_in, (cuuint64_t)x_rows};
     const cuuint64_t strides[1] = {(cuuint64_t)xs * size};
@@ -334,6 +336,12 @@ int rabbit_cuda_linear_grouped_dev(rabbit_cuda_linear *lin, const void *d_x, int
     if (!d_offsets) return fail(RABBIT_CUDA_ERR_ARGS, "linear_grouped: NULL offsets");
     return lin_run(lin, "linear_grouped", d_x, x_stride, x_rows, d_x_scale, x_scale_stride, d_rows,
                    d_offsets, out_dtype, d_y, y_stride, n_rows, stream);
+}
+
+int rabbit_cuda_linear_debug_withhold(rabbit_cuda_linear *lin) {
+    if (!lin) return fail(RABBIT_CUDA_ERR_ARGS, "linear_debug_withhold: NULL object");
+    lin->withhold.store(true);
+    return ok();
 }
 
 int rabbit_cuda_linear_check(rabbit_cuda_linear *lin, void *stream) {

@@ -88,6 +88,7 @@ struct LinArgs {
     uint32_t format;      // operand format of the instruction descriptor
     int *err;
     uint64_t wait_ns;
+    bool withhold;        // test hook: the copies end before a tile's last step
 };
 
 // Shared memory: the ring (aligned to 1024), the outputs on their way, then LinShared,
@@ -453,7 +454,7 @@ __global__ void __launch_bounds__(kLinThreads, 1)
         int issued = 0;
         bool ok = true;
         const bool chosen = elect_one();
-        for (int i = first; ok && lin_tile(a, off, pre, i, t); i += stride) {
+        for (int i = first; ok && lin_tile(a, off, pre, i, t); i += a.withhold ? 1 << 30 : stride) {
             const int n0 = (PAIR ? 2 * t.mt + rank : t.mt) * outputs;
             const int here = PAIR ? t.cols / 2 : t.cols;  // token rows of this CTA
             const int boxes = a.rows ? 0 : (here + a.box - 1) / a.box;
@@ -471,7 +472,7 @@ __global__ void __launch_bounds__(kLinThreads, 1)
             // weights that no other tile of tokens reads leave the L2 first
             const uint64_t pol = pre[t.e + 1] - pre[t.e] > 1 ? keep : once;
             if (chosen) {
-                for (int k = k0; k < k1; ++k, ++issued) {
+                for (int k = k0; k < k1 - a.withhold; ++k, ++issued) {
                     if (!(ok = lin_wait1(&s.empty[st.at], st.phase ^ 1, a, abort))) break;
                     uint8_t *base = ring + (size_t)st.at * stage_bytes, *xb = base + kLinTile;
                     const int c0 = k * (F8 ? 128 : 64);

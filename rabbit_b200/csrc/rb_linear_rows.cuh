@@ -76,10 +76,10 @@ __global__ void __launch_bounds__(kLinThreads, 1)
                 int issued = 0;
                 bool ok = true;
                 const uint32_t bytes = 2 * (kLinTile + (a.rows ? 0 : kLinTile));
-                for (int i = first; ok && lin_tile(a, off, pre, i, t); i += stride) {
+                for (int i = first; ok && lin_tile(a, off, pre, i, t); i += a.withhold ? 1 << 30 : stride) {
                     const int n0 = GATED ? t.mt * 128 : t.mt * 256 + rank * 128;
                     const int r0 = t.row0 + rank * 128;
-                    for (int k = 0; k < a.steps; ++k, ++issued) {
+                    for (int k = 0; k < a.steps - a.withhold; ++k, ++issued) {
                         if (!(ok = lin_wait1(&s.empty[st.at], st.phase ^ 1, a, abort))) break;
                         uint8_t *base = ring + (size_t)st.at * kRowsStage;
                         const uint32_t bar = cluster_addr(&s.full[st.at], 0);

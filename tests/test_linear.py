@@ -78,6 +78,7 @@ def test_null_arguments_are_refused(rc):
     assert so.rabbit_cuda_linear_dev(None, P, 0, P, 0, 0, P, 0, 1, None) == rc.ERR_ARGS
     assert so.rabbit_cuda_linear_grouped_dev(None, P, 0, 1, P, 0, None, P, 0, P, 0, 1, None) == rc.ERR_ARGS
     assert so.rabbit_cuda_linear_check(None, None) == rc.ERR_ARGS
+    assert so.rabbit_cuda_linear_debug_withhold(None) == rc.ERR_ARGS
     assert so.rabbit_cuda_linear_free(None) == rc.OK
 
 
@@ -85,7 +86,7 @@ def test_null_arguments_are_refused(rc):
     dict(dtype=3), dict(dtype=-1), dict(n_rows=-1), dict(n_cols=0), dict(n_cols=(1 << 20) + 1),
     dict(block_rows=2), dict(block_rows=0), dict(d_x=None), dict(d_q=None), dict(d_scale=None),
     dict(d_x=P + 2), dict(dtype=1, d_x=P + 1), dict(d_scale=P + 1), dict(x_stride=99), dict(q_stride=99),
-    dict(d_rows=P, x_rows=4, block_rows=128), dict(d_rows=P, x_rows=0), dict(d_rows=P + 2, x_rows=4),
+    dict(n_rows=1 << 30, n_cols=300), dict(d_rows=P, x_rows=4, block_rows=128), dict(d_rows=P, x_rows=0), dict(d_rows=P + 2, x_rows=4),
 ])
 def test_quantise_refuses(rc, kw):
     d = dict(dtype=0, d_x=P, x_stride=0, x_rows=0, d_rows=None, d_q=P, q_stride=0, d_scale=P, n_rows=4,
@@ -118,7 +119,7 @@ def test_route_refuses(rc, kw):
     dict(dtype=3), dict(out_dtype=-1), dict(y_rows=-1), dict(n_tokens=-1), dict(k=0), dict(k=33), dict(n_cols=0),
     dict(d_y=None), dict(d_place=None), dict(d_weights=None), dict(d_out=None), dict(y_stride=63),
     dict(out_stride=63), dict(base_stride=63), dict(d_y=P + 2), dict(d_out=P + 2), dict(d_place=P + 1),
-    dict(d_base=P, d_out=P, base_stride=64, out_stride=72),
+    dict(d_base=P, d_out=P, base_stride=64, out_stride=72), dict(n_tokens=1 << 23),
 ])
 def test_combine_refuses(rc, kw):
     d = dict(dtype=0, d_y=P, y_stride=0, y_rows=8, d_place=P, d_weights=P, n_tokens=4, k=2, n_cols=64,

@@ -325,6 +325,61 @@ def test_same_bits_each_time(torch, rc):
         assert all((o == outs[0]).all() for o in outs)
 
 
+@pytest.mark.parametrize("name,R,N,K,out", [
+    ("bf16", 3, 128, 64, "bf16"), ("e4m3", 5, 256, 2048, "f32"), ("f16", 2, 64, 2048, "f32"),
+    ("bf16", 700, 3000, 256, "bf16"), ("f16", 700, 3000, 512, "f32"), ("e4m3", 700, 3000, 512, "bf16"),
+])
+@pytest.mark.parametrize("listed", [False, True])
+def test_waits_that_run_out(torch, rc, name, R, N, K, out, listed):
+    """Copies that end early end the call with a status, and the next call is whole."""
+    c = Case(torch, rc, name, R, N, K)
+    off, rows = dev(torch, np.array([0, R], np.int32)), dev(torch, np.arange(R, dtype=np.int32)[::-1])
+    y, code = c.out(out, R)
+    run = lambda: c.lin.grouped_dev(c.xd.data_ptr(), R, off.data_ptr(), code, y.data_ptr(), R,  # noqa: E731
+                                    d_rows=rows.data_ptr() if listed else 0, stream=stream(torch), **c.kw)
+    rc.check(rc.lib().rabbit_cuda_set_wait_limit_ms(20))
+    try:
+        rc.check(rc.lib().rabbit_cuda_linear_debug_withhold(c.lin.handle))
+        run()
+        with pytest.raises(rc.RabbitCudaError, match="wait ran out") as e:
+            c.lin.check(stream(torch))
+        assert e.value.status == rc.ERR_TIMEOUT
+    finally:
+        rc.check(rc.lib().rabbit_cuda_set_wait_limit_ms(2000))
+    run()
+    c.lin.check(stream(torch))
+    at = np.arange(0, R, max(1, R // 40))
+    c.close(f64(y)[at], c.x[::-1][at] if listed else c.x[at], 0, out)
+
+
+@pytest.mark.parametrize("name,R,N,K,gated,out", [
+    ("bf16", 20, 40, 20000, False, "bf16"), ("f16", 300, 300, 17000, True, "f16"), ("e4m3", 130, 140, 20001, False, "f16"),
+])
+def test_long_sums(torch, rc, name, R, N, K, gated, out):
+    """More channels than a 16-bit output's sum stays in tensor memory for."""
+    c = Case(torch, rc, name, R, N, K, gated)
+    y, code = c.out(out, R)
+    c.lin.apply_dev(c.xd.data_ptr(), code, y.data_ptr(), R, stream=stream(torch), **c.kw)
+    c.lin.check(stream(torch))
+    c.close(f64(y)[:R], c.x, 0, out)
+
+
+@pytest.mark.parametrize("name,K,out", [("e4m3", 140, "bf16"), ("e4m3", 500, "f32"), ("f16", 100, "f16"), ("bf16", 300, "f32")])
+@pytest.mark.parametrize("N,gap,shift", [(301, 0, 0), (302, 0, 0), (301, 3, 1), (304, 0, 1), (304, 4, 2), (303, 5, 0)])
+@pytest.mark.parametrize("gated", [False, True])
+def test_rows_of_y_that_do_not_lie_on_16_bytes(torch, rc, name, K, out, N, gap, shift, gated):
+    for R in (3, 600):  # one CTA a tile, pairs
+        c = Case(torch, rc, name, R, N, K, gated)
+        dt, code = types(torch, rc, out)
+        flat = torch.full(((R + 1) * (N + gap) + shift,), -777.0, dtype=dt, device="cuda")
+        y = flat[shift:].view(R + 1, N + gap)
+        c.lin.apply_dev(c.xd.data_ptr(), code, y.data_ptr(), R, y_stride=N + gap, stream=stream(torch), **c.kw)
+        c.lin.check(stream(torch))
+        got = f64(y)
+        c.close(got[:R, :N], c.x, 0, out)
+        assert (got[R:] == got[-1, -1]).all() and (got[:, N:] == got[-1, -1]).all() and (flat[:shift] == flat[-1]).all()
+
+
 def test_elements_past_32_bits(torch, rc):
     """Rows of x and y so far apart that their last elements lie past 2^32."""
     R, N, K = 140, 40, 64
