@@ -650,7 +650,7 @@ int rabbit_cuda_kv4_debug_withhold(rabbit_cuda_kv4 *kv);
  * s = NaN and codes NaN. q [n_rows] rows of q_stride bytes; d_scale [n_rows or its blocks][n_cols /
  * 128 rounded up]. With d_rows (block_rows 1 only) row i is row d_rows[i] of the x_rows rows
  * of x; where that is outside of them, row i of q and of d_scale is left as it was. x_rows is
- * not read without d_rows. n_rows 0 does nothing; n_rows * blocks of columns below 2^31. On the calling
+ * not read without d_rows. q must not overlap x. n_rows 0 does nothing; n_rows * blocks of columns below 2^31. On the calling
  * thread's device. */
 int rabbit_cuda_f8_quantise_dev(int dtype, const void *d_x, int64_t x_stride, int x_rows,
                                 const int *d_rows, void *d_q, int64_t q_stride, float *d_scale,
@@ -679,10 +679,14 @@ int rabbit_cuda_linear_free(rabbit_cuda_linear *lin);
 /* y [n_rows][n_out] (f32, f16 or bf16) = x [n_rows][n_in] times the one matrix. x of the weights'
  * type, 16-byte aligned, its stride a multiple of 16 bytes. E4M3: d_x_scale, rows of x_scale_stride
  * floats, n_in / 128 rounded up of them, and
- *   y = sum_b sx[row][b] sw[n / 128][b] sum_{k in block b} x[row][k] w[n][k].
- * Sums are fp32 (a block's on the tensor cores, then over the blocks in order), rounded to
- * out_dtype once; silu in fp32. Infinities and NaN go where the formula takes them, and to
- * no other row. y must not overlap an input. n_rows 0 does nothing. */
+ *   y = sum_b (sx[row][b] sw[n / 128][b]) sum_{k in block b} x[row][k] w[n][k],
+ * the product of the scales in fp32. Sums are fp32, rounded to out_dtype once: a block's on the
+ * tensor cores, then over the blocks in order; 16-bit products' over all of n_in on the tensor
+ * cores (which cut off what fp32 cannot hold: up to 2^-25 of the sum for each 16 channels) or, for fp32 outputs
+ * and n_in above 16384, in parts of 256 channels. silu in fp32 (to |gate| 2^-24 + 2^-21 of itself).
+ * Infinities and NaN go where the formula takes them, and to
+ * no other row. y must not overlap an input. n_rows up to 2^30; 0 does nothing. Strides of x up to
+ * 2^30 elements, of its scales up to 2^30. */
 int rabbit_cuda_linear_dev(rabbit_cuda_linear *lin, const void *d_x, int64_t x_stride,
                            const float *d_x_scale, int64_t x_scale_stride, int out_dtype, void *d_y,
                            int64_t y_stride, int n_rows, void *stream);

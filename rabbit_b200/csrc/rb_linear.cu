@@ -159,8 +159,8 @@ static int lin_run(rabbit_cuda_linear *lin, const char *what, const void *d_x, i
     const rabbit_cuda_linear_desc &d = lin->d;
     const int size = operand_size(d.dtype), out = dtype_size(out_dtype);
     const bool f8 = d.dtype == RABBIT_CUDA_E4M3;
-    if (!out || n_rows < 0)
-        return fail(RABBIT_CUDA_ERR_ARGS, "%s: unknown out_dtype or a negative count", what);
+    if (!out || n_rows < 0 || n_rows > 1 << 30)
+        return fail(RABBIT_CUDA_ERR_ARGS, "%s: unknown out_dtype, or n_rows not in 0..2^30", what);
     if (n_rows == 0) return ok();
     LinArgs a = {};
     a.N = d.n_out;

@@ -86,8 +86,9 @@ def product_bar(parts, mags, steps, half, tiny):
         g, up = parts
         s = silu(g)
         y = s * up
-        # |silu'| <= 1.1; exp and the division: 8 u; the product of the two
-        err = (1.1 * e[0] + 8 * u * np.abs(s)) * (np.abs(up) + e[1]) + (np.abs(s) + 1.1 * e[0]) * e[1] + u * np.abs(y)
+        # |silu'| <= 1.1; exp (|g| u + 4 u of itself), 1 + exp (u) and the division (4 u); the
+        # product of the two
+        err = (1.1 * e[0] + (9 + np.abs(g)) * u * np.abs(s)) * (np.abs(up) + e[1]) + (np.abs(s) + 1.1 * e[0]) * e[1] + u * np.abs(y)
     return err + half * (np.abs(y) + err) + tiny
 
 

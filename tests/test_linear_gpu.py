@@ -402,7 +402,7 @@ def test_arguments_are_refused(torch, rc):
     good = [h, x, 0, 8, s, 0, None, o, 0, y, 0, 8, None]
     for i, v in [(1, None), (1, x + 8), (2, 112), (2, 130), (2, -128), (3, 7), (3, 0), (4, None), (4, s + 2),
                  (5, -1), (6, o + 1), (7, None), (7, o + 2), (8, 3), (8, -1), (9, None), (9, y + 2),
-                 (10, 63), (11, -1)]:
+                 (10, 63), (11, -1), (11, (1 << 30) + 1), (5, (1 << 30) + 1)]:
         args = list(good)
         args[i] = v
         assert so.rabbit_cuda_linear_grouped_dev(*args) == rc.ERR_ARGS, (i, v)
