@@ -11,7 +11,8 @@
 //   warp 0       TMA: the step's weight rows and, without a list, token rows into a ring of
 //                stages (128-byte rows, 128-byte swizzle);
 //   warp 1       tensor memory; one thread issues the step's MMAs and commits;
-//   warps 2, 3   (e4m3) the step's scales, sw * sx for each token, into shared memory;
+//   warps 2, 3   (e4m3) the step's scales, sw * sx for each token, into shared memory; (16-bit)
+//                one thread's fence between the proxies for gathered rows;
 //   warps 4..11  readout: warp w reads lanes 32 (w % 4) .. + 31 (weight rows), and the
 //                even or odd blocks of 16 tokens; outputs go through shared memory, so that
 //                they leave in rows of 16 bytes a thread;
@@ -95,8 +96,8 @@ struct LinArgs {
 // the scales [bufs][1 or 2][bn, at least 32], off [E + 1] and pre [E + 1].
 struct LinShared {
     uint64_t full[kLinStages], empty[kLinStages];
-    uint64_t rows[kLinStages];  // with a list: this CTA's token rows have arrived
-    uint64_t told[kLinStages];  // and the other CTA's, in the leader
+    uint64_t rows[kLinStages];  // to gather: this CTA's token rows have arrived
+    uint64_t told[kLinStages];  // and the MMAs may read them (and the other CTA's), in the leader
     uint64_t dfull[kLinBufs], dempty[kLinBufs], mfree[kLinBufs];
     uint64_t mdone;
     uint32_t tmem;
@@ -388,6 +389,23 @@ __device__ __forceinline__ bool lin_gather(const LinArgs &a, LinShared &s, uint3
     return true;
 }
 
+// One thread, of each CTA of a pair: once this CTA's rows of a step are there, the fence
+// between the proxies, and word to the thread that issues the MMAs (of CTA `to`). In that thread
+// itself the fence held up the MMAs: 8192 tokens of 8 f16 experts took 0.3 ms more.
+__device__ __forceinline__ void lin_tell(const LinArgs &a, LinShared &s, const int *off, const int *pre,
+                                         int first, int stride, int k0, int k1, uint32_t to,
+                                         volatile int *abort) {
+    LinTile t;
+    LinRing st;
+    for (int i = first; lin_tile(a, off, pre, i, t); i += stride)
+        for (int k = k0; k < k1; ++k) {
+            if (!lin_wait1(&s.rows[st.at], st.phase, a, abort)) return;
+            fence_async();
+            cluster_bar_arrive(cluster_addr(&s.told[st.at], to));
+            st.next(a.stages);
+        }
+}
+
 template <int MODE, bool PAIR, bool GATED, typename OUT>
 __global__ void __launch_bounds__(kLinThreads, 1)
     k_linear(const __grid_constant__ LinArgs a, const __grid_constant__ CUtensorMap mw,
@@ -412,7 +430,7 @@ __global__ void __launch_bounds__(kLinThreads, 1)
             mbar_init(&s.full[i], 1);
             mbar_init(&s.empty[i], 1);
             mbar_init(&s.rows[i], 128);
-            mbar_init(&s.told[i], 1);
+            mbar_init(&s.told[i], PAIR ? 2 : 1);
         }
         for (int i = 0; i < a.bufs; ++i) {
             mbar_init(&s.dfull[i], F8 ? 3 : 1);  // the MMAs, and the scales' two warps
@@ -515,9 +533,8 @@ __global__ void __launch_bounds__(kLinThreads, 1)
                 for (int k = k0; k < k1; ++k) {
                     if (!(ok = lin_wait1(&s.full[st.at], st.phase, a, abort))) break;
                     if (a.gather) {
-                        if (PAIR) ok = lin_wait1(&s.told[st.at], st.phase, a, abort);
-                        if (!ok || !(ok = lin_wait1(&s.rows[st.at], st.phase, a, abort))) break;
-                        fence_async();
+                        if (!(ok = lin_wait1(F8 ? &s.rows[st.at] : &s.told[st.at], st.phase, a, abort))) break;
+                        if (F8) fence_async();  // (no warp is free to do it)
                     }
                     const uint64_t step = (uint64_t)(st.at * stage_bytes) >> 4;
                     if (part == 0)
@@ -544,18 +561,6 @@ __global__ void __launch_bounds__(kLinThreads, 1)
                 mbar_wait(&s.mdone, 0, a.wait_ns, nullptr, 0);
             }
         }
-        if (PAIR && !leader && a.gather && elect_one()) {  // word of this CTA's rows to the leader
-            LinRing st;
-            bool ok = true;
-            for (int i = first; ok && lin_tile(a, off, pre, i, t); i += stride)
-                for (int k = k0; k < k1; ++k) {
-                    if (!(ok = lin_wait1(&s.rows[st.at], st.phase, a, abort))) break;
-                    fence_async();
-                    cluster_bar_arrive(cluster_addr(&s.told[st.at], 0));
-                    st.next(a.stages);
-                }
-        }
-        __syncwarp();
     } else if (F8) {  // ---------------------------------------------- scales
         const int nb = (a.N + 127) / 128;  // rows of scale blocks of a matrix
         const int64_t up = (int64_t)nb * a.steps;
@@ -623,6 +628,9 @@ __global__ void __launch_bounds__(kLinThreads, 1)
             if (t.cols <= 32) tile(LinInt<1>(), LinInt<GATED ? 5 : 8>());
             else tile(LinInt<4>(), LinInt<2>());
         }
+    } else if (!F8 && warp == 2 && a.gather) {  // ------- word of gathered rows
+        if (elect_one()) lin_tell(a, s, off, pre, first, stride, k0, k1, PAIR ? 0 : rank, abort);
+        __syncwarp();
     }
     } else if (warp >= 12) {  // ------------------------------------- gather
         if constexpr (MODE != kLinWhole) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");

@@ -44,7 +44,7 @@ __global__ void __launch_bounds__(kLinThreads, 1)
             mbar_init(&s.full[i], 1);
             mbar_init(&s.empty[i], 1);
             mbar_init(&s.rows[i], 128);
-            mbar_init(&s.told[i], 1);
+            mbar_init(&s.told[i], 2);
         }
         for (int i = 0; i < 2; ++i) {
             mbar_init(&s.dfull[i], 1);
@@ -108,12 +108,7 @@ __global__ void __launch_bounds__(kLinThreads, 1)
                     for (int i = first; ok && lin_tile(a, off, pre, i, t); i += stride)
                         for (int k = 0; k < a.steps; ++k) {
                             if (!(ok = lin_wait1(&s.full[st.at], st.phase, a, abort))) break;
-                            if (a.rows) {
-                                if (!(ok = lin_wait1(&s.told[st.at], st.phase, a, abort) &&
-                                           lin_wait1(&s.rows[st.at], st.phase, a, abort)))
-                                    break;
-                                fence_async();
-                            }
+                            if (a.rows && !(ok = lin_wait1(&s.told[st.at], st.phase, a, abort))) break;
                             if (!(ok = lin_wait1(&s.mfree[db.at], db.phase ^ 1, a, abort))) break;
                             tc_fence_after();
                             const uint64_t step = (uint64_t)(st.at * kRowsStage) >> 4;
@@ -131,17 +126,11 @@ __global__ void __launch_bounds__(kLinThreads, 1)
                         mbar_wait(&s.mdone, 0, a.wait_ns, nullptr, 0);
                     }
                 }
-            } else if (a.rows && elect_one()) {  // word of this CTA's rows to the leader
-                LinRing st;
-                bool ok = true;
-                for (int i = first; ok && lin_tile(a, off, pre, i, t); i += stride)
-                    for (int k = 0; k < a.steps; ++k) {
-                        if (!(ok = lin_wait1(&s.rows[st.at], st.phase, a, abort))) break;
-                        fence_async();
-                        cluster_bar_arrive(cluster_addr(&s.told[st.at], 0));
-                        st.next(a.stages);
-                    }
             }
+            __syncwarp();
+        } else if (warp == 2 && a.rows) {  // ------------- word of gathered rows
+            if (elect_one())
+                lin_tell(a, s, off, pre, first, stride, 0, a.steps, 0, abort);
             __syncwarp();
         }
     } else if (warp >= 12) {  // ------------------------------------- gather

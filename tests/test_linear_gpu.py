@@ -597,6 +597,20 @@ def test_expert_layer(torch, rc, T, H, I, E, k):
     layer.verify()
 
 
+@pytest.mark.parametrize("name", ["e4m3", "f16"])
+@pytest.mark.parametrize("R", [7, 60, 200])
+def test_listed_rows_split_over_k(torch, rc, name, R):
+    """Few tiles and many channels: a cluster for each tile, rows gathered by either way."""
+    c = Case(torch, rc, name, 50, 100, 4000)
+    rows = np.random.default_rng(R).integers(0, 50, R)
+    off, rd = dev(torch, np.array([0, R], np.int32)), dev(torch, rows.astype(np.int32))
+    y, code = c.out("bf16", R)
+    c.lin.grouped_dev(c.xd.data_ptr(), 50, off.data_ptr(), code, y.data_ptr(), R, d_rows=rd.data_ptr(),
+                      stream=stream(torch), **c.kw)
+    c.lin.check(stream(torch))
+    c.close(f64(y)[:R], c.x[rows], 0, "bf16")
+
+
 def test_expert_layers_in_graphs_and_streams(torch, rc):
     """A layer captured once and replayed with other inputs in its buffers, while another
     runs on a second stream; a second graph of the same objects."""
