@@ -258,36 +258,45 @@ struct CombineArgs {
 
 constexpr int kCombineThreads = 256;
 
-// Eight elements as they lie in memory (VEC), or one.
+// Eight elements side by side as they lie in memory (VEC), or four `step` apart, `left` elements
+// from the first on.
 template <typename T, bool VEC>
 struct Piece {
+    static constexpr int V = VEC ? 8 : 4;
     using W = typename std::conditional<VEC, uint4, T>::type;
-    W w[VEC ? sizeof(T) / 2 : 1];
-    __device__ __forceinline__ void load(const T *p) {
+    W w[VEC ? sizeof(T) / 2 : V];
+    __device__ __forceinline__ void load(const T *p, int step, int left) {
+        if constexpr (VEC) {
 #pragma unroll
-        for (int i = 0; i < (VEC ? (int)sizeof(T) / 2 : 1); ++i) w[i] = reinterpret_cast<const W *>(p)[i];
+            for (int i = 0; i < (int)sizeof(T) / 2; ++i) w[i] = reinterpret_cast<const uint4 *>(p)[i];
+        } else {
+#pragma unroll
+            for (int i = 0; i < V; ++i) w[i] = i * step < left ? p[i * step] : from_f32<T>(0.f);
+        }
     }
-    __device__ __forceinline__ void values(float (&v)[VEC ? 8 : 1]) const {
+    __device__ __forceinline__ void values(float (&v)[V]) const {
         const T *e = reinterpret_cast<const T *>(w);
 #pragma unroll
-        for (int i = 0; i < (VEC ? 8 : 1); ++i) v[i] = to_f32(e[i]);
+        for (int i = 0; i < V; ++i) v[i] = to_f32(e[i]);
     }
 };
 
 // Bound by memory: each row of y is read once. 2^shift threads have a token, a thread eight
-// columns at a time (scalar form: one).
+// columns at a time (rows that do not lie on 16 bytes: four, 2^shift apart).
 template <typename Y, typename O, bool VEC>
 __global__ void __launch_bounds__(kCombineThreads, 4) k_combine(const __grid_constant__ CombineArgs a) {
-    constexpr int V = VEC ? 8 : 1, B = 2;  // B rows of y in flight
+    constexpr int V = VEC ? 8 : 4, B = 2;  // B rows of y in flight
     launch_dependents();
     wait_prerequisite();
     const int t = (blockIdx.x * kCombineThreads + threadIdx.x) >> a.shift;
     if (t >= a.T) return;
     const int *place = a.place + (int64_t)t * a.k;
     const float *weights = a.weights + (int64_t)t * a.k;
-    for (int c = (threadIdx.x & ((1 << a.shift) - 1)) * V; c < a.cols; c += V << a.shift) {
+    const int step = 1 << a.shift;
+    for (int c = (threadIdx.x & (step - 1)) * (VEC ? V : 1); c < a.cols; c += V * step) {
+        const int left = a.cols - c;
         Piece<O, VEC> base;
-        if (a.base) base.load(static_cast<const O *>(a.base) + t * a.bs + c);
+        if (a.base) base.load(static_cast<const O *>(a.base) + t * a.bs + c, step, left);
         float acc[V], v[V];
 #pragma unroll
         for (int e = 0; e < V; ++e) acc[e] = 0.f;
@@ -301,7 +310,7 @@ __global__ void __launch_bounds__(kCombineThreads, 4) k_combine(const __grid_con
                 some[b] = p >= 0 && p < a.y_rows;
                 if (some[b]) {
                     w[b] = __ldg(weights + j0 + b);
-                    d[b].load(static_cast<const Y *>(a.y) + p * a.ys + c);
+                    d[b].load(static_cast<const Y *>(a.y) + p * a.ys + c, step, left);
                 }
             }
 #pragma unroll
@@ -318,8 +327,13 @@ __global__ void __launch_bounds__(kCombineThreads, 4) k_combine(const __grid_con
             for (int e = 0; e < V; ++e) acc[e] = v[e] + acc[e];
         }
         O *o = static_cast<O *>(a.out) + t * a.os + c;
-        if constexpr (VEC) store8<true>(o, acc);
-        else *o = from_f32<O>(acc[0]);
+        if constexpr (VEC) {
+            store8<true>(o, acc);
+        } else {
+#pragma unroll
+            for (int e = 0; e < V; ++e)
+                if (e * step < left) o[e * step] = from_f32<O>(acc[e]);
+        }
     }
 }
 
@@ -434,7 +448,7 @@ int rabbit_cuda_experts_combine_dev(int dtype, const void *d_y, int64_t y_stride
     const bool vec = (y & 15) == 0 && (o & 15) == 0 && a.ys * ys % 16 == 0 && a.os * os % 16 == 0 &&
                      (!d_base || a.bs * os % 16 == 0) && n_cols % 8 == 0;
     a.shift = 0;  // up to a CTA's threads to a token
-    while (a.shift < 8 && (1 << a.shift) * (vec ? 8 : 1) < n_cols) ++a.shift;
+    while (a.shift < 8 && (1 << a.shift) * (vec ? 8 : 4) < n_cols) ++a.shift;
     const int64_t threads = (int64_t)n_tokens << a.shift;  // below 2^31
     DeviceScope scope(current_device());
     if (scope.status != RABBIT_CUDA_OK) return scope.status;
