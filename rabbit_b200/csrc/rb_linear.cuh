@@ -351,6 +351,16 @@ __device__ __forceinline__ void lin_experts(const LinArgs &a, int *off, int *pre
     if (lane == 0) pre[0] = 0;
 }
 
+// The ring's last `issued` uses have been given back. The commits that do it arrive in both CTAs
+// of a pair, whenever the products are through; until each has arrived neither CTA may end,
+// or the arrival would go to the shared memory of another block. (The products' own commits have
+// all been waited for by the readout.)
+__device__ __forceinline__ bool lin_emptied(const LinArgs &a, LinShared &s, int issued, volatile int *abort) {
+    for (int j = max(0, issued - a.stages); j < issued; ++j)
+        if (!lin_wait1(&s.empty[j % a.stages], (j / a.stages) & 1, a, abort)) return false;
+    return true;
+}
+
 // The gathering warps' part of a tile: tokens c0 .. c0 + here - 1 of it into rows 0.. of the
 // token rows `at` bytes into each stage, ROWS of them a thread (part, part + 16, ..).
 template <int ROWS>
@@ -516,6 +526,7 @@ __global__ void __launch_bounds__(kLinThreads, 1)
             }
             ok = __all_sync(0xffffffffu, ok);
         }
+        if (chosen && ok) ok = lin_emptied(a, s, issued, abort);
         // copies under way (the pair's complete on the leader's barriers) end before
         // the block does
         if (chosen && !ok && leader)

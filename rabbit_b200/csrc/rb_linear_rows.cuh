@@ -92,6 +92,7 @@ __global__ void __launch_bounds__(kLinThreads, 1)
                         st.next(a.stages);
                     }
                 }
+                if (ok) ok = lin_emptied(a, s, issued, abort);
                 // copies under way (they complete on the leader's barriers) end before the block does
                 if (!ok && leader)
                     for (int j = max(0, issued - a.stages); j < issued; ++j)
