@@ -707,6 +707,8 @@ int rabbit_cuda_linear_check(rabbit_cuda_linear *lin, void *stream);
 /* Test hook: in the next call with `lin` the copies end one step early, so that waits in it run
  * out; it ends with RABBIT_CUDA_ERR_TIMEOUT in the check, rows of it not written. */
 int rabbit_cuda_linear_debug_withhold(rabbit_cuda_linear *lin);
+/* The same for one CTA, 0 or 1, of each pair that shares a tile, if the call has pairs (else as above). */
+int rabbit_cuda_linear_debug_withhold_cta(rabbit_cuda_linear *lin, int cta);
 
 /* k experts for each of n_tokens tokens, and the order by expert. With d_scores [n_tokens]
  * rows of n_experts (stride score_stride): the k largest scores, the lower id first among

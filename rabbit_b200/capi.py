@@ -167,6 +167,7 @@ SIGNATURES = {
     "rabbit_cuda_linear_grouped_dev": (_I, [_P, _P, _L, _I, _P, _L, _P, _P, _I, _P, _L, _I, _P]),
     "rabbit_cuda_linear_check": (_I, [_P, _P]),
     "rabbit_cuda_linear_debug_withhold": (_I, [_P]),
+    "rabbit_cuda_linear_debug_withhold_cta": (_I, [_P, _I]),
     "rabbit_cuda_experts_route_dev": (_I, [_P, _L, _I, _I, _I, _I, _P, _P, _P, _P, _P, _P]),
     "rabbit_cuda_experts_combine_dev": (_I, [_I, _P, _L, _I, _P, _P, _I, _I, _I, _I, _P, _L, _P,
                                              _L, _P]),

@@ -17,7 +17,7 @@ struct rabbit_cuda_linear {
     PFN_cuTensorMapEncodeTiled_v12000 encode = nullptr;
     int *d_err = nullptr;  // the error word, and what a check took of it
     std::mutex taking;     // one check at a time
-    std::atomic<bool> withhold{false};  // test hook for the next call
+    std::atomic<int> withhold{0};  // test hook for the next call: a bit for each CTA of a pair
 };
 
 namespace rb {
@@ -209,7 +209,8 @@ static int lin_run(rabbit_cuda_linear *lin, const char *what, const void *d_x, i
     a.format = d.dtype == RABBIT_CUDA_BF16;
     a.err = lin->d_err;
     a.wait_ns = wait_limit_ns();
-    a.withhold = lin->withhold.exchange(false);
+    a.withhold = lin->withhold.exchange(0);
+    if (!pair && a.withhold) a.withhold = 1;
     CUtensorMap mx;
     const cuuint64_t dims[2] = {(cuuint64_t)d.n_in, (cuuint64_t)x_rows};
     const cuuint64_t strides[1] = {(cuuint64_t)xs * size};
@@ -340,7 +341,14 @@ int rabbit_cuda_linear_grouped_dev(rabbit_cuda_linear *lin, const void *d_x, int
 
 int rabbit_cuda_linear_debug_withhold(rabbit_cuda_linear *lin) {
     if (!lin) return fail(RABBIT_CUDA_ERR_ARGS, "linear_debug_withhold: NULL object");
-    lin->withhold.store(true);
+    lin->withhold.store(3);
+    return ok();
+}
+
+int rabbit_cuda_linear_debug_withhold_cta(rabbit_cuda_linear *lin, int cta) {
+    if (!lin || (cta & ~1))
+        return fail(RABBIT_CUDA_ERR_ARGS, "linear_debug_withhold_cta: NULL object, or a CTA other than 0 and 1");
+    lin->withhold.store(1 << cta);
     return ok();
 }
 
@@ -359,9 +367,10 @@ int rabbit_cuda_linear_check(rabbit_cuda_linear *lin, void *stream) {
         RB_CUDA(cudaStreamSynchronize(s));
     }
     if (h == 0) return ok();
-    return fail(h & RB_LIN_ERR_WAIT ? RABBIT_CUDA_ERR_TIMEOUT : RABBIT_CUDA_ERR_ARGS, "linear: %s%s%s%s",
+    return fail(h & RB_LIN_ERR_WAIT ? RABBIT_CUDA_ERR_TIMEOUT : RABBIT_CUDA_ERR_ARGS, "linear: %s%s%s%s%s",
                 h & RB_LIN_ERR_WAIT ? "a bounded device wait ran out; " : "",
-                h & ~RB_LIN_ERR_WAIT ? "out of range on the device:" : "",
+                h & RB_LIN_ERR_OPEN ? "copies or products did not end; " : "",
+                h & (RB_LIN_ERR_OFFSETS | RB_LIN_ERR_ROWS) ? "out of range on the device:" : "",
                 h & RB_LIN_ERR_OFFSETS ? " offsets" : "", h & RB_LIN_ERR_ROWS ? " rows" : "");
 }
 

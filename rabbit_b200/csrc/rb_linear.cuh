@@ -61,6 +61,7 @@ constexpr uint32_t kLinOut = 32 * 128 * 4;  // outputs on their way: 32 tokens
 #define RB_LIN_ERR_OFFSETS 16
 #define RB_LIN_ERR_ROWS 32
 #define RB_LIN_ERR_WAIT 256
+#define RB_LIN_ERR_OPEN 512  // after it, what was under way did not end either
 
 struct LinArgs {
     const int *offsets;   // [E + 1], or NULL: one expert with all rows
@@ -89,7 +90,7 @@ struct LinArgs {
     uint32_t format;      // operand format of the instruction descriptor
     int *err;
     uint64_t wait_ns;
-    bool withhold;        // test hook: the copies end before a tile's last step
+    int withhold;         // test hook: the copies end before a tile's last step; a bit for each CTA of a pair
 };
 
 // Shared memory: the ring (aligned to 1024), the outputs on their way, then LinShared,
@@ -102,6 +103,10 @@ struct LinShared {
     uint64_t mdone;
     uint32_t tmem;
     int abort;
+    // for lin_settle: steps copied, the bytes of each stage's last by this CTA; steps and buffers
+    // committed, whether on mdone, too
+    int issued, stepped, filled, ended;
+    uint32_t bytes[kLinStages];
     int4 src[8];  // a list's rows of x, gathered by TMA
     uint32_t written[2][8];  // of the tile, and of the one before: a bit for each token to write
 };
@@ -229,6 +234,15 @@ __device__ __forceinline__ void fma2(uint64_t &acc, uint64_t v, uint64_t f) {
 }
 __device__ __forceinline__ void add2(uint64_t &acc, uint64_t v) {
     asm("add.rn.f32x2 %0, %0, %1;" : "+l"(acc) : "l"(v));
+}
+__device__ __forceinline__ int cluster_ld1(uint32_t at) {
+    int v;
+    asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(at) : "memory");
+    return v;
+}
+// Counts `bytes` of a barrier's phase as arrived.
+__device__ __forceinline__ void mbar_complete_tx(uint64_t *bar, uint32_t bytes) {
+    asm volatile("mbarrier.complete_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)), "r"(bytes) : "memory");
 }
 __device__ __forceinline__ float4 cluster_ld4(uint32_t at) {
     float4 v;
@@ -361,6 +375,41 @@ __device__ __forceinline__ bool lin_emptied(const LinArgs &a, LinShared &s, int 
     return true;
 }
 
+// At the end of a block in which a wait ran out, after the (pair's) last barrier but one: what is
+// under way ends before the tensor memory is given back and the block ends. Thread 0: the products (mdone),
+// what they were committed to in this CTA (`bufs` buffers, where nobody else arrives on those
+// barriers: there mdone is all), and the copies of both CTAs, which complete on the leader's barriers. A pair's CTAs
+// may have got to different steps, at most the ring's stages apart; a barrier's count is made up by
+// what the one behind did not copy, or did not expect. In a CTA without a wait that ran out all of
+// this has been waited for; then nothing of the other's arrives there, either.
+template <bool PAIR>
+__device__ __forceinline__ void lin_settle(const LinArgs &a, LinShared &s, int bufs) {
+    if (threadIdx.x == 0) {
+        const bool leader = !PAIR || cluster_rank() == 0;
+        auto of = [&](const int *p, uint32_t r) {  // a number of CTA r
+            return PAIR ? cluster_ld1(cluster_addr(p, r)) : *p;
+        };
+        bool closed = true;
+        auto wait = [&](uint64_t *bar, int n, int size) {  // for the last uses of a ring of n so far
+            for (int j = max(0, n - size); j < n; ++j)
+                closed &= mbar_wait(&bar[j % size], (j / size) & 1, a.wait_ns, nullptr, 0);
+        };
+        if (of(&s.ended, 0)) wait(&s.mdone, 1, 1);
+        wait(s.empty, of(&s.stepped, 0), a.stages);
+        if (bufs) wait(s.dfull, of(&s.filled, 0), bufs);
+        if (leader) {
+            const int n0 = s.issued, n1 = of(&s.issued, 1);
+            for (int j = n0; j < n1; ++j)  // only the other CTA's
+                mbar_arrive_expect_tx(&s.full[j % a.stages], of(reinterpret_cast<const int *>(&s.bytes[j % a.stages]), 1));
+            for (int j = n1; j < n0; ++j)  // expected, and not copied
+                mbar_complete_tx(&s.full[j % a.stages], s.bytes[j % a.stages]);
+            wait(s.full, max(n0, n1), a.stages);
+        }
+        if (!closed) atomicOr(a.err, RB_LIN_ERR_OPEN);
+    }
+    __syncthreads();
+}
+
 // The gathering warps' part of a tile: tokens c0 .. c0 + here - 1 of it into rows 0.. of the
 // token rows `at` bytes into each stage, ROWS of them a thread (part, part + 16, ..).
 template <int ROWS>
@@ -449,6 +498,7 @@ __global__ void __launch_bounds__(kLinThreads, 1)
         }
         mbar_init(&s.mdone, 1);
         s.abort = 0;
+        s.issued = s.stepped = s.filled = s.ended = 0;
         mbar_init_fence();
     }
     if (warp == 1) {
@@ -482,6 +532,7 @@ __global__ void __launch_bounds__(kLinThreads, 1)
         int issued = 0;
         bool ok = true;
         const bool chosen = elect_one();
+        const int held = a.withhold >> (PAIR ? rank : 0) & 1;
         for (int i = first; ok && lin_tile(a, off, pre, i, t); i += a.withhold ? 1 << 30 : stride) {
             const int n0 = (PAIR ? 2 * t.mt + rank : t.mt) * outputs;
             const int here = PAIR ? t.cols / 2 : t.cols;  // token rows of this CTA
@@ -500,10 +551,11 @@ __global__ void __launch_bounds__(kLinThreads, 1)
             // weights that no other tile of tokens reads leave the L2 first
             const uint64_t pol = pre[t.e + 1] - pre[t.e] > 1 ? keep : once;
             if (chosen) {
-                for (int k = k0; k < k1 - a.withhold; ++k, ++issued) {
+                for (int k = k0; k < k1 - held; ++k, ++issued) {
                     if (!(ok = lin_wait1(&s.empty[st.at], st.phase ^ 1, a, abort))) break;
                     uint8_t *base = ring + (size_t)st.at * stage_bytes, *xb = base + kLinTile;
                     const int c0 = k * (F8 ? 128 : 64);
+                    s.bytes[st.at] = PAIR ? bytes / 2 : bytes;
                     if (leader) mbar_arrive_expect_tx(&s.full[st.at], bytes);
                     if constexpr (PAIR) {
                         const uint32_t bar = cluster_addr(&s.full[st.at], 0);
@@ -526,17 +578,16 @@ __global__ void __launch_bounds__(kLinThreads, 1)
             }
             ok = __all_sync(0xffffffffu, ok);
         }
-        if (chosen && ok) ok = lin_emptied(a, s, issued, abort);
-        // copies under way (the pair's complete on the leader's barriers) end before
-        // the block does
-        if (chosen && !ok && leader)
-            for (int j = max(0, issued - a.stages); j < issued; ++j)
-                mbar_wait(&s.full[j % a.stages], (j / a.stages) & 1, a.wait_ns, nullptr, 0);
+        if (chosen) {
+            if (ok) lin_emptied(a, s, issued, abort);
+            s.issued = issued;
+        }
         __syncwarp();
     } else if (warp == 1) {  // ------------------------------------------ MMA
         if (leader && elect_one()) {
             LinRing st, db;
             bool ok = true;
+            int stepped = 0, filled = 0;
             const uint64_t wd0 = swizzled_desc(smem_u32(ring)), xd0 = swizzled_desc(smem_u32(ring + kLinTile));
             for (int i = first; ok && lin_tile(a, off, pre, i, t); i += stride) {
                 const uint32_t idesc = float_idesc(a.format, PAIR ? 256 : 128, t.cols);
@@ -557,20 +608,24 @@ __global__ void __launch_bounds__(kLinThreads, 1)
                         mma_float_ss<F8, PAIR>(d, wd0 + step + 2 * j, xd0 + step + 2 * j, idesc, j > 0 || part > 0);
                     if (PAIR) mma_commit_pair(&s.empty[st.at]);
                     else mma_commit(&s.empty[st.at]);
+                    ++stepped;
                     st.next(a.stages);
                     if (++part == PART || k == k1 - 1) {
                         if (PAIR) mma_commit_pair(&s.dfull[db.at]);
                         else mma_commit(&s.dfull[db.at]);
+                        ++filled;
                         db.next(a.bufs);
                         part = 0;
                     }
                 }
             }
-            if (!ok) {  // products under way end before their memory is given back
+            if (!ok) {  // lin_settle waits for it
                 if (PAIR) mma_commit_pair(&s.mdone);
                 else mma_commit(&s.mdone);
-                mbar_wait(&s.mdone, 0, a.wait_ns, nullptr, 0);
             }
+            s.stepped = stepped;
+            s.filled = filled;
+            s.ended = !ok;
         }
     } else if (F8) {  // ---------------------------------------------- scales
         const int nb = (a.N + 127) / 128;  // rows of scale blocks of a matrix
@@ -807,6 +862,7 @@ __global__ void __launch_bounds__(kLinThreads, 1)
     tc_fence_before();
     __syncthreads();
     if (PAIR) cluster_sync_all();  // both have read their products
+    if (*abort) lin_settle<PAIR>(a, s, F8 && !PAIR ? 0 : a.bufs);
     tc_fence_after();
     if (warp == 1) {
         if (PAIR) tmem_dealloc_pair(tmem, 512);

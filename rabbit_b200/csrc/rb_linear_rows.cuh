@@ -52,6 +52,7 @@ __global__ void __launch_bounds__(kLinThreads, 1)
         }
         mbar_init(&s.mdone, 1);
         s.abort = 0;
+        s.issued = s.stepped = s.filled = s.ended = 0;
         mbar_init_fence();
     }
     if (warp == 1) tmem_alloc_pair(&s.tmem, 512);
@@ -77,13 +78,15 @@ __global__ void __launch_bounds__(kLinThreads, 1)
                 int issued = 0;
                 bool ok = true;
                 const uint32_t bytes = 2 * (kLinTile + (a.rows ? 0 : kLinTile));
+                const int held = a.withhold >> rank & 1;
                 for (int i = first; ok && lin_tile(a, off, pre, i, t); i += a.withhold ? 1 << 30 : stride) {
                     const int n0 = GATED ? t.mt * 128 : t.mt * 256 + rank * 128;
                     const int r0 = t.row0 + rank * 128;
-                    for (int k = 0; k < a.steps - a.withhold; ++k, ++issued) {
+                    for (int k = 0; k < a.steps - held; ++k, ++issued) {
                         if (!(ok = lin_wait1(&s.empty[st.at], st.phase ^ 1, a, abort))) break;
                         uint8_t *base = ring + (size_t)st.at * kRowsStage;
                         const uint32_t bar = cluster_addr(&s.full[st.at], 0);
+                        s.bytes[st.at] = bytes / 2;
                         if (leader) mbar_arrive_expect_tx(&s.full[st.at], bytes);
                         for (int b = 0; b < 128; b += GATED ? 64 : 128)  // (the map's boxes)
                             tma_load_4d_pair(base + kLinTile + b * 128, &mw, k * 128, n0 + b, GATED ? rank : 0,
@@ -92,11 +95,8 @@ __global__ void __launch_bounds__(kLinThreads, 1)
                         st.next(a.stages);
                     }
                 }
-                if (ok) ok = lin_emptied(a, s, issued, abort);
-                // copies under way (they complete on the leader's barriers) end before the block does
-                if (!ok && leader)
-                    for (int j = max(0, issued - a.stages); j < issued; ++j)
-                        mbar_wait(&s.full[j % a.stages], (j / a.stages) & 1, a.wait_ns, nullptr, 0);
+                if (ok) lin_emptied(a, s, issued, abort);
+                s.issued = issued;
             }
             __syncwarp();
         } else if (warp == 1) {  // -------------------------------------- MMA
@@ -104,6 +104,7 @@ __global__ void __launch_bounds__(kLinThreads, 1)
                 if (elect_one()) {
                     LinRing st, db;
                     bool ok = true;
+                    int stepped = 0;
                     const uint64_t xd0 = swizzled_desc(smem_u32(ring)), wd0 = swizzled_desc(smem_u32(ring + kLinTile));
                     const uint32_t idesc = float_idesc(a.format, 256, 256);
                     for (int i = first; ok && lin_tile(a, off, pre, i, t); i += stride)
@@ -119,13 +120,13 @@ __global__ void __launch_bounds__(kLinThreads, 1)
                                                          idesc, j > 0);
                             mma_commit_pair(&s.dfull[db.at]);
                             mma_commit_pair(&s.empty[st.at]);
+                            ++stepped;
                             st.next(a.stages);
                             db.next(2);
                         }
-                    if (!ok) {  // products under way end before their memory is given back
-                        mma_commit_pair(&s.mdone);
-                        mbar_wait(&s.mdone, 0, a.wait_ns, nullptr, 0);
-                    }
+                    if (!ok) mma_commit_pair(&s.mdone);  // lin_settle waits for it
+                    s.stepped = s.filled = stepped;
+                    s.ended = !ok;
                 }
             }
             __syncwarp();
@@ -278,6 +279,7 @@ __global__ void __launch_bounds__(kLinThreads, 1)
     tc_fence_before();
     __syncthreads();
     cluster_sync_all();  // both have read their products
+    if (*abort) lin_settle<true>(a, s, 2);
     tc_fence_after();
     if (warp == 1) tmem_dealloc_pair(tmem, 512);
     cluster_sync_all();

@@ -37,3 +37,32 @@ def test_pairs_that_follow_one_another(torch, rc):
         c.lin.apply_dev(c.xd.data_ptr(), code, y.data_ptr(), c.R, stream=base.stream(torch), **c.kw)
         torch.cuda.synchronize()
         assert torch.equal(y, first)
+
+
+@pytest.mark.parametrize("name,R,N,K,gated,out", [
+    ("bf16", 700, 3000, 256, False, "bf16"), ("f16", 700, 3000, 512, False, "f32"),
+    ("e4m3", 700, 3000, 512, False, "bf16"), ("e4m3", 600, 700, 2500, True, "f32"), ("f16", 600, 2000, 200, True, "f16"),
+])
+@pytest.mark.parametrize("listed", [False, True])
+@pytest.mark.parametrize("cta", [0, 1])
+def test_a_pair_of_which_one_gives_up_first(torch, rc, name, R, N, K, gated, out, listed, cta):
+    """One CTA of each pair copies a step less than the other. The call ends with a status, nothing of it
+    is still under way then (the check would say so), and the next call is whole."""
+    c = base.Case(torch, rc, name, R, N, K, gated)
+    off, rows = base.dev(torch, np.array([0, R], np.int32)), base.dev(torch, np.arange(R, dtype=np.int32)[::-1])
+    y, code = c.out(out, R)
+    run = lambda: c.lin.grouped_dev(c.xd.data_ptr(), R, off.data_ptr(), code, y.data_ptr(), R,  # noqa: E731
+                                    d_rows=rows.data_ptr() if listed else 0, stream=base.stream(torch), **c.kw)
+    rc.check(rc.lib().rabbit_cuda_set_wait_limit_ms(20))
+    try:
+        rc.check(rc.lib().rabbit_cuda_linear_debug_withhold_cta(c.lin.handle, cta))
+        run()
+        with pytest.raises(rc.RabbitCudaError, match="wait ran out") as e:
+            c.lin.check(base.stream(torch))
+        assert e.value.status == rc.ERR_TIMEOUT and "did not end" not in str(e.value)
+    finally:
+        rc.check(rc.lib().rabbit_cuda_set_wait_limit_ms(2000))
+    run()
+    c.lin.check(base.stream(torch))
+    at = np.arange(0, R, max(1, R // 40))
+    c.close(base.f64(y)[at], c.x[::-1][at] if listed else c.x[at], 0, out)
