@@ -3,6 +3,7 @@
 // experts' rows (:356-357, 398-399).
 #include <math.h>
 
+#include <atomic>
 #include <type_traits>
 
 #include "rb_device.cuh"
@@ -243,6 +244,22 @@ __global__ void __launch_bounds__(kRouteThreads, 1) k_route_order(const __grid_c
         asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
 }
 
+constexpr size_t route_smem_bytes(int E) { return sizeof(int) * (size_t)E * (kRouteWarps + 2); }
+
+// What a kernel may take of shared memory belongs to it, for every thread's calls: the most that
+// any call takes, once for each device. (With experts chosen in it k_route_order has at most 256.)
+static cudaError_t route_prepare() {
+    static_assert(route_smem_bytes(256) < 48 * 1024 - 256, "a launch has that unasked");
+    static std::atomic<bool> done[kMaxDevices];
+    std::atomic<bool> &mine = done[current_device()];
+    if (mine.load()) return cudaSuccess;
+    const cudaError_t e = cudaFuncSetAttribute(reinterpret_cast<const void *>(k_route_order<0>),
+                                               cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                               (int)route_smem_bytes(kRouteExperts));
+    if (e == cudaSuccess) mine.store(true);
+    return e;
+}
+
 struct CombineArgs {
     const void *y;
     int64_t ys;
@@ -375,12 +392,14 @@ int rabbit_cuda_experts_route_dev(const float *d_scores, int64_t score_stride, i
     DeviceScope scope(current_device());
     if (scope.status != RABBIT_CUDA_OK) return scope.status;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    const size_t smem = sizeof(int) * (size_t)a.E * (kRouteWarps + 2);
+    const size_t smem = route_smem_bytes(a.E);
     // Up to a token a warp of the cluster the picks are made by the kernel that orders: one launch.
     // (With more than 256 experts a lane has too many for that kernel's registers.)
     const int v = n_experts <= 32 ? 1 : n_experts <= 64 ? 2 : n_experts <= 128 ? 4 : n_experts <= 256 ? 8 : 32;
     const bool pick = d_scores && n_tokens <= kRouteCluster * kRouteWarps && v <= 8;
     const unsigned ctas = n_tokens <= kRouteWarps ? 1 : kRouteCluster;
+    scope.launch(route_prepare(), "experts_route: shared memory");
+    if (scope.status != RABBIT_CUDA_OK) return scope.status;
     if (d_scores && !pick) {
         const int sms = device_sms();
         const int64_t want = ((int64_t)n_tokens + 7) / 8;
@@ -390,10 +409,6 @@ int rabbit_cuda_experts_route_dev(const float *d_scores, int64_t score_stride, i
     }
     auto kern = !pick ? k_route_order<0> : v == 1 ? k_route_order<1> : v == 2 ? k_route_order<2>
                 : v == 4 ? k_route_order<4> : k_route_order<8>;
-    if (smem > 48 * 1024 - 256)
-        scope.launch(cudaFuncSetAttribute(reinterpret_cast<const void *>(kern),
-                                          cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem),
-                     "experts_route: shared memory");
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;

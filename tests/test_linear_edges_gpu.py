@@ -66,3 +66,39 @@ def test_a_pair_of_which_one_gives_up_first(torch, rc, name, R, N, K, gated, out
     c.lin.check(base.stream(torch))
     at = np.arange(0, R, max(1, R // 40))
     c.close(base.f64(y)[at], c.x[::-1][at] if listed else c.x[at], 0, out)
+
+
+def test_two_threads_route_among_different_numbers_of_experts(torch, rc):
+    """Both need more shared memory than a launch has unasked, and not the same: what the kernel may take
+    belongs to the kernel, not to a call."""
+    import threading
+
+    T, k, wrong = 40, 8, []
+    rng = np.random.default_rng(11)
+    ids = {E: rng.integers(0, E, (T, k)).astype(np.int32) for E in (360, 700, 1024)}
+    idd = {E: base.dev(torch, v) for E, v in ids.items()}
+    got = {E: [torch.zeros(n, dtype=torch.int32, device="cuda") for n in (E + 1, T * k, T * k)] for E in ids}
+    streams = {E: torch.cuda.Stream() for E in ids}
+    torch.cuda.synchronize()
+    start = threading.Barrier(len(ids))
+
+    def go(E):
+        off, rows, place = (t.data_ptr() for t in got[E])
+        start.wait()
+        for _ in range(1500):
+            try:
+                rc.experts_route_dev(0, T, E, k, idd[E].data_ptr(), 0, off, rows, place, stream=streams[E].cuda_stream)
+            except rc.RabbitCudaError as e:
+                wrong.append((E, str(e)))
+                return
+
+    threads = [threading.Thread(target=go, args=(E,)) for E in ids]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert not wrong
+    for E in ids:
+        for t, exact in zip(got[E], lo.order(ids[E], E)):
+            np.testing.assert_array_equal(t.cpu().numpy(), exact.reshape(-1))
