@@ -683,7 +683,8 @@ int rabbit_cuda_linear_free(rabbit_cuda_linear *lin);
  * the product of the scales in fp32. Sums are fp32, rounded to out_dtype once: a block's on the
  * tensor cores, then over the blocks in order; 16-bit products' over all of n_in on the tensor
  * cores (which cut off what fp32 cannot hold: up to 2^-25 of the sum for each 16 channels) or, for fp32 outputs
- * and n_in above 16384, in parts of 256 channels. silu in fp32 (to |gate| 2^-24 + 2^-21 of itself).
+ * and n_in above 16384, in parts of 256 channels. silu in fp32, to 2^-20 of itself
+ * for fp32 outputs and to (10 + |gate|) 2^-23 for others, wherever gate exp(gate) is a normal fp32 number.
  * Infinities and NaN go where the formula takes them, and to
  * no other row. y must not overlap an input. n_rows up to 2^30; 0 does nothing. Strides of x up to
  * 2^30 elements, of its scales up to 2^30. */

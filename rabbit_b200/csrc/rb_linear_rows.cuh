@@ -240,7 +240,7 @@ __global__ void __launch_bounds__(kLinThreads, 1)
                         float v[8];
 #pragma unroll
                         for (int e = 0; e < 8; ++e)
-                            v[e] = GATED ? lin_silu(g[l + e]) * acc[(o * NB + b + 4) & 7][l + e] : g[l + e];
+                            v[e] = GATED ? lin_silu<OUT>(g[l + e]) * acc[(o * NB + b + 4) & 7][l + e] : g[l + e];
                         store8<true>(reinterpret_cast<OUT *>(outs + mine * kRowsPitch) + (2 * b + h) * 16 + l, v);
                     }
                 }

@@ -102,3 +102,52 @@ def test_two_threads_route_among_different_numbers_of_experts(torch, rc):
     for E in ids:
         for t, exact in zip(got[E], lo.order(ids[E], E)):
             np.testing.assert_array_equal(t.cpu().numpy(), exact.reshape(-1))
+
+
+@pytest.mark.parametrize("name,R,K", [("bf16", 7, 512), ("bf16", 99, 128), ("bf16", 700, 128),  # one CTA, pairs
+                                      ("e4m3", 40, 128), ("e4m3", 99, 128), ("e4m3", 700, 128)])
+@pytest.mark.parametrize("out", ["f32", "bf16"])
+def test_far_gates(torch, rc, name, R, K, out):
+    """silu(g) u where exp(-g) leaves fp32 and g exp(g) does not yet: gates down to -104, each product exact
+    (one channel the gate, one the up). Bar, u = 2^-24: fp32 outputs take exp(-|g| / 2) to a step (2 u), its square and
+    the gate times it twice (2 * 2 u + 2 u), 1 + its square (half of 5 u, and u), the division (4 u) and up (u): 15 u.
+    bf16's: exp(-|g| / 2) to 4 u and 3/4 |g| u, so 8 u + 3/2 |g| u and 2 u above, 1 + its square at most half of 9 u,
+    3/4 of |g| / (1 + e^|g|) < 0.3 and u below, the division 4 u and up u: (21 + 1.5 |g|) u, then half a step of bf16.
+    Below 2^-126 fp32's smallest step, times up."""
+    N = 40
+    gates = np.concatenate([-np.arange(87, 104.5, 0.5), -np.arange(0, 16, 0.5), [0.25, 1, 3, 8, 40, 80, 88, 100, 120],
+                            -np.arange(16, 87, 1.5)])
+    if name == "e4m3":  # codes of 4 bits: the scale makes the rest
+        x, w = np.zeros((R, K)), np.zeros((2, N, K))
+        g = np.resize(gates, R)
+        x[:, 0], x[:, 1] = 1, 1
+        w[0, :, 0], w[1, :, 1] = 1, 1
+        xq, one = (x * 0x38).astype(np.uint8), 0x38  # the code of 1
+        c = base.Case(torch, rc, name, R, N, K, True)
+        c.xd[:R, :K] = base.dev(torch, xq)
+        c.wd[0, :, :, :K] = base.dev(torch, (w * one).astype(np.uint8))
+        up = 2.0 ** 60
+        # the token's scale is |g|, the gate's its sign, the up's 2^60 / |g| cannot be exact for each: up = |g| 2^60
+        c.sx[:] = base.dev(torch, np.abs(g)[:, None].astype(np.float32))
+        c.sw[:] = 0
+        c.sw[0, 0], c.sw[0, 1] = -1.0, up
+        g, u = -np.abs(g), np.abs(g) * up
+    else:
+        c = base.Case(torch, rc, name, R, N, K, True)
+        g = np.resize(gates, R)
+        x, w = np.zeros((R, K)), np.zeros((2, N, K))
+        x[:, 0], x[:, 1] = g, 1
+        w[0, :, 0], w[1, :, 1] = 1, 2.0 ** 60
+        c.xd[:R, :K], c.wd[0, :, :, :K] = base.dev(torch, x).bfloat16(), base.dev(torch, w).bfloat16()
+        u = np.full(R, 2.0 ** 60)
+    y, code = c.out(out, R)
+    c.lin.apply_dev(c.xd.data_ptr(), code, y.data_ptr(), R, stream=base.stream(torch), **c.kw)
+    c.lin.check(base.stream(torch))
+    want = lo.silu(g) * u
+    a = np.abs(g)
+    steps = 15 if out == "f32" else 21 + 1.5 * a
+    bar = steps * base.U * np.abs(want) + 2.0 ** -148 * np.abs(u)
+    bar = bar + base.HALF[out] * (np.abs(want) + bar)
+    off = np.abs(base.f64(y)[:R] - want[:, None])
+    wrong = ~(off <= bar[:, None]).all(1)
+    assert not wrong.any(), list(zip(g[wrong], base.f64(y)[:R][wrong, 0], want[wrong]))[:8]
