@@ -184,10 +184,12 @@ static int lin_run(rabbit_cuda_linear *lin, const char *what, const void *d_x, i
         return fail(RABBIT_CUDA_ERR_ARGS, "%s: x_scale_stride below its row or above 2^30, or scales not aligned", what);
     if (x_rows < 1 || (!d_rows && x_rows < n_rows))
         return fail(RABBIT_CUDA_ERR_ARGS, "%s: x_rows of %d for %d rows", what, x_rows, n_rows);
-    // The tensor cores' sums of 16-bit products lose up to 2^-25 of the result at each of K / 16
-    // steps: nothing beside a 16-bit output's half step up to K 16384 (2^-15), parts beyond
-    // and for fp32 outputs.
-    const int mode = f8 ? kLinF8 : out == 4 || d.n_in > 16384 ? kLinParts : kLinWhole;
+    // The tensor cores' sums of 16-bit products lose up to 2^-22 of the sum so far at each of K / 16
+    // steps: of terms of one sign 2.5e-5 at K 4096 and 1.0e-4 at 16384. Kept to a tenth of half a step of the
+    // output (f16: 2^-12 and more, bf16: 2^-9), parts beyond and for fp32 outputs. (8192 x 4096 x 14336 to f16: 780 us in
+    // parts, 720 whole; 8192 x 4096 x 4096: 240 and 190.)
+    const int whole = out_dtype == RABBIT_CUDA_F16 ? 4096 : out_dtype == RABBIT_CUDA_BF16 ? 16384 : 0;
+    const int mode = f8 ? kLinF8 : d.n_in > whole ? kLinParts : kLinWhole;
     int64_t tiles;
     size_t smem;
     const int sms = lin->ctx->sm_count;

@@ -22,10 +22,10 @@
 //                proxies, some 0.3 us a step.)
 // Accumulation (MODE):
 //   kLinWhole  16-bit: in tensor memory over all of K, read once;
-//   kLinParts  16-bit, for fp32 outputs or a very long K: the tensor cores' sum is cut off,
-//              not rounded, at each MMA, an error that grows with their number (K 2048: 2e-6 of
-//              the result, K 14336: 1.4e-5); so each 256 channels are read out and added
-//              in 32-bit registers;
+//   kLinParts  16-bit, for fp32 outputs or a long K: the tensor cores' sum is cut off,
+//              not rounded, at each MMA, an error that grows with their number (K 2048 and 14336:
+//              2.3e-6 and 1.8e-5 of random terms' sum, 1.2e-5 and 9.3e-5 of terms' of one sign); so each 256
+//              channels are read out and added in 32-bit registers (4e-7, 1.2e-6);
 //   kLinF8     e4m3: each step is a scale block, read out and added to 32-bit registers as
 //              acc += (sw sx) * product, while the MMAs of the next steps fill other buffers
 //              of tensor memory (512 columns / the tile's, at least two).

@@ -151,3 +151,54 @@ def test_far_gates(torch, rc, name, R, K, out):
     off = np.abs(base.f64(y)[:R] - want[:, None])
     wrong = ~(off <= bar[:, None]).all(1)
     assert not wrong.any(), list(zip(g[wrong], base.f64(y)[:R][wrong, 0], want[wrong]))[:8]
+
+
+@pytest.mark.parametrize("name,R,N,K,out", [
+    ("bf16", 3, 70, 14336, "f32"), ("f16", 300, 130, 14336, "f32"), ("bf16", 600, 9600, 14336, "f32"),  # pairs at last
+    ("e4m3", 7, 70, 14336, "f32"), ("e4m3", 600, 3000, 14336, "f32"), ("f16", 5, 9600, 32768, "f16"),
+    ("f16", 600, 9600, 4096, "f16"), ("f16", 600, 9600, 14336, "f16"), ("bf16", 600, 9600, 16384, "bf16"),
+    ("bf16", 600, 9600, 8192, "f16"), ("bf16", 40, 70, 17000, "bf16"),
+])
+def test_sums_of_one_sign(torch, rc, name, R, N, K, out):
+    """Terms of one sign, so that every partial sum counts in full. Bar, u = 2^-24: each tensor-core step (32
+    bytes of channels) is off by 4 u of the sum it leaves there, which starts anew with each part of 256
+    channels (e4m3: block of 128); each part's addition by u of the sum so far (e4m3: a scale's product, one more u of
+    the part), the sum over a cluster's eight parts and the rest by 8 u of the whole. Summed in tensor memory
+    over all channels, a step's error goes by the whole sum so far: several times this bar, and the bar for
+    16-bit outputs of fewer channels."""
+    rng = np.random.default_rng(R + K)
+    f8 = name == "e4m3"
+    dt, code = base.types(torch, rc, name)
+    gen = torch.Generator("cuda").manual_seed(3)
+    some = lambda *s: torch.rand(*s, generator=gen, device="cuda") * 0.35 + 0.05  # noqa: E731
+    x, w = some(R, K), some(N, K)
+    if f8:  # codes 0x20 .. 0x40: 2^-3 .. 2
+        x, w = (torch.randint(0x20, 0x40, s, generator=gen, device="cuda", dtype=torch.uint8) for s in ((R, K), (N, K)))
+        nb = K // 128
+        sx, sw = some(R, nb), some(-(-N // 128), nb)
+    else:
+        x, w = x.to(dt), w.to(dt)
+    lin = rc.Linear(code, N, K, w.data_ptr(), d_scale=sw.data_ptr() if f8 else 0)
+    yt, ycode = base.types(torch, rc, out)
+    y = torch.zeros(R, N, dtype=yt, device="cuda")
+    lin.apply_dev(x.data_ptr(), ycode, y.data_ptr(), R, d_x_scale=sx.data_ptr() if f8 else 0, stream=base.stream(torch))
+    lin.check(base.stream(torch))
+    step, part = (32, 128) if f8 else (16, 256)
+    if K <= {"f16": 4096, "bf16": 16384, "f32": 0}[out]:
+        part = K
+    pad = -K % part  # (zeros: nothing is added)
+    outs = np.arange(N) if N < 200 else rng.integers(0, N, 90)
+    ww = lo.VALUES[w[outs].cpu().numpy()] if f8 else base.f64(w[outs])
+    for r in sorted({0, R - 1, R // 2, R // 3}):
+        xx = lo.VALUES[x[r].cpu().numpy()] if f8 else base.f64(x[r])
+        # [outputs, parts, steps]: sums that the tensor cores leave after each step
+        held = np.pad(ww * xx, ((0, 0), (0, pad))).reshape(len(outs), -1, part // step, step).sum(-1).cumsum(-1)
+        if f8:
+            held = held * (base.f64(sx[r]) * base.f64(sw)[outs // 128])[..., None]
+        sums = held[..., -1].cumsum(-1)
+        want = sums[:, -1]
+        bar = base.U * (4 * held.sum((1, 2)) + sums.sum(1) + (8 + f8) * want)
+        if out != "f32":  # half of the step between the numbers around it
+            bar = bar + 2.0 ** (np.floor(np.log2(want)) - (11 if out == "f16" else 8))
+        off = np.abs(base.f64(y[r])[outs] - want)
+        assert (off <= bar).all(), (r, (off / bar).max())
