@@ -202,3 +202,43 @@ def test_sums_of_one_sign(torch, rc, name, R, N, K, out):
             bar = bar + 2.0 ** (np.floor(np.log2(want)) - (11 if out == "f16" else 8))
         off = np.abs(base.f64(y[r])[outs] - want)
         assert (off <= bar).all(), (r, (off / bar).max())
+
+
+@pytest.mark.parametrize("name", ["e4m3", "f16"])
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("listed", [False, True])
+def test_what_is_not_finite_stays_in_its_row_of_many(torch, rc, name, gated, listed):
+    """Tiles of 256 tokens by pairs of CTAs: NaN in a token's row, in an output's weights and in a scale
+    reach no other row or output, nor the other expert."""
+    R, N, K = 600, 300, 256
+    c = base.Case(torch, rc, name, R, N, K, gated, experts=2)
+    rows = np.random.default_rng(2).integers(0, R, R) if listed else np.arange(R)
+    half = 290
+    off, rd = base.dev(torch, np.array([0, half, R], np.int32)), base.dev(torch, rows.astype(np.int32))
+    y, code = c.out("f32", R)
+
+    def run():
+        c.lin.grouped_dev(c.xd.data_ptr(), R, off.data_ptr(), code, y.data_ptr(), R,
+                          d_rows=rd.data_ptr() if listed else 0, stream=base.stream(torch), **c.kw)
+        c.lin.check(base.stream(torch))
+        return y.clone()
+
+    clean = run()
+    assert clean[:R].isfinite().all()
+    nan = 0x7F if name == "e4m3" else float("nan")
+    some = [7, 289, 290, 511]
+    for r in some:
+        c.xd[int(rows[r]), 100] = nan
+    c.wd[1, 0, 130, 5] = nan
+    bad = torch.zeros_like(y, dtype=torch.bool)
+    bad[:R][base.dev(torch, np.isin(rows, rows[some]))] = True
+    bad[half:R, 130] = True
+    got = run()
+    assert got[bad].isnan().all() and torch.equal(got[~bad], clean[~bad])
+    if name == "e4m3":
+        c.sx[int(rows[33]), 1] = float("nan")
+        c.sw[0, 0, 1, 0] = float("nan")
+        bad[:R][base.dev(torch, rows == rows[33])] = True
+        bad[:half, 128:256] = True
+        got = run()
+        assert got[bad].isnan().all() and torch.equal(got[~bad], clean[~bad])
