@@ -341,7 +341,7 @@ extern "C" int rabbit_cuda_f8_quantise_dev(int dtype, const void *d_x, int64_t x
     // Rows: blocks are handed out warp by warp, in one wave of the SMs at most.
     const int64_t ctas = ((int64_t)n_rows * a.nb + kF8Threads / 8 - 1) / (kF8Threads / 8);
     const dim3 grid = block_rows == 1 ? dim3((unsigned)(ctas < kF8Resident * sms ? ctas : kF8Resident * sms))
-                                      : dim3((n_rows + 127) / 128, a.nb);
+                                      : dim3((n_rows - 1) / 128 + 1, a.nb);
     with_dtype(dtype, [&](auto t) {
         using T = decltype(t);
         auto k = block_rows == 1 ? (vec ? k_f8_rows<T, true> : k_f8_rows<T, false>)

@@ -242,3 +242,20 @@ def test_what_is_not_finite_stays_in_its_row_of_many(torch, rc, name, gated, lis
         bad[:half, 128:256] = True
         got = run()
         assert got[bad].isnan().all() and torch.equal(got[~bad], clean[~bad])
+
+
+def test_blocks_of_as_many_rows_as_there_may_be(torch, rc):
+    """2^31 - 1 rows of one column: the last block has 127."""
+    R = 2 ** 31 - 1
+    x = torch.zeros(R, dtype=torch.bfloat16, device="cuda")
+    q = torch.full((R + 1,), 0x55, dtype=torch.uint8, device="cuda")
+    s = torch.full((2 ** 24 + 1,), 7.0, device="cuda")
+    x[:3], x[-127], x[-1], x[-128] = 3.0, -2.0, 1.0, 448.0
+    rc.f8_quantise_dev(rc.BF16, x.data_ptr(), q.data_ptr(), s.data_ptr(), R, 1, block_rows=128,
+                       stream=base.stream(torch))
+    torch.cuda.synchronize()
+    for a, b, block in ((0, 128, 0), (R - 127, R, 2 ** 24 - 1), (R - 255, R - 127, 2 ** 24 - 2), (2 ** 30, 2 ** 30 + 128, 2 ** 23)):
+        base.same_codes((q[a:b, None].cpu().numpy(), s[block:block + 1, None].cpu().numpy()),
+                        lo.quantise(base.f64(x[a:b])[:, None], 128))
+    assert q[-1] == 0x55 and s[-1] == 7.0
+    assert int((q[:R] != 0).sum()) == 6
