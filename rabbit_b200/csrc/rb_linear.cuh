@@ -168,16 +168,42 @@ struct LinRing {
     }
 };
 
-// Bounded wait of one thread. (Arrivals and waits between the CTAs of a pair have the
-// default scope: with the cluster's on every barrier a step took 0.2 us more. What crosses
-// from one to the other is either read by the tensor cores of its own CTA after a proxy
-// fence there, or no memory at all.)
+// An arrival in either CTA of a pair, and mbar_try_wait for such, of the cluster's scope. What changes hands is
+// tensor memory, which the tcgen05 fences on both sides order, or rows in shared memory, for which the two fences
+// below are: before the arrival and behind the wait. So both are relaxed. (With a release and an acquire of all memory
+// a step of 0.44 us took 0.8 and 8192 tokens of 8 f16 experts 5.8 ms instead of 3.4: they wait for the
+// thread's accesses under way.)
+__device__ __forceinline__ void cluster_bar_arrive(uint32_t bar) {
+    asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+// Fences of the cluster's scope for shared memory alone: this CTA's before an arrival, either's behind a wait.
+__device__ __forceinline__ void cluster_release_shared() {
+    asm volatile("fence.release.sync_restrict::shared::cta.cluster;" ::: "memory");
+}
+__device__ __forceinline__ void cluster_acquire_shared() {
+    asm volatile("fence.acquire.sync_restrict::shared::cluster.cluster;" ::: "memory");
+}
+__device__ __forceinline__ bool cluster_try_wait(uint64_t *bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.relaxed.cluster.shared::cta.b64 p, [%1], %2, %3;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(smem_u32(bar)), "r"(parity), "r"(1000000u)
+        : "memory");
+    return ok != 0;
+}
+
+// Bounded wait of one thread. OTHER: on a barrier at which the pair's other CTA arrives (cluster_bar_arrive).
+template <bool OTHER = false>
 __device__ __forceinline__ bool lin_wait1(uint64_t *bar, uint32_t parity, const LinArgs &a,
                                           volatile int *abort) {
-    if (mbar_try_wait(bar, parity)) return true;
+    auto passed = [&] { return OTHER ? cluster_try_wait(bar, parity) : mbar_try_wait(bar, parity); };
+    if (passed()) return true;
     const uint64_t t0 = globaltimer_ns();
     for (uint32_t it = 1;; ++it) {
-        if (mbar_try_wait(bar, parity)) return true;
+        if (passed()) return true;
         if ((it & 15u) == 0) {
             if (*abort) return false;
             if (globaltimer_ns() - t0 > a.wait_ns) {
@@ -208,9 +234,6 @@ __device__ __forceinline__ uint32_t cluster_addr(const void *p, uint32_t rank) {
     uint32_t at;
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(p)), "r"(rank));
     return at;
-}
-__device__ __forceinline__ void cluster_bar_arrive(uint32_t bar) {
-    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 __device__ __forceinline__ void cluster_sync_all() {
     asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
@@ -462,18 +485,23 @@ __device__ __forceinline__ bool lin_gather(const LinArgs &a, LinShared &s, uint3
 }
 
 // One thread, of each CTA of a pair: once this CTA's rows of a step are there, the fence
-// between the proxies, and word to the thread that issues the MMAs (of CTA `to`). In that thread
+// between the proxies, and word to the thread that issues the MMAs (of CTA 0). In that thread
 // itself the fence held up the MMAs: 8192 tokens of 8 f16 experts took 0.3 ms more.
+template <bool PAIR>
 __device__ __forceinline__ void lin_tell(const LinArgs &a, LinShared &s, const int *off, const int *pre,
-                                         int first, int stride, int k0, int k1, uint32_t to,
-                                         volatile int *abort) {
+                                         int first, int stride, int k0, int k1, volatile int *abort) {
     LinTile t;
     LinRing st;
     for (int i = first; lin_tile(a, off, pre, i, t); i += stride)
         for (int k = k0; k < k1; ++k) {
             if (!lin_wait1(&s.rows[st.at], st.phase, a, abort)) return;
             fence_async();
-            cluster_bar_arrive(cluster_addr(&s.told[st.at], to));
+            if (PAIR) {
+                cluster_release_shared();
+                cluster_bar_arrive(cluster_addr(&s.told[st.at], 0));
+            } else {
+                mbar_arrive(&s.told[st.at]);
+            }
             st.next(a.stages);
         }
 }
@@ -606,14 +634,15 @@ __global__ void __launch_bounds__(kLinThreads, 1)
                 const uint32_t idesc = float_idesc(a.format, PAIR ? 256 : 128, t.cols);
                 int part = 0;
                 for (int k = k0; k < k1; ++k) {
-                    if (!(ok = lin_wait1(&s.full[st.at], st.phase, a, abort))) break;
+                    if (!(ok = lin_wait1<PAIR>(&s.full[st.at], st.phase, a, abort))) break;
                     if (a.gather) {
-                        if (!(ok = lin_wait1(F8 ? &s.rows[st.at] : &s.told[st.at], st.phase, a, abort))) break;
+                        if (!(ok = lin_wait1<PAIR>(F8 ? &s.rows[st.at] : &s.told[st.at], st.phase, a, abort))) break;
                         if (F8) fence_async();  // (no warp is free to do it)
                     }
+                    if (PAIR) cluster_acquire_shared();
                     const uint64_t step = (uint64_t)(st.at * stage_bytes) >> 4;
                     if (part == 0)
-                        if (!(ok = lin_wait1(PAIR ? &s.mfree[db.at] : &s.dempty[db.at], db.phase ^ 1, a, abort))) break;
+                        if (!(ok = lin_wait1<PAIR>(PAIR ? &s.mfree[db.at] : &s.dempty[db.at], db.phase ^ 1, a, abort))) break;
                     tc_fence_after();
                     const uint32_t d = tmem + db.at * a.bn;
 #pragma unroll
@@ -708,7 +737,7 @@ __global__ void __launch_bounds__(kLinThreads, 1)
             else tile(LinInt<4>(), LinInt<2>());
         }
     } else if (!F8 && warp == 2 && a.gather) {  // ------- word of gathered rows
-        if (elect_one()) lin_tell(a, s, off, pre, first, stride, k0, k1, PAIR ? 0 : rank, abort);
+        if (elect_one()) lin_tell<PAIR>(a, s, off, pre, first, stride, k0, k1, abort);
         __syncwarp();
     }
     } else if (warp >= 12) {  // ------------------------------------- gather

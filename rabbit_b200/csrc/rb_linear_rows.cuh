@@ -109,9 +109,10 @@ __global__ void __launch_bounds__(kLinThreads, 1)
                     const uint32_t idesc = float_idesc(a.format, 256, 256);
                     for (int i = first; ok && lin_tile(a, off, pre, i, t); i += stride)
                         for (int k = 0; k < a.steps; ++k) {
-                            if (!(ok = lin_wait1(&s.full[st.at], st.phase, a, abort))) break;
-                            if (a.rows && !(ok = lin_wait1(&s.told[st.at], st.phase, a, abort))) break;
-                            if (!(ok = lin_wait1(&s.mfree[db.at], db.phase ^ 1, a, abort))) break;
+                            if (!(ok = lin_wait1<true>(&s.full[st.at], st.phase, a, abort))) break;
+                            if (a.rows && !(ok = lin_wait1<true>(&s.told[st.at], st.phase, a, abort))) break;
+                            cluster_acquire_shared();
+                            if (!(ok = lin_wait1<true>(&s.mfree[db.at], db.phase ^ 1, a, abort))) break;
                             tc_fence_after();
                             const uint64_t step = (uint64_t)(st.at * kRowsStage) >> 4;
 #pragma unroll
@@ -132,7 +133,7 @@ __global__ void __launch_bounds__(kLinThreads, 1)
             __syncwarp();
         } else if (warp == 2 && a.rows) {  // ------------- word of gathered rows
             if (elect_one())
-                lin_tell(a, s, off, pre, first, stride, 0, a.steps, 0, abort);
+                lin_tell<true>(a, s, off, pre, first, stride, 0, a.steps, abort);
             __syncwarp();
         }
     } else if (warp >= 12) {  // ------------------------------------- gather
