@@ -207,7 +207,6 @@ static int lin_run(rabbit_cuda_linear *lin, const char *what, const void *d_x, i
     a.xs = d_x_scale;
     a.ws = d.d_scale;
     a.y = d_y;
-    a.out_dtype = out_dtype;
     a.format = d.dtype == RABBIT_CUDA_BF16;
     a.err = lin->d_err;
     a.wait_ns = wait_limit_ns();

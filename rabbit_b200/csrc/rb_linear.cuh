@@ -74,7 +74,6 @@ struct LinArgs {
     uint32_t xs_stride;
     void *y;
     int64_t y_stride;
-    int out_dtype;
     bool vec, pairs;      // y's rows take pieces of 16 bytes, of two elements
     int gated;
     int N, E, R, x_rows;
@@ -512,6 +511,7 @@ __global__ void __launch_bounds__(kLinThreads, 1)
              const __grid_constant__ CUtensorMap mx) {
     extern __shared__ uint8_t lin_raw[];
     constexpr bool F8 = MODE == kLinF8;
+    static_assert(!F8 || !PAIR, "k_linear_rows has these");
     constexpr int PART = MODE == kLinF8 ? 1 : MODE == kLinParts ? kLinPart : 1 << 30;
     uint8_t *ring = lin_raw + ((1024u - (smem_u32(lin_raw) & 1023u)) & 1023u);
     const uint32_t stage_bytes = lin_stage_bytes(PAIR, a.bn);
@@ -694,7 +694,7 @@ __global__ void __launch_bounds__(kLinThreads, 1)
                 }
                 if (c >= t.n) r[j] = -1;
             }
-            const int n0 = (PAIR ? 2 * t.mt + rank : t.mt) * outputs;
+            const int n0 = t.mt * outputs;
             const float *ws = a.ws + ((int64_t)t.e * (1 + GATED) * nb + min(n0 / 128, nb - 1)) * a.steps;
             float v[AHEAD][NT], w[AHEAD][2];
             auto fetch = [&](int k, int h) {
@@ -767,8 +767,8 @@ __global__ void __launch_bounds__(kLinThreads, 1)
             tc_fence_before();
             __syncwarp();
             if (lane == 0) {
-                if (!PAIR || F8) mbar_arrive(&s.dempty[db.at]);
                 if (PAIR) cluster_bar_arrive(mfree + db.at * 8);
+                else mbar_arrive(&s.dempty[db.at]);
             }
             db.next(a.bufs);
         };
@@ -904,7 +904,7 @@ __global__ void __launch_bounds__(kLinThreads, 1)
     tc_fence_before();
     __syncthreads();
     if (PAIR) cluster_sync_all();  // both have read their products
-    if (*abort) lin_settle<PAIR>(a, s, F8 && !PAIR ? 0 : a.bufs);
+    if (*abort) lin_settle<PAIR>(a, s, F8 ? 0 : a.bufs);
     tc_fence_after();
     if (warp == 1) {
         if (PAIR) tmem_dealloc_pair(tmem, 512);
