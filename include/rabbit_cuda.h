@@ -682,9 +682,9 @@ int rabbit_cuda_linear_free(rabbit_cuda_linear *lin);
  *   y = sum_b (sx[row][b] sw[n / 128][b]) sum_{k in block b} x[row][k] w[n][k],
  * the product of the scales in fp32. Sums are fp32, rounded to out_dtype once: a block's on the
  * tensor cores, then over the blocks in order; 16-bit products' over all of n_in on the tensor
- * cores, which cut off what fp32 cannot hold, up to 2^-22 of the sum so far for each 16 channels (4096 terms of
- * one sign: 2.5e-5 of their sum, 16384: 1.0e-4), or in parts of 256 channels (1.2e-6): for fp32 outputs, for f16
- * ones from n_in 4097 on and for bf16 ones from 16385 on. silu in fp32, to 2^-20 of itself
+ * cores, which cut off what fp32 cannot hold, up to 2^-22 of the largest of the sum so far and its terms for each
+ * 16 channels (4096 terms of one sign: 2.5e-5 of their sum, 16384: 1.0e-4), or in parts of 256 channels (1.2e-6): for
+ * fp32 outputs, for f16 ones from n_in 4097 on and for bf16 ones from 16385 on. silu in fp32, to 2^-20 of itself
  * for fp32 outputs and to (10 + |gate|) 2^-23 for others, wherever gate exp(gate) is a normal fp32 number.
  * Infinities and NaN go where the formula takes them, and to
  * no other row. y must not overlap an input. n_rows up to 2^30; 0 does nothing. Strides of x up to
